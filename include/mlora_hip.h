@@ -369,6 +369,127 @@ int mlora_decode_attention(const void* q, int64_t q_row_stride, const void* k, i
 int mlora_silu_mul(const void* gate, const void* up, int64_t in_row_stride, void* out, int32_t rows, int32_t width,
                    int32_t dtype, void* stream);
 
+/* ---- paged KV cache ------------------------------------------------------
+ * A cache in pages of `page` positions (a power of two, 8 to 1024) that ragged
+ * requests share.  One layer's pool is
+ *   keys   [num_pages, kv_heads, page, D]
+ *   values [num_pages, kv_heads, D, page]   (transposed inside a page)
+ * with any stride between pages; position l of request i is in page
+ * table[i][l / page] at l % page.  New tokens of a step are packed rows:
+ * request i has rows [row_indptr[i], row_indptr[i + 1]), the last ones of its
+ * kv_lens[i] positions.  No counterpart in the reference, whose decode runs
+ * over transformers.StaticCache (multi_lora/graph_decode.py:23-111). */
+
+/* State of the pages, all on the device and changed in place: request i holds
+ * the first held[i] entries of table row i, and free[0 .. counts[0]) are the
+ * pages that none holds, taken from the end.  counts[1]: pages that the last
+ * call could not give. */
+typedef struct mlora_pages {
+  int32_t* table;       /* [n, width], table_stride elements between rows */
+  int64_t table_stride;
+  int32_t* held;        /* [n] */
+  int32_t* free;        /* [num_pages] */
+  int32_t* counts;      /* [2] */
+  int32_t n;
+  int32_t width;
+  int32_t num_pages;
+  int32_t page;
+} mlora_pages;
+
+/* A step's rows over the pages.  `rows`, `max_new` and the table's width are
+ * host bounds that size the launches (rows in the packed tensors, new tokens
+ * of one request); the lengths are read on the device.  The plan is the
+ * attention's work list, the workspace holds the parts of split ranges; both
+ * belong to the step (calls that overlap in time need steps of their own) and
+ * need no initialisation. */
+typedef struct mlora_paged_step {
+  int32_t* row_indptr;  /* [n + 1] */
+  int32_t* kv_lens;     /* [n] */
+  int32_t* positions;   /* [rows] */
+  int32_t* slots;       /* [rows]: page * page size + offset, -1: no place */
+  int32_t* plan;
+  void* workspace;
+  size_t plan_bytes;
+  size_t workspace_bytes;
+  int32_t rows;
+  int32_t max_new;
+} mlora_paged_step;
+
+/* Bytes of a step's plan and attention workspace, for n requests of up to
+ * max_kv = width * page positions; returns 0, or < 0 for an unsupported shape. */
+int mlora_paged_step_bytes(int32_t n, int32_t rows, int32_t max_new, int64_t max_kv, int32_t heads, int32_t kv_heads,
+                           int32_t head_dim, size_t* plan_bytes, size_t* workspace_bytes);
+
+/* int32 words of scratch that mlora_page_tables needs for n requests. */
+int32_t mlora_page_tables_scratch(int32_t n);
+
+/* Pages, slots and positions of a step in which request i keeps start_lens[i]
+ * cached positions and gets new_lens[i] tokens.  With need_i = pages for
+ * start + new positions (at most `width`), a request that holds more gives
+ * entries [need, held) back and one that holds fewer takes the rest.  Pages
+ * given back and pages taken are each counted in request and page order: the
+ * t-th page taken is the t-th one given back, or once there are none the
+ * stack's top.  Pages given back that nobody takes go on the stack, the last
+ * one first: a call that takes pages and a call that gives the same ones back
+ * restore it.  A page that the pool cannot give is -1 (later requests get
+ * none; held counts those given; asked for again by the next call).
+ * Writes row_indptr (prefix sums of new_lens, at most `rows`), kv_lens =
+ * start + new, positions and slots (0 and -1 for rows behind the last
+ * request's), and, if the step has a plan, the work list for `heads` query
+ * heads over `kv_heads` key heads of head_dim.  Table entries past the pages
+ * held are left as they were.  rows at most 2^20, num_pages * page and n *
+ * width below 2^31. */
+int mlora_page_tables(const mlora_pages* pages, const int32_t* start_lens, const int32_t* new_lens,
+                      const mlora_paged_step* step, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t* scratch,
+                      void* stream);
+
+/* Rotary on q [rows, heads * D] and k [rows, kv_heads * D] (x * cos + roll(x,
+ * D / 2) * sin, cos and sin [rows or 1, D] in the data type or fp32, row
+ * stride rot_row_stride, 0 to share one row; fp32 math, one rounding); q into
+ * q_out (may be q), k and v into their slots of the cache.  Rows whose slot
+ * lies outside the pool write only q_out.  Slots of one call must differ.
+ * bf16 or fp16, D 64 or 128 (else -2). */
+int mlora_rotary_paged_write(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
+                             int64_t v_row_stride, const void* cos, const void* sin, int64_t rot_row_stride,
+                             int32_t rot_dtype, const int32_t* slots, int32_t rows, int32_t heads, int32_t kv_heads,
+                             int32_t head_dim, void* keys, int64_t key_page_stride, void* values,
+                             int64_t value_page_stride, int32_t num_pages, int32_t page, void* q_out,
+                             int64_t q_out_row_stride, int32_t dtype, void* stream);
+
+/* Causal attention of a step's rows over their requests' pages:
+ *   out[row, h] = sum_l softmax_l(scale * q[row, h] . k[l, h / rep]) * v[l, h / rep]
+ * over the positions l <= the row's own; fp32 sums, P rounded to the data type
+ * for its product with V, one rounding of the result.  `step` is one that
+ * mlora_page_tables filled for these heads.  Rows behind the last request's
+ * are left as they were.  A row that would attend to a page outside the pool,
+ * or past the table, is NaN.  What lies in positions that a row does not
+ * attend to (NaN too) does not reach it.
+ * Requirements (else -2): bf16 or fp16; D 64 or 128; 16-byte aligned rows of
+ * q, out and pages. */
+int mlora_paged_attention(const void* q, int64_t q_row_stride, const void* keys, int64_t key_page_stride,
+                          const void* values, int64_t value_page_stride, const mlora_pages* pages,
+                          const mlora_paged_step* step, void* out, int64_t out_row_stride, int32_t heads,
+                          int32_t kv_heads, int32_t head_dim, float scale, int32_t dtype, void* stream);
+
+/* Verification of drafted tokens.  Request i has rows [row_indptr[i],
+ * row_indptr[i + 1]) of target [rows, vocab], one more than it has drafts
+ * (drafts past `most` are not looked at); tokens, draft and accept are
+ * [n, most], [n, most, vocab] and [n, most] (draft NULL: drafts that were
+ * certain).  Draft j is accepted while accept * draft[x] < target[x]; the
+ * token after the accepted ones is the lowest x with cum(x) > last[i] * total
+ * of max(target - draft, 0) at the first rejection, of the target's row after
+ * the last draft.  accepted[n]; out[n, most + 1] = accepted drafts, that
+ * token, then -1; all -1 and 0 for a request without rows.  Probabilities of
+ * `dtype` (fp32 too), products and sums in fp64; what is not positive counts
+ * as no mass, a residual without mass falls back to the target's row, and a
+ * row without mass gives -1.  workspace: mlora_verify_workspace_bytes. */
+size_t mlora_verify_workspace_bytes(int32_t n, int32_t vocab);
+int mlora_verify_drafts(const void* target, int64_t target_row_stride, int32_t rows, const void* draft,
+                        int64_t draft_stride0, int64_t draft_stride1, const int64_t* tokens, int64_t token_stride,
+                        const int32_t* row_indptr, const float* accept, int64_t accept_stride, const float* last,
+                        int32_t n, int32_t most, int32_t vocab, int32_t* accepted, int64_t* out, int32_t dtype,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

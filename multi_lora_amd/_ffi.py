@@ -44,6 +44,13 @@ EXPORTS = (
     "mlora_rmsnorm_apply_grouped",
     "mlora_decode_attention",
     "mlora_silu_mul",
+    "mlora_paged_step_bytes",
+    "mlora_page_tables_scratch",
+    "mlora_page_tables",
+    "mlora_rotary_paged_write",
+    "mlora_paged_attention",
+    "mlora_verify_workspace_bytes",
+    "mlora_verify_drafts",
 )
 
 # include/mlora_hip.h: MLORA_STATIC_SCRATCH_BYTES
@@ -121,6 +128,41 @@ class PoolKey(ctypes.Structure):
         ("out_dim", ctypes.c_int32),
     ]
 
+
+
+class Pages(ctypes.Structure):
+    """struct mlora_pages."""
+
+    _fields_ = [
+        ("table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("held", ctypes.c_void_p),
+        ("free", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("n", ctypes.c_int32),
+        ("width", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("page", ctypes.c_int32),
+    ]
+
+
+class PagedStep(ctypes.Structure):
+    """struct mlora_paged_step."""
+
+    _fields_ = [
+        ("row_indptr", ctypes.c_void_p),
+        ("kv_lens", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("plan", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("plan_bytes", ctypes.c_size_t),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("rows", ctypes.c_int32),
+        ("max_new", ctypes.c_int32),
+    ]
+
+
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None
 
@@ -174,6 +216,27 @@ _SIGNATURES = {
          _i32, _f32, _i32, _vp],
     ),
     "mlora_silu_mul": (ctypes.c_int, [_vp, _vp, _i64, _vp, _i32, _i32, _i32, _vp]),
+    "mlora_paged_step_bytes": (ctypes.c_int, [_i32, _i32, _i32, _i64, _i32, _i32, _i32, ctypes.POINTER(_sz),
+                                              ctypes.POINTER(_sz)]),
+    "mlora_page_tables_scratch": (_i32, [_i32]),
+    "mlora_page_tables": (ctypes.c_int, [ctypes.POINTER(Pages), _vp, _vp, ctypes.POINTER(PagedStep), _i32, _i32, _i32,
+                                         _vp, _vp]),
+    "mlora_rotary_paged_write": (
+        ctypes.c_int,
+        [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64,
+         _i32, _i32, _vp, _i64, _i32, _vp],
+    ),
+    "mlora_paged_attention": (
+        ctypes.c_int,
+        [_vp, _i64, _vp, _i64, _vp, _i64, ctypes.POINTER(Pages), ctypes.POINTER(PagedStep), _vp, _i64, _i32, _i32,
+         _i32, _f32, _i32, _vp],
+    ),
+    "mlora_verify_workspace_bytes": (_sz, [_i32, _i32]),
+    "mlora_verify_drafts": (
+        ctypes.c_int,
+        [_vp, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _sz,
+         _vp],
+    ),
     "mlora_build_plan": (ctypes.c_int, [ctypes.POINTER(SegMeta), _i32, _vp, _i32, _vp]),
     "mlora_rmsnorm_apply_grouped": (
         ctypes.c_int,

@@ -4,11 +4,13 @@
 // frees or synchronises.
 #include <algorithm>
 #include <cstdarg>
+#include <cstdint>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
 
 #include "kernels.h"
+#include "paged.h"
 
 namespace {
 
@@ -85,6 +87,39 @@ mlora::SliceView slice_view(const mlora_slice& s) {
   v.out_dim = s.out_dim;
   v.out_col = s.out_col;
   return v;
+}
+
+// Pages of a cache: sizes, and log2 of the page size.
+int check_pages(const mlora_pages* p, int* shift) {
+  if (p == nullptr) return fail(kBadArg, "pages are null");
+  if (p->n < 0 || p->width < 0 || p->num_pages < 0) return fail(kBadArg, "n %d, width %d, num_pages %d", p->n, p->width, p->num_pages);
+  if (p->page < 8 || p->page > 1024 || (p->page & (p->page - 1)) != 0)
+    return fail(kUnsupported, "pages of a power of two positions from 8 to 1024, got %d", p->page);
+  if (static_cast<int64_t>(p->num_pages) * p->page > INT32_MAX || static_cast<int64_t>(p->n) * std::max(p->width, 1) > INT32_MAX ||
+      p->n > (1 << 24))
+    return fail(kUnsupported, "num_pages * page and n * width must be below 2^31 (%d * %d, %d * %d)", p->num_pages, p->page, p->n, p->width);
+  if (p->n > 1 && p->table_stride < p->width) return fail(kBadArg, "table row stride %lld below width %d", (long long)p->table_stride, p->width);
+  *shift = __builtin_ctz(static_cast<unsigned>(p->page));
+  return 0;
+}
+
+int check_step(const mlora_paged_step* s) {
+  if (s == nullptr) return fail(kBadArg, "step is null");
+  if (s->rows < 0 || s->max_new < 0) return fail(kBadArg, "rows %d, max_new %d", s->rows, s->max_new);
+  if (s->rows > (1 << 20)) return fail(kUnsupported, "%d rows, a step takes 2^20", s->rows);
+  return 0;
+}
+
+bool paged_step_shape(int n, int rows, int max_new, int64_t max_kv, int heads, int kv_heads, int head_dim,
+                      mlora::PagedShape* s) {
+  if ((head_dim != 64 && head_dim != 128) || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads > 1024 ||
+      n < 0 || rows < 0 || rows > (1 << 20) || max_new < 0 || max_kv < 0 ||
+      !mlora::paged_shape(n, rows, max_new, max_kv, heads, kv_heads, head_dim, num_cus(), s)) {
+    fail(kUnsupported, "paged attention takes head_dim 64 or 128 (got %d) and heads a multiple of kv_heads (%d, %d); %d requests, %d rows",
+         head_dim, heads, kv_heads, n, rows);
+    return false;
+  }
+  return true;
 }
 
 // Bytes of the mid region at the start of a segment workspace (256-byte
@@ -747,6 +782,175 @@ int mlora_pool_scatter(const void* stage, int64_t stage_row_stride, int32_t h, c
   a.vec = al16(stage) && (stage_row_stride * eb) % 16 == 0;
   const hipError_t e = mlora::launch_scatter(a, max_numel, eb, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "pool scatter launch");
+  return 0;
+}
+
+int mlora_paged_step_bytes(int32_t n, int32_t rows, int32_t max_new, int64_t max_kv, int32_t heads, int32_t kv_heads,
+                           int32_t head_dim, size_t* plan_bytes, size_t* workspace_bytes) {
+  g_err[0] = '\0';
+  mlora::PagedShape s;
+  if (plan_bytes == nullptr || workspace_bytes == nullptr) return fail(kBadArg, "null pointer");
+  if (!paged_step_shape(n, rows, max_new, max_kv, heads, kv_heads, head_dim, &s)) return kUnsupported;
+  *plan_bytes = s.plan_bytes;
+  *workspace_bytes = s.ws_bytes;
+  return 0;
+}
+
+int32_t mlora_page_tables_scratch(int32_t n) { return n < 0 || n > (1 << 24) ? 0 : mlora::tables_scratch_words(n); }
+
+int mlora_page_tables(const mlora_pages* pages, const int32_t* start_lens, const int32_t* new_lens,
+                      const mlora_paged_step* step, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t* scratch,
+                      void* stream) {
+  g_err[0] = '\0';
+  int shift;
+  if (const int rc = check_pages(pages, &shift)) return rc;
+  if (const int rc = check_step(step)) return rc;
+  mlora::TablesArgs a{};
+  if (step->plan != nullptr) {
+    const int64_t max_kv = static_cast<int64_t>(pages->width) * pages->page;
+    if (!paged_step_shape(pages->n, step->rows, step->max_new, max_kv, heads, kv_heads, head_dim, &a.shape)) return kUnsupported;
+    if (step->plan_bytes < a.shape.plan_bytes)
+      return fail(kWorkspace, "plan of %zu bytes, needs %zu", step->plan_bytes, a.shape.plan_bytes);
+  }
+  if (pages->n == 0 && step->rows == 0 && step->plan == nullptr) return 0;
+  if (scratch == nullptr || step->row_indptr == nullptr || (step->rows > 0 && (!step->positions || !step->slots)) ||
+      (pages->n > 0 && (!pages->table || !pages->held || !start_lens || !new_lens || !step->kv_lens)) ||
+      pages->counts == nullptr || (pages->num_pages > 0 && pages->free == nullptr))
+    return fail(kBadArg, "null pointer");
+  a.table = pages->table, a.table_stride = pages->table_stride;
+  a.held = pages->held, a.free = pages->free, a.counts = pages->counts;
+  a.width = pages->width, a.num_pages = pages->num_pages, a.page_shift = shift;
+  a.n = pages->n;
+  a.start = start_lens, a.add = new_lens;
+  a.rows = step->rows;
+  a.row_indptr = step->row_indptr, a.kv_lens = step->kv_lens, a.positions = step->positions, a.slots = step->slots;
+  a.scratch = scratch;
+  a.plan = step->plan;
+  a.kv_heads = kv_heads;
+  const hipError_t e = mlora::launch_page_tables(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "page tables launch");
+  return 0;
+}
+
+int mlora_rotary_paged_write(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
+                             int64_t v_row_stride, const void* cos, const void* sin, int64_t rot_row_stride,
+                             int32_t rot_dtype, const int32_t* slots, int32_t rows, int32_t heads, int32_t kv_heads,
+                             int32_t head_dim, void* keys, int64_t key_page_stride, void* values,
+                             int64_t value_page_stride, int32_t num_pages, int32_t page, void* q_out,
+                             int64_t q_out_row_stride, int32_t dtype, void* stream) {
+  g_err[0] = '\0';
+  if (dtype != MLORA_BF16 && dtype != MLORA_F16) return fail(kUnsupported, "paged write needs bf16 or fp16, got dtype %d", dtype);
+  if (rot_dtype != dtype && rot_dtype != MLORA_F32) return fail(kUnsupported, "rotary tables of the data type or fp32, got dtype %d", rot_dtype);
+  if (head_dim != 64 && head_dim != 128) return fail(kUnsupported, "head_dim 64 or 128, got %d", head_dim);
+  mlora_pages p{};
+  p.num_pages = num_pages, p.page = page, p.width = 1;
+  int shift;
+  if (const int rc = check_pages(&p, &shift)) return rc;
+  if (rows < 0 || heads < 1 || kv_heads < 1) return fail(kBadArg, "rows %d, heads %d, kv_heads %d", rows, heads, kv_heads);
+  const int64_t qw = static_cast<int64_t>(heads) * head_dim, kw = static_cast<int64_t>(kv_heads) * head_dim;
+  if (q_row_stride < qw || k_row_stride < kw || v_row_stride < kw || q_out_row_stride < qw || rot_row_stride < 0 ||
+      key_page_stride < kw * page || value_page_stride < kw * page)
+    return fail(kBadArg, "strides do not hold the rows or pages");
+  if (rows == 0) return 0;
+  if (!q || !k || !v || !cos || !sin || !slots || !keys || !values || !q_out) return fail(kBadArg, "null pointer");
+  mlora::WriteArgs a{};
+  a.q = q, a.k = k, a.v = v;
+  a.q_stride = q_row_stride, a.k_stride = k_row_stride, a.v_stride = v_row_stride;
+  a.cos = cos, a.sin = sin, a.rot_stride = rot_row_stride, a.rot_f32 = rot_dtype == MLORA_F32;
+  a.slots = slots;
+  a.rows = rows, a.heads = heads, a.kv_heads = kv_heads;
+  a.keys = keys, a.values = values;
+  a.key_stride = key_page_stride, a.value_stride = value_page_stride;
+  a.num_pages = num_pages, a.page_shift = shift;
+  a.q_out = q_out, a.q_out_stride = q_out_row_stride;
+  const bool aligned = al16(q) && al16(k) && al16(v) && al16(keys) && al16(values) && al16(q_out) && al16(cos) && al16(sin) &&
+                       q_row_stride % 8 == 0 && k_row_stride % 8 == 0 && v_row_stride % 8 == 0 && q_out_row_stride % 8 == 0 &&
+                       rot_row_stride % 8 == 0 && key_page_stride % 8 == 0 && value_page_stride % 8 == 0;
+  const hipError_t e = mlora::launch_rotary_paged_write(a, dtype, head_dim, aligned, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "paged write launch");
+  return 0;
+}
+
+int mlora_paged_attention(const void* q, int64_t q_row_stride, const void* keys, int64_t key_page_stride,
+                          const void* values, int64_t value_page_stride, const mlora_pages* pages,
+                          const mlora_paged_step* step, void* out, int64_t out_row_stride, int32_t heads,
+                          int32_t kv_heads, int32_t head_dim, float scale, int32_t dtype, void* stream) {
+  g_err[0] = '\0';
+  if (dtype != MLORA_BF16 && dtype != MLORA_F16) return fail(kUnsupported, "paged attention needs bf16 or fp16, got dtype %d", dtype);
+  int shift;
+  if (const int rc = check_pages(pages, &shift)) return rc;
+  if (const int rc = check_step(step)) return rc;
+  mlora::PagedAttnArgs a{};
+  const int64_t max_kv = static_cast<int64_t>(pages->width) * pages->page;
+  if (!paged_step_shape(pages->n, step->rows, step->max_new, max_kv, heads, kv_heads, head_dim, &a.shape)) return kUnsupported;
+  const int64_t qw = static_cast<int64_t>(heads) * head_dim, pw = static_cast<int64_t>(kv_heads) * head_dim * pages->page;
+  if (q_row_stride < qw || out_row_stride < qw || key_page_stride < pw || value_page_stride < pw)
+    return fail(kBadArg, "strides do not hold the rows or pages");
+  if (pages->n == 0 || step->rows == 0 || pages->num_pages == 0 || pages->width == 0) {
+    if (pages->n > 0 && step->rows > 0) return fail(kBadArg, "attention over a cache without pages");
+    return 0;
+  }
+  if (!q || !keys || !values || !out || !pages->table || !step->row_indptr || !step->kv_lens || !step->plan)
+    return fail(kBadArg, "null pointer");
+  if (!al16(q) || !al16(keys) || !al16(values) || !al16(out) || q_row_stride % 8 != 0 || out_row_stride % 8 != 0 ||
+      key_page_stride % 8 != 0 || value_page_stride % 8 != 0)
+    return fail(kUnsupported, "paged attention needs 16-byte aligned rows and pages");
+  if (step->plan_bytes < a.shape.plan_bytes || step->workspace_bytes < a.shape.ws_bytes ||
+      (a.shape.ws_bytes > 0 && step->workspace == nullptr))
+    return fail(kWorkspace, "plan of %zu bytes and workspace of %zu, needs %zu and %zu", step->plan_bytes,
+                step->workspace_bytes, a.shape.plan_bytes, a.shape.ws_bytes);
+  a.q = q, a.q_stride = q_row_stride;
+  a.keys = keys, a.values = values;
+  a.key_stride = key_page_stride, a.value_stride = value_page_stride;
+  a.num_pages = pages->num_pages, a.page_shift = shift;
+  a.table = pages->table, a.table_stride = pages->table_stride, a.width = pages->width;
+  a.row_indptr = step->row_indptr, a.kv_lens = step->kv_lens;
+  a.n = pages->n, a.rows = step->rows;
+  a.plan = step->plan;
+  a.out = out, a.out_stride = out_row_stride;
+  a.part = static_cast<float*>(step->workspace);
+  a.ml = reinterpret_cast<float*>(static_cast<char*>(step->workspace) + a.shape.ml_off);
+  a.kv_heads = kv_heads, a.rep = heads / kv_heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  const hipError_t e = mlora::launch_paged_attention(a, dtype, head_dim, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "paged attention launch");
+  return 0;
+}
+
+size_t mlora_verify_workspace_bytes(int32_t n, int32_t vocab) {
+  if (n < 0 || vocab < 1) return 0;
+  const size_t chunks = (static_cast<size_t>(vocab) + mlora::kVerifyChunk - 1) / mlora::kVerifyChunk;
+  return static_cast<size_t>(n) * chunks * 2 * sizeof(double);
+}
+
+int mlora_verify_drafts(const void* target, int64_t target_row_stride, int32_t rows, const void* draft,
+                        int64_t draft_stride0, int64_t draft_stride1, const int64_t* tokens, int64_t token_stride,
+                        const int32_t* row_indptr, const float* accept, int64_t accept_stride, const float* last,
+                        int32_t n, int32_t most, int32_t vocab, int32_t* accepted, int64_t* out, int32_t dtype,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = '\0';
+  if (!valid_dtype(dtype)) return fail(kBadArg, "bad dtype %d", dtype);
+  if (n < 0 || most < 0 || rows < 0 || vocab < 1) return fail(kBadArg, "n %d, most %d, rows %d, vocab %d", n, most, rows, vocab);
+  if (target_row_stride < vocab || draft_stride0 < 0 || draft_stride1 < 0 || token_stride < 0 || accept_stride < 0)
+    return fail(kBadArg, "strides do not hold the rows");
+  if (vocab > (1 << 28)) return fail(kUnsupported, "vocab %d above 2^28", vocab);
+  if (n == 0) return 0;
+  if (!row_indptr || !last || !accepted || !out || (rows > 0 && !target) || (most > 0 && (!tokens || !accept)))
+    return fail(kBadArg, "null pointer");
+  const size_t need = mlora_verify_workspace_bytes(n, vocab);
+  if (workspace == nullptr || workspace_bytes < need) return fail(kWorkspace, "workspace of %zu bytes, needs %zu", workspace_bytes, need);
+  mlora::VerifyArgs a{};
+  a.target = target, a.target_stride = target_row_stride;
+  a.draft = draft, a.draft_stride0 = draft_stride0, a.draft_stride1 = draft_stride1;
+  a.tokens = tokens, a.token_stride = token_stride;
+  a.row_indptr = row_indptr;
+  a.accept = accept, a.accept_stride = accept_stride, a.last = last;
+  a.n = n, a.most = most, a.rows = rows, a.vocab = vocab;
+  a.chunks = (vocab + mlora::kVerifyChunk - 1) / mlora::kVerifyChunk;
+  a.sums = static_cast<double*>(workspace);
+  a.accepted = accepted, a.out = out;
+  const hipError_t e = mlora::launch_verify(a, dtype, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "verify launch");
   return 0;
 }
 

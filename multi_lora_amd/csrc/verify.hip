@@ -1,0 +1,252 @@
+// Verification of drafted tokens against the target's probabilities (gfx950).
+//
+// Request i has rows [row_indptr[i], row_indptr[i + 1]) of `target`, one more
+// than it has drafts x_0 .. x_{k-1}.  Draft j is accepted while
+// u_j * q_j(x_j) < p_j(x_j).  The token after the accepted ones is drawn from
+// max(p_j - q_j, 0) at the first rejection j (certain drafts: q is 1 at x_j,
+// 0 elsewhere), from p_k after k acceptances: the lowest x whose cumulated
+// mass exceeds w times the row's mass.  Products, sums and cumulated sums are
+// fp64, so a draw does not depend on how the row is cut.  Mass that is not
+// positive (NaN too) counts as none; a residual without mass falls back to
+// p_j, and a row without mass has no answer (-1).
+//
+// Two launches, for one row's sums are needed before its draw: a workgroup
+// per 4096 columns of a request's row, which finds the row itself, then a
+// workgroup per request that reads the one chunk its draw falls in.
+#include "kernels.h"
+#include "loads.h"
+#include "paged.h"
+
+namespace mlora {
+
+namespace {
+
+template <class T>
+__device__ __forceinline__ double mass(float f) {
+  return f > 0.f ? static_cast<double>(f) : 0.0;
+}
+
+struct Row {
+  int accepted;   // drafts accepted; the row drawn from is the accepted-th
+  bool rejected;  // a draft stands at that row
+  int64_t token;  // that draft
+  bool live;      // the request has rows in this call
+};
+
+// Every wave finds the row for itself, 64 drafts at a time.
+template <class T>
+__device__ Row find_row(const VerifyArgs& a, int i) {
+  using raw = typename T::raw_t;
+  const int first = min(max(a.row_indptr[i], 0), a.rows);
+  const int end = min(max(a.row_indptr[i + 1], first), a.rows);
+  const int k = min(end - first - 1, a.most);
+  Row r{0, false, -1, end > first};
+  const int lane = threadIdx.x & 63;
+  for (int j0 = 0; j0 < k; j0 += kWave) {
+    const int j = j0 + lane;
+    bool no = false;
+    int64_t x = -1;
+    if (j < k) {
+      x = a.tokens[i * a.token_stride + j];
+      no = true;
+      if (x >= 0 && x < a.vocab) {
+        const double p = T::to_f32(static_cast<const raw*>(a.target)[(first + j) * a.target_stride + x]);
+        const double q = a.draft == nullptr
+                             ? 1.0
+                             : static_cast<double>(T::to_f32(static_cast<const raw*>(
+                                   a.draft)[i * a.draft_stride0 + j * a.draft_stride1 + x]));
+        no = !(static_cast<double>(a.accept[i * a.accept_stride + j]) * q < p);
+      }
+    }
+    const uint64_t hit = __ballot(no);
+    if (hit != 0) {
+      const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+      r.accepted = j0 + l;
+      r.rejected = true;
+      r.token = __shfl(x, l, kWave);
+      return r;
+    }
+  }
+  r.accepted = max(k, 0);
+  return r;
+}
+
+// Mass of column x of the row drawn from: of the residual, and of p.
+template <class T>
+__device__ __forceinline__ void column(const VerifyArgs& a, const Row& r, const typename T::raw_t* p,
+                                       const typename T::raw_t* q, int x, double* rest, double* full) {
+  const float f = T::to_f32(p[x]);
+  *full = mass<T>(f);
+  if (!r.rejected) {
+    *rest = *full;
+  } else if (q != nullptr) {
+    const double less = static_cast<double>(f) - static_cast<double>(T::to_f32(q[x]));
+    *rest = less > 0.0 ? less : 0.0;
+  } else {
+    *rest = x == r.token ? 0.0 : *full;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void row_ptrs(const VerifyArgs& a, const Row& r, int i, const typename T::raw_t** p,
+                                         const typename T::raw_t** q) {
+  using raw = typename T::raw_t;
+  const int first = min(max(a.row_indptr[i], 0), a.rows);
+  *p = static_cast<const raw*>(a.target) + static_cast<int64_t>(first + r.accepted) * a.target_stride;
+  *q = r.rejected && a.draft != nullptr
+           ? static_cast<const raw*>(a.draft) + i * a.draft_stride0 + r.accepted * a.draft_stride1
+           : nullptr;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void verify_sum_kernel(VerifyArgs a) {
+  using raw = typename T::raw_t;
+  const int i = blockIdx.x / a.chunks;
+  const int c = blockIdx.x - i * a.chunks;
+  const Row r = find_row<T>(a, i);
+  if (!r.live) return;
+  const raw *p, *q;
+  row_ptrs<T>(a, r, i, &p, &q);
+  double rest = 0.0, full = 0.0;
+  const int end = min((c + 1) * kVerifyChunk, a.vocab);
+  for (int x = c * kVerifyChunk + threadIdx.x; x < end; x += 256) {
+    double m, f;
+    column<T>(a, r, p, q, x, &m, &f);
+    rest += m;
+    full += f;
+  }
+  for (int off = 1; off < kWave; off <<= 1) {
+    rest += __shfl_xor(rest, off, kWave);
+    full += __shfl_xor(full, off, kWave);
+  }
+  __shared__ double part[4][2];
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    part[wave][0] = rest;
+    part[wave][1] = full;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2)
+    a.sums[static_cast<int64_t>(blockIdx.x) * 2 + threadIdx.x] =
+        part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
+  using raw = typename T::raw_t;
+  constexpr int PT = kVerifyChunk / 256;  // columns a thread
+  const int i = blockIdx.x;
+  const int tid = threadIdx.x;
+  const Row r = find_row<T>(a, i);
+  int64_t* out = a.out + static_cast<int64_t>(i) * (a.most + 1);
+  for (int j = tid; j <= a.most; j += 256)
+    if (j != r.accepted || !r.live) out[j] = r.live && j < r.accepted ? a.tokens[i * a.token_stride + j] : -1;
+  if (tid == 0) a.accepted[i] = r.accepted;
+  if (!r.live) return;
+  const double* sums = a.sums + static_cast<int64_t>(i) * a.chunks * 2;
+  __shared__ double before_s, total_s;
+  __shared__ int chunk_s, full_s, found_s;
+  if (tid == 0) {
+    // Chunks of a row are few (32 for 128 k columns): one thread adds them up.
+    double rest = 0.0, full = 0.0;
+    for (int c = 0; c < a.chunks; ++c) {
+      rest += sums[c * 2];
+      full += sums[c * 2 + 1];
+    }
+    const int use = rest > 0.0 ? 0 : 1;
+    const double total = use == 0 ? rest : full;
+    const double want = static_cast<double>(a.last[i]) * total;
+    double cum = 0.0, before = 0.0;
+    int at = -1, last = -1;
+    for (int c = 0; c < a.chunks; ++c) {
+      const double m = sums[c * 2 + use];
+      if (m > 0.0) last = c;
+      if (m > 0.0 && cum + m > want) {
+        at = c;
+        before = cum;
+        break;
+      }
+      cum += m;
+    }
+    if (at < 0 && last >= 0) {  // a number of 1 or more: the last column with mass
+      at = last;
+      before = -INFINITY;
+    }
+    before_s = before;
+    total_s = want;
+    chunk_s = at;
+    full_s = use;
+    found_s = INT32_MAX;
+  }
+  __syncthreads();
+  if (chunk_s < 0) {
+    if (tid == 0) out[r.accepted] = -1;
+    return;
+  }
+  const raw *p, *q;
+  row_ptrs<T>(a, r, i, &p, &q);
+  const int x0 = chunk_s * kVerifyChunk + tid * PT;
+  double m[PT], mine = 0.0;
+  int last = -1;
+#pragma unroll
+  for (int e = 0; e < PT; ++e) {
+    m[e] = 0.0;
+    if (x0 + e < a.vocab) {
+      double rest, full;
+      column<T>(a, r, p, q, x0 + e, &rest, &full);
+      m[e] = full_s ? full : rest;
+    }
+    if (m[e] > 0.0) last = x0 + e;
+    mine += m[e];
+  }
+  // Mass of the threads before this one.
+  double incl = mine;
+  const int lane = tid & 63, wave = tid >> 6;
+  for (int off = 1; off < kWave; off <<= 1) {
+    const double y = __shfl_up(incl, off, kWave);
+    if (lane >= off) incl += y;
+  }
+  __shared__ double waves[4];
+  __shared__ int last_s[4];
+  for (int off = 1; off < kWave; off <<= 1) last = max(last, __shfl_xor(last, off, kWave));
+  if (lane == kWave - 1) {
+    waves[wave] = incl;
+    last_s[wave] = last;
+  }
+  __syncthreads();
+  double cum = before_s;
+  for (int v = 0; v < wave; ++v) cum += waves[v];
+  cum += incl - mine;
+#pragma unroll
+  for (int e = 0; e < PT; ++e) {
+    cum += m[e];
+    if (m[e] > 0.0 && cum > total_s) {
+      atomicMin(&found_s, x0 + e);
+      break;
+    }
+  }
+  __syncthreads();
+  if (tid == 0)
+    out[r.accepted] = found_s != INT32_MAX ? found_s : max(max(last_s[0], last_s[1]), max(last_s[2], last_s[3]));
+}
+
+template <class T>
+hipError_t launch(const VerifyArgs& a, hipStream_t stream) {
+  const int64_t blocks = static_cast<int64_t>(a.n) * a.chunks;
+  if (!grid_fits(blocks)) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL((verify_sum_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((verify_draw_kernel<T>), dim3(static_cast<unsigned>(a.n)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_verify(const VerifyArgs& a, int dtype, hipStream_t stream) {
+  if (a.n == 0) return hipSuccess;
+  if (dtype == MLORA_F32) return launch<F32>(a, stream);
+  return dtype == MLORA_BF16 ? launch<BF16>(a, stream) : launch<F16>(a, stream);
+}
+
+}  // namespace mlora

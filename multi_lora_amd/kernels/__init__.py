@@ -7,6 +7,7 @@ from .lora_ops import (
     sgemm_lora_b_fwd,
     sgemm_lora_b_multi_fwd,
 )
+from .paged import PagedStep, PageState, page_tables, paged_attention, rotary_paged_write, verify_drafts
 from .rmsnorm import fuse_rmsnorm, fused_add_rmsnorm, rmsnorm_fwd
 from .scatter_bank import scatter_stage
 
@@ -20,4 +21,10 @@ __all__ = [
     "rmsnorm_fwd",
     "fuse_rmsnorm",
     "fused_add_rmsnorm",
+    "PageState",
+    "PagedStep",
+    "page_tables",
+    "rotary_paged_write",
+    "paged_attention",
+    "verify_drafts",
 ]
