@@ -908,8 +908,7 @@ int mlora_paged_attention(const void* q, int64_t q_row_stride, const void* keys,
   a.n = pages->n, a.rows = step->rows;
   a.plan = step->plan;
   a.out = out, a.out_stride = out_row_stride;
-  a.part = static_cast<float*>(step->workspace);
-  a.ml = reinterpret_cast<float*>(static_cast<char*>(step->workspace) + a.shape.ml_off);
+  a.workspace = static_cast<char*>(step->workspace);
   a.kv_heads = kv_heads, a.rep = heads / kv_heads;
   a.scale_log2 = scale * 1.4426950408889634f;
   const hipError_t e = mlora::launch_paged_attention(a, dtype, head_dim, static_cast<hipStream_t>(stream));

@@ -20,6 +20,7 @@
 namespace mlora {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -47,6 +48,13 @@ struct BF16 {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
   }
+  // One K-step (16) of a 32x32 tile: lane l holds row / column l & 31 and the
+  // chunk k = 8 * (l >> 5); the result's register r is row 8 * (r >> 2) +
+  // 4 * (l >> 5) + (r & 3) of column l & 31.
+  __device__ static __forceinline__ f32x16 mma32(f32x16 acc, u32x4 a, u32x4 b) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  }
 };
 
 struct F16 {
@@ -64,6 +72,10 @@ struct F16 {
   }
   __device__ static __forceinline__ f32x4 mma(f32x4 acc, u32x4 a, u32x4 b) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+  }
+  __device__ static __forceinline__ f32x16 mma32(f32x16 acc, u32x4 a, u32x4 b) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
   }
 };

@@ -12,29 +12,35 @@ namespace mlora {
 // tables.  One item is a tile of query rows over a range of positions; every
 // key head runs the same items.  Query rows are (token, query head of the key
 // head) pairs, token-major: row m of a request is token m / rep, head m % rep.
+// Requests of few rows are short: their tiles are streamed by a workgroup
+// whose waves share the range.  The others are long: tiles of kApLongRows rows
+// whose waves share the rows.
 constexpr int kApHeaderWords = 16;
-constexpr int kApItems = 0;      // items
-constexpr int kApJoins = 1;      // tiles whose range is split
+constexpr int kApShort = 0;      // items; joins (tiles whose range is split) in the next word
+constexpr int kApLong = 2;       // the same
 constexpr int kApItemWords = 8;  // request, first row, first position, end, slot (-1: none)
 constexpr int kApJoinWords = 4;  // request, first row, first slot, slots
 
-// Rows a tile of the streaming kernel holds.
-constexpr int kApShortRows = 16;
+constexpr int kApLongRows = 128;
 // A range is split only into parts of at least this many positions.
 constexpr int kApMinSplit = 256;
 // Tiles that fill the chip this many times over are not split.
 constexpr int kApWhole = 4;
 
+// One kind of item: how many the plan and the workspace have room for, and
+// where they are.
+struct PagedKind {
+  int bm;            // query rows a tile
+  int item_cap, join_cap, slot_cap;
+  size_t items_off, joins_off;  // words of the plan
+  size_t part_off, ml_off;      // bytes of the workspace
+};
 struct PagedShape {
   int rep;
-  int bm;          // query rows a tile
-  int target;      // parts (of all key heads) that fill the chip
-  int item_cap;    // items and joins the plan has room for
-  int join_cap;
-  int slot_cap;    // partial results the workspace has room for
+  int target;        // parts (of all key heads) that fill the chip
   bool can_split;
-  size_t items_off, joins_off, plan_bytes;  // words, words, bytes
-  size_t ml_off, ws_bytes;                  // bytes
+  PagedKind kind[2]; // short, long (no caps: none can occur)
+  size_t plan_bytes, ws_bytes;
 };
 // Host bounds only: rows of the step, requests, new tokens of one request,
 // longest cache.  False: unsupported.
@@ -56,7 +62,7 @@ struct TablesArgs {
   PagedShape shape;
   int kv_heads;
 };
-constexpr int tables_scratch_words(int n) { return 16 + 3 * n; }
+constexpr int tables_scratch_words(int n) { return 16 + 7 * n; }
 hipError_t launch_page_tables(const TablesArgs& a, hipStream_t stream);
 
 struct WriteArgs {
@@ -89,8 +95,9 @@ struct PagedAttnArgs {
   const int32_t* plan;
   void* out;
   int64_t out_stride;
-  float* part;       // [slot][kv_heads][bm][D] sums
-  float* ml;         // [slot][kv_heads][bm][2] maximum (log2), sum
+  // Of each kind at its offsets: sums [slot][kv_heads][bm][D], and the
+  // maximum (log2) and sum of weights [slot][kv_heads][bm][2].
+  char* workspace;
   int kv_heads, rep;
   float scale_log2;  // scale * log2(e)
   PagedShape shape;

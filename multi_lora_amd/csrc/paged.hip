@@ -13,9 +13,10 @@ namespace {
 constexpr int kScanThreads = 1024;
 constexpr int kScanWaves = kScanThreads / kWave;
 
-// Scratch words: [0] pages on the stack before the call, [1] pages given
-// back, [2] pages wanted, then per request its first freed and first taken
-// page (exclusive prefix sums) and the pages it held.
+// Scratch words: pages on the stack before the call, pages given back, pages
+// wanted, the lengths at which ranges split; then per request its first freed
+// and first taken page (exclusive prefix sums), the pages it held, and of the
+// work list its first item, slot and join and its parts a tile.
 constexpr int kTsTop = 0;
 constexpr int kTsFreed = 1;
 constexpr int kTsTaken = 2;
@@ -51,151 +52,181 @@ __device__ int take_page(const TablesArgs& a, int t, int top, int freed) {
   return a.table[static_cast<int64_t>(lo) * a.table_stride + pages_for(l.x + l.y, a) + (t - freed0[lo])];
 }
 
-// Exclusive sum over the workgroup of a value that fits 31 bits.
-__device__ __forceinline__ int scan(int v, int* tmp, int* total) { return block_exclusive_scan<kScanWaves>(v, tmp, total); }
+// Exclusive sums over the workgroup of N values that fit 31 bits, and their
+// totals; the values share the two barriers.
+template <int N>
+__device__ __forceinline__ void scan(int (&v)[N], int (&total)[N], int (*tmp)[kScanWaves]) {
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  int x[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) x[k] = wave_incl_sum(v[k]);
+  if (lane == kWave - 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) tmp[k][wave] = x[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kScanWaves; ++w) {
+      const int t = tmp[k][w];
+      before += w < wave ? t : 0;
+      all += t;
+    }
+    v[k] = before + x[k] - v[k];
+    total[k] = all;
+  }
+  __syncthreads();
+}
 
-// Prefix sums of rows and pages; one workgroup.
-__device__ void scan_requests(const TablesArgs& a, int* tmp) {
+// Tiles of a request's c new tokens, and which kind they are.
+__device__ __forceinline__ int kind_of(const PagedShape& s, int c) {
+  return static_cast<int64_t>(c) * s.rep > s.kind[0].bm ? 1 : 0;
+}
+__device__ __forceinline__ int tiles_of(const PagedShape& s, int c, int kind) {
+  const int bm = s.kind[kind].bm;
+  return static_cast<int>((static_cast<int64_t>(c) * s.rep + bm - 1) / bm);
+}
+__device__ __forceinline__ int table_room(const TablesArgs& a) {
+  return static_cast<int>(min(static_cast<int64_t>(a.width) << a.page_shift, static_cast<int64_t>(1 << 30)));
+}
+
+// Prefix sums of rows, pages and items; one workgroup.
+__global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a) {
+  __shared__ int tmp[4][kScanWaves];
+  __shared__ unsigned long long wide[4];
   int32_t* freed0 = a.scratch + kTsArrays;
   int32_t* taken0 = freed0 + a.n;
   int32_t* held0 = taken0 + a.n;
+  int32_t* item0 = held0 + a.n;
+  int32_t* slot0 = item0 + a.n;
+  int32_t* join0 = slot0 + a.n;
+  int32_t* parts0 = join0 + a.n;
+  const PagedShape& s = a.shape;
+  const bool plan = a.plan != nullptr;
+  const int room = table_room(a);
+  if (threadIdx.x < 4) wide[threadIdx.x] = 0;
   int rows = 0, freed = 0, taken = 0;
+  unsigned long long work[2] = {0, 0}, count[2] = {0, 0};
   for (int i0 = 0; i0 < a.n; i0 += kScanThreads) {
     const int i = i0 + threadIdx.x;
-    int c = 0, f = 0, t = 0;
+    int v[3] = {0, 0, 0}, total[3];
+    int len = 0;
     if (i < a.n) {
       const int2 l = lens_of(a, i);
-      c = l.y;
-      const int need = pages_for(l.x + l.y, a);
+      len = l.x + l.y;
+      const int need = pages_for(len, a);
       const int held = min(max(a.held[i], 0), a.width);
-      f = max(held - need, 0);
-      t = max(need - held, 0);
-      a.kv_lens[i] = l.x + l.y;
+      v[0] = min(l.y, a.rows);
+      v[1] = max(held - need, 0);
+      v[2] = max(need - held, 0);
+      a.kv_lens[i] = len;
       held0[i] = held;
     }
-    int total;
-    // Rows saturate at the call's rows: later requests then get none.
-    const int r0 = scan(min(c, a.rows), tmp, &total);
-    if (i < a.n) a.row_indptr[i] = min(rows + r0, a.rows);
-    rows = min(rows + total, a.rows);
-    const int f0 = scan(f, tmp, &total);
-    if (i < a.n) freed0[i] = freed + f0;
-    freed += total;
-    const int t0 = scan(t, tmp, &total);
-    if (i < a.n) taken0[i] = taken + t0;
-    taken += total;
+    const int c = v[0];
+    scan(v, total, tmp);
+    if (i < a.n) {
+      // Rows saturate at the call's rows: later requests then get none.
+      const int first = min(rows + v[0], a.rows);
+      a.row_indptr[i] = first;
+      freed0[i] = freed + v[1];
+      taken0[i] = taken + v[2];
+      if (plan) {
+        const int mine = min(c, a.rows - first);
+        const int kind = kind_of(s, mine);
+        const unsigned long long tiles = tiles_of(s, mine, kind);
+        len = min(len, room);
+        const unsigned long long w = tiles * (len - min(mine, len) / 2);
+        work[kind] += w;
+        count[kind] += tiles;
+      }
+    }
+    rows = min(rows + total[0], a.rows);
+    freed += total[1];
+    taken += total[2];
   }
   const int top = min(max(a.counts[0], 0), a.num_pages);
-  __syncthreads();  // every thread has read counts
-  const int have = top + freed;
-  for (int i = threadIdx.x; i < a.n; i += kScanThreads) {
-    const int2 l = lens_of(a, i);
-    const int need = pages_for(l.x + l.y, a);
-    const int held = held0[i];
-    a.held[i] = need > held ? held + min(need - held, max(have - taken0[i], 0)) : need;
+  if (plan) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      for (int off = 1; off < kWave; off <<= 1) {
+        work[k] += __shfl_xor(work[k], off, kWave);
+        count[k] += __shfl_xor(count[k], off, kWave);
+      }
+      if ((threadIdx.x & 63) == 0 && count[k] != 0) {
+        atomicAdd(&wide[k], work[k]);
+        atomicAdd(&wide[2 + k], count[k]);
+      }
+    }
   }
+  __syncthreads();  // every thread has read counts, and written what others read below
   if (threadIdx.x == 0) {
     a.row_indptr[a.n] = rows;
     a.scratch[kTsTop] = top;
     a.scratch[kTsFreed] = freed;
     a.scratch[kTsTaken] = taken;
-    a.counts[0] = max(have - taken, 0);
-    a.counts[1] = max(taken - have, 0);
+    a.counts[0] = max(top + freed - taken, 0);
+    a.counts[1] = max(taken - top - freed, 0);
   }
-}
-
-// Work list of the step's attention; one workgroup, after scan_requests.
-__device__ void build_items(const TablesArgs& a, int* tmp, unsigned long long* wide) {
-  const PagedShape& s = a.shape;
-  const int room = static_cast<int>(min(static_cast<int64_t>(a.width) << a.page_shift, static_cast<int64_t>(INT32_MAX)));
-  if (threadIdx.x < 2) wide[threadIdx.x] = 0;
-  __syncthreads();
-  unsigned long long work = 0, count = 0;
-  for (int i = threadIdx.x; i < a.n; i += kScanThreads) {
-    const int c = a.row_indptr[i + 1] - a.row_indptr[i];
-    const unsigned long long tiles = (static_cast<unsigned long long>(c) * s.rep + s.bm - 1) / s.bm;
-    const int len = min(a.kv_lens[i], room);
-    work += tiles * (len - min(c, len) / 2);
-    count += tiles;
-  }
-  for (int off = 1; off < kWave; off <<= 1) {
-    work += __shfl_xor(work, off, kWave);
-    count += __shfl_xor(count, off, kWave);
-  }
-  if ((threadIdx.x & 63) == 0) {
-    atomicAdd(&wide[0], work);
-    atomicAdd(&wide[1], count);
-  }
-  __syncthreads();
   // Parts of equal length, so that all of them together fill the chip once;
   // tiles that fill it several times over stay whole.
-  const unsigned long long part = (wide[0] * a.kv_heads + s.target - 1) / s.target;
-  const bool whole = !s.can_split || wide[1] * a.kv_heads >= static_cast<unsigned long long>(kApWhole) * s.target;
-  const int split = whole ? INT32_MAX
-                          : static_cast<int>(min((max(part, static_cast<unsigned long long>(kApMinSplit)) + 63) / 64 * 64, 1ull << 30));
-  int32_t* items = a.plan + s.items_off;
-  int32_t* joins = a.plan + s.joins_off;
-  int item0 = 0, slot0 = 0, join0 = 0;
+  int split[2] = {INT32_MAX, INT32_MAX};
+  if (plan && s.can_split) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const unsigned long long part = (wide[k] * a.kv_heads + s.target - 1) / s.target;
+      if (wide[2 + k] * a.kv_heads < static_cast<unsigned long long>(kApWhole) * s.target)
+        split[k] = static_cast<int>((min(max(part, static_cast<unsigned long long>(kApMinSplit)), 1ull << 30) + 63) / 64 * 64);
+    }
+  }
+  const int have = top + freed;
+  int base[2][3] = {{0, 0, 0}, {0, 0, 0}};  // items, slots, joins so far of each kind
   for (int i0 = 0; i0 < a.n; i0 += kScanThreads) {
     const int i = i0 + threadIdx.x;
-    int c = 0, len = 0, tiles = 0, parts = 1;
+    int c = 0, len = 0;
     if (i < a.n) {
-      c = a.row_indptr[i + 1] - a.row_indptr[i];
-      len = min(a.kv_lens[i], room);
-      tiles = static_cast<int>((static_cast<int64_t>(c) * s.rep + s.bm - 1) / s.bm);
-      if (len > split) parts = (len + split - 1) / split;
+      const int2 l = lens_of(a, i);
+      const int need = pages_for(l.x + l.y, a);
+      const int held = held0[i];
+      a.held[i] = need > held ? held + min(need - held, max(have - taken0[i], 0)) : need;
+      const int first = a.row_indptr[i];
+      c = min(l.y, a.rows - first);
+      len = min(l.x + l.y, room);
     }
-    int n_items, n_slots, n_joins;
-    int it = item0 + scan(tiles * parts, tmp, &n_items);
-    int sl = slot0 + scan(parts > 1 ? tiles * parts : 0, tmp, &n_slots);
-    int jn = join0 + scan(parts > 1 ? tiles : 0, tmp, &n_joins);
-    for (int k = tiles - 1; k >= 0; --k) {  // the longest ranges first
-      const int last = min((k + 1) * s.bm, c * s.rep) - 1;
-      // Positions the tile's last row sees.
-      const int end = i < a.n ? min(a.kv_lens[i] - c + last / s.rep + 1, room) : 0;
-      const int step = parts > 1 ? ((end + parts - 1) / parts + 63) / 64 * 64 : end;
-      const bool fits = it + parts <= s.item_cap && (parts == 1 || (sl + parts <= s.slot_cap && jn < s.join_cap));
-      if (!fits) continue;  // the host's bounds rule it out
-      if (parts > 1) {
-        int32_t* j = joins + static_cast<int64_t>(jn++) * kApJoinWords;
-        j[0] = i;
-        j[1] = k * s.bm;
-        j[2] = sl;
-        j[3] = parts;
-      }
-      for (int p = 0; p < parts; ++p, ++it) {
-        int32_t* w = items + static_cast<int64_t>(it) * kApItemWords;
-        w[0] = i;
-        w[1] = k * s.bm;
-        w[2] = min(p * step, end);
-        w[3] = p + 1 == parts ? end : min((p + 1) * step, end);
-        w[4] = parts > 1 ? sl++ : -1;
-      }
+    if (!plan) continue;
+    const int kind = kind_of(s, c);
+    const int tiles = tiles_of(s, c, kind);
+    const int at = kind ? split[1] : split[0];
+    const int parts = len > at ? (len + at - 1) / at : 1;
+    const int items = tiles * parts;
+    int v[3] = {kind ? 0 : items, kind ? 0 : (parts > 1 ? items : 0), kind ? 0 : (parts > 1 ? tiles : 0)}, t[3];
+    int u[3] = {kind ? items : 0, kind && parts > 1 ? items : 0, kind && parts > 1 ? tiles : 0}, tu[3];
+    scan(v, t, tmp);
+    scan(u, tu, tmp);
+    if (i < a.n) {
+      item0[i] = kind ? base[1][0] + u[0] : base[0][0] + v[0];
+      slot0[i] = kind ? base[1][1] + u[1] : base[0][1] + v[1];
+      join0[i] = kind ? base[1][2] + u[2] : base[0][2] + v[2];
+      parts0[i] = parts;
     }
-    item0 += n_items;
-    slot0 += n_slots;
-    join0 += n_joins;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      base[0][k] += t[k];
+      base[1][k] += tu[k];
+    }
   }
-  if (threadIdx.x == 0) {
-    a.plan[kApItems] = min(item0, s.item_cap);
-    a.plan[kApJoins] = min(join0, s.join_cap);
-  }
-}
-
-__global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a) {
-  __shared__ int tmp[kScanWaves];
-  __shared__ unsigned long long wide[2];
-  scan_requests(a, tmp);
-  if (a.plan != nullptr) {
-    __syncthreads();
-    build_items(a, tmp, wide);
+  if (plan && threadIdx.x < 2) {
+    const int k = threadIdx.x;
+    a.plan[(k ? kApLong : kApShort)] = min(k ? base[1][0] : base[0][0], s.kind[k].item_cap);
+    a.plan[(k ? kApLong : kApShort) + 1] = min(k ? base[1][2] : base[0][2], s.kind[k].join_cap);
   }
 }
 
 // Blocks [0, row_blocks): positions and slots of 256 rows each; the rest:
-// four requests each, one a wave, their pages.  Nothing that one block
-// writes is read by another: a freeing request's entries and the stack below
-// the pages taken are only read, a taking request's new entries and the
+// four requests each, one a wave, their pages and items.  Nothing that one
+// block writes is read by another: a freeing request's entries and the stack
+// below the pages taken are only read, a taking request's new entries and the
 // stack above the pages left only written.
 __global__ __launch_bounds__(256) void tables_fill_kernel(TablesArgs a, int row_blocks) {
   const int32_t* freed0 = a.scratch + kTsArrays;
@@ -227,15 +258,53 @@ __global__ __launch_bounds__(256) void tables_fill_kernel(TablesArgs a, int row_
   }
   const int i = (blockIdx.x - row_blocks) * 4 + (threadIdx.x >> 6);
   if (i >= a.n) return;
+  const int lane = threadIdx.x & 63;
   const int2 l = lens_of(a, i);
   const int need = pages_for(l.x + l.y, a);
   const int held = held0[i];
   int32_t* row = a.table + static_cast<int64_t>(i) * a.table_stride;
-  for (int j = held + (threadIdx.x & 63); j < need; j += kWave) row[j] = take_page(a, taken0[i] + (j - held), top, freed);
-  for (int j = need + (threadIdx.x & 63); j < held; j += kWave) {
+  for (int j = held + lane; j < need; j += kWave) row[j] = take_page(a, taken0[i] + (j - held), top, freed);
+  for (int j = need + lane; j < held; j += kWave) {
     const int f = freed0[i] + (j - need);
     const int to = top + freed - 1 - f;
     if (f >= taken && to < a.num_pages) a.free[to] = row[j];
+  }
+  if (a.plan == nullptr) return;
+  // The request's tiles, those of the longest ranges first.
+  const PagedShape& s = a.shape;
+  const int32_t* item0 = held0 + a.n;
+  const int c = a.row_indptr[i + 1] - a.row_indptr[i];
+  const int len = l.x + l.y;
+  const int kind = kind_of(s, c);
+  const PagedKind kd = kind ? s.kind[1] : s.kind[0];
+  const int tiles = tiles_of(s, c, kind);
+  const int first_item = item0[i], first_slot = item0[a.n + i], first_join = item0[2 * a.n + i], parts = item0[3 * a.n + i];
+  const int room = table_room(a);
+  for (int t = lane; t < tiles; t += kWave) {
+    const int row0 = (tiles - 1 - t) * kd.bm;
+    const int last = min(row0 + kd.bm, c * s.rep) - 1;
+    const int end = min(len - c + last / s.rep + 1, room);  // positions the tile's last row sees
+    const int step = ((end + parts - 1) / parts + 63) / 64 * 64;
+    const int it = first_item + t * parts;
+    const int sl = first_slot + t * parts;
+    const int jn = first_join + t;
+    // The host's bounds leave room for all of them.
+    if (it + parts > kd.item_cap || (parts > 1 && (sl + parts > kd.slot_cap || jn >= kd.join_cap))) continue;
+    for (int p = 0; p < parts; ++p) {
+      int32_t* w = a.plan + kd.items_off + static_cast<int64_t>(it + p) * kApItemWords;
+      w[0] = i;
+      w[1] = row0;
+      w[2] = min(p * step, end);
+      w[3] = p + 1 == parts ? end : min((p + 1) * step, end);
+      w[4] = parts > 1 ? sl + p : -1;
+    }
+    if (parts > 1) {
+      int32_t* j = a.plan + kd.joins_off + static_cast<int64_t>(jn) * kApJoinWords;
+      j[0] = i;
+      j[1] = row0;
+      j[2] = sl;
+      j[3] = parts;
+    }
   }
 }
 
@@ -331,24 +400,39 @@ bool paged_shape(int n, int rows, int max_new, int64_t max_kv, int heads, int kv
   *s = PagedShape{};
   if (n < 0 || rows < 0 || max_new < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0) return false;
   s->rep = heads / kv_heads;
-  s->bm = kApShortRows;
   s->target = 2 * cus;
   s->can_split = max_kv > kApMinSplit;
-  const int64_t tiles = static_cast<int64_t>(rows) * s->rep / s->bm + std::min(n, rows);
-  // Parts of a tile: at most its length / split + 1, and the lengths of all
-  // tiles sum to at most twice the plan's estimate (len - new / 2).
-  const int64_t extra = s->can_split ? 2 * (s->target / kv_heads + 1) : 0;
-  const int64_t items = tiles + extra;
-  const int64_t slots = s->can_split ? std::min(tiles, kApWhole * static_cast<int64_t>(s->target) / kv_heads + 1) + extra : 0;
-  s->item_cap = static_cast<int>(std::min<int64_t>(items, INT32_MAX / 64));
-  s->join_cap = static_cast<int>(std::min<int64_t>(tiles, slots / 2));
-  if (s->item_cap < items) return false;
-  s->slot_cap = static_cast<int>(slots);
-  s->items_off = kApHeaderWords;
-  s->joins_off = s->items_off + static_cast<size_t>(s->item_cap) * kApItemWords;
-  s->plan_bytes = 4 * (s->joins_off + static_cast<size_t>(s->join_cap) * kApJoinWords);
-  s->ml_off = static_cast<size_t>(s->slot_cap) * kv_heads * s->bm * head_dim * 4;
-  s->ws_bytes = s->ml_off + static_cast<size_t>(s->slot_cap) * kv_heads * s->bm * 2 * 4;
+  const int64_t most = static_cast<int64_t>(std::min(max_new, rows)) * s->rep;  // rows of one request
+  const int64_t all = static_cast<int64_t>(rows) * s->rep;
+  s->kind[0].bm = most <= 16 ? 16 : 32;
+  s->kind[1].bm = kApLongRows;
+  size_t words = kApHeaderWords, bytes = 0;
+  for (int k = 0; k < 2; ++k) {
+    PagedKind& kd = s->kind[k];
+    const bool occurs = k == 0 ? n > 0 && rows > 0 : most > s->kind[0].bm;
+    // A short request has one tile, a long one more than short rows.
+    const int64_t tiles = !occurs ? 0
+                          : k == 0 ? std::min(n, rows)
+                                   : all / kd.bm + std::min<int64_t>(n, all / (s->kind[0].bm + 1));
+    // Parts of a tile: at most its length / split + 1, and the lengths of all
+    // tiles sum to at most twice the plan's estimate (len - new / 2).
+    const int64_t extra = occurs && s->can_split ? 2 * (s->target / kv_heads + 1) : 0;
+    const int64_t slots = extra > 0 ? std::min(tiles, static_cast<int64_t>(kApWhole) * s->target / kv_heads + 1) + extra : 0;
+    if (tiles + extra > INT32_MAX / 64) return false;
+    kd.item_cap = static_cast<int>(tiles + extra);
+    kd.slot_cap = static_cast<int>(slots);
+    kd.join_cap = static_cast<int>(std::min(tiles, slots / 2));
+    kd.items_off = words;
+    words += static_cast<size_t>(kd.item_cap) * kApItemWords;
+    kd.joins_off = words;
+    words += static_cast<size_t>(kd.join_cap) * kApJoinWords;
+    kd.part_off = bytes;
+    bytes += static_cast<size_t>(kd.slot_cap) * kv_heads * kd.bm * head_dim * 4;
+    kd.ml_off = bytes;
+    bytes += static_cast<size_t>(kd.slot_cap) * kv_heads * kd.bm * 2 * 4;
+  }
+  s->plan_bytes = 4 * words;
+  s->ws_bytes = bytes;
   return true;
 }
 

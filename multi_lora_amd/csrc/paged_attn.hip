@@ -38,6 +38,61 @@ __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {
   return m;
 }
 
+// A zero the compiler does not know, made anew at each use: loads at an
+// address that has it are not kept in registers over a rare loop.
+__device__ __forceinline__ int opaque_zero() {
+  int z = 0;
+  asm volatile("" : "+s"(z));
+  return z;
+}
+
+// Element e of a chunk if it is not finite, zeros elsewhere (e < 0: nowhere).
+template <class T>
+__device__ __forceinline__ u32x4 odd_values(u32x4 v, int e) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] &= (e >> 1) == i ? nonfinite_mask<T>(v[i]) & ((e & 1) ? 0xffff0000u : 0xffffu) : 0u;
+  return v;
+}
+
+// exp2 of what a softmax needs: arguments at most 0 (or NaN); results below
+// the smallest normal number are 0.
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// An item of the plan, as every wave of its workgroup reads it.
+struct Item {
+  int req, row0, kv0, kv1, slot;
+  int first, c, past;  // its request's first packed row, new tokens, and position of the first
+  int rows;            // query rows of the tile, at most bm
+};
+__device__ __forceinline__ bool load_item(const PagedAttnArgs& a, const PagedKind& kd, int counter, int item, Item* t) {
+  if (item >= a.plan[counter]) return false;
+  const int32_t* w = a.plan + kd.items_off + static_cast<int64_t>(item) * kApItemWords;
+  t->req = w[0], t->row0 = w[1], t->kv0 = w[2], t->kv1 = w[3], t->slot = w[4];
+  t->first = a.row_indptr[t->req];
+  t->c = a.row_indptr[t->req + 1] - t->first;
+  t->past = a.kv_lens[t->req] - t->c;
+  t->rows = min(kd.bm, t->c * a.rep - t->row0);
+  return t->rows > 0;
+}
+
+// Element offset of query row m of a request inside q or out.
+__device__ __forceinline__ int64_t row_offset(const PagedAttnArgs& a, const Item& t, int head, int m, int64_t stride, int d) {
+  const int tok = m / a.rep;
+  return static_cast<int64_t>(t.first + tok) * stride + static_cast<int64_t>(head * a.rep + (m - tok * a.rep)) * d;
+}
+
+// Four columns of a row's result.  Every row sees its own position, so a sum
+// of 0 means scores of -inf only.
+template <class T>
+__device__ __forceinline__ void store_row(typename T::raw_t* out, f32x4 o, float l) {
+  const float inv = l == 0.f ? NAN : 1.f / l;
+  uint2 y;
+  y.x = T::pack2(o[0] * inv, o[1] * inv);
+  y.y = T::pack2(o[2] * inv, o[3] * inv);
+  *reinterpret_cast<uint2*>(out) = y;
+}
+
 template <int D, int NW, int MT>
 struct StreamLds {
   float m[NW][MT * 16];
@@ -46,32 +101,23 @@ struct StreamLds {
   float o[NW][MT * 16][D + 4];
 };
 
-// Workgroup = (item, key head).  Wave w of NW takes tiles w, w + NW, ... of
-// 32 positions, straight from memory into MFMA operands; the waves meet in
-// LDS at the end.
+// Short items: wave w of NW takes tiles w, w + NW, ... of 32 positions,
+// straight from memory into MFMA operands; the waves meet in LDS at the end.
 template <class T, int D, int NW, int MT>
-__global__ __launch_bounds__(NW * 64) void paged_attn_kernel(PagedAttnArgs a) {
+__device__ __forceinline__ void stream_item(const PagedAttnArgs& a, StreamLds<D, NW, MT>& s, int item, int head) {
   using raw = typename T::raw_t;
   constexpr int KS = D / 32;  // k-steps of the scores
   constexpr int DT = D / 16;  // 16-row tiles of O^T
   constexpr int BM = MT * 16;
-  __shared__ StreamLds<D, NW, MT> s;
-  const int item = blockIdx.x / a.kv_heads;
-  const int head = blockIdx.x - item * a.kv_heads;
-  if (item >= a.plan[kApItems]) return;
-  const int32_t* w = a.plan + a.shape.items_off + static_cast<int64_t>(item) * kApItemWords;
-  const int req = w[0], row0 = w[1], kv0 = w[2], kv1 = w[3], slot = w[4];
-  const int first = a.row_indptr[req];
-  const int c = a.row_indptr[req + 1] - first;
-  const int past = a.kv_lens[req] - c;  // position of the first new token
-  const int rows = min(BM, c * a.rep - row0);
-  if (rows <= 0) return;
+  Item it;
+  if (!load_item(a, a.shape.kind[0], kApShort, item, &it)) return;
+  const int row0 = it.row0, rows = it.rows, past = it.past, kv0 = it.kv0, kv1 = it.kv1;
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const int col = lane & 15;
   const int g = lane >> 4;
   const int page = 1 << a.page_shift;
-  const int32_t* table = a.table + static_cast<int64_t>(req) * a.table_stride;
+  const int32_t* table = a.table + static_cast<int64_t>(it.req) * a.table_stride;
   const raw* keys = static_cast<const raw*>(a.keys) + static_cast<int64_t>(head) * page * D;
   const raw* values = static_cast<const raw*>(a.values) + static_cast<int64_t>(head) * page * D;
 
@@ -81,10 +127,8 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int m = row0 + min(t * 16 + col, rows - 1);
-    const int tok = m / a.rep;
-    lim[t] = past + tok + 1;
-    const raw* q = static_cast<const raw*>(a.q) + static_cast<int64_t>(first + tok) * a.q_stride +
-                   static_cast<int64_t>(head * a.rep + (m - tok * a.rep)) * D;
+    lim[t] = past + m / a.rep + 1;
+    const raw* q = static_cast<const raw*>(a.q) + row_offset(a, it, head, m, a.q_stride, D);
 #pragma unroll
     for (int k = 0; k < KS; ++k) qf[t][k] = ld_chunk(q + k * 32 + g * 8);
   }
@@ -159,12 +203,12 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_kernel(PagedAttnArgs a) {
       top = fmaxf(top, __shfl_xor(top, 32, kWave));
       const float now = fmaxf(mx[t], top);
       const float ref = now == -INFINITY ? 0.f : now;  // nothing seen yet: every term below is 0
-      const float keep = exp2f(mx[t] - ref);
+      const float keep = exp2_fast(mx[t] - ref);
       mx[t] = now;
       float add = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        p[i] = exp2f(p[i] - ref);
+        p[i] = exp2_fast(p[i] - ref);
         add += p[i];
       }
       sum[t] = sum[t] * keep + add;  // this lane's positions; joined over the column at the end
@@ -178,31 +222,17 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_kernel(PagedAttnArgs a) {
         acc[t][d] = T::mma(acc[t][d], vf[d], pf);
       }
       if (any_odd) {
-        // The values left out, for the rows that see them: position z of the
-        // tile is in lane group z / 8; row 16 d + 4 g + i of V^T in its lane
-        // 4 g + i.
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const u32x4 vd = ld_chunk(vr + static_cast<int64_t>(d) * 16 * page);
+        // The values left out: one position's at a time, for the rows that see it.
 #pragma unroll 1
-          for (int z = 0; z < kPos; ++z) {
-            const int e = z & 7;
-            const int from = (z >> 3) * 16;
-            float pe = p[0];
+        for (int z = 0; z < kPos; ++z) {
+          const int again = opaque_zero();
+          const bool sees = base + z < min(lim[t], kv1);
 #pragma unroll
-            for (int i = 1; i < 8; ++i) pe = e == i ? p[i] : pe;
-            pe = __shfl(pe, from + col, kWave);
-            uint32_t word = vd[0];
-#pragma unroll
-            for (int i = 1; i < 4; ++i) word = (e >> 1) == i ? vd[i] : word;
-            word &= nonfinite_mask<T>(word);
-            const bool sees = base + z < min(lim[t], kv1);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t other = __shfl(word, from + g * 4 + i, kWave);
-              const float v = T::to_f32(static_cast<raw>((e & 1) ? other >> 16 : other & 0xffffu));
-              if (sees && v != 0.f) acc[t][d][i] += pe * v;
-            }
+          for (int d = 0; d < DT; ++d) {
+            const u32x4 v = odd_values<T>(ld_chunk(vr + again + static_cast<int64_t>(d) * 16 * page), (z >> 3) == g ? z & 7 : -1);
+            if (__ballot((v[0] | v[1] | v[2] | v[3]) != 0) == 0) continue;
+            const f32x4 part = T::mma(f32x4{0.f, 0.f, 0.f, 0.f}, v, pf);
+            if (sees) acc[t][d] += part;
           }
         }
       }
@@ -238,89 +268,337 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_kernel(PagedAttnArgs a) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < NW; ++v) {
-      const float f = exp2f(s.m[v][r] - ref);
+      const float f = exp2_fast(s.m[v][r] - ref);
       l += s.l[v][r] * f;
       o += *reinterpret_cast<const f32x4*>(&s.o[v][r][d]) * f;
     }
-    if (slot >= 0) {
-      const int64_t at = (static_cast<int64_t>(slot) * a.kv_heads + head) * BM + r;
-      *reinterpret_cast<f32x4*>(a.part + at * D + d) = o;
-      if (d == 0) {
-        a.ml[at * 2] = m;
-        a.ml[at * 2 + 1] = l;
-      }
-      continue;
+    if (it.slot >= 0) {
+      const int64_t at = (static_cast<int64_t>(it.slot) * a.kv_heads + head) * BM + r;
+      *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.workspace + a.shape.kind[0].part_off) + at * D + d) = o;
+      if (d == 0) *reinterpret_cast<float2*>(a.workspace + a.shape.kind[0].ml_off + at * 8) = make_float2(m, l);
+    } else {
+      store_row<T>(static_cast<raw*>(a.out) + row_offset(a, it, head, row0 + r, a.out_stride, D) + d, o, l);
     }
-    const int mr = row0 + r;
-    const int tok = mr / a.rep;
-    raw* out = static_cast<raw*>(a.out) + static_cast<int64_t>(first + tok) * a.out_stride +
-               static_cast<int64_t>(head * a.rep + (mr - tok * a.rep)) * D + d;
-    // Every row sees its own position, so a sum of 0 means scores of -inf only.
-    const float inv = l == 0.f ? NAN : 1.f / l;
-    uint2 y;
-    y.x = T::pack2(o[0] * inv, o[1] * inv);
-    y.y = T::pack2(o[2] * inv, o[3] * inv);
-    *reinterpret_cast<uint2*>(out) = y;
   }
+}
+
+constexpr int kTile = 64;  // positions of a long item's step
+
+// Long items: 128 rows, 32 a wave, over the same 64 positions; K and V^T of a
+// step go through LDS, read a step ahead into registers and stored into the
+// other of two buffers after the products.  Chunk p of a row lies at p ^
+// (row's low bits), which spreads a fragment's rows over the banks.
+template <int D>
+struct TileLds {
+  u32x4 k[2][kTile * D / 8];  // [position][D / 8 chunks]
+  u32x4 v[2][D * kTile / 8];  // [D][8 chunks of positions]
+};
+template <int D>
+__device__ __forceinline__ int k_at(int row, int chunk) {
+  return row * (D / 8) + (chunk ^ (row & (D / 8 - 1)));
+}
+__device__ __forceinline__ int v_at(int row, int chunk) { return row * 8 + (chunk ^ ((row >> 1) & 7)); }
+
+template <class T, int D>
+__device__ __forceinline__ void tile_item(const PagedAttnArgs& a, TileLds<D>& s, int item, int head) {
+  using raw = typename T::raw_t;
+  constexpr int KS = D / 16;                     // k-steps of the scores
+  constexpr int DT = D / 32;                     // 32-row tiles of O^T
+  constexpr int NL = kTile * D / 8 / 256;        // chunks a thread loads of each of K and V
+  Item it;
+  if (!load_item(a, a.shape.kind[1], kApLong, item, &it)) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int col = lane & 31;
+  const int h = lane >> 5;
+  const int page = 1 << a.page_shift;
+  const int kv0 = it.kv0, kv1 = it.kv1;
+  const int32_t* table = a.table + static_cast<int64_t>(it.req) * a.table_stride;
+  const raw* keys = static_cast<const raw*>(a.keys) + static_cast<int64_t>(head) * page * D;
+  const raw* values = static_cast<const raw*>(a.values) + static_cast<int64_t>(head) * page * D;
+
+  // The wave's rows; a negative scale goes into q, so that the largest scaled
+  // score is the scaled largest one.
+  const float scale = fabsf(a.scale_log2);
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  const int m = it.row0 + min(wave * 32 + col, it.rows - 1);
+  const int lim = it.past + m / a.rep + 1;
+  u32x4 qf[KS];
+  {
+    const raw* q = static_cast<const raw*>(a.q) + row_offset(a, it, head, m, a.q_stride, D) + h * 8;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qf[k] = ld_chunk(q + k * 16) ^ flip;
+  }
+  const bool live = wave * 32 < it.rows;
+  const int last_row = min(wave * 32 + 31, it.rows - 1);
+  const int open = it.past + (it.row0 + min(wave * 32, it.rows - 1)) / a.rep + 1;  // all of the wave's rows see [0, open)
+  const int shut = min(it.past + (it.row0 + last_row) / a.rep + 1, kv1);            // none sees past it
+
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+  float mx = -INFINITY, sum = 0.f;  // of this lane's positions; the two lanes of a row share mx
+  int broken = INT32_MAX;           // first position without a page in the pool
+
+  // Lane l's page is that of position base + l of the step.
+  auto load_ids = [&](int base) {
+    const int p = base + lane;
+    return p < kv1 ? table[min(p >> a.page_shift, a.width - 1)] : 0;
+  };
+  auto check_ids = [&](int ids, int base) {
+    if (ids < 0 || ids >= a.num_pages) {
+      broken = min(broken, base + lane);
+      ids = 0;
+    }
+    return ids;
+  };
+  u32x4 kr[NL], vr[NL];
+  auto load_tile = [&](int base, int ids) {
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int i = j * 256 + static_cast<int>(threadIdx.x);
+      const int row = i / (D / 8);
+      const int64_t id = __shfl(ids, row, kWave);
+      kr[j] = ld_chunk(keys + id * a.key_stride + ((base + row) & (page - 1)) * D + (i & (D / 8 - 1)) * 8);
+    }
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int i = j * 256 + static_cast<int>(threadIdx.x);
+      const int64_t id = __shfl(ids, (i & 7) * 8, kWave);
+      vr[j] = ld_chunk(values + id * a.value_stride + static_cast<int64_t>(i >> 3) * page + ((base + (i & 7) * 8) & (page - 1)));
+    }
+  };
+  auto store_tile = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int i = j * 256 + static_cast<int>(threadIdx.x);
+      s.k[buf][k_at<D>(i / (D / 8), i & (D / 8 - 1))] = kr[j];
+      s.v[buf][v_at(i >> 3, i & 7)] = vr[j];
+    }
+  };
+  int ids = 0;
+  if (kv0 < kv1) {
+    ids = check_ids(load_ids(kv0), kv0);
+    load_tile(kv0, ids);
+    ids = load_ids(kv0 + kTile);
+    store_tile(0);
+  }
+  int buf = 0;
+  for (int base = kv0; base < kv1; base += kTile, buf ^= 1) {
+    __syncthreads();
+    const bool more = base + kTile < kv1;
+    if (more) {
+      ids = check_ids(ids, base + kTile);
+      load_tile(base + kTile, ids);
+      ids = load_ids(base + 2 * kTile);
+    }
+    if (live && base < shut) {
+      // S^T of 64 positions x 32 rows.  Row rho of an MFMA tile is position
+      // rho with bits 2 and 3 exchanged: a lane's registers 8 s + i are then
+      // positions 16 s + 8 h + i.
+      const int krow = (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1);
+      f32x16 sc[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[t][r] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) sc[t] = T::mma32(sc[t], s.k[buf][k_at<D>(t * 32 + krow, k * 2 + h)], qf[k]);
+      }
+      const bool masked = base + kTile > min(open, kv1);
+      if (masked) {
+        const int seen = min(lim, kv1) - base - h * 8;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (t * 32 + (r >> 3) * 16 + (r & 7) >= seen) sc[t][r] = -INFINITY;
+      }
+      float top = fmaxf(sc[0][0], sc[1][0]);
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, fmaxf(sc[0][r], sc[1][r]));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave)) * scale;
+      if (__any(top > mx)) {
+        const float now = fmaxf(mx, top);
+        const float keep = exp2_fast(mx - (now == -INFINITY ? 0.f : now));
+        mx = now;
+        sum *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[d][r] *= keep;
+      }
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      u32x4 pf[4];
+      float add = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          sc[t][r] = exp2_fast(__builtin_fmaf(sc[t][r], scale, -ref));
+          add += sc[t][r];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) pf[t * 2 + (r >> 3)][(r & 7) >> 1] = T::pack2(sc[t][r], sc[t][r + 1]);
+      }
+      sum += add;
+      if (!masked) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int z = 0; z < 4; ++z) acc[d] = T::mma32(acc[d], s.v[buf][v_at(d * 32 + col, z * 2 + h)], pf[z]);
+      } else {
+        bool any_odd = false;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            u32x4 v = s.v[buf][v_at(d * 32 + col, z * 2 + h)];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t nf = nonfinite_mask<T>(v[i]);
+              any_odd |= nf != 0;
+              v[i] &= ~nf;
+            }
+            acc[d] = T::mma32(acc[d], v, pf[z]);
+          }
+        if (__ballot(any_odd) != 0) {
+          // The values left out: one position's at a time, for the rows that see it.
+#pragma unroll
+          for (int z = 0; z < 4; ++z)
+#pragma unroll 1
+            for (int e = 0; e < 16; ++e) {
+              const int again = opaque_zero();
+              const bool sees = base + z * 16 + e < min(lim, kv1);
+#pragma unroll
+              for (int d = 0; d < DT; ++d) {
+                const u32x4 v = odd_values<T>(s.v[buf][v_at(d * 32 + col, z * 2 + h) + again], (e >> 3) == h ? e & 7 : -1);
+                if (__ballot((v[0] | v[1] | v[2] | v[3]) != 0) == 0) continue;
+                f32x16 part;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) part[r] = 0.f;
+                part = T::mma32(part, v, pf[z]);
+                if (sees)
+#pragma unroll
+                  for (int r = 0; r < 16; ++r) acc[d][r] += part[r];
+              }
+            }
+        }
+      }
+    }
+    if (more) store_tile(buf ^ 1);
+  }
+
+  sum += __shfl_xor(sum, 32, kWave);
+  for (int off = 1; off < kWave; off <<= 1) broken = min(broken, __shfl_xor(broken, off, kWave));
+  if (broken < lim || lim > (static_cast<int64_t>(a.width) << a.page_shift)) sum = NAN;
+  const int r0 = wave * 32 + col;
+  if (r0 >= it.rows) return;
+  if (it.slot >= 0) {
+    const int64_t at = (static_cast<int64_t>(it.slot) * a.kv_heads + head) * kApLongRows + r0;
+    float* part = reinterpret_cast<float*>(a.workspace + a.shape.kind[1].part_off) + at * D + h * 4;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        *reinterpret_cast<f32x4*>(part + d * 32 + r * 2) = f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]};
+    if (h == 0) *reinterpret_cast<float2*>(a.workspace + a.shape.kind[1].ml_off + at * 8) = make_float2(mx, sum);
+  } else {
+    raw* out = static_cast<raw*>(a.out) + row_offset(a, it, head, m, a.out_stride, D) + h * 4;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        store_row<T>(out + d * 32 + r * 2, f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]}, sum);
+  }
+}
+
+template <class T, int D, int NW, int MT>
+__global__ __launch_bounds__(NW * 64, 2) void paged_short_kernel(PagedAttnArgs a) {
+  __shared__ StreamLds<D, NW, MT> s;
+  const int item = blockIdx.x / a.kv_heads;
+  stream_item<T, D, NW, MT>(a, s, item, blockIdx.x - item * a.kv_heads);
+}
+
+// Long items first, then the short ones, which fill the chip as those end.
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void paged_mixed_kernel(PagedAttnArgs a, int long_items) {
+  __shared__ union {
+    TileLds<D> tile;
+    StreamLds<D, 4, 2> stream;
+  } s;
+  const int item = blockIdx.x / a.kv_heads;
+  const int head = blockIdx.x - item * a.kv_heads;
+  if (item < long_items)
+    tile_item<T, D>(a, s.tile, item, head);
+  else
+    stream_item<T, D, 4, 2>(a, s.stream, item - long_items, head);
 }
 
 // The parts of a split tile: workgroup = (tile, key head), thread = four
 // columns of a row.
 template <class T, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int long_joins) {
   using raw = typename T::raw_t;
   constexpr int C = D / 4;
-  const int join = blockIdx.x / a.kv_heads;
+  int join = blockIdx.x / a.kv_heads;
   const int head = blockIdx.x - join * a.kv_heads;
-  if (join >= a.plan[kApJoins]) return;
-  const int32_t* w = a.plan + a.shape.joins_off + static_cast<int64_t>(join) * kApJoinWords;
-  const int req = w[0], row0 = w[1], slot0 = w[2], parts = w[3];
-  const int bm = a.shape.bm;
-  const int first = a.row_indptr[req];
-  const int rows = min(bm, (a.row_indptr[req + 1] - first) * a.rep - row0);
-  for (int i = threadIdx.x; i < rows * C; i += 256) {
+  const int k = join < long_joins ? 1 : 0;
+  const PagedKind kd = k ? a.shape.kind[1] : a.shape.kind[0];
+  if (k == 0) join -= long_joins;
+  if (join >= a.plan[(k ? kApLong : kApShort) + 1]) return;
+  const int32_t* w = a.plan + kd.joins_off + static_cast<int64_t>(join) * kApJoinWords;
+  const int slot0 = w[2], parts = w[3];
+  Item it;
+  it.req = w[0], it.row0 = w[1];
+  it.first = a.row_indptr[it.req];
+  it.rows = min(kd.bm, (a.row_indptr[it.req + 1] - it.first) * a.rep - it.row0);
+  const float* part = reinterpret_cast<const float*>(a.workspace + kd.part_off);
+  const float* ml = reinterpret_cast<const float*>(a.workspace + kd.ml_off);
+  for (int i = threadIdx.x; i < it.rows * C; i += 256) {
     const int r = i / C;
     const int d = (i - r * C) * 4;
-    const int64_t step = static_cast<int64_t>(a.kv_heads) * bm;
-    const int64_t at = (static_cast<int64_t>(slot0) * a.kv_heads + head) * bm + r;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * kd.bm;
+    const int64_t at = (static_cast<int64_t>(slot0) * a.kv_heads + head) * kd.bm + r;
     float m = -INFINITY;
-    for (int p = 0; p < parts; ++p) m = fmaxf(m, a.ml[(at + p * step) * 2]);
+    for (int p = 0; p < parts; ++p) m = fmaxf(m, ml[(at + p * step) * 2]);
     const float ref = m == -INFINITY ? 0.f : m;
     float l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     for (int p = 0; p < parts; ++p) {
-      const float f = exp2f(a.ml[(at + p * step) * 2] - ref);
-      l += a.ml[(at + p * step) * 2 + 1] * f;
-      o += *reinterpret_cast<const f32x4*>(a.part + (at + p * step) * D + d) * f;
+      const float f = exp2_fast(ml[(at + p * step) * 2] - ref);
+      l += ml[(at + p * step) * 2 + 1] * f;
+      o += *reinterpret_cast<const f32x4*>(part + (at + p * step) * D + d) * f;
     }
-    const int mr = row0 + r;
-    const int tok = mr / a.rep;
-    raw* out = static_cast<raw*>(a.out) + static_cast<int64_t>(first + tok) * a.out_stride +
-               static_cast<int64_t>(head * a.rep + (mr - tok * a.rep)) * D + d;
-    const float inv = l == 0.f ? NAN : 1.f / l;
-    uint2 y;
-    y.x = T::pack2(o[0] * inv, o[1] * inv);
-    y.y = T::pack2(o[2] * inv, o[3] * inv);
-    *reinterpret_cast<uint2*>(out) = y;
+    store_row<T>(static_cast<raw*>(a.out) + row_offset(a, it, head, it.row0 + r, a.out_stride, D) + d, o, l);
   }
 }
 
 template <class T, int D>
 hipError_t launch(const PagedAttnArgs& a, hipStream_t stream) {
-  const int64_t blocks = static_cast<int64_t>(a.shape.item_cap) * a.kv_heads;
-  if (!grid_fits(blocks)) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL((paged_attn_kernel<T, D, 4, 1>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
+  const PagedKind &few = a.shape.kind[0], &many = a.shape.kind[1];
+  const int64_t blocks = (static_cast<int64_t>(few.item_cap) + many.item_cap) * a.kv_heads;
+  const int64_t joins = (static_cast<int64_t>(few.join_cap) + many.join_cap) * a.kv_heads;
+  if (!grid_fits(blocks) || !grid_fits(joins)) return hipErrorInvalidConfiguration;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (many.item_cap > 0)
+    hipLaunchKernelGGL((paged_mixed_kernel<T, D>), grid, dim3(256), 0, stream, a, many.item_cap);
+  else if (few.bm == 16)
+    hipLaunchKernelGGL((paged_short_kernel<T, D, 4, 1>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_short_kernel<T, D, 4, 2>), grid, dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.shape.join_cap == 0) return e;
-  hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(static_cast<unsigned>(a.shape.join_cap * a.kv_heads)), dim3(256), 0,
-                     stream, a);
+  if (e != hipSuccess || joins == 0) return e;
+  hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(static_cast<unsigned>(joins)), dim3(256), 0, stream, a, many.join_cap);
   return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, int dtype, int head_dim, hipStream_t stream) {
-  if (a.shape.item_cap == 0) return hipSuccess;
+  if (a.shape.kind[0].item_cap + a.shape.kind[1].item_cap == 0) return hipSuccess;
   if (dtype == MLORA_BF16) return head_dim == 64 ? launch<BF16, 64>(a, stream) : launch<BF16, 128>(a, stream);
   return head_dim == 64 ? launch<F16, 64>(a, stream) : launch<F16, 128>(a, stream);
 }
