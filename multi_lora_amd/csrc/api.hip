@@ -911,7 +911,7 @@ int mlora_paged_attention(const void* q, int64_t q_row_stride, const void* keys,
   a.workspace = static_cast<char*>(step->workspace);
   a.kv_heads = kv_heads, a.rep = heads / kv_heads;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const hipError_t e = mlora::launch_paged_attention(a, dtype, head_dim, static_cast<hipStream_t>(stream));
+  const hipError_t e = mlora::launch_paged_attention(a, step->max_new, dtype, head_dim, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "paged attention launch");
   return 0;
 }

@@ -102,7 +102,7 @@ struct PagedAttnArgs {
   float scale_log2;  // scale * log2(e)
   PagedShape shape;
 };
-hipError_t launch_paged_attention(const PagedAttnArgs& a, int dtype, int head_dim, hipStream_t stream);
+hipError_t launch_paged_attention(const PagedAttnArgs& a, int max_new, int dtype, int head_dim, hipStream_t stream);
 
 struct VerifyArgs {
   const void* target;

@@ -16,6 +16,7 @@
 // any, values that are not finite are left out of the product and added in
 // for the rows that see them, so what lies behind a request's end or in a
 // later token of the chunk reaches no row.
+#include <algorithm>
 #include <type_traits>
 
 #include "kernels.h"
@@ -537,17 +538,17 @@ __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(PagedAttnArgs a, in
     stream_item<T, D, 4, 2>(a, s.stream, item - long_items, head);
 }
 
-// The parts of a split tile: workgroup = (tile, key head), thread = four
-// columns of a row.
-template <class T, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int long_joins) {
+// The parts of a split tile: workgroup = (tile, key head, block of RB rows),
+// thread = four columns of a row.  Short tiles have few rows and up to a
+// hundred parts, so the threads left over share the parts (G groups); long
+// ones the other way round.  One thread a column group over 34 parts took
+// 24 us (three requests of up to 32,000 positions), four 6.
+template <class T, int D, int RB>
+__device__ __forceinline__ void join_rows(const PagedAttnArgs& a, int k, int join, int head, int block, f32x4* os, float* ls) {
   using raw = typename T::raw_t;
   constexpr int C = D / 4;
-  int join = blockIdx.x / a.kv_heads;
-  const int head = blockIdx.x - join * a.kv_heads;
-  const int k = join < long_joins ? 1 : 0;
+  constexpr int G = 256 / (RB * C);
   const PagedKind kd = k ? a.shape.kind[1] : a.shape.kind[0];
-  if (k == 0) join -= long_joins;
   if (join >= a.plan[(k ? kApLong : kApShort) + 1]) return;
   const int32_t* w = a.plan + kd.joins_off + static_cast<int64_t>(join) * kApJoinWords;
   const int slot0 = w[2], parts = w[3];
@@ -555,32 +556,71 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int lo
   it.req = w[0], it.row0 = w[1];
   it.first = a.row_indptr[it.req];
   it.rows = min(kd.bm, (a.row_indptr[it.req + 1] - it.first) * a.rep - it.row0);
-  const float* part = reinterpret_cast<const float*>(a.workspace + kd.part_off);
-  const float* ml = reinterpret_cast<const float*>(a.workspace + kd.ml_off);
-  for (int i = threadIdx.x; i < it.rows * C; i += 256) {
-    const int r = i / C;
-    const int d = (i - r * C) * 4;
-    const int64_t step = static_cast<int64_t>(a.kv_heads) * kd.bm;
-    const int64_t at = (static_cast<int64_t>(slot0) * a.kv_heads + head) * kd.bm + r;
-    float m = -INFINITY;
-    for (int p = 0; p < parts; ++p) m = fmaxf(m, ml[(at + p * step) * 2]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < parts; ++p) {
-      const float f = exp2_fast(ml[(at + p * step) * 2] - ref);
-      l += ml[(at + p * step) * 2 + 1] * f;
-      o += *reinterpret_cast<const f32x4*>(part + (at + p * step) * D + d) * f;
+  if (block * RB >= it.rows) return;
+  const int group = threadIdx.x / (RB * C);
+  const int i = threadIdx.x - group * (RB * C);
+  const int r = min(block * RB + i / C, it.rows - 1);
+  const int d = (i & (C - 1)) * 4;
+  const int64_t step = static_cast<int64_t>(a.kv_heads) * kd.bm;
+  const int64_t at = (static_cast<int64_t>(slot0) * a.kv_heads + head) * kd.bm + r;
+  const float* part = reinterpret_cast<const float*>(a.workspace + kd.part_off) + at * D + d;
+  const float2* ml = reinterpret_cast<const float2*>(a.workspace + kd.ml_off) + at;
+  float m = -INFINITY;
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p) m = fmaxf(m, ml[p * step].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = group; p < parts; p += G) {
+    const float2 x = ml[p * step];
+    const float f = exp2_fast(x.x - ref);
+    l += x.y * f;
+    o += *reinterpret_cast<const f32x4*>(part + p * step * D) * f;
+  }
+  if constexpr (G > 1) {
+    os[threadIdx.x] = o;
+    ls[threadIdx.x] = l;
+    lds_barrier();
+    if (group > 0) return;
+#pragma unroll
+    for (int v = 1; v < G; ++v) {
+      o += os[v * RB * C + i];
+      l += ls[v * RB * C + i];
     }
-    store_row<T>(static_cast<raw*>(a.out) + row_offset(a, it, head, it.row0 + r, a.out_stride, D) + d, o, l);
+  }
+  if (block * RB + i / C >= it.rows) return;
+  store_row<T>(static_cast<raw*>(a.out) + row_offset(a, it, head, it.row0 + r, a.out_stride, D) + d, o, l);
+}
+
+constexpr int join_block(int d, int kind) { return kind ? 1024 / d : 256 / d; }  // rows: 8 or 2 of 128 columns
+
+template <class T, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int long_blocks, int long_per, int short_per) {
+  __shared__ f32x4 os[256];
+  __shared__ float ls[256];
+  int b = blockIdx.x;
+  if (b < long_blocks) {
+    const int tile = b / long_per;
+    const int join = tile / a.kv_heads;
+    join_rows<T, D, join_block(D, 1)>(a, 1, join, tile - join * a.kv_heads, b - tile * long_per, os, ls);
+  } else {
+    b -= long_blocks;
+    const int tile = b / short_per;
+    const int join = tile / a.kv_heads;
+    join_rows<T, D, join_block(D, 0)>(a, 0, join, tile - join * a.kv_heads, b - tile * short_per, os, ls);
   }
 }
 
 template <class T, int D>
-hipError_t launch(const PagedAttnArgs& a, hipStream_t stream) {
+hipError_t launch(const PagedAttnArgs& a, int max_rows, hipStream_t stream) {
   const PagedKind &few = a.shape.kind[0], &many = a.shape.kind[1];
   const int64_t blocks = (static_cast<int64_t>(few.item_cap) + many.item_cap) * a.kv_heads;
-  const int64_t joins = (static_cast<int64_t>(few.join_cap) + many.join_cap) * a.kv_heads;
+  // Row blocks of a tile that hold rows at all.
+  const int long_per = cdiv(std::min(many.bm, max_rows), join_block(D, 1));
+  const int short_per = cdiv(std::min(few.bm, max_rows), join_block(D, 0));
+  const int64_t long_blocks = static_cast<int64_t>(many.join_cap) * a.kv_heads * long_per;
+  const int64_t joins = long_blocks + static_cast<int64_t>(few.join_cap) * a.kv_heads * short_per;
   if (!grid_fits(blocks) || !grid_fits(joins)) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(blocks));
   if (many.item_cap > 0)
@@ -591,16 +631,19 @@ hipError_t launch(const PagedAttnArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((paged_short_kernel<T, D, 4, 2>), grid, dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || joins == 0) return e;
-  hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(static_cast<unsigned>(joins)), dim3(256), 0, stream, a, many.join_cap);
+  hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(static_cast<unsigned>(joins)), dim3(256), 0, stream, a,
+                     static_cast<int>(long_blocks), long_per, short_per);
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_paged_attention(const PagedAttnArgs& a, int dtype, int head_dim, hipStream_t stream) {
+hipError_t launch_paged_attention(const PagedAttnArgs& a, int max_new, int dtype, int head_dim, hipStream_t stream) {
   if (a.shape.kind[0].item_cap + a.shape.kind[1].item_cap == 0) return hipSuccess;
-  if (dtype == MLORA_BF16) return head_dim == 64 ? launch<BF16, 64>(a, stream) : launch<BF16, 128>(a, stream);
-  return head_dim == 64 ? launch<F16, 64>(a, stream) : launch<F16, 128>(a, stream);
+  const int max_rows = std::min(std::min(max_new, a.rows), kApLongRows) * a.rep;  // of one request, as far as it matters
+  if (dtype == MLORA_BF16)
+    return head_dim == 64 ? launch<BF16, 64>(a, max_rows, stream) : launch<BF16, 128>(a, max_rows, stream);
+  return head_dim == 64 ? launch<F16, 64>(a, max_rows, stream) : launch<F16, 128>(a, max_rows, stream);
 }
 
 }  // namespace mlora

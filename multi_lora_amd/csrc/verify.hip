@@ -21,11 +21,6 @@ namespace mlora {
 
 namespace {
 
-template <class T>
-__device__ __forceinline__ double mass(float f) {
-  return f > 0.f ? static_cast<double>(f) : 0.0;
-}
-
 struct Row {
   int accepted;   // drafts accepted; the row drawn from is the accepted-th
   bool rejected;  // a draft stands at that row
@@ -73,14 +68,14 @@ __device__ Row find_row(const VerifyArgs& a, int i) {
 
 // Mass of column x of the row drawn from: of the residual, and of p.
 template <class T>
-__device__ __forceinline__ void column(const VerifyArgs& a, const Row& r, const typename T::raw_t* p,
-                                       const typename T::raw_t* q, int x, double* rest, double* full) {
-  const float f = T::to_f32(p[x]);
-  *full = mass<T>(f);
+__device__ __forceinline__ void column(const Row& r, typename T::raw_t p, bool has_q, typename T::raw_t q, int x,
+                                       double* rest, double* full) {
+  const float f = T::to_f32(p);
+  *full = f > 0.f ? static_cast<double>(f) : 0.0;
   if (!r.rejected) {
     *rest = *full;
-  } else if (q != nullptr) {
-    const double less = static_cast<double>(f) - static_cast<double>(T::to_f32(q[x]));
+  } else if (has_q) {
+    const double less = static_cast<double>(f) - static_cast<double>(T::to_f32(q));
     *rest = less > 0.0 ? less : 0.0;
   } else {
     *rest = x == r.token ? 0.0 : *full;
@@ -98,22 +93,38 @@ __device__ __forceinline__ void row_ptrs(const VerifyArgs& a, const Row& r, int 
            : nullptr;
 }
 
+constexpr int kPer = kVerifyChunk / 256;  // columns a thread
+
 template <class T>
 __global__ __launch_bounds__(256) void verify_sum_kernel(VerifyArgs a) {
   using raw = typename T::raw_t;
   const int i = blockIdx.x / a.chunks;
   const int c = blockIdx.x - i * a.chunks;
   const Row r = find_row<T>(a, i);
+  if (c == 0 && threadIdx.x == 0) a.accepted[i] = r.accepted;
   if (!r.live) return;
   const raw *p, *q;
   row_ptrs<T>(a, r, i, &p, &q);
+  // Every load is issued before the first is used; columns past the row's end
+  // read its last one again and count nothing.
+  raw pv[kPer], qv[kPer];
+  const int x0 = c * kVerifyChunk + static_cast<int>(threadIdx.x);
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) pv[e] = p[min(x0 + e * 256, a.vocab - 1)];
+  if (q != nullptr) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) qv[e] = q[min(x0 + e * 256, a.vocab - 1)];
+  }
   double rest = 0.0, full = 0.0;
-  const int end = min((c + 1) * kVerifyChunk, a.vocab);
-  for (int x = c * kVerifyChunk + threadIdx.x; x < end; x += 256) {
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const int x = x0 + e * 256;
     double m, f;
-    column<T>(a, r, p, q, x, &m, &f);
-    rest += m;
-    full += f;
+    column<T>(r, pv[e], q != nullptr, qv[e], x, &m, &f);
+    if (x < a.vocab) {
+      rest += m;
+      full += f;
+    }
   }
   for (int off = 1; off < kWave; off <<= 1) {
     rest += __shfl_xor(rest, off, kWave);
@@ -131,103 +142,128 @@ __global__ __launch_bounds__(256) void verify_sum_kernel(VerifyArgs a) {
         part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
-  using raw = typename T::raw_t;
-  constexpr int PT = kVerifyChunk / 256;  // columns a thread
-  const int i = blockIdx.x;
-  const int tid = threadIdx.x;
-  const Row r = find_row<T>(a, i);
-  int64_t* out = a.out + static_cast<int64_t>(i) * (a.most + 1);
-  for (int j = tid; j <= a.most; j += 256)
-    if (j != r.accepted || !r.live) out[j] = r.live && j < r.accepted ? a.tokens[i * a.token_stride + j] : -1;
-  if (tid == 0) a.accepted[i] = r.accepted;
-  if (!r.live) return;
-  const double* sums = a.sums + static_cast<int64_t>(i) * a.chunks * 2;
-  __shared__ double before_s, total_s;
-  __shared__ int chunk_s, full_s, found_s;
-  if (tid == 0) {
-    // Chunks of a row are few (32 for 128 k columns): one thread adds them up.
-    double rest = 0.0, full = 0.0;
-    for (int c = 0; c < a.chunks; ++c) {
-      rest += sums[c * 2];
-      full += sums[c * 2 + 1];
-    }
-    const int use = rest > 0.0 ? 0 : 1;
-    const double total = use == 0 ? rest : full;
-    const double want = static_cast<double>(a.last[i]) * total;
-    double cum = 0.0, before = 0.0;
-    int at = -1, last = -1;
-    for (int c = 0; c < a.chunks; ++c) {
-      const double m = sums[c * 2 + use];
-      if (m > 0.0) last = c;
-      if (m > 0.0 && cum + m > want) {
-        at = c;
-        before = cum;
-        break;
-      }
-      cum += m;
-    }
-    if (at < 0 && last >= 0) {  // a number of 1 or more: the last column with mass
-      at = last;
-      before = -INFINITY;
-    }
-    before_s = before;
-    total_s = want;
-    chunk_s = at;
-    full_s = use;
-    found_s = INT32_MAX;
-  }
-  __syncthreads();
-  if (chunk_s < 0) {
-    if (tid == 0) out[r.accepted] = -1;
-    return;
-  }
-  const raw *p, *q;
-  row_ptrs<T>(a, r, i, &p, &q);
-  const int x0 = chunk_s * kVerifyChunk + tid * PT;
-  double m[PT], mine = 0.0;
-  int last = -1;
-#pragma unroll
-  for (int e = 0; e < PT; ++e) {
-    m[e] = 0.0;
-    if (x0 + e < a.vocab) {
-      double rest, full;
-      column<T>(a, r, p, q, x0 + e, &rest, &full);
-      m[e] = full_s ? full : rest;
-    }
-    if (m[e] > 0.0) last = x0 + e;
-    mine += m[e];
-  }
-  // Mass of the threads before this one.
+// Exclusive sum over the workgroup's 256 threads of `mine`, and the total.
+__device__ __forceinline__ double scan256(double mine, double* tmp, double* total) {
   double incl = mine;
-  const int lane = tid & 63, wave = tid >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
   for (int off = 1; off < kWave; off <<= 1) {
     const double y = __shfl_up(incl, off, kWave);
     if (lane >= off) incl += y;
   }
-  __shared__ double waves[4];
-  __shared__ int last_s[4];
-  for (int off = 1; off < kWave; off <<= 1) last = max(last, __shfl_xor(last, off, kWave));
-  if (lane == kWave - 1) {
-    waves[wave] = incl;
-    last_s[wave] = last;
-  }
+  if (lane == kWave - 1) tmp[wave] = incl;
   __syncthreads();
-  double cum = before_s;
-  for (int v = 0; v < wave; ++v) cum += waves[v];
-  cum += incl - mine;
-#pragma unroll
-  for (int e = 0; e < PT; ++e) {
-    cum += m[e];
-    if (m[e] > 0.0 && cum > total_s) {
-      atomicMin(&found_s, x0 + e);
-      break;
+  double before = 0.0;
+  for (int v = 0; v < wave; ++v) before += tmp[v];
+  *total = (tmp[0] + tmp[1]) + (tmp[2] + tmp[3]);
+  __syncthreads();
+  return before + (incl - mine);
+}
+
+struct DrawLds {
+  double tmp[4];
+  double before;
+  int hit, last;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
+  using raw = typename T::raw_t;
+  __shared__ DrawLds s;
+  const int i = blockIdx.x;
+  const int tid = threadIdx.x;
+  // The row, from the first launch's count.
+  const int first = min(max(a.row_indptr[i], 0), a.rows);
+  const int end = min(max(a.row_indptr[i + 1], first), a.rows);
+  Row r{a.accepted[i], false, -1, end > first};
+  r.rejected = r.accepted < min(end - first - 1, a.most);
+  if (r.rejected) r.token = a.tokens[i * a.token_stride + r.accepted];
+  int64_t* out = a.out + static_cast<int64_t>(i) * (a.most + 1);
+  for (int j = tid; j <= a.most; j += 256)
+    if (j != r.accepted || !r.live) out[j] = r.live && j < r.accepted ? a.tokens[i * a.token_stride + j] : -1;
+  if (!r.live) return;
+
+  // The chunk that the draw falls in; a thread takes `per` neighbouring ones.
+  const double* sums = a.sums + static_cast<int64_t>(i) * a.chunks * 2;
+  const int per = (a.chunks + 255) / 256;
+  const int c0 = tid * per, c1 = min(c0 + per, a.chunks);
+  double rest = 0.0, full = 0.0, total_rest, total_full;
+  for (int c = c0; c < c1; ++c) {
+    rest += sums[c * 2];
+    full += sums[c * 2 + 1];
+  }
+  if (tid == 0) {
+    s.hit = INT32_MAX;
+    s.last = -1;
+  }
+  const double rest0 = scan256(rest, s.tmp, &total_rest);
+  const double full0 = scan256(full, s.tmp, &total_full);
+  const int use = total_rest > 0.0 ? 0 : 1;
+  const double want = static_cast<double>(a.last[i]) * (use == 0 ? total_rest : total_full);
+  double cum = use == 0 ? rest0 : full0;
+  int hit = INT32_MAX, last = -1;
+  double before = 0.0;
+  for (int c = c0; c < c1; ++c) {
+    const double m = sums[c * 2 + use];
+    if (m > 0.0) {
+      last = c;
+      if (hit == INT32_MAX && cum + m > want) {
+        hit = c;
+        before = cum;
+      }
     }
+    cum += m;
+  }
+  if (hit != INT32_MAX) atomicMin(&s.hit, hit);
+  if (last >= 0) atomicMax(&s.last, last);
+  __syncthreads();
+  int chunk = s.hit;
+  if (chunk == hit && hit != INT32_MAX) s.before = before;
+  if (chunk == INT32_MAX) {  // a number of 1 or more: the last column with mass
+    chunk = s.last;
+    if (tid == 0) s.before = -INFINITY;
   }
   __syncthreads();
-  if (tid == 0)
-    out[r.accepted] = found_s != INT32_MAX ? found_s : max(max(last_s[0], last_s[1]), max(last_s[2], last_s[3]));
+  before = s.before;
+  if (chunk < 0) {
+    if (tid == 0) out[r.accepted] = -1;
+    return;
+  }
+  if (tid == 0) {
+    s.hit = INT32_MAX;
+    s.last = -1;
+  }
+  const raw *p, *q;
+  row_ptrs<T>(a, r, i, &p, &q);
+  const int x0 = chunk * kVerifyChunk + tid * kPer;
+  raw pv[kPer], qv[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) pv[e] = p[min(x0 + e, a.vocab - 1)];
+  if (q != nullptr) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) qv[e] = q[min(x0 + e, a.vocab - 1)];
+  }
+  double m[kPer], mine = 0.0, total;
+  last = -1;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    double re, fu;
+    column<T>(r, pv[e], q != nullptr, qv[e], x0 + e, &re, &fu);
+    m[e] = x0 + e < a.vocab ? (use ? fu : re) : 0.0;
+    if (m[e] > 0.0) last = x0 + e;
+    mine += m[e];
+  }
+  cum = before + scan256(mine, s.tmp, &total);
+  hit = INT32_MAX;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    cum += m[e];
+    if (hit == INT32_MAX && m[e] > 0.0 && cum > want) hit = x0 + e;
+  }
+  if (hit != INT32_MAX) atomicMin(&s.hit, hit);
+  if (last >= 0) atomicMax(&s.last, last);
+  __syncthreads();
+  if (tid == 0) out[r.accepted] = s.hit != INT32_MAX ? s.hit : s.last;
 }
 
 template <class T>
