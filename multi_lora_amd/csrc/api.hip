@@ -886,6 +886,8 @@ int mlora_paged_attention(const void* q, int64_t q_row_stride, const void* keys,
   const int64_t qw = static_cast<int64_t>(heads) * head_dim, pw = static_cast<int64_t>(kv_heads) * head_dim * pages->page;
   if (q_row_stride < qw || out_row_stride < qw || key_page_stride < pw || value_page_stride < pw)
     return fail(kBadArg, "strides do not hold the rows or pages");
+  if (key_page_stride > INT32_MAX / 2 || value_page_stride > INT32_MAX / 2)
+    return fail(kUnsupported, "pages more than 2^30 elements apart");
   if (pages->n == 0 || step->rows == 0 || pages->num_pages == 0 || pages->width == 0) {
     if (pages->n > 0 && step->rows > 0) return fail(kBadArg, "attention over a cache without pages");
     return 0;

@@ -22,8 +22,11 @@ constexpr int kApItemWords = 8;  // request, first row, first position, end, slo
 constexpr int kApJoinWords = 4;  // request, first row, first slot, slots
 
 constexpr int kApLongRows = 128;
-// A range is split only into parts of at least this many positions.
+// A range is split only into parts of at least this many positions.  A part of
+// a long tile writes and reads again 128 rows of sums: prompts of 512 tokens in
+// two parts cost 21 us of joins for 34 MB, and 8 steps less of a tile.
 constexpr int kApMinSplit = 256;
+constexpr int kApMinSplitLong = 1024;
 // Tiles that fill the chip this many times over are not split.
 constexpr int kApWhole = 4;
 
@@ -38,7 +41,6 @@ struct PagedKind {
 struct PagedShape {
   int rep;
   int target;        // parts (of all key heads) that fill the chip
-  bool can_split;
   PagedKind kind[2]; // short, long (no caps: none can occur)
   size_t plan_bytes, ws_bytes;
 };

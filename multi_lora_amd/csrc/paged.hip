@@ -172,12 +172,12 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
   // Parts of equal length, so that all of them together fill the chip once;
   // tiles that fill it several times over stay whole.
   int split[2] = {INT32_MAX, INT32_MAX};
-  if (plan && s.can_split) {
+  if (plan) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const unsigned long long part = (wide[k] * a.kv_heads + s.target - 1) / s.target;
       if (wide[2 + k] * a.kv_heads < static_cast<unsigned long long>(kApWhole) * s.target)
-        split[k] = static_cast<int>((min(max(part, static_cast<unsigned long long>(kApMinSplit)), 1ull << 30) + 63) / 64 * 64);
+        split[k] = static_cast<int>((min(max(part, static_cast<unsigned long long>(k ? kApMinSplitLong : kApMinSplit)), 1ull << 30) + 63) / 64 * 64);
     }
   }
   const int have = top + freed;
@@ -401,7 +401,6 @@ bool paged_shape(int n, int rows, int max_new, int64_t max_kv, int heads, int kv
   if (n < 0 || rows < 0 || max_new < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0) return false;
   s->rep = heads / kv_heads;
   s->target = 2 * cus;
-  s->can_split = max_kv > kApMinSplit;
   const int64_t most = static_cast<int64_t>(std::min(max_new, rows)) * s->rep;  // rows of one request
   const int64_t all = static_cast<int64_t>(rows) * s->rep;
   s->kind[0].bm = most <= 16 ? 16 : 32;
@@ -414,9 +413,12 @@ bool paged_shape(int n, int rows, int max_new, int64_t max_kv, int heads, int kv
     const int64_t tiles = !occurs ? 0
                           : k == 0 ? std::min(n, rows)
                                    : all / kd.bm + std::min<int64_t>(n, all / (s->kind[0].bm + 1));
-    // Parts of a tile: at most its length / split + 1, and the lengths of all
-    // tiles sum to at most twice the plan's estimate (len - new / 2).
-    const int64_t extra = occurs && s->can_split ? 2 * (s->target / kv_heads + 1) : 0;
+    // Parts of a tile: at most its length / split + 1.  The plan's estimate of
+    // a tile's length is len - new / 2: at least half of it, and of a short
+    // request that is split (more than 256 positions, at most 32 of them new)
+    // at least 15 of 16.
+    const int64_t fill = s->target / kv_heads + 1;
+    const int64_t extra = !occurs || max_kv <= (k ? kApMinSplitLong : kApMinSplit) ? 0 : k ? 2 * fill : fill + fill / 15 + 1;
     const int64_t slots = extra > 0 ? std::min(tiles, static_cast<int64_t>(kApWhole) * s->target / kv_heads + 1) + extra : 0;
     if (tiles + extra > INT32_MAX / 64) return false;
     kd.item_cap = static_cast<int>(tiles + extra);

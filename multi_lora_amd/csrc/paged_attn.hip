@@ -29,6 +29,9 @@ namespace {
 
 constexpr int kPos = 32;  // positions a wave takes at once
 
+typedef const __attribute__((address_space(1))) void gvoid_t;
+typedef __attribute__((address_space(3))) void lvoid_t;
+
 // All ones in the 16-bit halves of a word that are infinite or NaN.
 template <class T>
 __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {
@@ -286,9 +289,9 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, StreamLds<D,
 constexpr int kTile = 64;  // positions of a long item's step
 
 // Long items: 128 rows, 32 a wave, over the same 64 positions; K and V^T of a
-// step go through LDS, read a step ahead into registers and stored into the
-// other of two buffers after the products.  Chunk p of a row lies at p ^
-// (row's low bits), which spreads a fragment's rows over the banks.
+// step go straight into LDS, a step ahead, in one of two buffers.  Chunk p of
+// a row lies at p ^ (row's low bits), which spreads a fragment's rows over the
+// banks.
 template <int D>
 struct TileLds {
   u32x4 k[2][kTile * D / 8];  // [position][D / 8 chunks]
@@ -300,23 +303,30 @@ __device__ __forceinline__ int k_at(int row, int chunk) {
 }
 __device__ __forceinline__ int v_at(int row, int chunk) { return row * 8 + (chunk ^ ((row >> 1) & 7)); }
 
+// The softmax's reference of a row is not its largest score so far but one
+// against which no weight is above kOver: weights stay in the data type's range,
+// and the sums are rescaled a few times a range instead of at every new maximum
+// (whose search over raw scores costs as much as the exponentials' arguments).
+constexpr float kOver = 256.f;
+constexpr float kNoScore = -3e38f;  // a row's reference before it has seen a score
+
 template <class T, int D>
 __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, TileLds<D>& s, int item, int head) {
   using raw = typename T::raw_t;
   constexpr int KS = D / 16;                     // k-steps of the scores
   constexpr int DT = D / 32;                     // 32-row tiles of O^T
-  constexpr int NL = kTile * D / 8 / 256;        // chunks a thread loads of each of K and V
+  constexpr int NL = kTile * D / 8 / 256;        // instructions a wave loads each of K and V with
+  constexpr int KC = D / 8;                      // chunks of a key
   Item it;
   if (!load_item(a, a.shape.kind[1], kApLong, item, &it)) return;
-  const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31;
   const int h = lane >> 5;
   const int page = 1 << a.page_shift;
   const int kv0 = it.kv0, kv1 = it.kv1;
   const int32_t* table = a.table + static_cast<int64_t>(it.req) * a.table_stride;
-  const raw* keys = static_cast<const raw*>(a.keys) + static_cast<int64_t>(head) * page * D;
-  const raw* values = static_cast<const raw*>(a.values) + static_cast<int64_t>(head) * page * D;
 
   // The wave's rows; a negative scale goes into q, so that the largest scaled
   // score is the scaled largest one.
@@ -331,16 +341,16 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, TileLds<D>& s,
     for (int k = 0; k < KS; ++k) qf[k] = ld_chunk(q + k * 16) ^ flip;
   }
   const bool live = wave * 32 < it.rows;
-  const int last_row = min(wave * 32 + 31, it.rows - 1);
-  const int open = it.past + (it.row0 + min(wave * 32, it.rows - 1)) / a.rep + 1;  // all of the wave's rows see [0, open)
-  const int shut = min(it.past + (it.row0 + last_row) / a.rep + 1, kv1);            // none sees past it
+  // All of the wave's rows see [0, open), none sees past shut.
+  const int open = min(it.past + (it.row0 + min(wave * 32, it.rows - 1)) / a.rep + 1, kv1);
+  const int shut = min(it.past + (it.row0 + min(wave * 32 + 31, it.rows - 1)) / a.rep + 1, kv1);
 
   f32x16 acc[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
-  float mx = -INFINITY, sum = 0.f;  // of this lane's positions; the two lanes of a row share mx
+  float ref = kNoScore, sum = 0.f;  // sum: of this lane's positions; the two lanes of a row share ref
   int broken = INT32_MAX;           // first position without a page in the pool
 
   // Lane l's page is that of position base + l of the step.
@@ -349,147 +359,151 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, TileLds<D>& s,
     return p < kv1 ? table[min(p >> a.page_shift, a.width - 1)] : 0;
   };
   auto check_ids = [&](int ids, int base) {
-    if (ids < 0 || ids >= a.num_pages) {
+    if (static_cast<uint32_t>(ids) >= static_cast<uint32_t>(a.num_pages)) {
       broken = min(broken, base + lane);
       ids = 0;
     }
-    return ids;
+    return static_cast<uint32_t>(ids);
   };
-  u32x4 kr[NL], vr[NL];
-  auto load_tile = [&](int base, int ids) {
+  // An instruction of a wave fills 1 KB of a tile: K rows kr0 + j * 256 / KC,
+  // V rows vr0 + j * 32, and chunk p of a row comes from chunk p ^ (row's low
+  // bits), the same for every j.  Steps begin at multiples of 64 and pages are
+  // powers of two, so a lane's place inside a page moves with the step's only.
+  const int kr0 = wave * (64 / KC) + lane / KC;
+  const int vr0 = wave * 8 + (lane >> 3);
+  const int kc = (lane & (KC - 1)) ^ (kr0 & (KC - 1));
+  const int vc = (lane & 7) ^ ((vr0 >> 1) & 7);
+  const char* kb = reinterpret_cast<const char*>(a.keys) + (static_cast<int64_t>(head) * page * D + kc * 8) * 2;
+  const char* vb = reinterpret_cast<const char*>(a.values) +
+                   ((static_cast<int64_t>(head) * D + vr0) * page + (vc * 8 & (page - 1))) * 2;
+  const uint32_t kstep = static_cast<uint32_t>(a.key_stride * 2), vstep = static_cast<uint32_t>(a.value_stride * 2);
+  auto load_tile = [&](int base, uint32_t ids, int buf) {
+    const int in_page = base & (page - 1);
+    const char* kp = kb + static_cast<int64_t>(in_page) * (D * 2);
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
-      const int i = j * 256 + static_cast<int>(threadIdx.x);
-      const int row = i / (D / 8);
-      const int64_t id = __shfl(ids, row, kWave);
-      kr[j] = ld_chunk(keys + id * a.key_stride + ((base + row) & (page - 1)) * D + (i & (D / 8 - 1)) * 8);
+      const int row = j * (256 / KC) + kr0;
+      const uint32_t id = __shfl(ids, row, kWave);
+      const char* p = kp + (row & (page - 1)) * (D * 2) + static_cast<uint64_t>(id) * kstep;
+      __builtin_amdgcn_global_load_lds((gvoid_t*)p, (lvoid_t*)(&s.k[buf][(j * 4 + wave) * 64]), 16, 0, 0);
     }
+    const char* vp = vb + in_page * 2 + static_cast<uint64_t>(static_cast<uint32_t>(__shfl(ids, vc * 8, kWave))) * vstep;
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      const int i = j * 256 + static_cast<int>(threadIdx.x);
-      const int64_t id = __shfl(ids, (i & 7) * 8, kWave);
-      vr[j] = ld_chunk(values + id * a.value_stride + static_cast<int64_t>(i >> 3) * page + ((base + (i & 7) * 8) & (page - 1)));
-    }
+    for (int j = 0; j < NL; ++j)
+      __builtin_amdgcn_global_load_lds((gvoid_t*)(vp + static_cast<int64_t>(j * 32 * 2) * page),
+                                       (lvoid_t*)(&s.v[buf][(j * 4 + wave) * 64]), 16, 0, 0);
   };
-  auto store_tile = [&](int buf) {
+
+  // Row rho of an MFMA tile is position rho with bits 2 and 3 exchanged: a
+  // lane's registers 8 s + i are then positions 16 s + 8 h + i.
+  const int krow = (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1);
+  auto step = [&](int base, int buf, auto is_masked) {
+    constexpr bool MASKED = decltype(is_masked)::value;
+    const int seen = min(lim, kv1) - base - h * 8;
+    // S^T of 32 positions x 32 rows.
+    auto scores = [&](int t) {
+      f32x16 sc;
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      const int i = j * 256 + static_cast<int>(threadIdx.x);
-      s.k[buf][k_at<D>(i / (D / 8), i & (D / 8 - 1))] = kr[j];
-      s.v[buf][v_at(i >> 3, i & 7)] = vr[j];
-    }
-  };
-  int ids = 0;
-  if (kv0 < kv1) {
-    ids = check_ids(load_ids(kv0), kv0);
-    load_tile(kv0, ids);
-    ids = load_ids(kv0 + kTile);
-    store_tile(0);
-  }
-  int buf = 0;
-  for (int base = kv0; base < kv1; base += kTile, buf ^= 1) {
-    __syncthreads();
-    const bool more = base + kTile < kv1;
-    if (more) {
-      ids = check_ids(ids, base + kTile);
-      load_tile(base + kTile, ids);
-      ids = load_ids(base + 2 * kTile);
-    }
-    if (live && base < shut) {
-      // S^T of 64 positions x 32 rows.  Row rho of an MFMA tile is position
-      // rho with bits 2 and 3 exchanged: a lane's registers 8 s + i are then
-      // positions 16 s + 8 h + i.
-      const int krow = (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1);
-      f32x16 sc[2];
+      for (int r = 0; r < 16; ++r) sc[r] = 0.f;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int k = 0; k < KS; ++k) sc = T::mma32(sc, s.k[buf][k_at<D>(t * 32 + krow, k * 2 + h)], qf[k]);
+      if constexpr (MASKED) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sc[t][r] = 0.f;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) sc[t] = T::mma32(sc[t], s.k[buf][k_at<D>(t * 32 + krow, k * 2 + h)], qf[k]);
+        for (int r = 0; r < 16; ++r)
+          if (t * 32 + (r >> 3) * 16 + (r & 7) >= seen) sc[r] = -INFINITY;
       }
-      const bool masked = base + kTile > min(open, kv1);
-      if (masked) {
-        const int seen = min(lim, kv1) - base - h * 8;
+      return sc;
+    };
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
+      f32x16 p = scores(t);
+      float top = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (t * 32 + (r >> 3) * 16 + (r & 7) >= seen) sc[t][r] = -INFINITY;
-      }
-      float top = fmaxf(sc[0][0], sc[1][0]);
+      for (int r = 0; r < 16; ++r) p[r] = exp2_fast(__builtin_fmaf(p[r], scale, -ref));
 #pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, fmaxf(sc[0][r], sc[1][r]));
-      top = fmaxf(top, __shfl_xor(top, 32, kWave)) * scale;
-      if (__any(top > mx)) {
-        const float now = fmaxf(mx, top);
-        const float keep = exp2_fast(mx - (now == -INFINITY ? 0.f : now));
-        mx = now;
+      for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(top, p[r]), p[r + 1]);
+      if (__any(top > kOver)) {
+        p = scores(t);  // again: the weights took their place
+        float now = p[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) now = fmaxf(now, p[r]);
+        now = fmaxf(now, __shfl_xor(now, 32, kWave)) * scale;
+        now = fmaxf(now, ref);
+        const float keep = exp2_fast(ref - now);
+        ref = now;
         sum *= keep;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[d][r] *= keep;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = exp2_fast(__builtin_fmaf(p[r], scale, -ref));
       }
-      const float ref = mx == -INFINITY ? 0.f : mx;
-      u32x4 pf[4];
-      float add = 0.f;
+      u32x4 pf[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int r = 0; r < 16; r += 2) pf[r >> 3][(r & 7) >> 1] = T::pack2(p[r], p[r + 1]);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          sc[t][r] = exp2_fast(__builtin_fmaf(sc[t][r], scale, -ref));
-          add += sc[t][r];
-        }
+      for (int r = 0; r < 16; r += 2) sum += p[r] + p[r + 1];
+      bool any_odd = false;
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) pf[t * 2 + (r >> 3)][(r & 7) >> 1] = T::pack2(sc[t][r], sc[t][r + 1]);
-      }
-      sum += add;
-      if (!masked) {
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int z = 0; z < 4; ++z) acc[d] = T::mma32(acc[d], s.v[buf][v_at(d * 32 + col, z * 2 + h)], pf[z]);
-      } else {
-        bool any_odd = false;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            u32x4 v = s.v[buf][v_at(d * 32 + col, z * 2 + h)];
+        for (int z = 0; z < 2; ++z) {
+          u32x4 v = s.v[buf][v_at(d * 32 + col, t * 4 + z * 2 + h)];
+          if constexpr (MASKED) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t nf = nonfinite_mask<T>(v[i]);
               any_odd |= nf != 0;
               v[i] &= ~nf;
             }
-            acc[d] = T::mma32(acc[d], v, pf[z]);
           }
-        if (__ballot(any_odd) != 0) {
-          // The values left out: one position's at a time, for the rows that see it.
-#pragma unroll
-          for (int z = 0; z < 4; ++z)
-#pragma unroll 1
-            for (int e = 0; e < 16; ++e) {
-              const int again = opaque_zero();
-              const bool sees = base + z * 16 + e < min(lim, kv1);
-#pragma unroll
-              for (int d = 0; d < DT; ++d) {
-                const u32x4 v = odd_values<T>(s.v[buf][v_at(d * 32 + col, z * 2 + h) + again], (e >> 3) == h ? e & 7 : -1);
-                if (__ballot((v[0] | v[1] | v[2] | v[3]) != 0) == 0) continue;
-                f32x16 part;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) part[r] = 0.f;
-                part = T::mma32(part, v, pf[z]);
-                if (sees)
-#pragma unroll
-                  for (int r = 0; r < 16; ++r) acc[d][r] += part[r];
-              }
-            }
+          acc[d] = T::mma32(acc[d], v, pf[z]);
         }
+      if (MASKED && __ballot(any_odd) != 0) {
+        // The values left out: one position's at a time, for the rows that see it.
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+#pragma unroll 1
+          for (int e = 0; e < 16; ++e) {
+            const int again = opaque_zero();
+            const bool sees = base + t * 32 + z * 16 + e < min(lim, kv1);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+              const u32x4 v = odd_values<T>(s.v[buf][v_at(d * 32 + col, t * 4 + z * 2 + h) + again], (e >> 3) == h ? e & 7 : -1);
+              if (__ballot((v[0] | v[1] | v[2] | v[3]) != 0) == 0) continue;
+              f32x16 part;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) part[r] = 0.f;
+              part = T::mma32(part, v, pf[z]);
+              if (sees)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] += part[r];
+            }
+          }
       }
     }
-    if (more) store_tile(buf ^ 1);
+  };
+
+  uint32_t ids = 0;
+  if (kv0 < kv1) {
+    load_tile(kv0, check_ids(load_ids(kv0), kv0), 0);
+    ids = load_ids(kv0 + kTile);
+  }
+  int buf = 0;
+  for (int base = kv0; base < kv1; base += kTile, buf ^= 1) {
+    wait_vmcnt<0>();  // this wave's part of the step has landed
+    lds_barrier();    // everyone's has, and nobody reads the other buffer
+    if (base + kTile < kv1) {
+      load_tile(base + kTile, check_ids(ids, base + kTile), buf ^ 1);
+      ids = load_ids(base + 2 * kTile);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // the next step's loads go out before this one's products
+    if (!live || base >= shut) continue;
+    if (__builtin_expect(base + kTile > open, 0))
+      step(base, buf, std::true_type{});
+    else
+      step(base, buf, std::false_type{});
   }
 
   sum += __shfl_xor(sum, 32, kWave);
@@ -505,7 +519,8 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, TileLds<D>& s,
 #pragma unroll
       for (int r = 0; r < 16; r += 4)
         *reinterpret_cast<f32x4*>(part + d * 32 + r * 2) = f32x4{acc[d][r], acc[d][r + 1], acc[d][r + 2], acc[d][r + 3]};
-    if (h == 0) *reinterpret_cast<float2*>(a.workspace + a.shape.kind[1].ml_off + at * 8) = make_float2(mx, sum);
+    if (h == 0)
+      *reinterpret_cast<float2*>(a.workspace + a.shape.kind[1].ml_off + at * 8) = make_float2(ref == kNoScore ? -INFINITY : ref, sum);
   } else {
     raw* out = static_cast<raw*>(a.out) + row_offset(a, it, head, m, a.out_stride, D) + h * 4;
 #pragma unroll
@@ -549,7 +564,6 @@ __device__ __forceinline__ void join_rows(const PagedAttnArgs& a, int k, int joi
   constexpr int C = D / 4;
   constexpr int G = 256 / (RB * C);
   const PagedKind kd = k ? a.shape.kind[1] : a.shape.kind[0];
-  if (join >= a.plan[(k ? kApLong : kApShort) + 1]) return;
   const int32_t* w = a.plan + kd.joins_off + static_cast<int64_t>(join) * kApJoinWords;
   const int slot0 = w[2], parts = w[3];
   Item it;
@@ -593,22 +607,28 @@ __device__ __forceinline__ void join_rows(const PagedAttnArgs& a, int k, int joi
   store_row<T>(static_cast<raw*>(a.out) + row_offset(a, it, head, it.row0 + r, a.out_stride, D) + d, o, l);
 }
 
+constexpr int kJoinGrid = 2048;  // eight workgroups a CU
 constexpr int join_block(int d, int kind) { return kind ? 1024 / d : 256 / d; }  // rows: 8 or 2 of 128 columns
 
+// Workgroups take the row blocks in turn: the host's bound on them is many
+// times what most steps have, and starting that many idle ones cost 10 us.
 template <class T, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int long_blocks, int long_per, int short_per) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int long_per, int short_per) {
   __shared__ f32x4 os[256];
   __shared__ float ls[256];
-  int b = blockIdx.x;
-  if (b < long_blocks) {
-    const int tile = b / long_per;
-    const int join = tile / a.kv_heads;
-    join_rows<T, D, join_block(D, 1)>(a, 1, join, tile - join * a.kv_heads, b - tile * long_per, os, ls);
-  } else {
-    b -= long_blocks;
-    const int tile = b / short_per;
-    const int join = tile / a.kv_heads;
-    join_rows<T, D, join_block(D, 0)>(a, 0, join, tile - join * a.kv_heads, b - tile * short_per, os, ls);
+  const int long_blocks = a.plan[kApLong + 1] * a.kv_heads * long_per;
+  const int blocks = long_blocks + a.plan[kApShort + 1] * a.kv_heads * short_per;
+  for (int u = blockIdx.x; u < blocks; u += gridDim.x) {
+    if (u < long_blocks) {
+      const int tile = u / long_per;
+      const int join = tile / a.kv_heads;
+      join_rows<T, D, join_block(D, 1)>(a, 1, join, tile - join * a.kv_heads, u - tile * long_per, os, ls);
+    } else {
+      const int tile = (u - long_blocks) / short_per;
+      const int join = tile / a.kv_heads;
+      join_rows<T, D, join_block(D, 0)>(a, 0, join, tile - join * a.kv_heads, u - long_blocks - tile * short_per, os, ls);
+      lds_barrier();  // before the next block's sums go where these were read
+    }
   }
 }
 
@@ -619,8 +639,8 @@ hipError_t launch(const PagedAttnArgs& a, int max_rows, hipStream_t stream) {
   // Row blocks of a tile that hold rows at all.
   const int long_per = cdiv(std::min(many.bm, max_rows), join_block(D, 1));
   const int short_per = cdiv(std::min(few.bm, max_rows), join_block(D, 0));
-  const int64_t long_blocks = static_cast<int64_t>(many.join_cap) * a.kv_heads * long_per;
-  const int64_t joins = long_blocks + static_cast<int64_t>(few.join_cap) * a.kv_heads * short_per;
+  const int64_t joins = static_cast<int64_t>(many.join_cap) * a.kv_heads * long_per +
+                        static_cast<int64_t>(few.join_cap) * a.kv_heads * short_per;
   if (!grid_fits(blocks) || !grid_fits(joins)) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(blocks));
   if (many.item_cap > 0)
@@ -631,8 +651,8 @@ hipError_t launch(const PagedAttnArgs& a, int max_rows, hipStream_t stream) {
     hipLaunchKernelGGL((paged_short_kernel<T, D, 4, 2>), grid, dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || joins == 0) return e;
-  hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(static_cast<unsigned>(joins)), dim3(256), 0, stream, a,
-                     static_cast<int>(long_blocks), long_per, short_per);
+  hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(static_cast<unsigned>(std::min<int64_t>(joins, kJoinGrid))), dim3(256), 0,
+                     stream, a, long_per, short_per);
   return hipGetLastError();
 }
 
