@@ -6,7 +6,7 @@
 
 namespace mlora {
 
-inline int cdiv(int a, int b) { return (a + b - 1) / b; }
+__host__ __device__ inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 
 // A launch's work-items per grid dimension must fit in 32 bits: at most this
 // many 256-thread workgroups.  Launchers return hipErrorInvalidConfiguration

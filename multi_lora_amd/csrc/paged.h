@@ -18,6 +18,7 @@ namespace mlora {
 constexpr int kApHeaderWords = 16;
 constexpr int kApShort = 0;      // items; joins (tiles whose range is split) in the next word
 constexpr int kApLong = 2;       // the same
+constexpr int kApJoinRows = 4;   // most rows of a split short tile
 constexpr int kApItemWords = 8;  // request, first row, first position, end, slot (-1: none)
 constexpr int kApJoinWords = 4;  // request, first row, first slot, slots
 

@@ -96,6 +96,7 @@ __device__ __forceinline__ int table_room(const TablesArgs& a) {
 __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a) {
   __shared__ int tmp[4][kScanWaves];
   __shared__ unsigned long long wide[4];
+  __shared__ int join_rows;
   int32_t* freed0 = a.scratch + kTsArrays;
   int32_t* taken0 = freed0 + a.n;
   int32_t* held0 = taken0 + a.n;
@@ -107,6 +108,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
   const bool plan = a.plan != nullptr;
   const int room = table_room(a);
   if (threadIdx.x < 4) wide[threadIdx.x] = 0;
+  if (threadIdx.x == 4) join_rows = 0;
   int rows = 0, freed = 0, taken = 0;
   unsigned long long work[2] = {0, 0}, count[2] = {0, 0};
   for (int i0 = 0; i0 < a.n; i0 += kScanThreads) {
@@ -200,6 +202,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
     const int at = kind ? split[1] : split[0];
     const int parts = len > at ? (len + at - 1) / at : 1;
     const int items = tiles * parts;
+    if (kind == 0 && parts > 1 && tiles > 0) atomicMax(&join_rows, c * s.rep);
     int v[3] = {kind ? 0 : items, kind ? 0 : (parts > 1 ? items : 0), kind ? 0 : (parts > 1 ? tiles : 0)}, t[3];
     int u[3] = {kind ? items : 0, kind && parts > 1 ? items : 0, kind && parts > 1 ? tiles : 0}, tu[3];
     scan(v, t, tmp);
@@ -216,7 +219,10 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
       base[1][k] += tu[k];
     }
   }
-  if (plan && threadIdx.x < 2) {
+  if (!plan) return;
+  __syncthreads();
+  if (threadIdx.x == 0) a.plan[kApJoinRows] = join_rows;
+  if (threadIdx.x < 2) {
     const int k = threadIdx.x;
     a.plan[(k ? kApLong : kApShort)] = min(k ? base[1][0] : base[0][0], s.kind[k].item_cap);
     a.plan[(k ? kApLong : kApShort) + 1] = min(k ? base[1][2] : base[0][2], s.kind[k].join_cap);

@@ -287,6 +287,12 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, StreamLds<D,
 }
 
 constexpr int kTile = 64;  // positions of a long item's step
+// Chunks from one 1 KB block of a tile (what one load instruction of a wave
+// fills) to the next.  With chunk p of a row at p ^ (two of the row's low bits)
+// and blocks 64 bytes further apart than they are long, the 16 rows that a
+// fragment load takes a chunk of lie in different banks, and all of a lane's
+// addresses are two registers and constants.
+constexpr int kBlock = 68;
 
 // Long items: 128 rows, 32 a wave, over the same 64 positions; K and V^T of a
 // step go straight into LDS, a step ahead, in one of two buffers.  Chunk p of
@@ -294,14 +300,17 @@ constexpr int kTile = 64;  // positions of a long item's step
 // banks.
 template <int D>
 struct TileLds {
-  u32x4 k[2][kTile * D / 8];  // [position][D / 8 chunks]
-  u32x4 v[2][D * kTile / 8];  // [D][8 chunks of positions]
+  u32x4 k[2][kTile * D / 8 / 64 * kBlock];  // [position][D / 8 chunks]
+  u32x4 v[2][D * kTile / 8 / 64 * kBlock];  // [D][8 chunks of positions]
 };
-template <int D>
-__device__ __forceinline__ int k_at(int row, int chunk) {
-  return row * (D / 8) + (chunk ^ (row & (D / 8 - 1)));
+// Chunk index of (row, chunk) in a tile whose rows have CPR chunks.
+template <int CPR>
+__device__ __forceinline__ int swizzle(int row) { return CPR == 16 ? row & 3 : (row >> 1) & 3; }
+template <int CPR>
+__device__ __forceinline__ int chunk_at(int row, int chunk) {
+  constexpr int R = 64 / CPR;  // rows a block
+  return row / R * kBlock + (row & (R - 1)) * CPR + (chunk ^ swizzle<CPR>(row));
 }
-__device__ __forceinline__ int v_at(int row, int chunk) { return row * 8 + (chunk ^ ((row >> 1) & 7)); }
 
 // The softmax's reference of a row is not its largest score so far but one
 // against which no weight is above kOver: weights stay in the data type's range,
@@ -371,8 +380,8 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, TileLds<D>& s,
   // powers of two, so a lane's place inside a page moves with the step's only.
   const int kr0 = wave * (64 / KC) + lane / KC;
   const int vr0 = wave * 8 + (lane >> 3);
-  const int kc = (lane & (KC - 1)) ^ (kr0 & (KC - 1));
-  const int vc = (lane & 7) ^ ((vr0 >> 1) & 7);
+  const int kc = (lane & (KC - 1)) ^ swizzle<KC>(kr0);
+  const int vc = (lane & 7) ^ swizzle<8>(vr0);
   const char* kb = reinterpret_cast<const char*>(a.keys) + (static_cast<int64_t>(head) * page * D + kc * 8) * 2;
   const char* vb = reinterpret_cast<const char*>(a.values) +
                    ((static_cast<int64_t>(head) * D + vr0) * page + (vc * 8 & (page - 1))) * 2;
@@ -385,104 +394,173 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, TileLds<D>& s,
       const int row = j * (256 / KC) + kr0;
       const uint32_t id = __shfl(ids, row, kWave);
       const char* p = kp + (row & (page - 1)) * (D * 2) + static_cast<uint64_t>(id) * kstep;
-      __builtin_amdgcn_global_load_lds((gvoid_t*)p, (lvoid_t*)(&s.k[buf][(j * 4 + wave) * 64]), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gvoid_t*)p, (lvoid_t*)(&s.k[buf][(j * 4 + wave) * kBlock]), 16, 0, 0);
     }
     const char* vp = vb + in_page * 2 + static_cast<uint64_t>(static_cast<uint32_t>(__shfl(ids, vc * 8, kWave))) * vstep;
 #pragma unroll
     for (int j = 0; j < NL; ++j)
       __builtin_amdgcn_global_load_lds((gvoid_t*)(vp + static_cast<int64_t>(j * 32 * 2) * page),
-                                       (lvoid_t*)(&s.v[buf][(j * 4 + wave) * 64]), 16, 0, 0);
+                                       (lvoid_t*)(&s.v[buf][(j * 4 + wave) * kBlock]), 16, 0, 0);
   };
 
   // Row rho of an MFMA tile is position rho with bits 2 and 3 exchanged: a
   // lane's registers 8 s + i are then positions 16 s + 8 h + i.
   const int krow = (col & ~12) | ((col & 4) << 1) | ((col & 8) >> 1);
-  auto step = [&](int base, int buf, auto is_masked) {
-    constexpr bool MASKED = decltype(is_masked)::value;
+  // Fragments: k-step k of positions 32 t + krow, and positions 32 t + 16 z of
+  // V^T's rows 32 d + col.
+  const int ka[2] = {chunk_at<KC>(krow, h), chunk_at<KC>(krow, 2 + h)};
+  const int va[2] = {chunk_at<8>(col, h), chunk_at<8>(col, 2 + h)};
+  auto k_frag = [&](int buf, int t, int k) { return s.k[buf][ka[k & 1] + t * (32 * KC / 64 * kBlock) + (k >> 1) * 4]; };
+  auto v_frag = [&](int buf, int t, int z, int d) { return s.v[buf][va[z] + d * (4 * kBlock) + t * 4]; };
+  auto step = [&](int base, int buf) {
+    const bool masked = base + kTile > open;  // of the wave
     const int seen = min(lim, kv1) - base - h * 8;
-    // S^T of 32 positions x 32 rows.
-    auto scores = [&](int t) {
-      f32x16 sc;
+    u32x4 kf[2][KS], vf[2][DT][2], pf[2];
+    f32x16 p[2];  // of 32 positions each: scores, then weights
+    float top;
+    auto load_k = [&](int t) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[r] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) sc = T::mma32(sc, s.k[buf][k_at<D>(t * 32 + krow, k * 2 + h)], qf[k]);
-      if constexpr (MASKED) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (t * 32 + (r >> 3) * 16 + (r & 7) >= seen) sc[r] = -INFINITY;
-      }
-      return sc;
+      for (int k = 0; k < KS; ++k) kf[t][k] = k_frag(buf, t, k);
     };
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      f32x16 p = scores(t);
-      float top = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] = exp2_fast(__builtin_fmaf(p[r], scale, -ref));
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(top, p[r]), p[r + 1]);
-      if (__any(top > kOver)) {
-        p = scores(t);  // again: the weights took their place
-        float now = p[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) now = fmaxf(now, p[r]);
-        now = fmaxf(now, __shfl_xor(now, 32, kWave)) * scale;
-        now = fmaxf(now, ref);
-        const float keep = exp2_fast(ref - now);
-        ref = now;
-        sum *= keep;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[d][r] *= keep;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = exp2_fast(__builtin_fmaf(p[r], scale, -ref));
-      }
-      u32x4 pf[2];
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) pf[r >> 3][(r & 7) >> 1] = T::pack2(p[r], p[r + 1]);
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) sum += p[r] + p[r + 1];
-      bool any_odd = false;
+    auto load_v = [&](int t) {
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          u32x4 v = s.v[buf][v_at(d * 32 + col, t * 4 + z * 2 + h)];
-          if constexpr (MASKED) {
+        for (int z = 0; z < 2; ++z) vf[t][d][z] = v_frag(buf, t, z, d);
+    };
+    // S^T of 32 positions x 32 rows.
+    auto scores = [&](int t) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t nf = nonfinite_mask<T>(v[i]);
-              any_odd |= nf != 0;
-              v[i] &= ~nf;
-            }
-          }
-          acc[d] = T::mma32(acc[d], v, pf[z]);
-        }
-      if (MASKED && __ballot(any_odd) != 0) {
-        // The values left out: one position's at a time, for the rows that see it.
+      for (int r = 0; r < 16; ++r) p[t][r] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) p[t] = T::mma32(p[t], kf[t][k], qf[k]);
+    };
+    auto hide = [&](int t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (t * 32 + (r >> 3) * 16 + (r & 7) >= seen) p[t][r] = -INFINITY;
+    };
+    auto weights = [&](int t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[t][r] = exp2_fast(__builtin_fmaf(p[t][r], scale, -ref));
+      top = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(top, p[t][r]), p[t][r + 1]);
+    };
+    auto rescale = [&](int t) {
+      // The scores again: the weights took their place.
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[t][r] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) p[t] = T::mma32(p[t], k_frag(buf, t, k), qf[k]);
+      if (masked) {
+        asm volatile("");
+        hide(t);
+      }
+      float now = p[t][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) now = fmaxf(now, p[t][r]);
+      now = fmaxf(now, __shfl_xor(now, 32, kWave)) * scale;
+      now = fmaxf(now, ref);
+      const float keep = exp2_fast(ref - now);
+      ref = now;
+      sum *= keep;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[d][r] *= keep;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[t][r] = exp2_fast(__builtin_fmaf(p[t][r], scale, -ref));
+    };
+    auto pack = [&](int t) {
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) pf[r >> 3][(r & 7) >> 1] = T::pack2(p[t][r], p[t][r + 1]);
+    };
+    auto add_up = [&](int t) {
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) sum += p[t][r] + p[t][r + 1];
+    };
+    auto product = [&](int t) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) acc[d] = T::mma32(acc[d], vf[t][d][z], pf[z]);
+    };
+    auto drop_odd = [&](int t) {
+      bool any = false;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int z = 0; z < 2; ++z)
-#pragma unroll 1
-          for (int e = 0; e < 16; ++e) {
-            const int again = opaque_zero();
-            const bool sees = base + t * 32 + z * 16 + e < min(lim, kv1);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-              const u32x4 v = odd_values<T>(s.v[buf][v_at(d * 32 + col, t * 4 + z * 2 + h) + again], (e >> 3) == h ? e & 7 : -1);
-              if (__ballot((v[0] | v[1] | v[2] | v[3]) != 0) == 0) continue;
-              f32x16 part;
-#pragma unroll
-              for (int r = 0; r < 16; ++r) part[r] = 0.f;
-              part = T::mma32(part, v, pf[z]);
-              if (sees)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[d][r] += part[r];
-            }
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t nf = nonfinite_mask<T>(vf[t][d][z][i]);
+            any |= nf != 0;
+            vf[t][d][z][i] &= ~nf;
           }
-      }
+      return __ballot(any) != 0;
+    };
+    // The values left out: one position's at a time, for the rows that see it.
+    auto add_odd = [&](int t) {
+#pragma unroll
+      for (int z = 0; z < 2; ++z)
+#pragma unroll 1
+        for (int e = 0; e < 16; ++e) {
+          const int again = opaque_zero();
+          const bool sees = base + t * 32 + z * 16 + e < min(lim, kv1);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const u32x4 v = odd_values<T>(v_frag(buf, t + again, z, d), (e >> 3) == h ? e & 7 : -1);
+            if (__ballot((v[0] | v[1] | v[2] | v[3]) != 0) == 0) continue;
+            f32x16 part;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) part[r] = 0.f;
+            part = T::mma32(part, v, pf[z]);
+            if (sees)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) acc[d][r] += part[r];
+          }
+        }
+    };
+    bool odd = false;
+
+    // The second half's scores come before the first half's weights, and the
+    // first half's product before the second's weights: matrix and vector
+    // instructions that do not wait for each other stand next to each other.
+    load_k(0);
+    load_k(1);
+    scores(0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (masked) {
+      asm volatile("");
+      hide(0);
     }
+    load_v(0);
+    scores(1);
+    weights(0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (__any(top > kOver)) rescale(0);
+    if (masked) {
+      asm volatile("");
+      hide(1);
+      odd = drop_odd(0);
+    }
+    pack(0);
+    if (odd) add_odd(0);
+    product(0);
+    weights(1);
+    add_up(0);
+    load_v(1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (__any(top > kOver)) rescale(1);
+    if (masked) {
+      asm volatile("");
+      odd = drop_odd(1);
+    }
+    pack(1);
+    if (odd) add_odd(1);
+    product(1);
+    add_up(1);
   };
 
   uint32_t ids = 0;
@@ -499,11 +577,7 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, TileLds<D>& s,
       ids = load_ids(base + 2 * kTile);
     }
     __builtin_amdgcn_sched_barrier(0);  // the next step's loads go out before this one's products
-    if (!live || base >= shut) continue;
-    if (__builtin_expect(base + kTile > open, 0))
-      step(base, buf, std::true_type{});
-    else
-      step(base, buf, std::false_type{});
+    if (live && base < shut) step(base, buf);
   }
 
   sum += __shfl_xor(sum, 32, kWave);
@@ -613,9 +687,10 @@ constexpr int join_block(int d, int kind) { return kind ? 1024 / d : 256 / d; } 
 // Workgroups take the row blocks in turn: the host's bound on them is many
 // times what most steps have, and starting that many idle ones cost 10 us.
 template <class T, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int long_per, int short_per) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int long_per) {
   __shared__ f32x4 os[256];
   __shared__ float ls[256];
+  const int short_per = cdiv(a.plan[kApJoinRows], join_block(D, 0));
   const int long_blocks = a.plan[kApLong + 1] * a.kv_heads * long_per;
   const int blocks = long_blocks + a.plan[kApShort + 1] * a.kv_heads * short_per;
   for (int u = blockIdx.x; u < blocks; u += gridDim.x) {
@@ -638,9 +713,8 @@ hipError_t launch(const PagedAttnArgs& a, int max_rows, hipStream_t stream) {
   const int64_t blocks = (static_cast<int64_t>(few.item_cap) + many.item_cap) * a.kv_heads;
   // Row blocks of a tile that hold rows at all.
   const int long_per = cdiv(std::min(many.bm, max_rows), join_block(D, 1));
-  const int short_per = cdiv(std::min(few.bm, max_rows), join_block(D, 0));
   const int64_t joins = static_cast<int64_t>(many.join_cap) * a.kv_heads * long_per +
-                        static_cast<int64_t>(few.join_cap) * a.kv_heads * short_per;
+                        static_cast<int64_t>(few.join_cap) * a.kv_heads * cdiv(std::min(few.bm, max_rows), join_block(D, 0));
   if (!grid_fits(blocks) || !grid_fits(joins)) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(blocks));
   if (many.item_cap > 0)
@@ -652,7 +726,7 @@ hipError_t launch(const PagedAttnArgs& a, int max_rows, hipStream_t stream) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || joins == 0) return e;
   hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3(static_cast<unsigned>(std::min<int64_t>(joins, kJoinGrid))), dim3(256), 0,
-                     stream, a, long_per, short_per);
+                     stream, a, long_per);
   return hipGetLastError();
 }
 
