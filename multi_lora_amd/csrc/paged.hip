@@ -409,7 +409,7 @@ bool paged_shape(int n, int rows, int max_new, int64_t max_kv, int heads, int kv
   s->target = 2 * cus;
   const int64_t most = static_cast<int64_t>(std::min(max_new, rows)) * s->rep;  // rows of one request
   const int64_t all = static_cast<int64_t>(rows) * s->rep;
-  s->kind[0].bm = most <= 16 ? 16 : 32;
+  s->kind[0].bm = most <= 16 || most > 32 ? 16 : 32;
   s->kind[1].bm = kApLongRows;
   size_t words = kApHeaderWords, bytes = 0;
   for (int k = 0; k < 2; ++k) {

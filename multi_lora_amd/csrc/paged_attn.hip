@@ -117,7 +117,7 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, StreamLds<D,
   if (!load_item(a, a.shape.kind[0], kApShort, item, &it)) return;
   const int row0 = it.row0, rows = it.rows, past = it.past, kv0 = it.kv0, kv1 = it.kv1;
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15;
   const int g = lane >> 4;
   const int page = 1 << a.page_shift;
@@ -152,25 +152,65 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, StreamLds<D,
   }
 
   const int ka = (col >> 2) * 8 + (col & 3);  // position of K row `col` of the first tile; the second's is 4 on
-  for (int base = kv0 + wave * kPos; base < kv1; base += NW * kPos) {
-    // Pages of the chunk of positions this lane loads keys and values of.
-    // Chunks past the range read page 0 (their scores are masked).
-    const int kp = base + ka, vp = base + g * 8;
-    int kid = kp < kv1 ? table[min(kp >> a.page_shift, a.width - 1)] : 0;
-    int vid = vp < kv1 ? table[min(vp >> a.page_shift, a.width - 1)] : 0;
-    const bool missing = vid < 0 || vid >= a.num_pages;
-    if (missing) vid = 0;
-    if (kid < 0 || kid >= a.num_pages) kid = 0;
-    const raw* kr = keys + static_cast<int64_t>(kid) * a.key_stride + static_cast<int64_t>(kp & (page - 1)) * D + g * 8;
-    const raw* vr = values + static_cast<int64_t>(vid) * a.value_stride + static_cast<int64_t>(col) * page + (vp & (page - 1));
-    u32x4 kf[2][KS], vf[DT];
+  u32x4 kf[2][KS], vf[DT];
+  // Pages of the chunks of positions that this lane loads keys and values of.
+  // Chunks past the range read page 0 (their scores are masked).
+  auto key_page = [&](int base) {
+    const int p = base + ka;
+    return p < kv1 ? table[min(p >> a.page_shift, a.width - 1)] : 0;
+  };
+  auto value_page = [&](int base) {
+    const int p = base + g * 8;
+    return p < kv1 ? table[min(p >> a.page_shift, a.width - 1)] : 0;
+  };
+  auto in_pool = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.num_pages); };
+  auto load_keys = [&](int base, int id) {
+    const raw* k = keys + static_cast<int64_t>(in_pool(id) ? id : 0) * a.key_stride +
+                   static_cast<int64_t>((base + ka) & (page - 1)) * D + g * 8;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      kf[0][k] = ld_chunk(kr + k * 32);
-      kf[1][k] = ld_chunk(kr + 4 * D + k * 32);
+    for (int i = 0; i < KS; ++i) {
+      kf[0][i] = ld_chunk(k + i * 32);
+      kf[1][i] = ld_chunk(k + 4 * D + i * 32);
     }
+  };
+  auto value_rows = [&](int base, int id) {
+    return values + static_cast<int64_t>(in_pool(id) ? id : 0) * a.value_stride + static_cast<int64_t>(col) * page +
+           ((base + g * 8) & (page - 1));
+  };
+  auto load_values = [&](const raw* v) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d) vf[d] = ld_chunk(vr + static_cast<int64_t>(d) * 16 * page);
+    for (int d = 0; d < DT; ++d) vf[d] = ld_chunk(v + static_cast<int64_t>(d) * 16 * page);
+  };
+
+  // Keys of the next tile are asked for as soon as this one's are used, values
+  // likewise, so that each is in flight for half of a tile's work at least.
+  int base = kv0 + wave * kPos;
+  int kid = 0, vid = 0;
+  const raw* vr = values;
+  if (base < kv1) {
+    kid = key_page(base);
+    vid = value_page(base);
+    load_keys(base, kid);
+    vr = value_rows(base, vid);
+    load_values(vr);
+    kid = key_page(base + NW * kPos);
+  }
+  for (; base < kv1; base += NW * kPos) {
+    const bool more = base + NW * kPos < kv1;
+    const bool missing = !in_pool(vid);
+    vid = value_page(base + NW * kPos);
+    f32x4 sc[MT][2];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      sc[t][0] = sc[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        sc[t][0] = T::mma(sc[t][0], kf[0][k], qf[t][k]);
+        sc[t][1] = T::mma(sc[t][1], kf[1][k], qf[t][k]);
+      }
+    }
+    if (more) load_keys(base + NW * kPos, kid);
+    kid = key_page(base + 2 * NW * kPos);
     const bool masked = base + kPos > min(open, kv1);  // wave-uniform
     bool any_odd = false;  // a value of the tile is not finite
     if (masked) {
@@ -186,19 +226,13 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, StreamLds<D,
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      f32x4 sc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        sc[0] = T::mma(sc[0], kf[0][k], qf[t][k]);
-        sc[1] = T::mma(sc[1], kf[1][k], qf[t][k]);
-      }
       // Lane (col, g): positions base + 8 g + i of row t * 16 + col.
       float p[8];
       const int seen = min(lim[t], kv1) - (base + g * 8);
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        p[i] = sc[i >> 2][i & 3] * a.scale_log2;
+        p[i] = sc[t][i >> 2][i & 3] * a.scale_log2;
         if (masked && i >= seen) p[i] = -INFINITY;
         top = fmaxf(top, p[i]);
       }
@@ -240,6 +274,10 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, StreamLds<D,
           }
         }
       }
+    }
+    if (more) {
+      vr = value_rows(base + NW * kPos, vid);
+      load_values(vr);
     }
   }
 
@@ -617,14 +655,14 @@ template <class T, int D>
 __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(PagedAttnArgs a, int long_items) {
   __shared__ union {
     TileLds<D> tile;
-    StreamLds<D, 4, 2> stream;
+    StreamLds<D, 4, 1> stream;
   } s;
   const int item = blockIdx.x / a.kv_heads;
   const int head = blockIdx.x - item * a.kv_heads;
   if (item < long_items)
     tile_item<T, D>(a, s.tile, item, head);
   else
-    stream_item<T, D, 4, 2>(a, s.stream, item - long_items, head);
+    stream_item<T, D, 4, 1>(a, s.stream, item - long_items, head);
 }
 
 // The parts of a split tile: workgroup = (tile, key head, block of RB rows),
