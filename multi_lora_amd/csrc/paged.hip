@@ -315,54 +315,67 @@ __global__ __launch_bounds__(256) void tables_fill_kernel(TablesArgs a, int row_
 }
 
 // ------------------------------------------------------------------- write
-// A chunk of 8 table values at p (element index e), as fp32.
-template <class T>
+// A chunk of 8 table values at element e, as fp32.
+template <class T, bool AL>
 __device__ __forceinline__ void rot_chunk(const void* p, int64_t e, bool f32, float* f) {
   if (f32) {
+    const float* t = static_cast<const float*>(p) + e;
+    if constexpr (AL) {
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(t), hi = *reinterpret_cast<const f32x4*>(t + 4);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = static_cast<const float*>(p)[e + i];
+      for (int i = 0; i < 4; ++i) f[i] = lo[i], f[4 + i] = hi[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = t[i];
+    }
   } else {
-    const typename T::raw_t* t = static_cast<const typename T::raw_t*>(p) + e;
+    const u32x4 v = load_row_chunk<T, AL>(static_cast<const typename T::raw_t*>(p), static_cast<int>(e), 8);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = T::to_f32(t[i]);
+    for (int i = 0; i < 8; ++i) f[i] = chunk_elem<T>(v, i);
   }
 }
 
 // Blocks [0, rot_blocks): a thread rotates 8 columns of a head's first half
 // and the 8 they pair with; x * cos + (x rolled by D / 2) * sin in fp32, one
-// rounding.  The rest: a wave takes a row's values of one key head.
+// rounding.  The rest, values: they lie transposed in a page, so a row alone
+// is D stores of 2 bytes.  A wave takes the run of up to 8 rows whose slots
+// fill one 16-byte chunk of a page, if its row is the run's first (others
+// leave), and stores chunks where the run is whole.
 template <class T, int D, bool AL>
 __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a, int rot_blocks) {
   using raw = typename T::raw_t;
   const int page = 1 << a.page_shift;
+  const int64_t slots = static_cast<int64_t>(a.num_pages) << a.page_shift;
   if (static_cast<int>(blockIdx.x) < rot_blocks) {
     constexpr int U = D / 16;  // units a head
     const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     const int per_row = (a.heads + a.kv_heads) * U;
-    const int64_t r = id / per_row;
+    const int r = static_cast<int>(id / per_row);
     if (r >= a.rows) return;
-    const int u = static_cast<int>(id - r * per_row);
+    const int u = static_cast<int>(id - static_cast<int64_t>(r) * per_row);
     const int h = u / U;
     const int e = (u - h * U) * 8;
     const bool is_q = h < a.heads;
     const raw* x = is_q ? static_cast<const raw*>(a.q) + r * a.q_stride + h * D
                         : static_cast<const raw*>(a.k) + r * a.k_stride + (h - a.heads) * D;
+    const u32x4 lo = load_row_chunk<T, AL>(x, e, 8);
+    const u32x4 hi = load_row_chunk<T, AL>(x, e + D / 2, 8);
+    float c0[8], c1[8], s0[8], s1[8], y0[8], y1[8];
+    const char* cs = static_cast<const char*>(a.cos) + r * a.rot_stride * (a.rot_f32 ? 4 : 2);
+    const char* sn = static_cast<const char*>(a.sin) + r * a.rot_stride * (a.rot_f32 ? 4 : 2);
+    rot_chunk<T, AL>(cs, e, a.rot_f32, c0);
+    rot_chunk<T, AL>(cs, e + D / 2, a.rot_f32, c1);
+    rot_chunk<T, AL>(sn, e, a.rot_f32, s0);
+    rot_chunk<T, AL>(sn, e + D / 2, a.rot_f32, s1);
     raw* to;
     if (is_q) {
       to = static_cast<raw*>(a.q_out) + r * a.q_out_stride + h * D;
     } else {
       const int slot = a.slots[r];
-      if (slot < 0 || (slot >> a.page_shift) >= a.num_pages) return;
+      if (slot < 0 || slot >= slots) return;
       to = static_cast<raw*>(a.keys) + static_cast<int64_t>(slot >> a.page_shift) * a.key_stride +
            (static_cast<int64_t>(h - a.heads) * page + (slot & (page - 1))) * D;
     }
-    const u32x4 lo = load_row_chunk<T, AL>(x, e, 8);
-    const u32x4 hi = load_row_chunk<T, AL>(x, e + D / 2, 8);
-    float c0[8], c1[8], s0[8], s1[8], y0[8], y1[8];
-    rot_chunk<T>(a.cos, r * a.rot_stride + e, a.rot_f32, c0);
-    rot_chunk<T>(a.cos, r * a.rot_stride + e + D / 2, a.rot_f32, c1);
-    rot_chunk<T>(a.sin, r * a.rot_stride + e, a.rot_f32, s0);
-    rot_chunk<T>(a.sin, r * a.rot_stride + e + D / 2, a.rot_f32, s1);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float x0 = chunk_elem<T>(lo, i), x1 = chunk_elem<T>(hi, i);
@@ -374,15 +387,36 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a, int rot_b
     return;
   }
   const int64_t w = (static_cast<int64_t>(blockIdx.x) - rot_blocks) * 4 + (threadIdx.x >> 6);
-  const int64_t r = w / a.kv_heads;
+  const int r = static_cast<int>(w / a.kv_heads);
   if (r >= a.rows) return;
-  const int g = static_cast<int>(w - r * a.kv_heads);
-  const int slot = a.slots[r];
-  if (slot < 0 || (slot >> a.page_shift) >= a.num_pages) return;
+  const int g = static_cast<int>(w - static_cast<int64_t>(r) * a.kv_heads);
+  const int lane = threadIdx.x & 63;
+  // Lane l looks at row r - 1 + l: is row r the first of its run, and how long is that?
+  const int look = r - 1 + lane;
+  const int seen = lane <= 8 && look >= 0 && look < a.rows ? a.slots[look] : -2;
+  const int slot = __builtin_amdgcn_readlane(seen, 1);
+  if (slot < 0 || slot >= slots) return;
+  if ((slot & 7) != 0 && __builtin_amdgcn_readlane(seen, 0) == slot - 1) return;  // in another row's run
+  const int room = 8 - (slot & 7);
+  const uint64_t next = __ballot(lane >= 1 && lane <= room && seen == slot + lane - 1) >> 1;
+  const int run = __builtin_amdgcn_readfirstlane(__builtin_ctzll(~next));  // rows r .. r + run - 1
   const raw* v = static_cast<const raw*>(a.v) + r * a.v_stride + g * D;
   raw* to = static_cast<raw*>(a.values) + static_cast<int64_t>(slot >> a.page_shift) * a.value_stride +
             static_cast<int64_t>(g) * D * page + (slot & (page - 1));
-  for (int e = threadIdx.x & 63; e < D; e += kWave) to[static_cast<int64_t>(e) * page] = v[e];
+  if (AL && run == 8) {
+#pragma unroll
+    for (int e0 = 0; e0 < D; e0 += kWave) {
+      const int e = e0 + lane;
+      u32x4 c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        c[i] = static_cast<uint32_t>(v[2 * i * a.v_stride + e]) | static_cast<uint32_t>(v[(2 * i + 1) * a.v_stride + e]) << 16;
+      st_chunk(to + static_cast<int64_t>(e) * page, c);
+    }
+    return;
+  }
+  for (int i = 0; i < run; ++i)
+    for (int e = lane; e < D; e += kWave) to[static_cast<int64_t>(e) * page + i] = v[i * a.v_stride + e];
 }
 
 template <class T, int D>

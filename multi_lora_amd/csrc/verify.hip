@@ -12,7 +12,8 @@
 //
 // Two launches, for one row's sums are needed before its draw: a workgroup
 // per 4096 columns of a request's row, which finds the row itself, then a
-// workgroup per request that reads the one chunk its draw falls in.
+// workgroup per request that reads the one chunk its draw falls in.  Rows of
+// one chunk are one launch.
 #include "kernels.h"
 #include "loads.h"
 #include "paged.h"
@@ -28,29 +29,35 @@ struct Row {
   bool live;      // the request has rows in this call
 };
 
-// Every wave finds the row for itself, 64 drafts at a time.
+// Every wave finds the row for itself, 64 drafts at a time.  The drafts and
+// their numbers are asked for together with the row numbers, the two
+// probabilities together: two round trips to memory, not four.
 template <class T>
 __device__ Row find_row(const VerifyArgs& a, int i) {
   using raw = typename T::raw_t;
+  const int lane = threadIdx.x & 63;
+  int64_t x = lane < a.most ? a.tokens[i * a.token_stride + lane] : -1;
+  float u = lane < a.most ? a.accept[i * a.accept_stride + lane] : 0.f;
   const int first = min(max(a.row_indptr[i], 0), a.rows);
   const int end = min(max(a.row_indptr[i + 1], first), a.rows);
   const int k = min(end - first - 1, a.most);
   Row r{0, false, -1, end > first};
-  const int lane = threadIdx.x & 63;
   for (int j0 = 0; j0 < k; j0 += kWave) {
     const int j = j0 + lane;
-    bool no = false;
-    int64_t x = -1;
-    if (j < k) {
+    if (j0 > 0 && j < k) {
       x = a.tokens[i * a.token_stride + j];
+      u = a.accept[i * a.accept_stride + j];
+    }
+    bool no = false;
+    if (j < k) {
       no = true;
       if (x >= 0 && x < a.vocab) {
-        const double p = T::to_f32(static_cast<const raw*>(a.target)[(first + j) * a.target_stride + x]);
-        const double q = a.draft == nullptr
-                             ? 1.0
-                             : static_cast<double>(T::to_f32(static_cast<const raw*>(
-                                   a.draft)[i * a.draft_stride0 + j * a.draft_stride1 + x]));
-        no = !(static_cast<double>(a.accept[i * a.accept_stride + j]) * q < p);
+        const raw p = static_cast<const raw*>(a.target)[(first + j) * a.target_stride + x];
+        const raw q = a.draft == nullptr
+                          ? raw{}
+                          : static_cast<const raw*>(a.draft)[i * a.draft_stride0 + j * a.draft_stride1 + x];
+        const double qd = a.draft == nullptr ? 1.0 : static_cast<double>(T::to_f32(q));
+        no = !(static_cast<double>(u) * qd < static_cast<double>(T::to_f32(p)));
       }
     }
     const uint64_t hit = __ballot(no);
@@ -166,72 +173,84 @@ struct DrawLds {
   int hit, last;
 };
 
-template <class T>
+// Workgroup = request.  ONE: the row is a single chunk, and this is the only
+// launch.
+template <class T, bool ONE>
 __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
   using raw = typename T::raw_t;
   __shared__ DrawLds s;
   const int i = blockIdx.x;
   const int tid = threadIdx.x;
-  // The row, from the first launch's count.
-  const int first = min(max(a.row_indptr[i], 0), a.rows);
-  const int end = min(max(a.row_indptr[i + 1], first), a.rows);
-  Row r{a.accepted[i], false, -1, end > first};
-  r.rejected = r.accepted < min(end - first - 1, a.most);
-  if (r.rejected) r.token = a.tokens[i * a.token_stride + r.accepted];
+  Row r;
+  if constexpr (ONE) {
+    r = find_row<T>(a, i);
+    if (tid == 0) a.accepted[i] = r.accepted;
+  } else {  // from the first launch's count
+    const int first = min(max(a.row_indptr[i], 0), a.rows);
+    const int end = min(max(a.row_indptr[i + 1], first), a.rows);
+    r = Row{a.accepted[i], false, -1, end > first};
+    r.rejected = r.accepted < min(end - first - 1, a.most);
+    if (r.rejected) r.token = a.tokens[i * a.token_stride + r.accepted];
+  }
   int64_t* out = a.out + static_cast<int64_t>(i) * (a.most + 1);
   for (int j = tid; j <= a.most; j += 256)
     if (j != r.accepted || !r.live) out[j] = r.live && j < r.accepted ? a.tokens[i * a.token_stride + j] : -1;
   if (!r.live) return;
-
-  // The chunk that the draw falls in; a thread takes `per` neighbouring ones.
-  const double* sums = a.sums + static_cast<int64_t>(i) * a.chunks * 2;
-  const int per = (a.chunks + 255) / 256;
-  const int c0 = tid * per, c1 = min(c0 + per, a.chunks);
-  double rest = 0.0, full = 0.0, total_rest, total_full;
-  for (int c = c0; c < c1; ++c) {
-    rest += sums[c * 2];
-    full += sums[c * 2 + 1];
-  }
   if (tid == 0) {
     s.hit = INT32_MAX;
     s.last = -1;
   }
-  const double rest0 = scan256(rest, s.tmp, &total_rest);
-  const double full0 = scan256(full, s.tmp, &total_full);
-  const int use = total_rest > 0.0 ? 0 : 1;
-  const double want = static_cast<double>(a.last[i]) * (use == 0 ? total_rest : total_full);
-  double cum = use == 0 ? rest0 : full0;
-  int hit = INT32_MAX, last = -1;
-  double before = 0.0;
-  for (int c = c0; c < c1; ++c) {
-    const double m = sums[c * 2 + use];
-    if (m > 0.0) {
-      last = c;
-      if (hit == INT32_MAX && cum + m > want) {
-        hit = c;
-        before = cum;
-      }
+  int chunk = 0, use = 0;
+  double before = 0.0, want = 0.0;
+  if constexpr (!ONE) {
+    // The chunk that the draw falls in; a thread takes `per` neighbouring ones.
+    const double* sums = a.sums + static_cast<int64_t>(i) * a.chunks * 2;
+    const int per = (a.chunks + 255) / 256;
+    const int c0 = tid * per, c1 = min(c0 + per, a.chunks);
+    double rest = 0.0, full = 0.0, total_rest, total_full;
+    for (int c = c0; c < c1; ++c) {
+      rest += sums[c * 2];
+      full += sums[c * 2 + 1];
     }
-    cum += m;
-  }
-  if (hit != INT32_MAX) atomicMin(&s.hit, hit);
-  if (last >= 0) atomicMax(&s.last, last);
-  __syncthreads();
-  int chunk = s.hit;
-  if (chunk == hit && hit != INT32_MAX) s.before = before;
-  if (chunk == INT32_MAX) {  // a number of 1 or more: the last column with mass
-    chunk = s.last;
-    if (tid == 0) s.before = -INFINITY;
-  }
-  __syncthreads();
-  before = s.before;
-  if (chunk < 0) {
-    if (tid == 0) out[r.accepted] = -1;
-    return;
-  }
-  if (tid == 0) {
-    s.hit = INT32_MAX;
-    s.last = -1;
+    double cum = scan256(rest, s.tmp, &total_rest);
+    want = static_cast<double>(a.last[i]) * total_rest;
+    if (!(total_rest > 0.0)) {
+      cum = scan256(full, s.tmp, &total_full);
+      use = 1;
+      want = static_cast<double>(a.last[i]) * total_full;
+    }
+    int hit = INT32_MAX, last = -1;
+    double here = 0.0;
+    for (int c = c0; c < c1; ++c) {
+      const double m = sums[c * 2 + use];
+      if (m > 0.0) {
+        last = c;
+        if (hit == INT32_MAX && cum + m > want) {
+          hit = c;
+          here = cum;
+        }
+      }
+      cum += m;
+    }
+    if (hit != INT32_MAX) atomicMin(&s.hit, hit);
+    if (last >= 0) atomicMax(&s.last, last);
+    __syncthreads();
+    chunk = s.hit;
+    if (chunk == hit && hit != INT32_MAX) s.before = here;
+    if (chunk == INT32_MAX) {  // a number of 1 or more: the last column with mass
+      chunk = s.last;
+      if (tid == 0) s.before = -INFINITY;
+    }
+    __syncthreads();
+    before = s.before;
+    if (chunk < 0) {
+      if (tid == 0) out[r.accepted] = -1;
+      return;
+    }
+    if (tid == 0) {
+      s.hit = INT32_MAX;
+      s.last = -1;
+    }
   }
   const raw *p, *q;
   row_ptrs<T>(a, r, i, &p, &q);
@@ -243,8 +262,27 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
 #pragma unroll
     for (int e = 0; e < kPer; ++e) qv[e] = q[min(x0 + e, a.vocab - 1)];
   }
+  if constexpr (ONE) {
+    double rest = 0.0, full = 0.0, total_rest, total_full;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      double re, fu;
+      column<T>(r, pv[e], q != nullptr, qv[e], x0 + e, &re, &fu);
+      if (x0 + e < a.vocab) {
+        rest += re;
+        full += fu;
+      }
+    }
+    (void)scan256(rest, s.tmp, &total_rest);
+    want = static_cast<double>(a.last[i]) * total_rest;
+    if (!(total_rest > 0.0)) {
+      (void)scan256(full, s.tmp, &total_full);
+      use = 1;
+      want = static_cast<double>(a.last[i]) * total_full;
+    }
+  }
   double m[kPer], mine = 0.0, total;
-  last = -1;
+  int hit = INT32_MAX, last = -1;
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     double re, fu;
@@ -253,8 +291,7 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
     if (m[e] > 0.0) last = x0 + e;
     mine += m[e];
   }
-  cum = before + scan256(mine, s.tmp, &total);
-  hit = INT32_MAX;
+  double cum = before + scan256(mine, s.tmp, &total);
 #pragma unroll
   for (int e = 0; e < kPer; ++e) {
     cum += m[e];
@@ -263,17 +300,21 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
   if (hit != INT32_MAX) atomicMin(&s.hit, hit);
   if (last >= 0) atomicMax(&s.last, last);
   __syncthreads();
-  if (tid == 0) out[r.accepted] = s.hit != INT32_MAX ? s.hit : s.last;
+  if (tid == 0) out[r.accepted] = s.hit != INT32_MAX ? s.hit : s.last;  // no mass at all: -1
 }
 
 template <class T>
 hipError_t launch(const VerifyArgs& a, hipStream_t stream) {
   const int64_t blocks = static_cast<int64_t>(a.n) * a.chunks;
   if (!grid_fits(blocks)) return hipErrorInvalidConfiguration;
+  if (a.chunks == 1) {
+    hipLaunchKernelGGL((verify_draw_kernel<T, true>), dim3(static_cast<unsigned>(a.n)), dim3(256), 0, stream, a);
+    return hipGetLastError();
+  }
   hipLaunchKernelGGL((verify_sum_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((verify_draw_kernel<T>), dim3(static_cast<unsigned>(a.n)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((verify_draw_kernel<T, false>), dim3(static_cast<unsigned>(a.n)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
