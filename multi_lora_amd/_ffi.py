@@ -279,7 +279,8 @@ def lib() -> ctypes.CDLL:
 _CALLS_FUNCTIONS = ("mlora_last_error", "mlora_shrink_workspace_bytes", "mlora_shrink", "mlora_expand",
                     "mlora_apply_segments_workspace_bytes", "mlora_apply_segments", "mlora_rmsnorm",
                     "mlora_add_rmsnorm", "mlora_grouped_workspace_bytes", "mlora_apply_grouped",
-                    "mlora_rmsnorm_apply_grouped")
+                    "mlora_rmsnorm_apply_grouped", "mlora_page_tables", "mlora_rotary_paged_write",
+                    "mlora_paged_attention", "mlora_verify_workspace_bytes", "mlora_verify_drafts")
 _calls_module = None
 
 

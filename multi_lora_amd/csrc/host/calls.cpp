@@ -18,7 +18,12 @@
 #include <hip/hip_runtime.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <ATen/core/grad_mode.h>
+#include <c10/core/InferenceMode.h>
+#include <c10/hip/HIPFunctions.h>
+
 #include <algorithm>
+#include <initializer_list>
 
 #include "../../../include/mlora_hip.h"
 
@@ -38,6 +43,11 @@ struct Library {
   decltype(&mlora_rmsnorm_apply_grouped) rmsnorm_grouped;
   decltype(&mlora_rmsnorm) rmsnorm;
   decltype(&mlora_add_rmsnorm) add_rmsnorm;
+  decltype(&mlora_page_tables) page_tables;
+  decltype(&mlora_rotary_paged_write) paged_write;
+  decltype(&mlora_paged_attention) paged_attention;
+  decltype(&mlora_verify_workspace_bytes) verify_ws;
+  decltype(&mlora_verify_drafts) verify;
 };
 Library lib{};
 PyObject* launch_error = nullptr;  // exception type of a failed launch
@@ -484,6 +494,216 @@ PyObject* norm(PyObject* px, PyObject* pres, PyObject* pw, PyObject* peps, Took*
   return *took == Took::kYes ? THPVariable_Wrap(std::move(out)) : nullptr;
 }
 
+// ---- paged KV cache (kernels/paged.py)
+
+// What PagedStep._native holds: addresses of its C structs and of the tables'
+// scratch, and its heads.  The step keeps what they point into.
+struct Step {
+  const mlora_pages* pages;
+  const mlora_paged_step* step;
+  int32_t* scratch;
+  int32_t heads, kv_heads, head_dim;
+  int device;
+
+  bool read(PyObject* t) {
+    if (!PyTuple_CheckExact(t) || PyTuple_GET_SIZE(t) != 7) return false;
+    void* p[3];
+    for (int i = 0; i < 3; ++i) p[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(t, i));
+    long n[4];
+    for (int i = 0; i < 4; ++i) n[i] = PyLong_AsLong(PyTuple_GET_ITEM(t, 3 + i));
+    if (PyErr_Occurred() || p[0] == nullptr || p[1] == nullptr) return false;
+    pages = static_cast<const mlora_pages*>(p[0]);
+    step = static_cast<const mlora_paged_step*>(p[1]);
+    scratch = static_cast<int32_t*>(p[2]);
+    heads = static_cast<int32_t>(n[0]), kv_heads = static_cast<int32_t>(n[1]), head_dim = static_cast<int32_t>(n[2]);
+    device = static_cast<int>(n[3]);
+    return true;
+  }
+};
+
+bool is_current(at::Device dev) { return dev.is_cuda() && dev.index() == c10::hip::current_device(); }
+
+bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->requires_grad()) return true;
+  return false;
+}
+
+bool is_i32(const at::Tensor* t, at::Device dev, int64_t n) {
+  return t != nullptr && t->scalar_type() == at::kInt && t->device() == dev && t->dim() == 1 && t->size(0) == n && t->is_contiguous();
+}
+
+// Rows [rows, cols] of the type on the device, columns next to each other.
+bool is_rows_of(const at::Tensor* t, at::Device dev, at::ScalarType st, int64_t rows, int64_t cols) {
+  return t != nullptr && t->scalar_type() == st && t->device() == dev && t->dim() == 2 && t->size(0) == rows &&
+         t->size(1) == cols && t->stride(1) == 1 && (rows <= 1 || t->stride(0) >= cols);
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// One layer's pools, pages contiguous.
+struct Pool {
+  int64_t pages, kv_heads, page, d, key_stride, value_stride;
+  bool read(const at::Tensor* k, const at::Tensor* v) {
+    if (k == nullptr || v == nullptr || k->dim() != 4 || v->dim() != 4 || !k->is_cuda() || v->device() != k->device()) return false;
+    if ((k->scalar_type() != at::kBFloat16 && k->scalar_type() != at::kHalf) || v->scalar_type() != k->scalar_type()) return false;
+    pages = k->size(0), kv_heads = k->size(1), page = k->size(2), d = k->size(3);
+    if (pages < 1 || !fits_i32(pages) || v->size(0) != pages || v->size(1) != kv_heads || v->size(2) != d || v->size(3) != page) return false;
+    if (k->stride(3) != 1 || k->stride(2) != d || k->stride(1) != page * d) return false;
+    if (v->stride(3) != 1 || v->stride(2) != page || v->stride(1) != page * d) return false;
+    key_stride = pages > 1 ? k->stride(0) : kv_heads * page * d;
+    value_stride = pages > 1 ? v->stride(0) : kv_heads * page * d;
+    return true;
+  }
+};
+
+// kernels.paged.page_tables into a step.
+Took page_tables(PyObject* const* args) {
+  Step st;
+  const at::Tensor *start = tensor_of(args[1]), *add = tensor_of(args[2]);
+  if (!st.read(args[0]) || start == nullptr || add == nullptr || !start->is_cuda()) return Took::kNo;
+  const at::Device dev = start->device();
+  if (!is_current(dev) || dev.index() != st.device || !is_i32(start, dev, st.pages->n) || !is_i32(add, dev, st.pages->n)) return Took::kNo;
+  const hipStream_t stream = stream_of(dev);
+  const int32_t *sp = start->data_ptr<int32_t>(), *ap = add->data_ptr<int32_t>();
+  const int rc = unlocked([&] {
+    return lib.page_tables(st.pages, sp, ap, st.step, st.heads, st.kv_heads, st.head_dim, st.scratch, stream);
+  });
+  return outcome(rc, "mlora_page_tables");
+}
+
+// kernels.paged.paged_attention: the output, new or given.
+PyObject* paged_attention(PyObject* const* args, Took* took) {
+  const at::Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *v = tensor_of(args[2]);
+  Step st;
+  Pool pool;
+  if (q == nullptr || !pool.read(k, v) || !st.read(args[3]) || !PyFloat_CheckExact(args[4])) return nullptr;
+  const at::Device dev = k->device();
+  const at::ScalarType dt = k->scalar_type();
+  const int64_t rows = st.step->rows, width = static_cast<int64_t>(st.heads) * st.head_dim;
+  if (!is_current(dev) || dev.index() != st.device || st.step->plan == nullptr || rows == 0 || wants_grad({q, k, v}) ||
+      !is_rows_of(q, dev, dt, rows, width) || pool.kv_heads != st.kv_heads || pool.d != st.head_dim ||
+      pool.page != st.pages->page || pool.pages < st.pages->num_pages)
+    return nullptr;
+  at::Tensor out;
+  if (args[5] == Py_None) {
+    out = at::empty({rows, width}, q->options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+  } else {
+    const at::Tensor* o = tensor_of(args[5]);
+    if (!is_rows_of(o, dev, dt, rows, width) || wants_grad({o})) return nullptr;
+    out = *o;
+  }
+  const float scale = static_cast<float>(PyFloat_AS_DOUBLE(args[4]));
+  const hipStream_t stream = stream_of(dev);
+  const void *qp = q->data_ptr(), *kp = k->data_ptr(), *vp = v->data_ptr();
+  void* op = out.data_ptr();
+  const int code = dtype_code(dt);
+  const int64_t qs = row_stride(*q), os = row_stride(out);
+  const int rc = unlocked([&] {
+    return lib.paged_attention(qp, qs, kp, pool.key_stride, vp, pool.value_stride, st.pages, st.step, op, os, st.heads,
+                               st.kv_heads, st.head_dim, scale, code, stream);
+  });
+  *took = outcome(rc, "mlora_paged_attention");
+  return *took == Took::kYes ? THPVariable_Wrap(std::move(out)) : nullptr;
+}
+
+// kernels.paged.rotary_paged_write: the rotated q, new or given.
+PyObject* paged_write(PyObject* const* args, Took* took) {
+  const at::Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *v = tensor_of(args[2]), *cs = tensor_of(args[3]),
+                   *sn = tensor_of(args[4]), *kp = tensor_of(args[5]), *vp = tensor_of(args[6]), *slots = tensor_of(args[7]);
+  Pool pool;
+  if (q == nullptr || k == nullptr || v == nullptr || cs == nullptr || sn == nullptr || !pool.read(kp, vp)) return nullptr;
+  const at::Device dev = kp->device();
+  const at::ScalarType dt = kp->scalar_type();
+  if (!is_current(dev) || q->dim() != 2 || q->size(0) == 0 || !fits_i32(q->size(0)) || q->size(1) == 0 || q->size(1) % pool.d != 0)
+    return nullptr;
+  const int64_t rows = q->size(0), heads = q->size(1) / pool.d;
+  if (!is_rows_of(q, dev, dt, rows, heads * pool.d) || !is_rows_of(k, dev, dt, rows, pool.kv_heads * pool.d) ||
+      !is_rows_of(v, dev, dt, rows, pool.kv_heads * pool.d) || !is_i32(slots, dev, rows) ||
+      wants_grad({q, k, v, cs, sn, kp, vp}))
+    return nullptr;
+  if ((kp->is_inference() || vp->is_inference()) && !c10::InferenceMode::is_enabled()) return nullptr;
+  int64_t rot[2];
+  const at::Tensor* tabs[2] = {cs, sn};
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor& t = *tabs[i];
+    const bool three = t.dim() == 3 && t.size(1) == 1;
+    if ((t.dim() != 2 && !three) || t.device() != dev || t.scalar_type() != cs->scalar_type() ||
+        (t.size(0) != rows && t.size(0) != 1) || t.size(-1) != pool.d || t.stride(-1) != 1)
+      return nullptr;
+    rot[i] = t.size(0) == 1 ? 0 : t.stride(0);
+  }
+  if (rot[0] != rot[1] || (cs->scalar_type() != dt && cs->scalar_type() != at::kFloat)) return nullptr;
+  at::Tensor out;
+  if (args[8] == Py_None) {
+    out = at::empty({rows, heads * pool.d}, q->options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+  } else {
+    const at::Tensor* o = tensor_of(args[8]);
+    if (!is_rows_of(o, dev, dt, rows, heads * pool.d) || wants_grad({o})) return nullptr;
+    out = *o;
+  }
+  const hipStream_t stream = stream_of(dev);
+  const void *qd = q->data_ptr(), *kd = k->data_ptr(), *vd = v->data_ptr(), *cd = cs->data_ptr(), *sd = sn->data_ptr();
+  const int32_t* slotd = slots->data_ptr<int32_t>();
+  void *keyd = kp->data_ptr(), *vald = vp->data_ptr(), *od = out.data_ptr();
+  const int64_t qs = row_stride(*q), ks = row_stride(*k), vs = row_stride(*v), os = row_stride(out);
+  const int code = dtype_code(dt), rot_code = dtype_code(cs->scalar_type());
+  const int rc = unlocked([&] {
+    return lib.paged_write(qd, qs, kd, ks, vd, vs, cd, sd, rot[0], rot_code, slotd, static_cast<int32_t>(rows),
+                           static_cast<int32_t>(heads), static_cast<int32_t>(pool.kv_heads), static_cast<int32_t>(pool.d),
+                           keyd, pool.key_stride, vald, pool.value_stride, static_cast<int32_t>(pool.pages),
+                           static_cast<int32_t>(pool.page), od, os, code, stream);
+  });
+  *took = outcome(rc, "mlora_rotary_paged_write");
+  if (*took != Took::kYes) return nullptr;
+  kp->unsafeGetTensorImpl()->bump_version();  // written in place
+  vp->unsafeGetTensorImpl()->bump_version();
+  return THPVariable_Wrap(std::move(out));
+}
+
+// kernels.paged.verify_drafts: (accepted, tokens).
+PyObject* verify_drafts(PyObject* const* args, Took* took) {
+  const at::Tensor *target = tensor_of(args[0]), *tokens = tensor_of(args[2]), *indptr = tensor_of(args[3]),
+                   *accept = tensor_of(args[4]), *last = tensor_of(args[5]);
+  const at::Tensor* draft = args[1] == Py_None ? nullptr : tensor_of(args[1]);
+  if (target == nullptr || tokens == nullptr || accept == nullptr || last == nullptr || (draft == nullptr && args[1] != Py_None))
+    return nullptr;
+  const at::Device dev = target->device();
+  const int code = dtype_code(target->scalar_type());
+  if (!is_current(dev) || code < 0 || target->dim() != 2 || tokens->dim() != 2 || target->size(0) == 0 || target->size(1) == 0 ||
+      !fits_i32(target->size(0)) || !fits_i32(target->size(1)))
+    return nullptr;
+  const int64_t rows = target->size(0), vocab = target->size(1), n = tokens->size(0), most = tokens->size(1);
+  if (n == 0 || most == 0 || !fits_i32(n) || !fits_i32(most) || !is_rows_of(target, dev, target->scalar_type(), rows, vocab) ||
+      !is_rows_of(tokens, dev, at::kLong, n, most) || !is_rows_of(accept, dev, at::kFloat, n, most) || !is_i32(indptr, dev, n + 1) ||
+      last->scalar_type() != at::kFloat || last->device() != dev || last->dim() != 1 || last->size(0) != n || !last->is_contiguous())
+    return nullptr;
+  if (draft != nullptr && (draft->scalar_type() != target->scalar_type() || draft->device() != dev || draft->dim() != 3 ||
+                           draft->size(0) != n || draft->size(1) != most || draft->size(2) != vocab || draft->stride(2) != 1))
+    return nullptr;
+  const size_t need = lib.verify_ws(static_cast<int32_t>(n), static_cast<int32_t>(vocab));
+  at::Tensor accepted = at::empty({n}, indptr->options()), out = at::empty({n, most + 1}, tokens->options().memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor ws = at::empty({static_cast<int64_t>(need)}, tokens->options().dtype(at::kByte));
+  const hipStream_t stream = stream_of(dev);
+  const void *tp = target->data_ptr(), *dp = draft != nullptr ? draft->data_ptr() : nullptr;
+  const int64_t ds0 = draft != nullptr ? draft->stride(0) : 0, ds1 = draft != nullptr ? draft->stride(1) : 0;
+  const int64_t *tok = tokens->data_ptr<int64_t>();
+  const int32_t* ip = indptr->data_ptr<int32_t>();
+  const float *ap = accept->data_ptr<float>(), *lp = last->data_ptr<float>();
+  int32_t* accp = accepted.data_ptr<int32_t>();
+  int64_t* outp = out.data_ptr<int64_t>();
+  void* wp = ws.data_ptr();
+  const int64_t ts = row_stride(*target), ks = row_stride(*tokens), as = row_stride(*accept);
+  const int rc = unlocked([&] {
+    return lib.verify(tp, ts, static_cast<int32_t>(rows), dp, ds0, ds1, tok, ks, ip, ap, as, lp, static_cast<int32_t>(n),
+                      static_cast<int32_t>(most), static_cast<int32_t>(vocab), accp, outp, code, wp, need, stream);
+  });
+  *took = outcome(rc, "mlora_verify_drafts");
+  if (*took != Took::kYes) return nullptr;
+  Ref a(THPVariable_Wrap(std::move(accepted))), o(THPVariable_Wrap(std::move(out)));
+  return a.p != nullptr && o.p != nullptr ? PyTuple_Pack(2, a.p, o.p) : nullptr;
+}
+
 // f(&took) -> a new reference or nullptr, as the module's functions return it:
 // None when the call was not taken.  No C++ exception gets out (an error of
 // torch's, as for a tensor without storage, leaves the call to the caller).
@@ -549,14 +769,34 @@ PyObject* py_add_rmsnorm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&](Took* took) { return norm(args[0], args[1], args[2], args[3], took); });
 }
 
+PyObject* py_page_tables(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!arity(n, 3)) return nullptr;
+  return guarded([&](Took* took) { return yes(page_tables(args), took); });
+}
+
+PyObject* py_paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!arity(n, 6)) return nullptr;
+  return guarded([&](Took* took) { return paged_attention(args, took); });
+}
+
+PyObject* py_paged_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!arity(n, 9)) return nullptr;
+  return guarded([&](Took* took) { return paged_write(args, took); });
+}
+
+PyObject* py_verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!arity(n, 6)) return nullptr;
+  return guarded([&](Took* took) { return verify_drafts(args, took); });
+}
+
 // set_library(addresses, launch_error, meta_type): the library's functions in
 // the order of the struct Library.
 PyObject* py_set_library(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!arity(n, 3)) return nullptr;
-  constexpr int kFns = 11;
+  constexpr int kFns = 16;
   void* p[kFns];
   if (!PyTuple_CheckExact(args[0]) || PyTuple_GET_SIZE(args[0]) != kFns) {
-    PyErr_SetString(PyExc_TypeError, "a tuple of the library's eleven addresses is expected");
+    PyErr_SetString(PyExc_TypeError, "a tuple of the library's sixteen addresses is expected");
     return nullptr;
   }
   for (int i = 0; i < kFns; ++i) {
@@ -577,6 +817,11 @@ PyObject* py_set_library(PyObject*, PyObject* const* args, Py_ssize_t n) {
   lib.grouped_ws = reinterpret_cast<decltype(lib.grouped_ws)>(p[8]);
   lib.grouped = reinterpret_cast<decltype(lib.grouped)>(p[9]);
   lib.rmsnorm_grouped = reinterpret_cast<decltype(lib.rmsnorm_grouped)>(p[10]);
+  lib.page_tables = reinterpret_cast<decltype(lib.page_tables)>(p[11]);
+  lib.paged_write = reinterpret_cast<decltype(lib.paged_write)>(p[12]);
+  lib.paged_attention = reinterpret_cast<decltype(lib.paged_attention)>(p[13]);
+  lib.verify_ws = reinterpret_cast<decltype(lib.verify_ws)>(p[14]);
+  lib.verify = reinterpret_cast<decltype(lib.verify)>(p[15]);
   Py_INCREF(args[1]);
   Py_INCREF(args[2]);
   Py_XSETREF(launch_error, args[1]);
@@ -596,6 +841,12 @@ PyMethodDef methods[] = {
     MLORA_METHOD("sgemm_b", py_sgemm_b, "(mid, weights, meta, out) -> True, or None"),
     MLORA_METHOD("rmsnorm", py_rmsnorm, "(x, weight, eps) -> new tensor, or None"),
     MLORA_METHOD("add_rmsnorm", py_add_rmsnorm, "(x, residual, weight, eps) -> new tensor, or None"),
+    MLORA_METHOD("page_tables", py_page_tables, "(step's native, start_lens, new_lens) -> True, or None"),
+    MLORA_METHOD("paged_attention", py_paged_attention, "(q, keys, values, step's native, scale, out or None) -> out, or None"),
+    MLORA_METHOD("paged_write", py_paged_write,
+                 "(q, k, v, cos, sin, keys, values, slots, out or None) -> out, or None"),
+    MLORA_METHOD("verify_drafts", py_verify_drafts,
+                 "(target, draft or None, tokens, row_indptr, accept, last) -> (accepted, tokens), or None"),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Native form of the entry points' ordinary calls.", -1, methods,
                       nullptr,               nullptr,  nullptr,                                            nullptr};

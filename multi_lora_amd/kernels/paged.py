@@ -23,6 +23,7 @@ from __future__ import annotations
 import ctypes
 from contextlib import nullcontext
 from dataclasses import dataclass, field
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -98,60 +99,59 @@ class PageState:
                    counts=torch.tensor([num_pages, 0], **i32), page=page)
 
 
-@dataclass(frozen=True)
+@lru_cache(maxsize=256)
+def _step_sizes(n: int, rows: int, max_new: int, max_kv: int, heads: Optional[int], kv_heads: Optional[int],
+                head_dim: Optional[int]) -> Tuple[int, int, int]:
+    """(int32 words of scratch, of plan, bytes of workspace) of a step."""
+    lib = _ffi.lib()
+    scratch = lib.mlora_page_tables_scratch(n)
+    if heads is None:
+        return scratch, 0, 0
+    pb, wb = ctypes.c_size_t(), ctypes.c_size_t()
+    rc = lib.mlora_paged_step_bytes(n, rows, max_new, max_kv, heads, kv_heads, head_dim, ctypes.byref(pb), ctypes.byref(wb))
+    _ffi.check(rc, "mlora_paged_step_bytes")
+    return scratch, pb.value // 4, wb.value
+
+
 class PagedStep:
     """The packed rows of one step: request ``i`` has rows ``[row_indptr[i],
     row_indptr[i + 1])``, the last of its ``kv_lens[i]`` positions.  Filled by
     ``page_tables``; with ``heads``, it carries the attention's work list and
     the workspace of its split ranges, so steps whose attention may overlap in
-    time (on different streams) need to be different ``PagedStep``s."""
+    time (on different streams) need to be different ``PagedStep``s.
 
-    state: PageState
-    row_indptr: torch.Tensor  # [n + 1] int32
-    kv_lens: torch.Tensor     # [n] int32
-    positions: torch.Tensor   # [rows] int32
-    slots: torch.Tensor       # [rows] int32: page * page size + offset; -1: no place
-    scratch: torch.Tensor
-    plan: Optional[torch.Tensor]
-    workspace: Optional[torch.Tensor]
-    rows: int
-    max_new: int
-    heads: int
-    kv_heads: int
-    head_dim: int
-    _c: _ffi.PagedStep = field(init=False, repr=False, compare=False)
+    ``row_indptr [n + 1]``, ``kv_lens [n]``, ``positions [rows]`` and ``slots
+    [rows]`` (page * page size + offset; -1: no place) are int32 tensors.
+    """
 
-    def __post_init__(self) -> None:
-        plan, ws = self.plan, self.workspace
-        object.__setattr__(self, "_c", _ffi.PagedStep(
-            self.row_indptr.data_ptr(), self.kv_lens.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(),
-            plan.data_ptr() if plan is not None else None, ws.data_ptr() if ws is not None else None,
-            plan.numel() * 4 if plan is not None else 0, ws.numel() if ws is not None else 0, self.rows, self.max_new))
+    __slots__ = ("state", "rows", "max_new", "heads", "kv_heads", "head_dim", "row_indptr", "kv_lens", "positions",
+                 "slots", "has_plan", "_ints", "_workspace", "_c", "_native")
 
-    @classmethod
-    def new(cls, state: PageState, rows: int, max_new: int, heads: Optional[int] = None, kv_heads: Optional[int] = None,
-            head_dim: Optional[int] = None) -> "PagedStep":
+    def __init__(self, state: PageState, rows: int, max_new: int, heads: Optional[int] = None,
+                 kv_heads: Optional[int] = None, head_dim: Optional[int] = None) -> None:
         """Room for ``rows`` packed rows of at most ``max_new`` new tokens a request."""
         if rows < 0 or max_new < 0:
             raise ValueError(f"rows {rows}, max_new {max_new}")
-        given = [v is not None for v in (heads, kv_heads, head_dim)]
-        if any(given) and not all(given):
+        self.has_plan = heads is not None
+        if not self.has_plan == (kv_heads is not None) == (head_dim is not None):
             raise ValueError("heads, kv_heads and head_dim are given together")
         n, width = state.table.shape
+        scratch, plan, ws = _step_sizes(n, rows, max_new, width * state.page, heads, kv_heads, head_dim)
         dev = state.table.device
-        ints = torch.empty(n + 1 + n + 2 * rows + _ffi.lib().mlora_page_tables_scratch(n), dtype=torch.int32, device=dev)
-        indptr, lens, pos, slots, scratch = ints.split(
-            (n + 1, n, rows, rows, ints.numel() - 2 * n - 1 - 2 * rows))
-        plan = ws = None
-        if given[0]:
-            pb, wb = ctypes.c_size_t(), ctypes.c_size_t()
-            rc = _ffi.lib().mlora_paged_step_bytes(n, rows, max_new, width * state.page, heads, kv_heads, head_dim,
-                                                   ctypes.byref(pb), ctypes.byref(wb))
-            _ffi.check(rc, "mlora_paged_step_bytes")
-            plan = torch.empty(pb.value // 4, dtype=torch.int32, device=dev)
-            ws = torch.empty(wb.value, dtype=torch.uint8, device=dev) if wb.value else None
-        return cls(state, indptr, lens, pos, slots, scratch, plan, ws, rows, max_new, heads or 0, kv_heads or 0,
-                   head_dim or 0)
+        self.state, self.rows, self.max_new = state, rows, max_new
+        self.heads, self.kv_heads, self.head_dim = heads or 0, kv_heads or 0, head_dim or 0
+        # One buffer: the tensors below, the tables' scratch, the plan.
+        ends = (n + 1, 2 * n + 1, 2 * n + 1 + rows, 2 * n + 1 + 2 * rows)
+        self._ints = ints = torch.empty(ends[3] + scratch + plan, dtype=torch.int32, device=dev)
+        self.row_indptr, self.kv_lens = ints[:ends[0]], ints[ends[0]:ends[1]]
+        self.positions, self.slots = ints[ends[1]:ends[2]], ints[ends[2]:ends[3]]
+        self._workspace = torch.empty(ws, dtype=torch.uint8, device=dev) if ws else None
+        p = ints.data_ptr()
+        at = p + 4 * (ends[3] + scratch)
+        self._c = _ffi.PagedStep(p, p + 4 * ends[0], p + 4 * ends[1], p + 4 * ends[2], at if self.has_plan else None,
+                                 self._workspace.data_ptr() if ws else None, 4 * plan, ws, rows, max_new)
+        self._native = (ctypes.addressof(state._c), ctypes.addressof(self._c), p + 4 * ends[3], self.heads, self.kv_heads,
+                        self.head_dim, -1 if dev.index is None else dev.index)
 
 
 def page_tables(state: PageState, start_lens: torch.Tensor, new_lens: torch.Tensor, *, rows: Optional[int] = None,
@@ -174,22 +174,24 @@ def page_tables(state: PageState, start_lens: torch.Tensor, new_lens: torch.Tens
     one to fill again in place (its bounds and heads hold), as a captured step
     does; otherwise a new one is returned.
     """
-    dev = _on_gpu("page_tables", state.table, start_lens, new_lens)
-    n = state.table.shape[0]
-    _i32("start_lens", start_lens, n)
-    _i32("new_lens", new_lens, n)
     if step is None:
         if rows is None or max_new is None:
             raise ValueError("page_tables needs rows and max_new, or a step to fill")
-        step = PagedStep.new(state, rows, max_new, heads, kv_heads, head_dim)
+        step = PagedStep(state, rows, max_new, heads, kv_heads, head_dim)
     elif any(v is not None for v in (rows, max_new, heads, kv_heads, head_dim)):
         raise ValueError("a step to fill again keeps its own bounds and heads")
     elif step.state is not state:
         raise ValueError("the step belongs to another PageState")
+    if _ffi.calls().page_tables(step._native, start_lens, new_lens):
+        return step
+    dev = _on_gpu("page_tables", state.table, start_lens, new_lens)
+    n = state.table.shape[0]
+    _i32("start_lens", start_lens, n)
+    _i32("new_lens", new_lens, n)
     with _guard(dev):
         rc = _ffi.lib().mlora_page_tables(ctypes.byref(state._c), start_lens.data_ptr(), new_lens.data_ptr(),
                                           ctypes.byref(step._c), step.heads, step.kv_heads, step.head_dim,
-                                          step.scratch.data_ptr(), _ffi.stream_ptr(dev))
+                                          step._native[2], _ffi.stream_ptr(dev))
     _ffi.check(rc, "mlora_page_tables")
     return step
 
@@ -225,6 +227,11 @@ def rotary_paged_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: t
     roll(x, d/2) * sin`` in fp32, rounded once.  Rows with a slot outside the
     pool are rotated and not written.  The slots of one call must differ.
     """
+    # The ordinary call, checked and launched natively; what it does not take
+    # (None) runs, or raises, below.  So in the functions after this one.
+    done = _ffi.calls().paged_write(q, k, v, cos, sin, keys, values, slots, out)
+    if done is not None:
+        return done if out is None else out
     dev = _on_gpu("rotary_paged_write", q, k, v, cos, sin, keys, values, slots)
     _no_grad("rotary_paged_write", q, k, v, cos, sin, keys, values)
     pages, kv_heads, page, d = _pool("rotary_paged_write", keys, values)
@@ -278,10 +285,13 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, s
     result is rounded once.  Rows behind the last request's are left as they
     were in ``out`` (undefined without one).
     """
+    done = _ffi.calls().paged_attention(q, keys, values, step._native, scale, out)
+    if done is not None:
+        return done if out is None else out
     dev = _on_gpu("paged_attention", q, keys, values, step.row_indptr)
     _no_grad("paged_attention", q, keys, values)
     pages, kv_heads, page, d = _pool("paged_attention", keys, values)
-    if step.plan is None:
+    if not step.has_plan:
         raise ValueError("the step has no work list: give page_tables the heads")
     if (kv_heads, d, page) != (step.kv_heads, step.head_dim, step.state.page):
         raise ValueError(f"the step is for {step.kv_heads} key heads of {step.head_dim} and pages of {step.state.page}, the "
@@ -331,6 +341,9 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
     row without any mass, -1.  Probabilities are float32, float16 or bfloat16;
     all sums are fp64.
     """
+    done = _ffi.calls().verify_drafts(target, draft, tokens, row_indptr, accept, last)
+    if done is not None:
+        return done
     given = [t for t in (target, draft, tokens, row_indptr, accept, last) if t is not None]
     dev = _on_gpu("verify_drafts", *given)
     if tokens.dim() != 2 or tokens.dtype != torch.int64 or (tokens.numel() > 0 and tokens.stride(1) != 1):

@@ -420,7 +420,7 @@ def test_steps_captured_and_replayed(dev):
                 torch.zeros(200, kv_heads, d, page, device=dev).half())
 
     def make(state):
-        return PagedStep.new(state, rows, most + 1, heads, kv_heads, d)
+        return PagedStep(state, rows, most + 1, heads, kv_heads, d)
 
     def run(state, keys, values, step, out):
         page_tables(state, start, new, step=step)

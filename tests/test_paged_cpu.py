@@ -122,12 +122,12 @@ def test_python_checks():
     with pytest.raises(ValueError, match="counts"):
         PageState(table=st.table, held=st.held, free=st.free, counts=st.counts.long(), page=16)
     with pytest.raises(ValueError, match="together"):
-        PagedStep.new(st, 4, 4, heads=8)
+        PagedStep(st, 4, 4, heads=8)
     with pytest.raises(ValueError, match="rows"):
-        PagedStep.new(st, -1, 4)
+        PagedStep(st, -1, 4)
     with pytest.raises(ValueError, match="head_dim"):
-        PagedStep.new(st, 4, 4, heads=8, kv_heads=2, head_dim=80)
-    s = PagedStep.new(st, 4, 4, heads=8, kv_heads=2, head_dim=64)
+        PagedStep(st, 4, 4, heads=8, kv_heads=2, head_dim=80)
+    s = PagedStep(st, 4, 4, heads=8, kv_heads=2, head_dim=64)
     q = torch.zeros(4, 512, dtype=torch.bfloat16)
     keys, values = torch.zeros(10, 2, 16, 64).bfloat16(), torch.zeros(10, 2, 64, 16).bfloat16()
     with pytest.raises(RuntimeError, match="no CPU fallback"):
