@@ -12,6 +12,13 @@ namespace {
 
 constexpr int kScanThreads = 1024;
 constexpr int kScanWaves = kScanThreads / kWave;
+// Steps of up to this many requests and rows run as one launch of one
+// workgroup; beyond, one workgroup's turns cost more than a second launch.  A
+// step and its taking back, replayed: 168 requests of one token 12.0 us
+// against 19.1 with two launches each, eight prompts of 128 tokens 13.1
+// against 19.6, of 512 17.7 against 18.9, of 1024 24.0 against 19.0.
+constexpr int kSmallRequests = kScanThreads;
+constexpr int kSmallRows = 2048;
 
 // Scratch words: pages on the stack before the call, pages given back, pages
 // wanted, the lengths at which ranges split; then per request its first freed
@@ -90,6 +97,170 @@ __device__ __forceinline__ int tiles_of(const PagedShape& s, int c, int kind) {
 }
 __device__ __forceinline__ int table_room(const TablesArgs& a) {
   return static_cast<int>(min(static_cast<int64_t>(a.width) << a.page_shift, static_cast<int64_t>(1 << 30)));
+}
+
+// Lengths at which the ranges of each kind split: parts of equal length, so
+// that all of them together fill the chip once; tiles that fill it several
+// times over stay whole.  work: positions of all tiles of a kind, count: tiles.
+__device__ __forceinline__ void split_lengths(const TablesArgs& a, const unsigned long long* work, const unsigned long long* count,
+                                              int (&split)[2]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const unsigned long long part = (work[k] * a.kv_heads + a.shape.target - 1) / a.shape.target;
+    const unsigned long long least = max(part, static_cast<unsigned long long>(k ? kApMinSplitLong : kApMinSplit));
+    split[k] = count[k] * a.kv_heads >= static_cast<unsigned long long>(kApWhole) * a.shape.target
+                   ? INT32_MAX
+                   : static_cast<int>((min(least, 1ull << 30) + 63) / 64 * 64);
+  }
+}
+
+// Tile t of a request's `tiles`, those of the longest ranges first, in `parts`
+// items.  (The host's bounds leave room for all of them.)
+__device__ __forceinline__ void put_items(const TablesArgs& a, const PagedKind& kd, int i, int c, int len, int room, int tiles,
+                                          int t, int parts, int it, int sl, int jn) {
+  const int row0 = (tiles - 1 - t) * kd.bm;
+  const int last = min(row0 + kd.bm, c * a.shape.rep) - 1;
+  const int end = min(len - c + last / a.shape.rep + 1, room);  // positions the tile's last row sees
+  const int step = ((end + parts - 1) / parts + 63) / 64 * 64;
+  if (it + parts > kd.item_cap || (parts > 1 && (sl + parts > kd.slot_cap || jn >= kd.join_cap))) return;
+  for (int p = 0; p < parts; ++p) {
+    int32_t* w = a.plan + kd.items_off + static_cast<int64_t>(it + p) * kApItemWords;
+    w[0] = i;
+    w[1] = row0;
+    w[2] = min(p * step, end);
+    w[3] = p + 1 == parts ? end : min((p + 1) * step, end);
+    w[4] = parts > 1 ? sl + p : -1;
+  }
+  if (parts > 1) {
+    int32_t* j = a.plan + kd.joins_off + static_cast<int64_t>(jn) * kApJoinWords;
+    j[0] = i;
+    j[1] = row0;
+    j[2] = sl;
+    j[3] = parts;
+  }
+}
+
+// The last of n ascending numbers (the first is 0) that is at most v.
+__device__ __forceinline__ int last_at_most(const int* x, int n, int v) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (x[mid] <= v) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// A step of few requests and rows in one workgroup and one launch: thread =
+// request for the sums and the work list, then row, then page.
+__global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a) {
+  __shared__ int tmp[6][kScanWaves];
+  __shared__ unsigned long long wide[4];
+  __shared__ int join_rows;
+  __shared__ int first_s[kSmallRequests], freed_s[kSmallRequests], taken_s[kSmallRequests], need_s[kSmallRequests],
+      held_s[kSmallRequests], start_s[kSmallRequests];
+  const int i = threadIdx.x;
+  const bool plan = a.plan != nullptr;
+  const int top = min(max(a.counts[0], 0), a.num_pages);
+  int v[3] = {0, 0, 0}, total[3];
+  int len = 0, start = 0, need = 0, held = 0;
+  if (i < 4) wide[i] = 0;
+  if (i == 4) join_rows = 0;
+  if (i < a.n) {
+    const int2 l = lens_of(a, i);
+    start = l.x;
+    len = l.x + l.y;
+    need = pages_for(len, a);
+    held = min(max(a.held[i], 0), a.width);
+    v[0] = min(l.y, a.rows);
+    v[1] = max(held - need, 0);
+    v[2] = max(need - held, 0);
+  }
+  int c = v[0];
+  scan(v, total, tmp);
+  const int rows = min(total[0], a.rows), freed = total[1], taken = total[2];
+  if (i < a.n) {
+    const int first = min(v[0], a.rows);
+    c = min(c, a.rows - first);
+    first_s[i] = first;
+    freed_s[i] = v[1];
+    taken_s[i] = v[2];
+    need_s[i] = need;
+    held_s[i] = held;
+    start_s[i] = start;
+    a.row_indptr[i] = first;
+    a.kv_lens[i] = len;
+    a.held[i] = need > held ? held + min(need - held, max(top + freed - v[2], 0)) : need;
+  }
+  if (i == 0) {
+    a.row_indptr[a.n] = rows;
+    a.counts[0] = max(top + freed - taken, 0);
+    a.counts[1] = max(taken - top - freed, 0);
+  }
+  __syncthreads();
+
+  // As in take_page.
+  auto take = [&](int t) {
+    if (t >= freed) {
+      const int at = top - 1 - (t - freed);
+      return at >= 0 ? a.free[at] : -1;
+    }
+    const int lo = last_at_most(freed_s, a.n, t);
+    return a.table[static_cast<int64_t>(lo) * a.table_stride + need_s[lo] + (t - freed_s[lo])];
+  };
+  for (int r = i; r < a.rows; r += kScanThreads) {
+    int pos = 0, slot = -1;
+    if (r < rows) {
+      const int q = last_at_most(first_s, a.n, r);
+      pos = start_s[q] + (r - first_s[q]);
+      const int pg = pos >> a.page_shift;
+      if (pg < a.width) {
+        const int id = pg < held_s[q] ? a.table[static_cast<int64_t>(q) * a.table_stride + pg] : take(taken_s[q] + (pg - held_s[q]));
+        if (id >= 0 && id < a.num_pages) slot = (id << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+      }
+    }
+    a.positions[r] = pos;
+    a.slots[r] = slot;
+  }
+  for (int t = i; t < taken; t += kScanThreads) {
+    const int q = last_at_most(taken_s, a.n, t);
+    a.table[static_cast<int64_t>(q) * a.table_stride + held_s[q] + (t - taken_s[q])] = take(t);
+  }
+  for (int f = taken + i; f < freed; f += kScanThreads) {
+    const int q = last_at_most(freed_s, a.n, f);
+    const int to = top + freed - 1 - f;
+    if (to < a.num_pages) a.free[to] = a.table[static_cast<int64_t>(q) * a.table_stride + need_s[q] + (f - freed_s[q])];
+  }
+  if (!plan) return;
+
+  const PagedShape& s = a.shape;
+  const int room = table_room(a);
+  const int seen = min(len, room);
+  const int kind = kind_of(s, c);
+  const int tiles = tiles_of(s, c, kind);
+  if (tiles > 0) {
+    atomicAdd(&wide[kind], static_cast<unsigned long long>(tiles) * (seen - min(c, seen) / 2));
+    atomicAdd(&wide[2 + kind], static_cast<unsigned long long>(tiles));
+  }
+  __syncthreads();
+  int split[2];
+  split_lengths(a, wide, wide + 2, split);
+  const int at = kind ? split[1] : split[0];
+  const int parts = seen > at ? (seen + at - 1) / at : 1;
+  const int items = tiles * parts;
+  if (kind == 0 && parts > 1 && tiles > 0) atomicMax(&join_rows, c * s.rep);
+  int u[6] = {kind ? 0 : items, kind || parts == 1 ? 0 : items, kind || parts == 1 ? 0 : tiles,
+              kind ? items : 0, kind && parts > 1 ? items : 0,  kind && parts > 1 ? tiles : 0};
+  int sums[6];
+  scan(u, sums, tmp);
+  const PagedKind kd = kind ? s.kind[1] : s.kind[0];
+  const int it = kind ? u[3] : u[0], sl = kind ? u[4] : u[1], jn = kind ? u[5] : u[2];
+  for (int t = 0; t < tiles; ++t) put_items(a, kd, i, c, len, room, tiles, t, parts, it + t * parts, sl + t * parts, jn + t);
+  if (i < 2) {
+    a.plan[i ? kApLong : kApShort] = min(i ? sums[3] : sums[0], s.kind[i].item_cap);
+    a.plan[(i ? kApLong : kApShort) + 1] = min(i ? sums[5] : sums[2], s.kind[i].join_cap);
+  }
+  if (i == 2) a.plan[kApJoinRows] = join_rows;
 }
 
 // Prefix sums of rows, pages and items; one workgroup.
@@ -171,17 +342,8 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
     a.counts[0] = max(top + freed - taken, 0);
     a.counts[1] = max(taken - top - freed, 0);
   }
-  // Parts of equal length, so that all of them together fill the chip once;
-  // tiles that fill it several times over stay whole.
   int split[2] = {INT32_MAX, INT32_MAX};
-  if (plan) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const unsigned long long part = (wide[k] * a.kv_heads + s.target - 1) / s.target;
-      if (wide[2 + k] * a.kv_heads < static_cast<unsigned long long>(kApWhole) * s.target)
-        split[k] = static_cast<int>((min(max(part, static_cast<unsigned long long>(k ? kApMinSplitLong : kApMinSplit)), 1ull << 30) + 63) / 64 * 64);
-    }
-  }
+  if (plan) split_lengths(a, wide, wide + 2, split);
   const int have = top + freed;
   int base[2][3] = {{0, 0, 0}, {0, 0, 0}};  // items, slots, joins so far of each kind
   for (int i0 = 0; i0 < a.n; i0 += kScanThreads) {
@@ -276,7 +438,6 @@ __global__ __launch_bounds__(256) void tables_fill_kernel(TablesArgs a, int row_
     if (f >= taken && to < a.num_pages) a.free[to] = row[j];
   }
   if (a.plan == nullptr) return;
-  // The request's tiles, those of the longest ranges first.
   const PagedShape& s = a.shape;
   const int32_t* item0 = held0 + a.n;
   const int c = a.row_indptr[i + 1] - a.row_indptr[i];
@@ -286,32 +447,8 @@ __global__ __launch_bounds__(256) void tables_fill_kernel(TablesArgs a, int row_
   const int tiles = tiles_of(s, c, kind);
   const int first_item = item0[i], first_slot = item0[a.n + i], first_join = item0[2 * a.n + i], parts = item0[3 * a.n + i];
   const int room = table_room(a);
-  for (int t = lane; t < tiles; t += kWave) {
-    const int row0 = (tiles - 1 - t) * kd.bm;
-    const int last = min(row0 + kd.bm, c * s.rep) - 1;
-    const int end = min(len - c + last / s.rep + 1, room);  // positions the tile's last row sees
-    const int step = ((end + parts - 1) / parts + 63) / 64 * 64;
-    const int it = first_item + t * parts;
-    const int sl = first_slot + t * parts;
-    const int jn = first_join + t;
-    // The host's bounds leave room for all of them.
-    if (it + parts > kd.item_cap || (parts > 1 && (sl + parts > kd.slot_cap || jn >= kd.join_cap))) continue;
-    for (int p = 0; p < parts; ++p) {
-      int32_t* w = a.plan + kd.items_off + static_cast<int64_t>(it + p) * kApItemWords;
-      w[0] = i;
-      w[1] = row0;
-      w[2] = min(p * step, end);
-      w[3] = p + 1 == parts ? end : min((p + 1) * step, end);
-      w[4] = parts > 1 ? sl + p : -1;
-    }
-    if (parts > 1) {
-      int32_t* j = a.plan + kd.joins_off + static_cast<int64_t>(jn) * kApJoinWords;
-      j[0] = i;
-      j[1] = row0;
-      j[2] = sl;
-      j[3] = parts;
-    }
-  }
+  for (int t = lane; t < tiles; t += kWave)
+    put_items(a, kd, i, c, len, room, tiles, t, parts, first_item + t * parts, first_slot + t * parts, first_join + t);
 }
 
 // ------------------------------------------------------------------- write
@@ -483,6 +620,10 @@ hipError_t launch_page_tables(const TablesArgs& a, hipStream_t stream) {
   const int64_t row_blocks = (static_cast<int64_t>(a.rows) + 255) / 256;
   const int64_t blocks = row_blocks + (static_cast<int64_t>(a.n) + 3) / 4;
   if (!grid_fits(blocks)) return hipErrorInvalidConfiguration;
+  if (a.n <= kSmallRequests && a.rows <= kSmallRows) {
+    hipLaunchKernelGGL(tables_small_kernel, dim3(1), dim3(kScanThreads), 0, stream, a);
+    return hipGetLastError();
+  }
   hipLaunchKernelGGL(tables_scan_kernel, dim3(1), dim3(kScanThreads), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
