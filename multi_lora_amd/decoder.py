@@ -25,6 +25,11 @@ so a decode step touches fixed addresses and can be captured in a HIP graph.
 ``forward`` accepts the keyword arguments the reference passes to its model
 (input_ids, attention_mask, position_ids, past_key_values, cache_position,
 use_cache) and returns an object with ``.logits``.
+
+Ragged requests share a ``PagedKV``: ``forward_paged`` (``forward`` given one)
+runs the packed rows of a ``kernels.PagedStep``, whole prompts, chunks of them,
+decoding requests and drafted tokens alike, every row over its own request's
+pages (``kernels/paged.py``; GPU, 16-bit data).
 """
 
 from __future__ import annotations
@@ -39,6 +44,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .kernels.decode_attn import decode_attention, silu_mul
+from .kernels.paged import PagedStep, PageState, page_tables, paged_attention, rotary_paged_write
 
 
 @dataclass
@@ -92,6 +98,34 @@ class KVLayer:
 
     keys: torch.Tensor
     values: torch.Tensor
+
+
+class PagedKV:
+    """Per-layer pools of pages that up to ``seqs`` requests of up to
+    ``max_len`` positions share, and the page tables: keys ``[num_pages,
+    kv_heads, page, head_dim]``, values ``[num_pages, kv_heads, head_dim,
+    page]``.  By default there are pages for all of them at full length."""
+
+    def __init__(self, config: DecoderConfig, seqs: int, max_len: int, device, dtype, *, page: int = 16,
+                 num_pages: Optional[int] = None) -> None:
+        self.config, self.max_len, self.page = config, max_len, page
+        if num_pages is None:
+            num_pages = seqs * -(-max_len // page)
+        g, d = config.num_key_value_heads, config.head_dim
+        self.state = PageState.new(seqs, max_len, num_pages, page, device)
+        self.keys: List[torch.Tensor] = [torch.zeros((num_pages, g, page, d), device=device, dtype=dtype)
+                                         for _ in range(config.num_hidden_layers)]
+        self.values: List[torch.Tensor] = [torch.zeros((num_pages, g, d, page), device=device, dtype=dtype)
+                                           for _ in range(config.num_hidden_layers)]
+
+    def new_step(self, rows: int, max_new: int) -> PagedStep:
+        """A step of up to ``rows`` packed rows for ``tables`` to fill."""
+        c = self.config
+        return PagedStep(self.state, rows, max_new, c.num_attention_heads, c.num_key_value_heads, c.head_dim)
+
+    def tables(self, start_lens: torch.Tensor, new_lens: torch.Tensor, step: PagedStep) -> PagedStep:
+        """``kernels.page_tables`` of the step: request ``i`` keeps ``start_lens[i]`` positions and gets ``new_lens[i]``."""
+        return page_tables(self.state, start_lens, new_lens, step=step)
 
 
 class DecoderRMSNorm(nn.Module):
@@ -214,6 +248,12 @@ class Attention(nn.Module):
         out = torch.bmm(probs, v.to(dt).contiguous().view(b * kvh, length, d))    # [b*kvh, rep*t, d]
         return out.view(b, h, t, d).transpose(1, 2).reshape(b, t, h * d)
 
+    def forward_paged(self, x, rot: Rotary, kv: PagedKV, layer: int, step: PagedStep):
+        """Packed rows ``x [rows, hidden]`` of a step over the paged cache."""
+        q = rotary_paged_write(self.q_proj(x), self.k_proj(x), self.v_proj(x), rot.cos, rot.sin, kv.keys[layer],
+                               kv.values[layer], step.slots)
+        return self.o_proj(paged_attention(q, kv.keys[layer], kv.values[layer], step, self.scale))
+
     def forward_mixed(self, x, rot: Rotary, pre: "Packed", dec: "Packed", layer: int):
         """Packed rows ``x [R, hidden]``: ``pre.n`` prompts of ``pre.t`` tokens,
         then ``dec.n`` decode rows, with ``rot`` covering all R rows.  The
@@ -263,6 +303,11 @@ class Block(nn.Module):
         attn = self.self_attn(h, rot, hide, kv, layer, cache_position)
         return x, self.mlp(self.post_attention_layernorm.add_forward(attn, x))
 
+    def forward_paged(self, x, rot, kv, layer, step, pending=None):
+        h = self.input_layernorm(x) if pending is None else self.input_layernorm.add_forward(pending, x)
+        attn = self.self_attn.forward_paged(h, rot, kv, layer, step)
+        return x, self.mlp(self.post_attention_layernorm.add_forward(attn, x))
+
     def forward_mixed(self, x, rot, pre, dec, layer, pending=None):
         h = self.input_layernorm(x) if pending is None else self.input_layernorm.add_forward(pending, x)
         attn = self.self_attn.forward_mixed(h, rot, pre, dec, layer)
@@ -295,7 +340,10 @@ class Decoder(nn.Module):
 
     def forward(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                 position_ids: Optional[torch.Tensor] = None, past_key_values: Optional[StaticKV] = None,
-                cache_position: Optional[torch.Tensor] = None, use_cache: bool = True, **_):
+                cache_position: Optional[torch.Tensor] = None, use_cache: bool = True,
+                paged_step: Optional[PagedStep] = None, logit_rows: Optional[torch.Tensor] = None, **_):
+        if isinstance(past_key_values, PagedKV):
+            return SimpleNamespace(logits=self.forward_paged(input_ids.reshape(-1), past_key_values, paged_step, logit_rows))
         b, t = input_ids.shape
         dev = input_ids.device
         kv = past_key_values if use_cache else None
@@ -311,6 +359,22 @@ class Decoder(nn.Module):
         for i, layer in enumerate(self.layers):
             x, pending = layer(x, rot, hide, kv, i, cache_position, pending)
         return SimpleNamespace(logits=self.lm_head(self.norm.add_forward(pending, x)))
+
+    def forward_paged(self, ids: torch.Tensor, kv: PagedKV, step: PagedStep, logit_rows: Optional[torch.Tensor] = None):
+        """One step of ragged requests: packed token ids ``[rows]`` as ``step``
+        lists them, their keys and values into ``kv``'s pages, every row
+        attending to its request's positions up to its own.  Logits of every
+        row, or of ``logit_rows``; those of rows behind the last request's mean
+        nothing.  No host synchronisation: over resident tensors the step can
+        be captured in a graph and replayed with new ids and lengths."""
+        x = self.embed_tokens(ids)
+        rot = Rotary.make(step.positions, self.inv_freq, x.dtype)
+        pending = None
+        for i, layer in enumerate(self.layers):
+            x, pending = layer.forward_paged(x, rot, kv, i, step, pending)
+        if logit_rows is not None:
+            x, pending = x[logit_rows], pending[logit_rows]
+        return self.lm_head(self.norm(x + pending))
 
     def forward_mixed(self, prompt_ids: torch.Tensor, decode_ids: torch.Tensor, decode_kv: StaticKV,
                       decode_pos: torch.Tensor):

@@ -97,7 +97,8 @@ def capture_graph(mgr, step: DecodeStep, warmup: int = WARMUP_STEPS):
     The warm-up advances the state and is rewound; the capture only
     records, so the step is at ``start`` when this returns and the first
     replay decodes position ``start``.  ``output`` is the captured run's
-    result, whose tensors every replay overwrites.
+    result, whose tensors every replay overwrites.  (``step`` may be a
+    ``paged_decode.PagedDecode``, whose positions are one per request.)
     """
     if step.start + warmup + 1 > step.max_len:
         raise ValueError(f"max_len {step.max_len} leaves no room for {warmup} warm-up steps and the capture")
