@@ -920,8 +920,8 @@ int mlora_paged_attention(const void* q, int64_t q_row_stride, const void* keys,
 
 size_t mlora_verify_workspace_bytes(int32_t n, int32_t vocab) {
   if (n < 0 || vocab < 1) return 0;
-  const size_t chunks = (static_cast<size_t>(vocab) + mlora::kVerifyChunk - 1) / mlora::kVerifyChunk;
-  return static_cast<size_t>(n) * chunks * 2 * sizeof(double);
+  if (vocab > (1 << 28)) return 0;
+  return static_cast<size_t>(n) * mlora::verify_chunks(vocab) * 2 * sizeof(double);
 }
 
 int mlora_verify_drafts(const void* target, int64_t target_row_stride, int32_t rows, const void* draft,
@@ -947,7 +947,7 @@ int mlora_verify_drafts(const void* target, int64_t target_row_stride, int32_t r
   a.row_indptr = row_indptr;
   a.accept = accept, a.accept_stride = accept_stride, a.last = last;
   a.n = n, a.most = most, a.rows = rows, a.vocab = vocab;
-  a.chunks = (vocab + mlora::kVerifyChunk - 1) / mlora::kVerifyChunk;
+  a.chunks = mlora::verify_chunks(vocab);
   a.sums = static_cast<double*>(workspace);
   a.accepted = accepted, a.out = out;
   const hipError_t e = mlora::launch_verify(a, dtype, static_cast<hipStream_t>(stream));

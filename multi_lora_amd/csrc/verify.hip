@@ -11,9 +11,9 @@
 // p_j, and a row without mass has no answer (-1).
 //
 // Two launches, for one row's sums are needed before its draw: a workgroup
-// per 4096 columns of a request's row, which finds the row itself, then a
+// per 2048 columns of a request's row, which finds the row itself, then a
 // workgroup per request that reads the one chunk its draw falls in.  Rows of
-// one chunk are one launch.
+// up to 4096 columns are one launch.
 #include "kernels.h"
 #include "loads.h"
 #include "paged.h"
@@ -100,11 +100,10 @@ __device__ __forceinline__ void row_ptrs(const VerifyArgs& a, const Row& r, int 
            : nullptr;
 }
 
-constexpr int kPer = kVerifyChunk / 256;  // columns a thread
-
 template <class T>
 __global__ __launch_bounds__(256) void verify_sum_kernel(VerifyArgs a) {
   using raw = typename T::raw_t;
+  constexpr int kPer = kVerifyChunk / 256;  // columns a thread
   const int i = blockIdx.x / a.chunks;
   const int c = blockIdx.x - i * a.chunks;
   const Row r = find_row<T>(a, i);
@@ -178,6 +177,7 @@ struct DrawLds {
 template <class T, bool ONE>
 __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
   using raw = typename T::raw_t;
+  constexpr int kPer = (ONE ? kVerifyOne : kVerifyChunk) / 256;  // columns a thread
   __shared__ DrawLds s;
   const int i = blockIdx.x;
   const int tid = threadIdx.x;

@@ -328,7 +328,7 @@ def probabilities(g, shape, dtype, dev, std=2.0):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("ks,vocab,certain", [
-    ([4], 512, False), ([0, 1, 2, 3], 1, False), ([3, 0, 5], 4097, False), ([2, 2], 4096, True), ([70, 64, 1], 777, False),
+    ([4], 512, False), ([0, 1, 2, 3], 1, False), ([3, 0, 5], 4097, False), ([3, 1], 2049, False), ([2, 2], 4096, True), ([70, 64, 1], 777, False),
     ([4] * 20, 12289, False), ([1, 8, 0], 128256, True),
 ])
 def test_verify_drafts(dev, ks, vocab, certain, dtype):

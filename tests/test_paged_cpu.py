@@ -92,7 +92,7 @@ def test_attention_arguments():
 def test_verify_arguments():
     lib = _ffi.lib()
     need = lib.mlora_verify_workspace_bytes(3, 5000)
-    assert need == 3 * 2 * 2 * 8 and lib.mlora_verify_workspace_bytes(3, 0) == 0
+    assert need == 3 * 3 * 2 * 8 and lib.mlora_verify_workspace_bytes(3, 0) == 0
 
     def call(target=1 << 12, ts=5000, rows=9, draft=1 << 20, s0=20000, tokens=1 << 13, accept=1 << 14, last=64, n=3, most=4,
              vocab=5000, ws=1 << 22, bytes_=need, dt=F32, indptr=32):
