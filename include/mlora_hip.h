@@ -436,8 +436,11 @@ int32_t mlora_page_tables_scratch(int32_t n);
  * Writes row_indptr (prefix sums of new_lens, at most `rows`), kv_lens =
  * start + new, positions and slots (0 and -1 for rows behind the last
  * request's), and, if the step has a plan, the work list for `heads` query
- * heads over `kv_heads` key heads of head_dim.  Table entries past the pages
- * held are left as they were.  rows at most 2^20, num_pages * page and n *
+ * heads over `kv_heads` key heads of head_dim.  A new length above the step's
+ * max_new counts as max_new, and requests that the step's rows do not hold get
+ * fewer or none (row_indptr says so).  start_lens and new_lens may be the
+ * step's own kv_lens.  Table entries past the pages held are left as they
+ * were.  rows at most 2^20, num_pages * page and n *
  * width below 2^31. */
 int mlora_page_tables(const mlora_pages* pages, const int32_t* start_lens, const int32_t* new_lens,
                       const mlora_paged_step* step, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t* scratch,
@@ -460,7 +463,7 @@ int mlora_rotary_paged_write(const void* q, int64_t q_row_stride, const void* k,
  *   out[row, h] = sum_l softmax_l(scale * q[row, h] . k[l, h / rep]) * v[l, h / rep]
  * over the positions l <= the row's own; fp32 sums, P rounded to the data type
  * for its product with V, one rounding of the result.  `step` is one that
- * mlora_page_tables filled for these heads.  Rows behind the last request's
+ * mlora_page_tables filled for these heads (its plan is followed unchecked).  Rows behind the last request's
  * are left as they were.  A row that would attend to a page outside the pool,
  * or past the table, is NaN.  What lies in positions that a row does not
  * attend to (NaN too) does not reach it.

@@ -822,7 +822,7 @@ int mlora_page_tables(const mlora_pages* pages, const int32_t* start_lens, const
   a.width = pages->width, a.num_pages = pages->num_pages, a.page_shift = shift;
   a.n = pages->n;
   a.start = start_lens, a.add = new_lens;
-  a.rows = step->rows;
+  a.rows = step->rows, a.max_new = std::min(step->max_new, (1 << 30) - 1);
   a.row_indptr = step->row_indptr, a.kv_lens = step->kv_lens, a.positions = step->positions, a.slots = step->slots;
   a.scratch = scratch;
   a.plan = step->plan;

@@ -57,15 +57,15 @@ struct TablesArgs {
   int width, num_pages, page_shift;
   int n;
   const int32_t *start, *add;
-  int rows;
+  int rows, max_new;
   int32_t *row_indptr, *kv_lens, *positions, *slots;
-  int32_t* scratch;  // kTablesScratch(n) words
+  int32_t* scratch;  // tables_scratch_words(n) words
   // plan (nullptr: none)
   int32_t* plan;
   PagedShape shape;
   int kv_heads;
 };
-constexpr int tables_scratch_words(int n) { return 16 + 7 * n; }
+constexpr int tables_scratch_words(int n) { return 16 + 9 * n; }
 hipError_t launch_page_tables(const TablesArgs& a, hipStream_t stream);
 
 struct WriteArgs {

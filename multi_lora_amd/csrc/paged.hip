@@ -22,8 +22,8 @@ constexpr int kSmallRows = 2048;
 
 // Scratch words: pages on the stack before the call, pages given back, pages
 // wanted, the lengths at which ranges split; then per request its first freed
-// and first taken page (exclusive prefix sums), the pages it held, and of the
-// work list its first item, slot and join and its parts a tile.
+// and first taken page (exclusive prefix sums), the pages it held, of the work
+// list its first item, slot and join and its parts a tile, and its lengths.
 constexpr int kTsTop = 0;
 constexpr int kTsFreed = 1;
 constexpr int kTsTaken = 2;
@@ -34,11 +34,16 @@ __device__ __forceinline__ int pages_for(int tokens, const TablesArgs& a) {
   return static_cast<int>(min(p, static_cast<int64_t>(a.width)));
 }
 
-// Tokens request i keeps and gets; sums stay inside 31 bits.
+// Tokens request i keeps and gets, as the caller gives them: sums stay inside
+// 31 bits, and max_new is kept, for the work list has room for no more.
+__device__ __forceinline__ int2 given_lens(const TablesArgs& a, int i) {
+  return make_int2(min(max(a.start[i], 0), (1 << 30) - 1), min(max(a.add[i], 0), a.max_new));
+}
+// The same from scratch, once the first kernel has put them there (the
+// caller's may be the step's own kv_lens).
 __device__ __forceinline__ int2 lens_of(const TablesArgs& a, int i) {
-  const int s = min(max(a.start[i], 0), (1 << 30) - 1);
-  const int c = min(max(a.add[i], 0), (1 << 30) - 1);
-  return make_int2(s, c);
+  const int32_t* start0 = a.scratch + kTsArrays + 7 * a.n;
+  return make_int2(start0[i], start0[a.n + i]);
 }
 
 // Page number `t` of the pages wanted in this call: the t-th page given back
@@ -175,10 +180,9 @@ __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a
   if (i < 4) wide[i] = 0;
   if (i == 4) join_rows = 0;
   if (i < a.n) {
-    const int2 l = lens_of(a, i);
+    const int2 l = given_lens(a, i);
     start = l.x;
-    len = l.x + l.y;
-    need = pages_for(len, a);
+    need = pages_for(l.x + l.y, a);
     held = min(max(a.held[i], 0), a.width);
     v[0] = min(l.y, a.rows);
     v[1] = max(held - need, 0);
@@ -190,6 +194,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a
   if (i < a.n) {
     const int first = min(v[0], a.rows);
     c = min(c, a.rows - first);
+    len = start + c;
     first_s[i] = first;
     freed_s[i] = v[1];
     taken_s[i] = v[2];
@@ -293,16 +298,14 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
   for (int i0 = 0; i0 < a.n; i0 += kScanThreads) {
     const int i = i0 + threadIdx.x;
     int v[3] = {0, 0, 0}, total[3];
-    int len = 0;
+    int2 l = make_int2(0, 0);
     if (i < a.n) {
-      const int2 l = lens_of(a, i);
-      len = l.x + l.y;
-      const int need = pages_for(len, a);
+      l = given_lens(a, i);
+      const int need = pages_for(l.x + l.y, a);
       const int held = min(max(a.held[i], 0), a.width);
       v[0] = min(l.y, a.rows);
       v[1] = max(held - need, 0);
       v[2] = max(need - held, 0);
-      a.kv_lens[i] = len;
       held0[i] = held;
     }
     const int c = v[0];
@@ -310,14 +313,17 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
     if (i < a.n) {
       // Rows saturate at the call's rows: later requests then get none.
       const int first = min(rows + v[0], a.rows);
+      const int mine = min(c, a.rows - first);
       a.row_indptr[i] = first;
+      a.kv_lens[i] = l.x + mine;
+      parts0[a.n + i] = l.x;
+      parts0[2 * a.n + i] = l.y;
       freed0[i] = freed + v[1];
       taken0[i] = taken + v[2];
       if (plan) {
-        const int mine = min(c, a.rows - first);
         const int kind = kind_of(s, mine);
         const unsigned long long tiles = tiles_of(s, mine, kind);
-        len = min(len, room);
+        const int len = min(l.x + mine, room);
         const unsigned long long w = tiles * len;
         work[kind] += w;
         count[kind] += tiles;
@@ -362,9 +368,8 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
       const int need = pages_for(l.x + l.y, a);
       const int held = held0[i];
       a.held[i] = need > held ? held + min(need - held, max(have - taken0[i], 0)) : need;
-      const int first = a.row_indptr[i];
-      c = min(l.y, a.rows - first);
-      len = min(l.x + l.y, room);
+      c = min(l.y, a.rows - a.row_indptr[i]);
+      len = min(l.x + c, room);
     }
     if (!plan) continue;
     const int kind = kind_of(s, c);
@@ -449,7 +454,7 @@ __global__ __launch_bounds__(256) void tables_fill_kernel(TablesArgs a, int row_
   const PagedShape& s = a.shape;
   const int32_t* item0 = held0 + a.n;
   const int c = a.row_indptr[i + 1] - a.row_indptr[i];
-  const int len = l.x + l.y;
+  const int len = l.x + c;
   const int kind = kind_of(s, c);
   const PagedKind kd = kind ? s.kind[1] : s.kind[0];
   const int tiles = tiles_of(s, c, kind);

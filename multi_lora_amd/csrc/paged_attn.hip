@@ -12,6 +12,10 @@
 // lie transposed in the cache ([D, page]), so that a chunk of eight positions
 // is one 16-byte load; a page is at least eight positions and a power of two.
 //
+// Roundings: the weights, for the second product, to the data type (half a
+// step of each; their sum is taken before), the result once; scores, sums and
+// rescaling are fp32.
+//
 // Masked places: their scores become -inf by selection, and where a tile has
 // any, values that are not finite are left out of the product and added in
 // for the rows that see them, so what lies behind a request's end or in a
@@ -355,7 +359,7 @@ __device__ __forceinline__ int chunk_at(int row, int chunk) {
 // and the sums are rescaled a few times a range instead of at every new maximum
 // (whose search over raw scores costs as much as the exponentials' arguments).
 constexpr float kOver = 256.f;
-constexpr float kNoScore = -3e38f;  // a row's reference before it has seen a score
+constexpr float kNoScore = -3.40282347e38f;  // a row's reference before it has seen a score: the lowest number
 
 template <class T, int D>
 __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, TileLds<D>& s, int item, int head) {
@@ -376,8 +380,9 @@ __device__ __forceinline__ void tile_item(const PagedAttnArgs& a, TileLds<D>& s,
   const int32_t* table = a.table + static_cast<int64_t>(it.req) * a.table_stride;
 
   // The wave's rows; a negative scale goes into q, so that the largest scaled
-  // score is the scaled largest one.
-  const float scale = fabsf(a.scale_log2);
+  // score is the scaled largest one.  A scale of 0 is the least normal number:
+  // it makes scores 0 and leaves hidden ones at -inf.
+  const float scale = a.scale_log2 == 0.f ? 1.17549435e-38f : fabsf(a.scale_log2);
   const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
   const int m = it.row0 + min(wave * 32 + col, it.rows - 1);
   const int lim = it.past + m / a.rep + 1;

@@ -125,7 +125,7 @@ class PagedStep:
     """
 
     __slots__ = ("state", "rows", "max_new", "heads", "kv_heads", "head_dim", "row_indptr", "kv_lens", "positions",
-                 "slots", "has_plan", "_ints", "_workspace", "_c", "_native")
+                 "slots", "has_plan", "filled", "_ints", "_workspace", "_c", "_native")
 
     def __init__(self, state: PageState, rows: int, max_new: int, heads: Optional[int] = None,
                  kv_heads: Optional[int] = None, head_dim: Optional[int] = None) -> None:
@@ -139,6 +139,7 @@ class PagedStep:
         scratch, plan, ws = _step_sizes(n, rows, max_new, width * state.page, heads, kv_heads, head_dim)
         dev = state.table.device
         self.state, self.rows, self.max_new = state, rows, max_new
+        self.filled = False  # by page_tables
         self.heads, self.kv_heads, self.head_dim = heads or 0, kv_heads or 0, head_dim or 0
         # One buffer: the tensors below, the tables' scratch, the plan.
         ends = (n + 1, 2 * n + 1, 2 * n + 1 + rows, 2 * n + 1 + 2 * rows)
@@ -168,11 +169,14 @@ def page_tables(state: PageState, start_lens: torch.Tensor, new_lens: torch.Tens
     rows that would attend to it are NaN.
 
     ``rows`` (packed rows, at least the sum of the new lengths) and ``max_new``
-    (at least each of them) are the host's bounds; rows behind the last
-    request's get position 0 and slot -1.  With ``heads``, ``kv_heads`` and
+    (at least each of them) are the host's bounds: a longer new length counts
+    as ``max_new``, requests that the rows do not hold get fewer or none.  Rows
+    behind the last request's get position 0 and slot -1.  With ``heads``, ``kv_heads`` and
     ``head_dim`` the step carries what ``paged_attention`` needs.  ``step``:
     one to fill again in place (its bounds and heads hold), as a captured step
-    does; otherwise a new one is returned.
+    does (``start_lens`` may be its ``kv_lens``); otherwise a new one is
+    returned.  Calls on one state are made in order, on one stream or with the
+    streams made to wait.
     """
     if step is None:
         if rows is None or max_new is None:
@@ -183,6 +187,7 @@ def page_tables(state: PageState, start_lens: torch.Tensor, new_lens: torch.Tens
     elif step.state is not state:
         raise ValueError("the step belongs to another PageState")
     if _ffi.calls().page_tables(step._native, start_lens, new_lens):
+        step.filled = True
         return step
     dev = _on_gpu("page_tables", state.table, start_lens, new_lens)
     n = state.table.shape[0]
@@ -193,6 +198,7 @@ def page_tables(state: PageState, start_lens: torch.Tensor, new_lens: torch.Tens
                                           ctypes.byref(step._c), step.heads, step.kv_heads, step.head_dim,
                                           step._native[2], _ffi.stream_ptr(dev))
     _ffi.check(rc, "mlora_page_tables")
+    step.filled = True
     return step
 
 
@@ -285,6 +291,8 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, s
     result is rounded once.  Rows behind the last request's are left as they
     were in ``out`` (undefined without one).
     """
+    if not step.filled:
+        raise ValueError("the step is empty: page_tables fills it")
     done = _ffi.calls().paged_attention(q, keys, values, step._native, scale, out)
     if done is not None:
         return done if out is None else out

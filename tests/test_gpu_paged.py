@@ -74,10 +74,29 @@ def test_page_tables_past_the_table_and_bad_lengths(dev):
     assert state.held.tolist() == [2, 1, 2]
 
 
-def test_a_step_that_holds_too_few_rows_stays_inside_them(dev):
-    state = PageState.new(3, 64, 16, 16, dev)
-    step = page_tables(state, i32([0, 0, 0], dev), i32([10, 10, 10], dev), rows=15, max_new=10)
-    assert step.row_indptr.tolist() == [0, 10, 15, 15]
+@pytest.mark.parametrize("n", [3, 1200])  # one launch, and two
+def test_bounds_that_are_too_small_are_kept(dev, n):
+    """Rows and new tokens past the step's bounds are not given out, and what is given fits together."""
+    state = PageState.new(n, 64, 16 + n, 16, dev)
+    zeros = [0] * (n - 3)
+    step = page_tables(state, i32([7, 20, 0] + zeros, dev), i32([10, 12, 10] + zeros, dev), rows=15, max_new=11,
+                       heads=2, kv_heads=1, head_dim=64)
+    assert step.row_indptr.tolist() == [0, 10] + [15] * (n - 1) and step.kv_lens.tolist() == [17, 25, 0] + zeros
+    assert step.positions.tolist() == list(range(7, 17)) + list(range(20, 25))
+    step = page_tables(state, i32([7, 20, 0] + zeros, dev), i32([10, 12, 10] + zeros, dev), rows=40, max_new=11)
+    assert step.row_indptr.tolist()[:4] == [0, 10, 21, 31] and step.kv_lens.tolist()[:3] == [17, 31, 10]
+
+
+@pytest.mark.parametrize("n", [5, 1100])
+def test_a_step_continues_from_its_own_lengths(dev, n):
+    """start_lens is the step's kv_lens, which the call rewrites."""
+    state, sim = PageState.new(n, 400, 26 * n, 16, dev), ref.Pages(n, 25, 26 * n, 16)
+    new = [1 + i % 3 for i in range(n)]
+    step = page_tables(state, i32([0] * n, dev), i32(new, dev), rows=sum(new), max_new=3)
+    check_step(state, sim, step, sim.step([0] * n, new, sum(new)), sum(new))
+    for turn in range(1, 20):
+        page_tables(state, step.kv_lens, i32(new, dev), step=step)
+        check_step(state, sim, step, sim.step([turn * c for c in new], new, sum(new)), sum(new))
 
 
 # ---------------------------------------------------------------- rotary and write
@@ -252,6 +271,21 @@ def test_extreme_scores(dev):
         assert torch.equal(got[0, :d], values[int(table[0, at // 16]), 0, :, at % 16])
         keys.fill_(8.0)
         check_attention(paged_attention(q, keys, values, step, 1.0), q, keys, values, table, [299], [1], 1.0, torch.bfloat16)
+
+
+@pytest.mark.parametrize("new,start", [([1], [70]), ([50], [70])])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_scales_that_are_not_positive(dev, new, start, scale):
+    q, keys, values, table, step = cache_case(dev, new, start, 4, 2, 64, 16, torch.bfloat16, 2)
+    check_attention(paged_attention(q, keys, values, step, scale), q, keys, values, table, start, new, scale, torch.bfloat16)
+
+
+def test_an_empty_step_is_refused(dev):
+    state = PageState.new(2, 64, 8, 16, dev)
+    step = PagedStep(state, 2, 1, 2, 1, 64)
+    pool = torch.zeros(8, 1, 16, 64, device=dev).half()
+    with pytest.raises(ValueError, match="page_tables fills it"):
+        paged_attention(torch.zeros(2, 128, device=dev).half(), pool, pool.transpose(2, 3).contiguous(), step, 0.1)
 
 
 def test_rows_behind_the_last_request_are_left(dev):

@@ -130,6 +130,9 @@ def test_python_checks():
     s = PagedStep(st, 4, 4, heads=8, kv_heads=2, head_dim=64)
     q = torch.zeros(4, 512, dtype=torch.bfloat16)
     keys, values = torch.zeros(10, 2, 16, 64).bfloat16(), torch.zeros(10, 2, 64, 16).bfloat16()
+    with pytest.raises(ValueError, match="page_tables fills it"):
+        paged_attention(q, keys, values, s, 0.125)
+    s.filled = True
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         paged_attention(q, keys, values, s, 0.125)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
