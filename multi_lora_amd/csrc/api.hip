@@ -906,14 +906,12 @@ int mlora_paged_attention(const void* q, int64_t q_row_stride, const void* keys,
   a.key_stride = key_page_stride, a.value_stride = value_page_stride;
   a.num_pages = pages->num_pages, a.page_shift = shift;
   a.table = pages->table, a.table_stride = pages->table_stride, a.width = pages->width;
-  a.row_indptr = step->row_indptr, a.kv_lens = step->kv_lens;
-  a.n = pages->n, a.rows = step->rows;
   a.plan = step->plan;
   a.out = out, a.out_stride = out_row_stride;
   a.workspace = static_cast<char*>(step->workspace);
   a.kv_heads = kv_heads, a.rep = heads / kv_heads;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const hipError_t e = mlora::launch_paged_attention(a, step->max_new, dtype, head_dim, static_cast<hipStream_t>(stream));
+  const hipError_t e = mlora::launch_paged_attention(a, std::min(step->max_new, step->rows), dtype, head_dim, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "paged attention launch");
   return 0;
 }

@@ -19,8 +19,12 @@ constexpr int kApHeaderWords = 16;
 constexpr int kApShort = 0;      // items; joins (tiles whose range is split) in the next word
 constexpr int kApLong = 2;       // the same
 constexpr int kApJoinRows = 4;   // most rows of a split short tile
-constexpr int kApItemWords = 8;  // request, first row, first position, end, slot (-1: none)
-constexpr int kApJoinWords = 4;  // request, first row, first slot, slots
+// An item: request, first row, first position, end, slot (-1: none), the
+// request's first packed row, new tokens, and position of the first of them.
+// (What the tables know anyway: looked up, it is one more round trip to memory
+// in every workgroup, 0.7 us.)
+constexpr int kApItemWords = 8;
+constexpr int kApJoinWords = 8;  // first packed row, first row, first slot, slots, rows
 
 constexpr int kApLongRows = 128;
 // A range is split only into parts of at least this many positions.  A part of
@@ -93,8 +97,6 @@ struct PagedAttnArgs {
   const int32_t* table;
   int64_t table_stride;
   int width;
-  const int32_t *row_indptr, *kv_lens;
-  int n, rows;
   const int32_t* plan;
   void* out;
   int64_t out_stride;

@@ -129,8 +129,8 @@ __device__ __forceinline__ int parts_of(int len, int split, int kind) {
 
 // Tile t of a request's `tiles`, those of the longest ranges first, in `parts`
 // items.  (The host's bounds leave room for all of them.)
-__device__ __forceinline__ void put_items(const TablesArgs& a, const PagedKind& kd, int i, int c, int len, int room, int tiles,
-                                          int t, int parts, int it, int sl, int jn) {
+__device__ __forceinline__ void put_items(const TablesArgs& a, const PagedKind& kd, int i, int first, int c, int len, int room,
+                                          int tiles, int t, int parts, int it, int sl, int jn) {
   const int row0 = (tiles - 1 - t) * kd.bm;
   const int last = min(row0 + kd.bm, c * a.shape.rep) - 1;
   const int end = min(len - c + last / a.shape.rep + 1, room);  // positions the tile's last row sees
@@ -143,13 +143,17 @@ __device__ __forceinline__ void put_items(const TablesArgs& a, const PagedKind& 
     w[2] = min(p * step, end);
     w[3] = p + 1 == parts ? end : min((p + 1) * step, end);
     w[4] = parts > 1 ? sl + p : -1;
+    w[5] = first;
+    w[6] = c;
+    w[7] = len - c;
   }
   if (parts > 1) {
     int32_t* j = a.plan + kd.joins_off + static_cast<int64_t>(jn) * kApJoinWords;
-    j[0] = i;
+    j[0] = first;
     j[1] = row0;
     j[2] = sl;
     j[3] = parts;
+    j[4] = last + 1 - row0;
   }
 }
 
@@ -268,7 +272,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a
   scan(u, sums, tmp);
   const PagedKind kd = kind ? s.kind[1] : s.kind[0];
   const int it = kind ? u[3] : u[0], sl = kind ? u[4] : u[1], jn = kind ? u[5] : u[2];
-  for (int t = 0; t < tiles; ++t) put_items(a, kd, i, c, len, room, tiles, t, parts, it + t * parts, sl + t * parts, jn + t);
+  for (int t = 0; t < tiles; ++t) put_items(a, kd, i, first_s[i], c, len, room, tiles, t, parts, it + t * parts, sl + t * parts, jn + t);
   if (i < 2) {
     a.plan[i ? kApLong : kApShort] = min(i ? sums[3] : sums[0], s.kind[i].item_cap);
     a.plan[(i ? kApLong : kApShort) + 1] = min(i ? sums[5] : sums[2], s.kind[i].join_cap);
@@ -453,7 +457,8 @@ __global__ __launch_bounds__(256) void tables_fill_kernel(TablesArgs a, int row_
   if (a.plan == nullptr) return;
   const PagedShape& s = a.shape;
   const int32_t* item0 = held0 + a.n;
-  const int c = a.row_indptr[i + 1] - a.row_indptr[i];
+  const int first_row = a.row_indptr[i];
+  const int c = a.row_indptr[i + 1] - first_row;
   const int len = l.x + c;
   const int kind = kind_of(s, c);
   const PagedKind kd = kind ? s.kind[1] : s.kind[0];
@@ -461,7 +466,7 @@ __global__ __launch_bounds__(256) void tables_fill_kernel(TablesArgs a, int row_
   const int first_item = item0[i], first_slot = item0[a.n + i], first_join = item0[2 * a.n + i], parts = item0[3 * a.n + i];
   const int room = table_room(a);
   for (int t = lane; t < tiles; t += kWave)
-    put_items(a, kd, i, c, len, room, tiles, t, parts, first_item + t * parts, first_slot + t * parts, first_join + t);
+    put_items(a, kd, i, first_row, c, len, room, tiles, t, parts, first_item + t * parts, first_slot + t * parts, first_join + t);
 }
 
 // ------------------------------------------------------------------- write

@@ -77,9 +77,7 @@ __device__ __forceinline__ bool load_item(const PagedAttnArgs& a, const PagedKin
   if (item >= a.plan[counter]) return false;
   const int32_t* w = a.plan + kd.items_off + static_cast<int64_t>(item) * kApItemWords;
   t->req = w[0], t->row0 = w[1], t->kv0 = w[2], t->kv1 = w[3], t->slot = w[4];
-  t->first = a.row_indptr[t->req];
-  t->c = a.row_indptr[t->req + 1] - t->first;
-  t->past = a.kv_lens[t->req] - t->c;
+  t->first = w[5], t->c = w[6], t->past = w[7];
   t->rows = min(kd.bm, t->c * a.rep - t->row0);
   return t->rows > 0;
 }
@@ -676,7 +674,7 @@ __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(PagedAttnArgs a, in
 // ones the other way round.  One thread a column group over 34 parts took
 // 24 us (three requests of up to 32,000 positions), four 6.
 template <class T, int D, int RB>
-__device__ __forceinline__ void join_rows(const PagedAttnArgs& a, int k, int join, int head, int block, f32x4* os, float* ls) {
+__device__ __forceinline__ void join_rows(const PagedAttnArgs& a, int k, int join, int head, int block, f32x4* os) {
   using raw = typename T::raw_t;
   constexpr int C = D / 4;
   constexpr int G = 256 / (RB * C);
@@ -684,9 +682,7 @@ __device__ __forceinline__ void join_rows(const PagedAttnArgs& a, int k, int joi
   const int32_t* w = a.plan + kd.joins_off + static_cast<int64_t>(join) * kApJoinWords;
   const int slot0 = w[2], parts = w[3];
   Item it;
-  it.req = w[0], it.row0 = w[1];
-  it.first = a.row_indptr[it.req];
-  it.rows = min(kd.bm, (a.row_indptr[it.req + 1] - it.first) * a.rep - it.row0);
+  it.first = w[0], it.row0 = w[1], it.rows = w[4];
   if (block * RB >= it.rows) return;
   const int group = threadIdx.x / (RB * C);
   const int i = threadIdx.x - group * (RB * C);
@@ -696,29 +692,33 @@ __device__ __forceinline__ void join_rows(const PagedAttnArgs& a, int k, int joi
   const int64_t at = (static_cast<int64_t>(slot0) * a.kv_heads + head) * kd.bm + r;
   const float* part = reinterpret_cast<const float*>(a.workspace + kd.part_off) + at * D + d;
   const float2* ml = reinterpret_cast<const float2*>(a.workspace + kd.ml_off) + at;
+  // The C lanes of a row look at C parts' maxima and sums at once.
+  static_assert(RB * C % kWave == 0, "a wave's lanes share the parts they add");
+  const int lane = i & (C - 1);
   float m = -INFINITY;
-#pragma unroll 8
-  for (int p = 0; p < parts; ++p) m = fmaxf(m, ml[p * step].x);
+  for (int p = lane; p < parts; p += C) m = fmaxf(m, ml[p * step].x);
+#pragma unroll
+  for (int off = 1; off < C; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int p = group; p < parts; p += G) {
-    const float2 x = ml[p * step];
+  for (int p0 = 0; p0 < parts; p0 += C) {
+    const float2 x = p0 + lane < parts ? ml[(p0 + lane) * step] : make_float2(-INFINITY, 0.f);
     const float f = exp2_fast(x.x - ref);
     l += x.y * f;
-    o += *reinterpret_cast<const f32x4*>(part + p * step * D) * f;
+    const int here = min(C, parts - p0);
+#pragma unroll 4
+    for (int p = group; p < here; p += G)
+      o += *reinterpret_cast<const f32x4*>(part + (p0 + p) * step * D) * __shfl(f, (threadIdx.x & 63 & ~(C - 1)) + p, kWave);
   }
+#pragma unroll
+  for (int off = 1; off < C; off <<= 1) l += __shfl_xor(l, off, kWave);
   if constexpr (G > 1) {
     os[threadIdx.x] = o;
-    ls[threadIdx.x] = l;
     lds_barrier();
     if (group > 0) return;
 #pragma unroll
-    for (int v = 1; v < G; ++v) {
-      o += os[v * RB * C + i];
-      l += ls[v * RB * C + i];
-    }
+    for (int v = 1; v < G; ++v) o += os[v * RB * C + i];
   }
   if (block * RB + i / C >= it.rows) return;
   store_row<T>(static_cast<raw*>(a.out) + row_offset(a, it, head, it.row0 + r, a.out_stride, D) + d, o, l);
@@ -732,7 +732,6 @@ constexpr int join_block(int d, int kind) { return kind ? 1024 / d : 256 / d; } 
 template <class T, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int long_per) {
   __shared__ f32x4 os[256];
-  __shared__ float ls[256];
   const int short_per = cdiv(a.plan[kApJoinRows], join_block(D, 0));
   const int long_blocks = a.plan[kApLong + 1] * a.kv_heads * long_per;
   const int blocks = long_blocks + a.plan[kApShort + 1] * a.kv_heads * short_per;
@@ -740,11 +739,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int lo
     if (u < long_blocks) {
       const int tile = u / long_per;
       const int join = tile / a.kv_heads;
-      join_rows<T, D, join_block(D, 1)>(a, 1, join, tile - join * a.kv_heads, u - tile * long_per, os, ls);
+      join_rows<T, D, join_block(D, 1)>(a, 1, join, tile - join * a.kv_heads, u - tile * long_per, os);
     } else {
       const int tile = (u - long_blocks) / short_per;
       const int join = tile / a.kv_heads;
-      join_rows<T, D, join_block(D, 0)>(a, 0, join, tile - join * a.kv_heads, u - long_blocks - tile * short_per, os, ls);
+      join_rows<T, D, join_block(D, 0)>(a, 0, join, tile - join * a.kv_heads, u - long_blocks - tile * short_per, os);
       lds_barrier();  // before the next block's sums go where these were read
     }
   }
@@ -777,7 +776,7 @@ hipError_t launch(const PagedAttnArgs& a, int max_rows, hipStream_t stream) {
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, int max_new, int dtype, int head_dim, hipStream_t stream) {
   if (a.shape.kind[0].item_cap + a.shape.kind[1].item_cap == 0) return hipSuccess;
-  const int max_rows = std::min(std::min(max_new, a.rows), kApLongRows) * a.rep;  // of one request, as far as it matters
+  const int max_rows = std::min(max_new, kApLongRows) * a.rep;  // of one request, as far as it matters
   if (dtype == MLORA_BF16)
     return head_dim == 64 ? launch<BF16, 64>(a, max_rows, stream) : launch<BF16, 128>(a, max_rows, stream);
   return head_dim == 64 ? launch<F16, 64>(a, max_rows, stream) : launch<F16, 128>(a, max_rows, stream);
