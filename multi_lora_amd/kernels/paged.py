@@ -124,8 +124,8 @@ class PagedStep:
     [rows]`` (page * page size + offset; -1: no place) are int32 tensors.
     """
 
-    __slots__ = ("state", "rows", "max_new", "heads", "kv_heads", "head_dim", "row_indptr", "kv_lens", "positions",
-                 "slots", "has_plan", "filled", "_ints", "_workspace", "_c", "_native")
+    __slots__ = ("state", "rows", "max_new", "heads", "kv_heads", "head_dim", "has_plan", "filled", "_ints", "_ends",
+                 "_workspace", "_c", "_native")
 
     def __init__(self, state: PageState, rows: int, max_new: int, heads: Optional[int] = None,
                  kv_heads: Optional[int] = None, head_dim: Optional[int] = None) -> None:
@@ -142,10 +142,8 @@ class PagedStep:
         self.filled = False  # by page_tables
         self.heads, self.kv_heads, self.head_dim = heads or 0, kv_heads or 0, head_dim or 0
         # One buffer: the tensors below, the tables' scratch, the plan.
-        ends = (n + 1, 2 * n + 1, 2 * n + 1 + rows, 2 * n + 1 + 2 * rows)
+        self._ends = ends = (n + 1, 2 * n + 1, 2 * n + 1 + rows, 2 * n + 1 + 2 * rows)
         self._ints = ints = torch.empty(ends[3] + scratch + plan, dtype=torch.int32, device=dev)
-        self.row_indptr, self.kv_lens = ints[:ends[0]], ints[ends[0]:ends[1]]
-        self.positions, self.slots = ints[ends[1]:ends[2]], ints[ends[2]:ends[3]]
         self._workspace = torch.empty(ws, dtype=torch.uint8, device=dev) if ws else None
         p = ints.data_ptr()
         at = p + 4 * (ends[3] + scratch)
@@ -153,6 +151,22 @@ class PagedStep:
                                  self._workspace.data_ptr() if ws else None, 4 * plan, ws, rows, max_new)
         self._native = (ctypes.addressof(state._c), ctypes.addressof(self._c), p + 4 * ends[3], self.heads, self.kv_heads,
                         self.head_dim, -1 if dev.index is None else dev.index)
+
+    @property
+    def row_indptr(self) -> torch.Tensor:
+        return self._ints[:self._ends[0]]
+
+    @property
+    def kv_lens(self) -> torch.Tensor:
+        return self._ints[self._ends[0]:self._ends[1]]
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._ints[self._ends[1]:self._ends[2]]
+
+    @property
+    def slots(self) -> torch.Tensor:
+        return self._ints[self._ends[2]:self._ends[3]]
 
 
 def page_tables(state: PageState, start_lens: torch.Tensor, new_lens: torch.Tensor, *, rows: Optional[int] = None,
