@@ -126,9 +126,9 @@ struct VerifyArgs {
   int64_t* out;                    // [n, most + 1]
 };
 // Columns a workgroup sums, and columns up to which one workgroup does it all.
-// Chunks of 2048 against 4096: 32 requests over 128,256 columns alike, 8 of
-// them 16.6 us against 18.8, one over 32,000 14.0 against 14.9; of 1024, 64
-// requests 29.8 against 25.8.  One launch for 4096 columns 10.9, two 12.7.
+// Chunks of 2048 against 4096: 32 requests over 128,256 columns 13.6 us against
+// 15.1, one over 32,000 7.8 against 9.1; of 1024, 64 requests 21.6 against 17.7.
+// One launch for 4096 columns 6.7, two 8.2; for 8192 10.1, two 8.2.
 constexpr int kVerifyChunk = 2048;
 constexpr int kVerifyOne = 4096;
 constexpr int verify_chunks(int vocab) { return vocab <= kVerifyOne ? 1 : (vocab + kVerifyChunk - 1) / kVerifyChunk; }

@@ -13,9 +13,9 @@
 // Two launches, for one row's sums are needed before its draw: a workgroup
 // per 2048 columns of a request's row, which finds the row itself, then a
 // workgroup per request that reads the one chunk its draw falls in.  Rows of
-// up to 4096 columns are one launch, bound by its chain of reads: 4.6 us for
+// up to 4096 columns are one launch, bound by its chain of reads: 4.3 us for
 // one request.  Thirty-two requests of 128,256 fp32 columns (31.8 MB with the
-// drafts' rows) take 7.8 us for the sums, 4.1 TB/s, and 5.3 us for the draw.
+// drafts' rows) take 7.6 us for the sums, 4.2 TB/s, and 4.4 us for the draw.
 #include "kernels.h"
 #include "loads.h"
 #include "paged.h"
@@ -171,12 +171,18 @@ __global__ __launch_bounds__(256) void verify_sum_kernel(VerifyArgs a) {
 // Workgroup = request.  ONE: the row is a single chunk, and this is the only
 // launch.  Its time is the chain of what it reads; the waves find the chunk
 // each for itself, and meet twice over its columns.
+// Four columns a thread: with eight, on 256 and 512 threads, 0.9 us more (2.4
+// where a thread has sixteen); two, on 1024 for a chunk, 0.4 more.
+constexpr int kDrawColumns = 4;
+constexpr int draw_threads(bool one) { return (one ? kVerifyOne : kVerifyChunk) / kDrawColumns; }
 template <class T, bool ONE>
-__global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(draw_threads(ONE)) void verify_draw_kernel(VerifyArgs a) {
   using raw = typename T::raw_t;
-  constexpr int kPer = (ONE ? kVerifyOne : kVerifyChunk) / 256;  // columns a thread
-  __shared__ double part[4][2];
-  __shared__ int hit_s[4], last_s[4];
+  constexpr int kPer = kDrawColumns;
+  constexpr int kThreads = draw_threads(ONE);
+  constexpr int kWaves = kThreads / kWave;
+  __shared__ double part[kWaves][2];
+  __shared__ int hit_s[kWaves], last_s[kWaves];
   const int i = blockIdx.x;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -262,10 +268,12 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
     }
     __syncthreads();
     if constexpr (ONE) {
-      double total = part[0][0] + part[1][0] + part[2][0] + part[3][0];
+      double total = 0.0;
+      for (int v = 0; v < kWaves; ++v) total += part[v][0];
       if (!(total > 0.0)) {  // nothing left of the residual: the target's row
         use = 1;
-        total = part[0][1] + part[1][1] + part[2][1] + part[3][1];
+        total = 0.0;
+        for (int v = 0; v < kWaves; ++v) total += part[v][1];
         incl = incl_all;
         mine = all;
 #pragma unroll
@@ -296,12 +304,12 @@ __global__ __launch_bounds__(256) void verify_draw_kernel(VerifyArgs a) {
       last_s[wave] = last_mass;
     }
     __syncthreads();
-    for (int v = 0; v < 4; ++v) token = max(token, static_cast<int64_t>(last_s[v]));
-    for (int v = 3; v >= 0; --v)
+    for (int v = 0; v < kWaves; ++v) token = max(token, static_cast<int64_t>(last_s[v]));
+    for (int v = kWaves - 1; v >= 0; --v)
       if (hit_s[v] >= 0) token = hit_s[v];
   }
   int64_t* out = a.out + static_cast<int64_t>(i) * (a.most + 1);
-  for (int j = tid; j <= a.most; j += 256)
+  for (int j = tid; j <= a.most; j += kThreads)
     out[j] = !r.live ? -1 : j < r.accepted ? a.tokens[i * a.token_stride + j] : j == r.accepted ? token : -1;
   if (ONE && tid == 0) a.accepted[i] = r.accepted;
 }
@@ -311,13 +319,13 @@ hipError_t launch(const VerifyArgs& a, hipStream_t stream) {
   const int64_t blocks = static_cast<int64_t>(a.n) * a.chunks;
   if (!grid_fits(blocks)) return hipErrorInvalidConfiguration;
   if (a.chunks == 1) {
-    hipLaunchKernelGGL((verify_draw_kernel<T, true>), dim3(static_cast<unsigned>(a.n)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((verify_draw_kernel<T, true>), dim3(static_cast<unsigned>(a.n)), dim3(draw_threads(true)), 0, stream, a);
     return hipGetLastError();
   }
   hipLaunchKernelGGL((verify_sum_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((verify_draw_kernel<T, false>), dim3(static_cast<unsigned>(a.n)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((verify_draw_kernel<T, false>), dim3(static_cast<unsigned>(a.n)), dim3(draw_threads(false)), 0, stream, a);
   return hipGetLastError();
 }
 
