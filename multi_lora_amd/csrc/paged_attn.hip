@@ -74,7 +74,7 @@ struct Item {
   int rows;            // query rows of the tile, at most bm
 };
 __device__ __forceinline__ bool load_item(const PagedAttnArgs& a, const PagedKind& kd, int counter, int item, Item* t) {
-  if (item >= a.plan[counter]) return false;
+  if (item >= min(a.plan[counter], kd.item_cap)) return false;
   const int32_t* w = a.plan + kd.items_off + static_cast<int64_t>(item) * kApItemWords;
   t->req = w[0], t->row0 = w[1], t->kv0 = w[2], t->kv1 = w[3], t->slot = w[4];
   t->first = w[5], t->c = w[6], t->past = w[7];
@@ -653,15 +653,22 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_short_kernel(PagedAttnArgs a
   stream_item<T, D, NW, MT>(a, s, item, blockIdx.x - item * a.kv_heads);
 }
 
-// Long items first, then the short ones, which fill the chip as those end.
+// Long items first, then the short ones, which fill the chip as those end, and
+// last the workgroups that the host's bounds ask for and the step does not
+// need (between the two kinds: 139 us instead of 136 for a prompt of 2048
+// tokens beside 128 decoding requests, 114 instead of 99 with four times as
+// many of them).  Both kinds in turn from the start: four prompts of 1024
+// beside 128 requests 138 us against 157, but 344 against 288 for 2048 tokens
+// after 4096 beside 64 requests, whose last long items then start late.
 template <class T, int D>
-__global__ __launch_bounds__(256, 2) void paged_mixed_kernel(PagedAttnArgs a, int long_items) {
+__global__ __launch_bounds__(256, 2) void paged_mixed_kernel(PagedAttnArgs a) {
   __shared__ union {
     TileLds<D> tile;
     StreamLds<D, 4, 1> stream;
   } s;
   const int item = blockIdx.x / a.kv_heads;
   const int head = blockIdx.x - item * a.kv_heads;
+  const int long_items = min(a.plan[kApLong], a.shape.kind[1].item_cap);
   if (item < long_items)
     tile_item<T, D>(a, s.tile, item, head);
   else
@@ -760,7 +767,7 @@ hipError_t launch(const PagedAttnArgs& a, int max_rows, hipStream_t stream) {
   if (!grid_fits(blocks) || !grid_fits(joins)) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(blocks));
   if (many.item_cap > 0)
-    hipLaunchKernelGGL((paged_mixed_kernel<T, D>), grid, dim3(256), 0, stream, a, many.item_cap);
+    hipLaunchKernelGGL((paged_mixed_kernel<T, D>), grid, dim3(256), 0, stream, a);
   else if (few.bm == 16)
     hipLaunchKernelGGL((paged_short_kernel<T, D, 4, 1>), grid, dim3(256), 0, stream, a);
   else
