@@ -33,9 +33,9 @@ constexpr int kSmallRequests = kScanThreads;
 constexpr int kSmallRows = 2048;
 
 // Scratch words: pages on the stack before the call, pages given back, pages
-// wanted, the lengths at which ranges split; then per request its first freed
-// and first taken page (exclusive prefix sums), the pages it held, of the work
-// list its first item, slot and join and its parts a tile, and its lengths.
+// wanted; then per request its first freed and first taken page (exclusive
+// prefix sums), the pages it held, of the work list its first item, slot and
+// join and its parts a tile, and its lengths.
 constexpr int kTsTop = 0;
 constexpr int kTsFreed = 1;
 constexpr int kTsTaken = 2;
@@ -116,19 +116,47 @@ __device__ __forceinline__ int table_room(const TablesArgs& a) {
   return static_cast<int>(min(static_cast<int64_t>(a.width) << a.page_shift, static_cast<int64_t>(1 << 30)));
 }
 
-// Lengths at which the ranges of each kind split: parts of equal length, so
-// that all of them together fill the chip once; tiles that fill it several
-// times over stay whole.  work: positions of all tiles of a kind, count: tiles.
-__device__ __forceinline__ void split_lengths(const TablesArgs& a, const unsigned long long* work, const unsigned long long* count,
-                                              int (&split)[2]) {
+// What the ranges' split is found from, summed over the workgroup: positions of
+// all tiles and tiles of each kind, and the longest short range.
+struct Ranges {
+  unsigned long long work[2], tiles[2];
+  int longest;
+};
+
+__device__ __forceinline__ void add_ranges(Ranges& r, unsigned long long (&work)[2], int (&tiles)[2], int longest) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const unsigned long long part = (work[k] * a.kv_heads + a.shape.target - 1) / a.shape.target;
-    const unsigned long long least = max(part, static_cast<unsigned long long>(k ? kApMinSplitLong : kApMinSplit));
-    split[k] = count[k] * a.kv_heads >= static_cast<unsigned long long>(kApWhole) * a.shape.target
-                   ? INT32_MAX
-                   : static_cast<int>((min(least, 1ull << 30) + 63) / 64 * 64);
+    if (__ballot(tiles[k] != 0) == 0) continue;
+    for (int off = 1; off < kWave; off <<= 1) {
+      work[k] += __shfl_xor(work[k], off, kWave);
+      tiles[k] += __shfl_xor(tiles[k], off, kWave);
+    }
+    if ((threadIdx.x & 63) == 0) {
+      atomicAdd(&r.work[k], work[k]);
+      atomicAdd(&r.tiles[k], static_cast<unsigned long long>(tiles[k]));
+    }
+    if (k > 0) continue;
+    for (int off = 1; off < kWave; off <<= 1) longest = max(longest, __shfl_xor(longest, off, kWave));
+    if ((threadIdx.x & 63) == 0) atomicMax(&r.longest, longest);
   }
+}
+
+// Lengths at which the ranges of each kind split: parts of equal length, so
+// that all of them together fill the chip once; tiles that fill it several
+// times over stay whole.  So do short ranges if the longest is not much longer
+// than a part, for the join costs time of its own, more the more tiles it has.
+__device__ __forceinline__ void split_lengths(const TablesArgs& a, const Ranges& r, int (&split)[2]) {
+  const unsigned long long target = a.shape.target;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const unsigned long long part = (r.work[k] * a.kv_heads + target - 1) / target;
+    const unsigned long long least = max(part, static_cast<unsigned long long>(k ? kApMinSplitLong : kApMinSplit));
+    split[k] = static_cast<int>((min(least, 1ull << 29) + 63) / 64 * 64);
+    if (r.tiles[k] * a.kv_heads >= kApWhole * target) split[k] = INT32_MAX;
+  }
+  const unsigned long long filled = min(2 * r.tiles[0] * a.kv_heads, target);
+  const int keep = kApKeep + static_cast<int>(kApKeepFull * filled / target);
+  if (r.longest - keep <= split[0]) split[0] = INT32_MAX;
 }
 
 // Parts of a tile of `len` positions.  Short ones round up, so that none is
@@ -184,7 +212,7 @@ __device__ __forceinline__ int last_at_most(const int* x, int n, int v) {
 // request for the sums and the work list, then row, then page.
 __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a) {
   __shared__ int tmp[6][kScanWaves];
-  __shared__ unsigned long long wide[4];
+  __shared__ Ranges ranges;
   __shared__ int join_rows;
   __shared__ int first_s[kSmallRequests], freed_s[kSmallRequests], taken_s[kSmallRequests], need_s[kSmallRequests],
       held_s[kSmallRequests], start_s[kSmallRequests];
@@ -193,8 +221,10 @@ __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a
   const int top = min(max(a.counts[0], 0), a.num_pages);
   int v[3] = {0, 0, 0}, total[3];
   int len = 0, start = 0, need = 0, held = 0;
-  if (i < 4) wide[i] = 0;
-  if (i == 4) join_rows = 0;
+  if (i == 0) {
+    ranges = Ranges{};
+    join_rows = 0;
+  }
   if (i < a.n) {
     const int2 l = given_lens(a, i);
     start = l.x;
@@ -267,15 +297,14 @@ __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a
   const int seen = min(len, room);
   const int kind = kind_of(s, c);
   const int tiles = tiles_of(s, c, kind);
-  if (tiles > 0) {
-    atomicAdd(&wide[kind], static_cast<unsigned long long>(tiles) * seen);
-    atomicAdd(&wide[2 + kind], static_cast<unsigned long long>(tiles));
-  }
+  const unsigned long long positions = static_cast<unsigned long long>(tiles) * seen;
+  unsigned long long work[2] = {kind ? 0 : positions, kind ? positions : 0};
+  int count[2] = {kind ? 0 : tiles, kind ? tiles : 0};
+  add_ranges(ranges, work, count, tiles > 0 && kind == 0 ? seen : 0);
   __syncthreads();
   int split[2];
-  split_lengths(a, wide, wide + 2, split);
-  const int at = kind ? split[1] : split[0];
-  const int parts = parts_of(seen, at, kind);
+  split_lengths(a, ranges, split);
+  const int parts = parts_of(seen, kind ? split[1] : split[0], kind);
   const int items = tiles * parts;
   if (kind == 0 && parts > 1 && tiles > 0) atomicMax(&join_rows, c * s.rep);
   int u[6] = {kind ? 0 : items, kind || parts == 1 ? 0 : items, kind || parts == 1 ? 0 : tiles,
@@ -295,7 +324,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a
 // Prefix sums of rows, pages and items; one workgroup.
 __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a) {
   __shared__ int tmp[4][kScanWaves];
-  __shared__ unsigned long long wide[4];
+  __shared__ Ranges ranges;
   __shared__ int join_rows;
   int32_t* freed0 = a.scratch + kTsArrays;
   int32_t* taken0 = freed0 + a.n;
@@ -307,10 +336,13 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
   const PagedShape& s = a.shape;
   const bool plan = a.plan != nullptr;
   const int room = table_room(a);
-  if (threadIdx.x < 4) wide[threadIdx.x] = 0;
-  if (threadIdx.x == 4) join_rows = 0;
+  if (threadIdx.x == 0) {
+    ranges = Ranges{};
+    join_rows = 0;
+  }
   int rows = 0, freed = 0, taken = 0;
-  unsigned long long work[2] = {0, 0}, count[2] = {0, 0};
+  unsigned long long work[2] = {0, 0};
+  int count[2] = {0, 0}, longest = 0;
   for (int i0 = 0; i0 < a.n; i0 += kScanThreads) {
     const int i = i0 + threadIdx.x;
     int v[3] = {0, 0, 0}, total[3];
@@ -338,11 +370,11 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
       taken0[i] = taken + v[2];
       if (plan) {
         const int kind = kind_of(s, mine);
-        const unsigned long long tiles = tiles_of(s, mine, kind);
+        const int tiles = tiles_of(s, mine, kind);
         const int len = min(l.x + mine, room);
-        const unsigned long long w = tiles * len;
-        work[kind] += w;
+        work[kind] += static_cast<unsigned long long>(tiles) * len;
         count[kind] += tiles;
+        if (kind == 0 && tiles > 0) longest = max(longest, len);
       }
     }
     rows = min(rows + total[0], a.rows);
@@ -350,19 +382,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
     taken += total[2];
   }
   const int top = min(max(a.counts[0], 0), a.num_pages);
-  if (plan) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      for (int off = 1; off < kWave; off <<= 1) {
-        work[k] += __shfl_xor(work[k], off, kWave);
-        count[k] += __shfl_xor(count[k], off, kWave);
-      }
-      if ((threadIdx.x & 63) == 0 && count[k] != 0) {
-        atomicAdd(&wide[k], work[k]);
-        atomicAdd(&wide[2 + k], count[k]);
-      }
-    }
-  }
+  if (plan) add_ranges(ranges, work, count, longest);
   __syncthreads();  // every thread has read counts, and written what others read below
   if (threadIdx.x == 0) {
     a.row_indptr[a.n] = rows;
@@ -373,7 +393,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
     a.counts[1] = max(taken - top - freed, 0);
   }
   int split[2] = {INT32_MAX, INT32_MAX};
-  if (plan) split_lengths(a, wide, wide + 2, split);
+  if (plan) split_lengths(a, ranges, split);
   const int have = top + freed;
   int base[2][3] = {{0, 0, 0}, {0, 0, 0}};  // items, slots, joins so far of each kind
   for (int i0 = 0; i0 < a.n; i0 += kScanThreads) {
@@ -390,8 +410,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
     if (!plan) continue;
     const int kind = kind_of(s, c);
     const int tiles = tiles_of(s, c, kind);
-    const int at = kind ? split[1] : split[0];
-    const int parts = parts_of(len, at, kind);
+    const int parts = parts_of(len, kind ? split[1] : split[0], kind);
     const int items = tiles * parts;
     if (kind == 0 && parts > 1 && tiles > 0) atomicMax(&join_rows, c * s.rep);
     int v[3] = {kind ? 0 : items, kind ? 0 : (parts > 1 ? items : 0), kind ? 0 : (parts > 1 ? tiles : 0)}, t[3];
@@ -622,7 +641,7 @@ bool paged_shape(int n, int rows, int max_new, int64_t max_kv, int heads, int kv
                                    : all / kd.bm + std::min<int64_t>(n, all / (s->kind[0].bm + 1));
     // Parts of a tile: at most its length / split + 1, and the lengths of all
     // tiles over the split are at most the parts that fill the chip.
-    const int64_t extra = !occurs || max_kv <= (k ? kApMinSplitLong : kApMinSplit) ? 0 : s->target / kv_heads + 1;
+    const int64_t extra = !occurs || max_kv <= (k ? kApMinSplitLong : kApMinSplit + kApKeep) ? 0 : s->target / kv_heads + 1;
     const int64_t slots = extra > 0 ? std::min(tiles, static_cast<int64_t>(kApWhole) * s->target / kv_heads + 1) + extra : 0;
     if (tiles + extra > INT32_MAX / 64) return false;
     kd.item_cap = static_cast<int>(tiles + extra);

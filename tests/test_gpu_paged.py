@@ -221,7 +221,8 @@ def test_paged_attention_random_shapes(dev, seed):
     check_attention(got, q, keys, values, table, start, new, d ** -0.5, dtype)
 
 
-@pytest.mark.parametrize("new,start", [([1, 1], [40, 300]), ([20, 3], [7, 600]), ([150, 1], [33, 30])])
+@pytest.mark.parametrize("new,start", [([1, 1], [40, 300]), ([20, 3], [7, 600]), ([150, 1], [33, 30]),
+                                       ([3, 1], [1300, 90])])
 def test_nothing_behind_a_row_reaches_it(dev, new, start):
     """NaN and infinities in the free pages, in the pages behind the requests' ends and in later tokens of a chunk."""
     dtype, heads, kv_heads, d, page = torch.bfloat16, 8, 2, 128, 32
@@ -273,7 +274,7 @@ def test_extreme_scores(dev):
         check_attention(paged_attention(q, keys, values, step, 1.0), q, keys, values, table, [299], [1], 1.0, torch.bfloat16)
 
 
-@pytest.mark.parametrize("new,start", [([1], [70]), ([50], [70])])
+@pytest.mark.parametrize("new,start", [([1], [70]), ([50], [70]), ([1], [1500])])
 @pytest.mark.parametrize("scale", [0.0, -0.3])
 def test_scales_that_are_not_positive(dev, new, start, scale):
     q, keys, values, table, step = cache_case(dev, new, start, 4, 2, 64, 16, torch.bfloat16, 2)
