@@ -7,8 +7,8 @@
 // the free stack, so nothing is claimed by atomics and a step gives the same
 // pages every time.  The bytes are kilobytes: launches and the chain of reads
 // bound it, hence one workgroup and one launch for all but the largest steps:
-// 168 requests of one token 6.8 us on average, of a step and its taking back.
-// Beyond, two launches: 9.6 + 2.6 us for 4139 rows of 72 requests.
+// 168 requests of one token 6.6 us on average, of a step and its taking back.
+// Beyond, two launches: 9.4 + 3.1 us for 4139 rows of 72 requests.
 //
 // Write: bound by its bytes, read and written once each.  4075 rows of 32 + 2 *
 // 8 heads of 128, 102 MB, take 24.3 to 26.3 us, 3.9 to 4.2 TB/s; 64 rows 3.4.
@@ -26,9 +26,9 @@ constexpr int kScanThreads = 1024;
 constexpr int kScanWaves = kScanThreads / kWave;
 // Steps of up to this many requests and rows run as one launch of one
 // workgroup; beyond, one workgroup's turns cost more than a second launch.  A
-// step and its taking back, replayed: 168 requests of one token 12.0 us
-// against 19.1 with two launches each, eight prompts of 128 tokens 13.1
-// against 19.6, of 512 17.7 against 18.9, of 1024 24.0 against 19.0.
+// step and its taking back (of one launch), replayed: 168 requests of one token
+// 12.2 us against 18.1 with two launches each, eight prompts of 128 tokens 13.1
+// against 18.5; of 512 17.7 against 15.9, of 1024 24.1 against 15.9.
 constexpr int kSmallRequests = kScanThreads;
 constexpr int kSmallRows = 2048;
 
