@@ -530,6 +530,9 @@ bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
   return false;
 }
 
+// Inference tensors are written in inference mode only (no version counter).
+bool may_write(const at::Tensor& t) { return !t.is_inference() || c10::InferenceMode::is_enabled(); }
+
 bool is_i32(const at::Tensor* t, at::Device dev, int64_t n) {
   return t != nullptr && t->scalar_type() == at::kInt && t->device() == dev && t->dim() == 1 && t->size(0) == n && t->is_contiguous();
 }
@@ -590,7 +593,7 @@ PyObject* paged_attention(PyObject* const* args, Took* took) {
     out = at::empty({rows, width}, q->options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
   } else {
     const at::Tensor* o = tensor_of(args[5]);
-    if (!is_rows_of(o, dev, dt, rows, width) || wants_grad({o})) return nullptr;
+    if (!is_rows_of(o, dev, dt, rows, width) || wants_grad({o}) || !may_write(*o)) return nullptr;
     out = *o;
   }
   const float scale = static_cast<float>(PyFloat_AS_DOUBLE(args[4]));
@@ -604,7 +607,9 @@ PyObject* paged_attention(PyObject* const* args, Took* took) {
                                st.kv_heads, st.head_dim, scale, code, stream);
   });
   *took = outcome(rc, "mlora_paged_attention");
-  return *took == Took::kYes ? THPVariable_Wrap(std::move(out)) : nullptr;
+  if (*took != Took::kYes) return nullptr;
+  if (args[5] != Py_None) out.unsafeGetTensorImpl()->bump_version();  // written in place
+  return THPVariable_Wrap(std::move(out));
 }
 
 // kernels.paged.rotary_paged_write: the rotated q, new or given.
@@ -622,7 +627,7 @@ PyObject* paged_write(PyObject* const* args, Took* took) {
       !is_rows_of(v, dev, dt, rows, pool.kv_heads * pool.d) || !is_i32(slots, dev, rows) ||
       wants_grad({q, k, v, cs, sn, kp, vp}))
     return nullptr;
-  if ((kp->is_inference() || vp->is_inference()) && !c10::InferenceMode::is_enabled()) return nullptr;
+  if (!may_write(*kp) || !may_write(*vp)) return nullptr;
   int64_t rot[2];
   const at::Tensor* tabs[2] = {cs, sn};
   for (int i = 0; i < 2; ++i) {
@@ -639,7 +644,7 @@ PyObject* paged_write(PyObject* const* args, Took* took) {
     out = at::empty({rows, heads * pool.d}, q->options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
   } else {
     const at::Tensor* o = tensor_of(args[8]);
-    if (!is_rows_of(o, dev, dt, rows, heads * pool.d) || wants_grad({o})) return nullptr;
+    if (!is_rows_of(o, dev, dt, rows, heads * pool.d) || wants_grad({o}) || !may_write(*o)) return nullptr;
     out = *o;
   }
   const hipStream_t stream = stream_of(dev);
@@ -658,6 +663,7 @@ PyObject* paged_write(PyObject* const* args, Took* took) {
   if (*took != Took::kYes) return nullptr;
   kp->unsafeGetTensorImpl()->bump_version();  // written in place
   vp->unsafeGetTensorImpl()->bump_version();
+  if (args[8] != Py_None) out.unsafeGetTensorImpl()->bump_version();
   return THPVariable_Wrap(std::move(out));
 }
 

@@ -48,6 +48,13 @@ def _no_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
         raise RuntimeError(f"{what} has no backward pass; call it under torch.no_grad() or on detached tensors")
 
 
+def _writes(what: str, *tensors: torch.Tensor) -> None:
+    """Tensors that a call is going to write."""
+    _no_grad(what, *tensors)
+    if any(t.is_inference() for t in tensors) and not torch.is_inference_mode_enabled():
+        raise RuntimeError(f"{what} writes in place: inference tensors need inference mode")
+
+
 def _guard(device: torch.device):
     """A launch goes to the current device."""
     return nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
@@ -271,8 +278,8 @@ def rotary_paged_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: t
     rot_stride = [0 if t.shape[0] == 1 else t.stride(0) for t in (cos, sin)]
     if cos.dtype != sin.dtype or rot_stride[0] != rot_stride[1]:
         raise ValueError("cos and sin must have one dtype and row stride")
-    if (keys.is_inference() or values.is_inference()) and not torch.is_inference_mode_enabled():
-        raise RuntimeError("rotary_paged_write writes in place: inference tensors need inference mode")
+    written = (keys, values) if out is None else (keys, values, out)
+    _writes("rotary_paged_write", *written)
     if out is None:
         out = torch.empty((rows, heads * d), dtype=dt, device=dev)
     else:
@@ -289,7 +296,7 @@ def rotary_paged_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: t
             values.stride(0) if pages > 1 else kv_heads * page * d, pages, page, out.data_ptr(), stride(out),
             _ffi.dtype_code(dt), _ffi.stream_ptr(dev))
     _ffi.check(rc, "mlora_rotary_paged_write")
-    torch.autograd.graph.increment_version((keys, values))
+    torch.autograd.graph.increment_version(written)
     return out
 
 
@@ -325,12 +332,13 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, s
         raise ValueError(f"the pool has {pages} pages, the page tables give out {step.state.free.numel()}")
     if step.rows > 1 and q.stride(0) % 8 or q.data_ptr() % 16:
         q = q.contiguous() if not q.is_contiguous() else q.clone()
-    if out is None:
-        out = torch.empty((step.rows, width), dtype=dt, device=dev)
-    else:
+    given = out is not None
+    if given:
         _on_gpu("paged_attention", q, out)
-        _no_grad("paged_attention", out)
+        _writes("paged_attention", out)
         _rows("out", out, step.rows, width, dt)
+    else:
+        out = torch.empty((step.rows, width), dtype=dt, device=dev)
     stride = lambda t: t.stride(0) if step.rows > 1 else width  # noqa: E731
     with _guard(dev):
         rc = _ffi.lib().mlora_paged_attention(
@@ -339,6 +347,8 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, s
             ctypes.byref(step._c), out.data_ptr(), stride(out), step.heads, kv_heads, d, float(scale),
             _ffi.dtype_code(dt), _ffi.stream_ptr(dev))
     _ffi.check(rc, "mlora_paged_attention")
+    if given:
+        torch.autograd.graph.increment_version(out)
     return out
 
 

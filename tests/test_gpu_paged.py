@@ -1,10 +1,12 @@
 """The paged KV cache's operators (GPU) against plain 64-bit forms, at the sizes and masks where they can go wrong."""
 
 import random
+from types import SimpleNamespace
 
 import pytest
 import torch
 
+from multi_lora_amd import _ffi
 from multi_lora_amd.kernels import PagedStep, PageState, page_tables, paged_attention, rotary_paged_write, verify_drafts
 
 from tests import paged_ref as ref
@@ -295,6 +297,32 @@ def test_rows_behind_the_last_request_are_left(dev):
     assert paged_attention(q, keys, values, step, 0.125, out=out) is out
     assert bool((out[4:] == 7.0).all())
     check_attention(out, q, keys, values, table, [0, 20], [3, 1], 0.125, torch.float16)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_given_outputs_are_written_in_place(dev, monkeypatch, native):
+    """Autograd sees the write; what needs a gradient, or inference mode, is refused."""
+    q, keys, values, table, step = cache_case(dev, [3, 1], [0, 20], 4, 2, 64, 16, torch.float16, 3)
+    if not native:
+        monkeypatch.setattr(_ffi, "calls", lambda: SimpleNamespace(paged_write=lambda *a: None, paged_attention=lambda *a: None))
+    rows = q.shape[0]
+    k = torch.randn(rows, 128, device=dev).half()
+    cos = torch.randn(rows, 64, device=dev).half()
+    for call in (lambda out: paged_attention(q, keys, values, step, 0.125, out=out),
+                 lambda out: rotary_paged_write(q, k, k, cos, cos, keys, values, step.slots, out=out)):
+        out = torch.ones_like(q)
+        w = torch.ones_like(q, requires_grad=True)
+        y = w * out
+        assert call(out) is out
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            call(torch.ones_like(q, requires_grad=True))
+        with torch.inference_mode():
+            inside = torch.ones_like(q)
+            call(inside)
+        with pytest.raises(RuntimeError, match="inference mode"):
+            call(inside)
 
 
 def test_strided_rows_pages_and_outputs(dev):
