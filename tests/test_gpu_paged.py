@@ -392,7 +392,7 @@ def probabilities(g, shape, dtype, dev, std=2.0):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("ks,vocab,certain", [
     ([4], 512, False), ([0, 1, 2, 3], 1, False), ([3, 0, 5], 4097, False), ([3, 1], 2049, False), ([2, 2], 4096, True), ([70, 64, 1], 777, False),
-    ([4] * 20, 12289, False), ([1, 8, 0], 128256, True),
+    ([4] * 20, 12289, False), ([1, 8, 0], 128256, True), ([2, 0, 3, 1], 290001, False),
 ])
 def test_verify_drafts(dev, ks, vocab, certain, dtype):
     g = torch.Generator(dev).manual_seed(vocab + len(ks))
@@ -464,7 +464,8 @@ def test_verify_strided_and_empty(dev):
 
 
 # ---------------------------------------------------------------- together, captured
-def test_steps_captured_and_replayed(dev):
+@pytest.mark.parametrize("longest", [600, 1600])  # without and with room for split ranges
+def test_steps_captured_and_replayed(dev, longest):
     """Tables, write, attention and verification of a step in one graph, replayed with other lengths, equal the eager calls."""
     heads, kv_heads, d, page, n, most = 8, 2, 64, 16, 5, 3
     rows, vocab = n * (most + 1), 640
@@ -479,7 +480,7 @@ def test_steps_captured_and_replayed(dev):
     start, new = i32([0] * n, dev), i32([4] * n, dev)
 
     def fresh():
-        return (PageState.new(n, 600, 200, page, dev), torch.zeros(200, kv_heads, page, d, device=dev).half(),
+        return (PageState.new(n, longest, 200, page, dev), torch.zeros(200, kv_heads, page, d, device=dev).half(),
                 torch.zeros(200, kv_heads, d, page, device=dev).half())
 
     def make(state):
@@ -505,7 +506,7 @@ def test_steps_captured_and_replayed(dev):
     with torch.cuda.graph(graph, stream=side):
         res = run(*mine, sa, oa)
     for lens in ([[0] * n, [4, 1, 2, 3, 4]], [[4, 1, 2, 3, 4], [1] * n], [[300, 2, 0, 4, 5], [4, 0, 4, 1, 2]],
-                 [[0, 0, 590, 4, 5], [0, 1, 4, 4, 4]]):
+                 [[0, 0, 590, 4, 5], [0, 1, 4, 4, 4]], [[longest - 10, 2, 0, 4, 5], [4, 0, 4, 1, 2]]):
         start.copy_(i32(lens[0], dev))
         new.copy_(i32(lens[1], dev))
         oa.fill_(3.0), ob.fill_(3.0)
