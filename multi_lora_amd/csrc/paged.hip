@@ -76,30 +76,45 @@ __device__ int take_page(const TablesArgs& a, int t, int top, int freed) {
   return a.table[static_cast<int64_t>(lo) * a.table_stride + pages_for(l.x + l.y, a) + (t - freed0[lo])];
 }
 
+// Inclusive sums over the lanes of each row of 16, and over the wave, by lane
+// moves (a lane without a source gets 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int row_sum(int v) {
+  v += moved<0x111, 0xf>(v);  // row_shr:1
+  v += moved<0x112, 0xf>(v);  // row_shr:2
+  v += moved<0x114, 0xf>(v);  // row_shr:4
+  v += moved<0x118, 0xf>(v);  // row_shr:8
+  return v;
+}
+__device__ __forceinline__ int lane_sum(int v) {
+  v = row_sum(v);
+  v += moved<0x142, 0xa>(v);  // the last lane of rows 0 and 2 to rows 1 and 3
+  v += moved<0x143, 0xc>(v);  // lane 31 to the upper two rows
+  return v;
+}
+
 // Exclusive sums over the workgroup of N values that fit 31 bits, and their
 // totals; the values share the two barriers.
 template <int N>
 __device__ __forceinline__ void scan(int (&v)[N], int (&total)[N], int (*tmp)[kScanWaves]) {
+  static_assert(kScanWaves == 16, "the waves' sums are a row of lanes");
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
-  int x[N];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-  for (int k = 0; k < N; ++k) x[k] = wave_incl_sum(v[k]);
-  if (lane == kWave - 1)
-#pragma unroll
-    for (int k = 0; k < N; ++k) tmp[k][wave] = x[k];
+  for (int k = 0; k < N; ++k) {
+    const int x = lane_sum(v[k]);
+    if (lane == kWave - 1) tmp[k][wave] = x;
+    v[k] = x - v[k];
+  }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kScanWaves; ++w) {
-      const int t = tmp[k][w];
-      before += w < wave ? t : 0;
-      all += t;
-    }
-    v[k] = before + x[k] - v[k];
-    total[k] = all;
+    const int t = row_sum(tmp[k][lane & 15]);
+    total[k] = __builtin_amdgcn_readlane(t, 15);
+    if (wave > 0) v[k] += __builtin_amdgcn_readlane(t, wave - 1);
   }
   __syncthreads();
 }
@@ -167,6 +182,14 @@ __device__ __forceinline__ int parts_of(int len, int split, int kind) {
   return kind ? max(len / split, 1) : len > split ? (len + split - 1) / split : 1;
 }
 
+// Short items go on the list in three groups, the longest first: what starts
+// last then ends soon after the rest.  300 requests of 100 positions before 20
+// of 3000 took 98 us, behind them 82.
+__device__ __forceinline__ int group_of(int len, int parts, int longest) {
+  const int64_t all = static_cast<int64_t>(longest) * parts;
+  return 2ll * len > all ? 0 : 4ll * len > all ? 1 : 2;
+}
+
 // Tile t of a request's `tiles`, those of the longest ranges first, in `parts`
 // items.  (The host's bounds leave room for all of them.)
 __device__ __forceinline__ void put_items(const TablesArgs& a, const PagedKind& kd, int i, int first, int c, int len, int room,
@@ -211,7 +234,7 @@ __device__ __forceinline__ int last_at_most(const int* x, int n, int v) {
 // A step of few requests and rows in one workgroup and one launch: thread =
 // request for the sums and the work list, then row, then page.
 __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a) {
-  __shared__ int tmp[6][kScanWaves];
+  __shared__ int tmp[8][kScanWaves];
   __shared__ Ranges ranges;
   __shared__ int join_rows;
   __shared__ int first_s[kSmallRequests], freed_s[kSmallRequests], taken_s[kSmallRequests], need_s[kSmallRequests],
@@ -307,23 +330,26 @@ __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a
   const int parts = parts_of(seen, kind ? split[1] : split[0], kind);
   const int items = tiles * parts;
   if (kind == 0 && parts > 1 && tiles > 0) atomicMax(&join_rows, c * s.rep);
-  int u[6] = {kind ? 0 : items, kind || parts == 1 ? 0 : items, kind || parts == 1 ? 0 : tiles,
-              kind ? items : 0, kind && parts > 1 ? items : 0,  kind && parts > 1 ? tiles : 0};
-  int sums[6];
+  const int group = group_of(seen, parts, min(split[0], ranges.longest));
+  const int shorts = kind ? 0 : items;
+  int u[8] = {group == 0 ? shorts : 0, group == 1 ? shorts : 0, group == 2 ? shorts : 0, parts > 1 ? shorts : 0,
+              kind || parts == 1 ? 0 : tiles, kind ? items : 0, kind && parts > 1 ? items : 0, kind && parts > 1 ? tiles : 0};
+  int sums[8];
   scan(u, sums, tmp);
   const PagedKind kd = kind ? s.kind[1] : s.kind[0];
-  const int it = kind ? u[3] : u[0], sl = kind ? u[4] : u[1], jn = kind ? u[5] : u[2];
+  const int listed = group == 0 ? u[0] : group == 1 ? sums[0] + u[1] : sums[0] + sums[1] + u[2];
+  const int it = kind ? u[5] : listed, sl = kind ? u[6] : u[3], jn = kind ? u[7] : u[4];
   for (int t = 0; t < tiles; ++t) put_items(a, kd, i, first_s[i], c, len, room, tiles, t, parts, it + t * parts, sl + t * parts, jn + t);
   if (i < 2) {
-    a.plan[i ? kApLong : kApShort] = min(i ? sums[3] : sums[0], s.kind[i].item_cap);
-    a.plan[(i ? kApLong : kApShort) + 1] = min(i ? sums[5] : sums[2], s.kind[i].join_cap);
+    a.plan[i ? kApLong : kApShort] = min(i ? sums[5] : sums[0] + sums[1] + sums[2], s.kind[i].item_cap);
+    a.plan[(i ? kApLong : kApShort) + 1] = min(i ? sums[7] : sums[4], s.kind[i].join_cap);
   }
   if (i == 2) a.plan[kApJoinRows] = join_rows;
 }
 
 // Prefix sums of rows, pages and items; one workgroup.
 __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a) {
-  __shared__ int tmp[4][kScanWaves];
+  __shared__ int tmp[5][kScanWaves];
   __shared__ Ranges ranges;
   __shared__ int join_rows;
   int32_t* freed0 = a.scratch + kTsArrays;
@@ -413,21 +439,25 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
     const int parts = parts_of(len, kind ? split[1] : split[0], kind);
     const int items = tiles * parts;
     if (kind == 0 && parts > 1 && tiles > 0) atomicMax(&join_rows, c * s.rep);
-    int v[3] = {kind ? 0 : items, kind ? 0 : (parts > 1 ? items : 0), kind ? 0 : (parts > 1 ? tiles : 0)}, t[3];
+    const int group = group_of(len, parts, min(split[0], ranges.longest));
+    const int shorts = kind ? 0 : items;
+    int v[5] = {parts > 1 ? shorts : 0, kind || parts == 1 ? 0 : tiles, group == 0 ? shorts : 0, group == 1 ? shorts : 0,
+                group == 2 ? shorts : 0}, t[5];
     int u[3] = {kind ? items : 0, kind && parts > 1 ? items : 0, kind && parts > 1 ? tiles : 0}, tu[3];
     scan(v, t, tmp);
     scan(u, tu, tmp);
-    if (i < a.n) {
-      item0[i] = kind ? base[1][0] + u[0] : base[0][0] + v[0];
-      slot0[i] = kind ? base[1][1] + u[1] : base[0][1] + v[1];
-      join0[i] = kind ? base[1][2] + u[2] : base[0][2] + v[2];
+    if (i < a.n) {  // (the groups of 1024 requests at a time)
+      const int listed = group == 0 ? v[2] : group == 1 ? t[2] + v[3] : t[2] + t[3] + v[4];
+      item0[i] = kind ? base[1][0] + u[0] : base[0][0] + listed;
+      slot0[i] = kind ? base[1][1] + u[1] : base[0][1] + v[0];
+      join0[i] = kind ? base[1][2] + u[2] : base[0][2] + v[1];
       parts0[i] = parts;
     }
+    base[0][0] += t[2] + t[3] + t[4];
+    base[0][1] += t[0];
+    base[0][2] += t[1];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      base[0][k] += t[k];
-      base[1][k] += tu[k];
-    }
+    for (int k = 0; k < 3; ++k) base[1][k] += tu[k];
   }
   if (!plan) return;
   __syncthreads();
