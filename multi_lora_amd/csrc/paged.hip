@@ -7,8 +7,8 @@
 // the free stack, so nothing is claimed by atomics and a step gives the same
 // pages every time.  The bytes are kilobytes: launches and the chain of reads
 // bound it, hence one workgroup and one launch for all but the largest steps:
-// 168 requests of one token 6.6 us on average, of a step and its taking back.
-// Beyond, two launches: 9.4 + 3.1 us for 4139 rows of 72 requests.
+// 168 requests of one token 5.6 us on average, of a step and its taking back.
+// Beyond, two launches: 7.0 + 2.8 us for 4139 rows of 72 requests.
 //
 // Write: bound by its bytes, read and written once each.  4075 rows of 32 + 2 *
 // 8 heads of 128, 102 MB, take 24.3 to 26.3 us, 3.9 to 4.2 TB/s; 64 rows 3.4.
@@ -27,8 +27,8 @@ constexpr int kScanWaves = kScanThreads / kWave;
 // Steps of up to this many requests and rows run as one launch of one
 // workgroup; beyond, one workgroup's turns cost more than a second launch.  A
 // step and its taking back (of one launch), replayed: 168 requests of one token
-// 12.2 us against 18.1 with two launches each, eight prompts of 128 tokens 13.1
-// against 18.5; of 512 17.7 against 15.9, of 1024 24.1 against 15.9.
+// 9.4 us against 15.1 with two launches each, eight prompts of 128 tokens 10.5
+// against 15.2; of 512 15.6 against 12.9, of 1024 22.5 against 13.0.
 constexpr int kSmallRequests = kScanThreads;
 constexpr int kSmallRows = 2048;
 
@@ -184,7 +184,7 @@ __device__ __forceinline__ int parts_of(int len, int split, int kind) {
 
 // Short items go on the list in three groups, the longest first: what starts
 // last then ends soon after the rest.  300 requests of 100 positions before 20
-// of 3000 took 98 us, behind them 82.
+// of 3000 took 98 us in the requests' order, 81 in this.
 __device__ __forceinline__ int group_of(int len, int parts, int longest) {
   const int64_t all = static_cast<int64_t>(longest) * parts;
   return 2ll * len > all ? 0 : 4ll * len > all ? 1 : 2;
