@@ -132,27 +132,26 @@ __device__ __forceinline__ int table_room(const TablesArgs& a) {
 }
 
 // What the ranges' split is found from, summed over the workgroup: positions of
-// all tiles and tiles of each kind, and the longest short range.
+// all tiles, tiles and the longest range of each kind.
 struct Ranges {
   unsigned long long work[2], tiles[2];
-  int longest;
+  int longest[2];
 };
 
-__device__ __forceinline__ void add_ranges(Ranges& r, unsigned long long (&work)[2], int (&tiles)[2], int longest) {
+__device__ __forceinline__ void add_ranges(Ranges& r, unsigned long long (&work)[2], int (&tiles)[2], int (&longest)[2]) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     if (__ballot(tiles[k] != 0) == 0) continue;
     for (int off = 1; off < kWave; off <<= 1) {
       work[k] += __shfl_xor(work[k], off, kWave);
       tiles[k] += __shfl_xor(tiles[k], off, kWave);
+      longest[k] = max(longest[k], __shfl_xor(longest[k], off, kWave));
     }
     if ((threadIdx.x & 63) == 0) {
       atomicAdd(&r.work[k], work[k]);
       atomicAdd(&r.tiles[k], static_cast<unsigned long long>(tiles[k]));
+      atomicMax(&r.longest[k], longest[k]);
     }
-    if (k > 0) continue;
-    for (int off = 1; off < kWave; off <<= 1) longest = max(longest, __shfl_xor(longest, off, kWave));
-    if ((threadIdx.x & 63) == 0) atomicMax(&r.longest, longest);
   }
 }
 
@@ -171,7 +170,7 @@ __device__ __forceinline__ void split_lengths(const TablesArgs& a, const Ranges&
   }
   const unsigned long long filled = min(2 * r.tiles[0] * a.kv_heads, target);
   const int keep = kApKeep + static_cast<int>(kApKeepFull * filled / target);
-  if (r.longest - keep <= split[0]) split[0] = INT32_MAX;
+  if (r.longest[0] - keep <= split[0]) split[0] = INT32_MAX;
 }
 
 // Parts of a tile of `len` positions.  Short ones round up, so that none is
@@ -182,13 +181,21 @@ __device__ __forceinline__ int parts_of(int len, int split, int kind) {
   return kind ? max(len / split, 1) : len > split ? (len + split - 1) / split : 1;
 }
 
-// Short items go on the list in three groups, the longest first: what starts
-// last then ends soon after the rest.  300 requests of 100 positions before 20
-// of 3000 took 98 us in the requests' order, 81 in this.
-__device__ __forceinline__ int group_of(int len, int parts, int longest) {
-  const int64_t all = static_cast<int64_t>(longest) * parts;
+// The items of a kind go on the list in three groups of requests, the longest
+// first: what starts last then ends soon after the rest.  300 requests of 100
+// positions before 20 of 3000 took 98 us in the requests' order, 81 in this;
+// 20 prompts of 300 before four chunks of 300 after 3000 165 and 142.
+__device__ __forceinline__ int group_of(const Ranges& r, const int (&split)[2], int len, int parts, int kind) {
+  const int longest = kind ? r.longest[1] : min(split[0], r.longest[0]);
+  const int64_t all = static_cast<int64_t>(longest) * (kind ? 1 : parts);
   return 2ll * len > all ? 0 : 4ll * len > all ? 1 : 2;
 }
+struct Groups {  // an item's place from the groups' sums
+  int before[3], total[3];
+  __device__ int at(int group) const {
+    return group == 0 ? before[0] : group == 1 ? total[0] + before[1] : total[0] + total[1] + before[2];
+  }
+};
 
 // Tile t of a request's `tiles`, those of the longest ranges first, in `parts`
 // items.  (The host's bounds leave room for all of them.)
@@ -234,7 +241,7 @@ __device__ __forceinline__ int last_at_most(const int* x, int n, int v) {
 // A step of few requests and rows in one workgroup and one launch: thread =
 // request for the sums and the work list, then row, then page.
 __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a) {
-  __shared__ int tmp[8][kScanWaves];
+  __shared__ int tmp[10][kScanWaves];
   __shared__ Ranges ranges;
   __shared__ int join_rows;
   __shared__ int first_s[kSmallRequests], freed_s[kSmallRequests], taken_s[kSmallRequests], need_s[kSmallRequests],
@@ -323,26 +330,31 @@ __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a
   const unsigned long long positions = static_cast<unsigned long long>(tiles) * seen;
   unsigned long long work[2] = {kind ? 0 : positions, kind ? positions : 0};
   int count[2] = {kind ? 0 : tiles, kind ? tiles : 0};
-  add_ranges(ranges, work, count, tiles > 0 && kind == 0 ? seen : 0);
+  int longest[2] = {kind || tiles == 0 ? 0 : seen, kind && tiles > 0 ? seen : 0};
+  add_ranges(ranges, work, count, longest);
   __syncthreads();
   int split[2];
   split_lengths(a, ranges, split);
   const int parts = parts_of(seen, kind ? split[1] : split[0], kind);
   const int items = tiles * parts;
   if (kind == 0 && parts > 1 && tiles > 0) atomicMax(&join_rows, c * s.rep);
-  const int group = group_of(seen, parts, min(split[0], ranges.longest));
-  const int shorts = kind ? 0 : items;
-  int u[8] = {group == 0 ? shorts : 0, group == 1 ? shorts : 0, group == 2 ? shorts : 0, parts > 1 ? shorts : 0,
-              kind || parts == 1 ? 0 : tiles, kind ? items : 0, kind && parts > 1 ? items : 0, kind && parts > 1 ? tiles : 0};
-  int sums[8];
+  const int group = group_of(ranges, split, seen, parts, kind);
+  int u[10], sums[10];  // items by kind and group, then slots and joins
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int g = 0; g < 3; ++g) u[3 * k + g] = kind == k && group == g ? items : 0;
+    u[6 + k] = kind == k && parts > 1 ? items : 0;
+    u[8 + k] = kind == k && parts > 1 ? tiles : 0;
+  }
   scan(u, sums, tmp);
   const PagedKind kd = kind ? s.kind[1] : s.kind[0];
-  const int listed = group == 0 ? u[0] : group == 1 ? sums[0] + u[1] : sums[0] + sums[1] + u[2];
-  const int it = kind ? u[5] : listed, sl = kind ? u[6] : u[3], jn = kind ? u[7] : u[4];
+  const Groups listed = kind ? Groups{{u[3], u[4], u[5]}, {sums[3], sums[4], sums[5]}} : Groups{{u[0], u[1], u[2]}, {sums[0], sums[1], sums[2]}};
+  const int it = listed.at(group), sl = kind ? u[7] : u[6], jn = kind ? u[9] : u[8];
   for (int t = 0; t < tiles; ++t) put_items(a, kd, i, first_s[i], c, len, room, tiles, t, parts, it + t * parts, sl + t * parts, jn + t);
   if (i < 2) {
-    a.plan[i ? kApLong : kApShort] = min(i ? sums[5] : sums[0] + sums[1] + sums[2], s.kind[i].item_cap);
-    a.plan[(i ? kApLong : kApShort) + 1] = min(i ? sums[7] : sums[4], s.kind[i].join_cap);
+    a.plan[i ? kApLong : kApShort] = min(i ? sums[3] + sums[4] + sums[5] : sums[0] + sums[1] + sums[2], s.kind[i].item_cap);
+    a.plan[(i ? kApLong : kApShort) + 1] = min(i ? sums[9] : sums[8], s.kind[i].join_cap);
   }
   if (i == 2) a.plan[kApJoinRows] = join_rows;
 }
@@ -368,7 +380,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
   }
   int rows = 0, freed = 0, taken = 0;
   unsigned long long work[2] = {0, 0};
-  int count[2] = {0, 0}, longest = 0;
+  int count[2] = {0, 0}, longest[2] = {0, 0};
   for (int i0 = 0; i0 < a.n; i0 += kScanThreads) {
     const int i = i0 + threadIdx.x;
     int v[3] = {0, 0, 0}, total[3];
@@ -400,7 +412,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
         const int len = min(l.x + mine, room);
         work[kind] += static_cast<unsigned long long>(tiles) * len;
         count[kind] += tiles;
-        if (kind == 0 && tiles > 0) longest = max(longest, len);
+        if (tiles > 0) longest[kind] = max(longest[kind], len);
       }
     }
     rows = min(rows + total[0], a.rows);
@@ -439,25 +451,23 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
     const int parts = parts_of(len, kind ? split[1] : split[0], kind);
     const int items = tiles * parts;
     if (kind == 0 && parts > 1 && tiles > 0) atomicMax(&join_rows, c * s.rep);
-    const int group = group_of(len, parts, min(split[0], ranges.longest));
-    const int shorts = kind ? 0 : items;
-    int v[5] = {parts > 1 ? shorts : 0, kind || parts == 1 ? 0 : tiles, group == 0 ? shorts : 0, group == 1 ? shorts : 0,
-                group == 2 ? shorts : 0}, t[5];
-    int u[3] = {kind ? items : 0, kind && parts > 1 ? items : 0, kind && parts > 1 ? tiles : 0}, tu[3];
-    scan(v, t, tmp);
-    scan(u, tu, tmp);
-    if (i < a.n) {  // (the groups of 1024 requests at a time)
-      const int listed = group == 0 ? v[2] : group == 1 ? t[2] + v[3] : t[2] + t[3] + v[4];
-      item0[i] = kind ? base[1][0] + u[0] : base[0][0] + listed;
-      slot0[i] = kind ? base[1][1] + u[1] : base[0][1] + v[0];
-      join0[i] = kind ? base[1][2] + u[2] : base[0][2] + v[1];
-      parts0[i] = parts;
-    }
-    base[0][0] += t[2] + t[3] + t[4];
-    base[0][1] += t[0];
-    base[0][2] += t[1];
+    const int group = group_of(ranges, split, len, parts, kind);
 #pragma unroll
-    for (int k = 0; k < 3; ++k) base[1][k] += tu[k];
+    for (int k = 0; k < 2; ++k) {  // (the groups of 1024 requests at a time)
+      const int mine = kind == k ? items : 0;
+      int v[5] = {group == 0 ? mine : 0, group == 1 ? mine : 0, group == 2 ? mine : 0, parts > 1 ? mine : 0,
+                  kind == k && parts > 1 ? tiles : 0}, t[5];
+      scan(v, t, tmp);
+      if (i < a.n && kind == k) {
+        item0[i] = base[k][0] + Groups{{v[0], v[1], v[2]}, {t[0], t[1], t[2]}}.at(group);
+        slot0[i] = base[k][1] + v[3];
+        join0[i] = base[k][2] + v[4];
+        parts0[i] = parts;
+      }
+      base[k][0] += t[0] + t[1] + t[2];
+      base[k][1] += t[3];
+      base[k][2] += t[4];
+    }
   }
   if (!plan) return;
   __syncthreads();
