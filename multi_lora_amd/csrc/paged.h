@@ -92,6 +92,7 @@ struct WriteArgs {
   int num_pages, page_shift;
   void* q_out;
   int64_t q_out_stride;
+  int value_rows;    // rows whose values a wave looks after (at most 8); set by the launch
 };
 hipError_t launch_rotary_paged_write(const WriteArgs& a, int dtype, int head_dim, bool aligned, hipStream_t stream);
 

@@ -11,7 +11,8 @@
 // Beyond, two launches: 7.0 + 2.8 us for 4139 rows of 72 requests.
 //
 // Write: bound by its bytes, read and written once each.  4075 rows of 32 + 2 *
-// 8 heads of 128, 102 MB, take 24.3 to 26.3 us, 3.9 to 4.2 TB/s; 64 rows 3.4.
+// 8 heads of 128, 102 MB, take 20.2 us, 5.1 TB/s, the rate of a large copy; 64
+// rows 3.8.
 #include <algorithm>
 
 #include "kernels.h"
@@ -561,20 +562,21 @@ __device__ __forceinline__ void rot_chunk(const void* p, int64_t e, bool f32, fl
   }
 }
 
-// Blocks [0, rot_blocks): a thread rotates 8 columns of a head's first half
-// and the 8 they pair with; x * cos + (x rolled by D / 2) * sin in fp32, one
-// rounding.  The rest, values: they lie transposed in a page, so a row alone
-// is D stores of 2 bytes.  A wave takes the run of up to 8 rows whose slots
-// fill one 16-byte chunk of a page, if its row is the run's first (others
-// leave), and stores chunks where the run is whole.
+// Blocks [0, value_blocks): values; they lie transposed in a page, so a row
+// alone is D stores of 2 bytes.  A wave looks at the slots around a few rows:
+// eight rows whose slots fill a 16-byte chunk of a page are stored as chunks by
+// the wave that has the first of them, others one by one.  The rest of the
+// blocks: a thread rotates 8 columns of a head's first half and the 8 they pair
+// with; x * cos + (x rolled by D / 2) * sin in fp32, one rounding.  (Values
+// last: 24.1 us instead of 20.2 for 4075 rows.)
 template <class T, int D, bool AL>
-__global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a, int rot_blocks) {
+__global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a, int value_blocks) {
   using raw = typename T::raw_t;
   const int page = 1 << a.page_shift;
   const int64_t slots = static_cast<int64_t>(a.num_pages) << a.page_shift;
-  if (static_cast<int>(blockIdx.x) < rot_blocks) {
+  if (static_cast<int>(blockIdx.x) >= value_blocks) {
     constexpr int U = D / 16;  // units a head
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t id = (static_cast<int64_t>(blockIdx.x) - value_blocks) * 256 + threadIdx.x;
     const int per_row = (a.heads + a.kv_heads) * U;
     const int r = static_cast<int>(id / per_row);
     if (r >= a.rows) return;
@@ -612,50 +614,79 @@ __global__ __launch_bounds__(256) void paged_write_kernel(WriteArgs a, int rot_b
     store_row_chunk<T, AL>(to + e + D / 2, pack_chunk<T>(y1), 8);
     return;
   }
-  const int64_t w = (static_cast<int64_t>(blockIdx.x) - rot_blocks) * 4 + (threadIdx.x >> 6);
-  const int r = static_cast<int>(w / a.kv_heads);
-  if (r >= a.rows) return;
-  const int g = static_cast<int>(w - static_cast<int64_t>(r) * a.kv_heads);
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t first = w / a.kv_heads * a.value_rows;
+  if (first >= a.rows) return;
+  const int r0 = static_cast<int>(first);
+  const int g = static_cast<int>(w % a.kv_heads);
   const int lane = threadIdx.x & 63;
-  // Lane l looks at row r - 1 + l: is row r the first of its run, and how long is that?
-  const int look = r - 1 + lane;
-  const int seen = lane <= 8 && look >= 0 && look < a.rows ? a.slots[look] : -2;
-  const int slot = __builtin_amdgcn_readlane(seen, 1);
-  if (slot < 0 || slot >= slots) return;
-  if ((slot & 7) != 0 && __builtin_amdgcn_readlane(seen, 0) == slot - 1) return;  // in another row's run
-  const int room = 8 - (slot & 7);
-  const uint64_t next = __ballot(lane >= 1 && lane <= room && seen == slot + lane - 1) >> 1;
-  const int run = __builtin_amdgcn_readfirstlane(__builtin_ctzll(~next));  // rows r .. r + run - 1
-  const raw* v = static_cast<const raw*>(a.v) + r * a.v_stride + g * D;
-  raw* to = static_cast<raw*>(a.values) + static_cast<int64_t>(slot >> a.page_shift) * a.value_stride +
-            static_cast<int64_t>(g) * D * page + (slot & (page - 1));
-  if (AL && run == 8) {
+  // Lane l looks at row r0 - 7 + l.  Bits of lanes: rows with a slot, those in
+  // the slot behind the row before, first ones of eight that fill a chunk.
+  const int look = r0 - 7 + lane;
+  const int seen = lane < a.value_rows + 14 && look >= 0 && look < a.rows ? a.slots[look] : -1;
+  const int before = __shfl_up(seen, 1, kWave);
+  const uint64_t placed = __ballot(seen >= 0 && seen < slots);
+  const uint64_t follows = __ballot(lane > 0 && seen == before + 1);
+  uint64_t whole = AL ? placed & __ballot((seen & 7) == 0) : 0;
 #pragma unroll
-    for (int e0 = 0; e0 < D; e0 += kWave) {
-      const int e = e0 + lane;
+  for (int i = 1; i < 8; ++i) whole &= follows >> i;
+  uint64_t covered = whole;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) covered |= whole << i;
+  const uint64_t mine = ((1ull << a.value_rows) - 1) << 7;
+  const int64_t head = static_cast<int64_t>(g) * D * page;
+  const raw* v = static_cast<const raw*>(a.v) + g * D + lane;
+  raw* values = static_cast<raw*>(a.values) + head + static_cast<int64_t>(lane) * page;
+  auto place = [&](int slot) { return values + static_cast<int64_t>(slot >> a.page_shift) * a.value_stride + (slot & (page - 1)); };
+  for (uint64_t todo = whole & mine; todo != 0; todo &= todo - 1) {
+    const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(todo));
+    const raw* from = v + (r0 - 7 + l) * a.v_stride;
+    raw* to = place(__builtin_amdgcn_readlane(seen, l));
+#pragma unroll
+    for (int e = 0; e < D; e += kWave) {
       u32x4 c;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        c[i] = static_cast<uint32_t>(v[2 * i * a.v_stride + e]) | static_cast<uint32_t>(v[(2 * i + 1) * a.v_stride + e]) << 16;
+        c[i] = static_cast<uint32_t>(from[2 * i * a.v_stride + e]) | static_cast<uint32_t>(from[(2 * i + 1) * a.v_stride + e]) << 16;
       st_chunk(to + static_cast<int64_t>(e) * page, c);
     }
-    return;
   }
-  for (int i = 0; i < run; ++i)
-    for (int e = lane; e < D; e += kWave) to[static_cast<int64_t>(e) * page + i] = v[i * a.v_stride + e];
+  const uint64_t single = placed & mine & ~covered;
+  if (single == 0) return;
+  // The loads of all of the wave's rows go out before the first store.
+  raw x[8][D / kWave];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < a.value_rows)
+#pragma unroll
+      for (int e = 0; e < D / kWave; ++e) x[j][e] = v[min(r0 + j, a.rows - 1) * a.v_stride + e * kWave];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if ((single >> (7 + j) & 1) == 0) continue;
+    raw* to = place(__builtin_amdgcn_readlane(seen, 7 + j));
+#pragma unroll
+    for (int e = 0; e < D / kWave; ++e) to[static_cast<int64_t>(e * kWave) * page] = x[j][e];
+  }
 }
 
+// Rows whose values one wave looks after.  More share the look at the slots and
+// ask for more at once, fewer are more waves: 64 decoding requests 3.8 us with
+// one row, 4.1 with four, 4.9 with eight; 1000 15.9, 13.0, 13.3; 4096 tokens of
+// each of four prompts 136, 99, 92.
+constexpr int value_rows(int rows) { return rows < 128 ? 1 : rows < 2048 ? 4 : 8; }
+
 template <class T, int D>
-hipError_t launch_write(const WriteArgs& a, bool aligned, hipStream_t stream) {
+hipError_t launch_write(WriteArgs a, bool aligned, hipStream_t stream) {
+  a.value_rows = value_rows(a.rows);
   const int64_t units = static_cast<int64_t>(a.rows) * (a.heads + a.kv_heads) * (D / 16);
   const int64_t rot = (units + 255) / 256;
-  const int64_t val = (static_cast<int64_t>(a.rows) * a.kv_heads + 3) / 4;
+  const int64_t val = ((static_cast<int64_t>(a.rows) + a.value_rows - 1) / a.value_rows * a.kv_heads + 3) / 4;
   if (!grid_fits(rot + val)) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(rot + val));
   if (aligned)
-    hipLaunchKernelGGL((paged_write_kernel<T, D, true>), grid, dim3(256), 0, stream, a, static_cast<int>(rot));
+    hipLaunchKernelGGL((paged_write_kernel<T, D, true>), grid, dim3(256), 0, stream, a, static_cast<int>(val));
   else
-    hipLaunchKernelGGL((paged_write_kernel<T, D, false>), grid, dim3(256), 0, stream, a, static_cast<int>(rot));
+    hipLaunchKernelGGL((paged_write_kernel<T, D, false>), grid, dim3(256), 0, stream, a, static_cast<int>(val));
   return hipGetLastError();
 }
 

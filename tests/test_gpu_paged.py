@@ -111,6 +111,7 @@ def half_step(dtype):
     (4, 2, 64, 8, [1], [0], False, 0), (5, 1, 128, 16, [1, 0, 33, 2], [15, 9, 0, 31], False, 3),
     (8, 8, 64, 32, [70, 1, 7], [5, 200, 25], True, 0), (32, 8, 128, 16, [100, 1, 1, 13], [12, 40, 0, 3], True, 8),
     (2, 1, 128, 128, [300], [100], False, 1),
+    (2, 1, 64, 8, [1500, 1, 700, 9], [3, 7, 8, 15], False, 0), (1, 1, 128, 64, [1] * 190, list(range(190)), False, 0),
 ])
 def test_rotary_paged_write(dev, heads, kv_heads, d, page, new, start, f32_tables, pad, dtype):
     g = torch.Generator().manual_seed(sum(new) + d)
