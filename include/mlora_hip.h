@@ -432,7 +432,9 @@ int32_t mlora_page_tables_scratch(int32_t n);
  * stack's top.  Pages given back that nobody takes go on the stack, the last
  * one first: a call that takes pages and a call that gives the same ones back
  * restore it.  A page that the pool cannot give is -1 (later requests get
- * none; held counts those given; asked for again by the next call).
+ * none; held counts those given; asked for again by the next call).  Its
+ * tokens are not written: at most held[i] * page positions of request i are
+ * cached, and no later call's start length may be above that.
  * Writes row_indptr (prefix sums of new_lens, at most `rows`), kv_lens =
  * start + new, positions and slots (0 and -1 for rows behind the last
  * request's), and, if the step has a plan, the work list for `heads` query

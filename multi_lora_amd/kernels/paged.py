@@ -186,8 +186,10 @@ def page_tables(state: PageState, start_lens: torch.Tensor, new_lens: torch.Tens
     Requests take the pages that they lack and give back those past their new
     length (0 and 0: a request that is done; a smaller start: tokens taken
     back), in request order; ``state`` changes in place.  A page that the pool
-    cannot give is counted in ``state.counts[1]``, its tokens have slot -1 and
-    rows that would attend to it are NaN.
+    cannot give is counted in ``state.counts[1]``; its tokens have slot -1 and
+    are not written, and this step's rows that would attend to it are NaN.
+    Such tokens are not cached: the next call, which may get the page, keeps at
+    most ``torch.minimum(step.kv_lens, state.held * state.page)`` positions.
 
     ``rows`` (packed rows, at least the sum of the new lengths) and ``max_new``
     (at least each of them) are the host's bounds: a longer new length counts

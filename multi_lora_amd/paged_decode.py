@@ -17,6 +17,15 @@ those that the target accepts.
 Lengths, pages and positions live on the device (``kernels.page_tables``); no
 step synchronises with the host.  Pages that rejected drafts took go back to
 the pool with the next step's tables.  GPU, float16 or bfloat16 models.
+
+A token that finds no place (the pool is short of pages, or the request is at
+its table's end) is not cached and does not count: ``placed`` says how many of
+each request's tokens the last step had room for.  A request with none keeps
+its length and has to be given the same token again once others have left:
+
+    graph.replay()
+    nxt = out.logits.argmax(-1, keepdim=True)
+    step.input_ids.copy_(torch.where(step.placed[:, None] > 0, nxt, step.input_ids))
 """
 
 from __future__ import annotations
@@ -40,6 +49,7 @@ class PagedDecode:
         self.input_ids = torch.zeros((batch, 1), dtype=torch.long, device=device)
         self.lens = torch.zeros(batch, **i32)         # cached positions of each request
         self.start_lens = torch.zeros(batch, **i32)   # its prompt's length, for rewind
+        self.placed = torch.zeros(batch, **i32)       # tokens of each that the last step had room for
         self.one = torch.ones(batch, **i32)
         self.none = torch.zeros(batch, **i32)
         self.step = self.kv.new_step(batch, 1)
@@ -64,6 +74,9 @@ class PagedDecode:
         counts = [int(p.numel()) for p in prompts]
         if len(counts) != self.batch or min(counts) < 1 or max(counts) >= self.max_len:
             raise ValueError(f"{self.batch} prompts of 1 to {self.max_len - 1} tokens expected, got {counts}")
+        need, pages = sum(-(-c // self.kv.page) for c in counts), self.kv.state.free.numel()
+        if need > pages:
+            raise ValueError(f"the prompts need {need} pages of {self.kv.page} positions, the pool has {pages}")
         device = self.lens.device
         ends = torch.tensor(counts, dtype=torch.int32).cumsum(0) - 1
         self.start = max(counts)
@@ -77,10 +90,12 @@ class PagedDecode:
         return out.logits.argmax(dim=-1, keepdim=True)
 
     def run(self, mgr):
-        """One token of every request: ``input_ids`` at its position, which then advances."""
+        """One token of every request: ``input_ids`` at its position, which then
+        advances.  Logits of a request whose token has no place are NaN."""
         self.kv.tables(self.lens, self.one, self.step)
         out = mgr.model(input_ids=self.input_ids, past_key_values=self.kv, paged_step=self.step)
-        self.lens.add_(1)
+        torch.ge(self.step.slots, 0, out=self.placed)
+        self.lens.add_(self.placed)
         return out
 
     def verify(self, mgr, drafts: torch.Tensor, draft_probs: Optional[torch.Tensor], accept: torch.Tensor,
@@ -89,16 +104,25 @@ class PagedDecode:
         every request in one step; ``kernels.verify_drafts``' accepted counts and
         tokens for the numbers ``accept [batch, k]`` and ``last [batch]``.  Every
         request keeps its accepted drafts, and ``input_ids`` becomes the token
-        after them (0 where the probabilities had no mass)."""
+        after them (0 where the probabilities had no mass).  Drafts without a
+        place are not looked at; a request without any keeps its ``input_ids``,
+        and its tokens are -1."""
         k = int(drafts.shape[1])
         if k not in self._chunks:
             self._chunks[k] = (self.kv.new_step(self.batch * (k + 1), k + 1), torch.full_like(self.one, k + 1))
         step, new = self._chunks[k]
         self.kv.tables(self.lens, new, step)
         ids = torch.cat((self.input_ids, drafts), dim=1)
-        logits = mgr.model(input_ids=ids, past_key_values=self.kv, paged_step=step).logits
+        # A request's first rows are the ones with a place: they come first among the target's rows.
+        outside = (step.slots < 0).view(self.batch, k + 1)
+        torch.sum(~outside, 1, dtype=torch.int32, out=self.placed)
+        rows = torch.argsort(outside.view(-1), stable=True)
+        indptr = torch.cat((self.none[:1], self.placed.cumsum(0, dtype=torch.int32)))
+        logits = mgr.model(input_ids=ids, past_key_values=self.kv, paged_step=step, logit_rows=rows).logits
         probs = torch.softmax(logits.float(), dim=-1)
-        accepted, tokens = verify_drafts(probs, draft_probs, drafts, step.row_indptr, accept, last)
-        self.lens.add_(accepted).add_(1)
-        self.input_ids.copy_(tokens.gather(1, accepted.long()[:, None]).clamp_(min=0))
+        accepted, tokens = verify_drafts(probs, draft_probs, drafts, indptr, accept, last)
+        some = self.placed > 0
+        self.lens.add_(accepted).add_(some)
+        after = tokens.gather(1, accepted.long()[:, None]).clamp_(min=0)
+        self.input_ids.copy_(torch.where(some[:, None], after, self.input_ids))
         return accepted, tokens

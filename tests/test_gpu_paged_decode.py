@@ -161,3 +161,154 @@ def test_refusals(dev):
     fp32 = PagedKV(cfg, 2, 40, dev, torch.float32)
     with pytest.raises(ValueError, match="float16 or bfloat16"), torch.no_grad():
         Decoder(cfg).to(dev).forward_paged(ids[:2], fp32, fp32.tables(step.none, step.one, fp32.new_step(2, 1)))
+
+
+# ---------------------------------------------------------------- tokens without a place
+def short_of_pages():
+    """A decoder's requests 0 (14 tokens) and 1 (15 tokens) on three pages of 16 positions."""
+    mgr, cfg = build()
+    g = torch.Generator().manual_seed(11)
+    ps = [torch.randint(0, cfg.vocab_size, (n,), generator=g).to("cuda") for n in (14, 15)]
+    step = PagedDecode.new(mgr, 2, 96, num_pages=3)
+    step.input_ids.copy_(step.prefill(mgr, ps, ["a", "b"]))
+    return mgr, cfg, step, [torch.cat((p, t)) for p, t in zip(ps, step.input_ids)]
+
+
+def step_and_compare(mgr, step, seqs, names, live):
+    """One token of every request: those in ``live`` equal their whole sequences, the others' rows are NaN."""
+    mgr._setup_forward_batch(names, seq_lens=[1] * len(names))
+    before = step.lens.tolist()
+    got = step.run(mgr).logits
+    for i, (s, n) in enumerate(zip(seqs, names)):
+        if i in live:
+            torch.testing.assert_close(got[i].float(), whole(mgr, s, n)[-1].float(), atol=ATOL, rtol=ATOL)
+        else:
+            assert bool(got[i].isnan().all())
+    assert step.placed.tolist() == [int(i in live) for i in range(len(names))]
+    assert step.lens.tolist() == [b + int(i in live) for i, b in enumerate(before)]
+
+
+@torch.inference_mode()
+def test_drafts_without_a_page_are_not_kept(dev):
+    """Request 0 takes the last page and rejects its drafts; request 1's drafts have no place, and none of them counts as
+    cached: what follows attends to its own tokens, not to what request 0 left in the page."""
+    mgr, cfg, step, seqs = short_of_pages()
+    g = torch.Generator(dev).manual_seed(2)
+    drafts = torch.randint(0, cfg.vocab_size, (2, 3), generator=g, device=dev)
+    u = torch.tensor([[1.0] * 3, [0.0] * 3], device=dev)
+    mgr._setup_forward_batch(["a", "b"], seq_lens=[4, 4])
+    accepted, tokens = step.verify(mgr, drafts, None, u, torch.rand(2, generator=g, device=dev))
+    assert step.placed.tolist() == [4, 1] and accepted.tolist() == [0, 0] and step.lens.tolist() == [15, 16]
+    assert tokens[:, 1:].tolist() == [[-1] * 3] * 2 and bool((tokens[:, 0] >= 0).all())
+    assert torch.equal(step.input_ids, tokens[:, :1])
+    seqs = [torch.cat((s, t)) for s, t in zip(seqs, step.input_ids)]
+    for live in ((0, 1), (1,)):  # request 1 gets the page that request 0 gives back; then request 0 needs one
+        step_and_compare(mgr, step, seqs, ["a", "b"], live)
+        step.input_ids.copy_(torch.randint(0, cfg.vocab_size, (2, 1), generator=torch.Generator().manual_seed(len(live))))
+        if 0 not in live:
+            step.input_ids[0] = seqs[0][-1]
+        seqs = [torch.cat((s, t)) if i in live else s for i, (s, t) in enumerate(zip(seqs, step.input_ids))]
+        if len(live) == 2:
+            assert step.lens.tolist() == [16, 17]
+    # Verification of a request without any place: nothing accepted, nothing changed.
+    before, ids = step.lens.tolist(), step.input_ids.clone()
+    mgr._setup_forward_batch(["a", "b"], seq_lens=[4, 4])
+    accepted, tokens = step.verify(mgr, drafts, None, torch.ones(2, 3, device=dev), torch.rand(2, generator=g, device=dev))
+    assert step.placed.tolist() == [0, 4] and accepted.tolist() == [0, 0] and tokens[0].tolist() == [-1] * 4
+    assert step.lens.tolist() == [before[0], before[1] + 1] and torch.equal(step.input_ids[0], ids[0])
+    # Request 1 leaves: request 0 goes on where it was.
+    step.lens[1] = 0
+    seqs[1] = step.input_ids[1]
+    step_and_compare(mgr, step, seqs, ["a", "b"], (0, 1))
+
+
+@torch.inference_mode()
+def test_the_last_positions_of_the_table(dev):
+    """Drafts past the table's end are not looked at, and a full request stays as it is."""
+    mgr, cfg = build()
+    g = torch.Generator().manual_seed(4)
+    ps = [torch.randint(0, cfg.vocab_size, (n,), generator=g).to("cuda") for n in (30, 7)]
+    step = PagedDecode.new(mgr, 2, 32)
+    step.input_ids.copy_(step.prefill(mgr, ps, ["a", "b"]))
+    drafts = torch.randint(0, cfg.vocab_size, (2, 3), generator=g).to(dev)
+    seqs = [torch.cat((p, t, d)) for p, t, d in zip(ps, step.input_ids, drafts)]
+    mgr._setup_forward_batch(["a", "b"], seq_lens=[4, 4])
+    accepted, tokens = step.verify(mgr, drafts, None, torch.zeros(2, 3, device=dev), torch.full((2,), 0.5, device=dev))
+    assert step.placed.tolist() == [2, 4] and accepted.tolist() == [1, 3] and step.lens.tolist() == [32, 11]
+    assert tokens[0, 0] == drafts[0, 0] and tokens[0, 1] >= 0 and tokens[0, 2:].tolist() == [-1, -1]
+    # The token after the last draft that had a place is drawn from its row of the target.  Logits of at most 2 that are
+    # off by ATOL (1 + 2) = 0.18 at most move a cumulated half to 1 / (1 + exp(-0.36)) = 0.59.
+    p = torch.softmax(whole(mgr, seqs[0][:32], "a")[-1].double(), -1)
+    before = p.cumsum(0)[tokens[0, 1]] - p[tokens[0, 1]]
+    assert before - 0.1 < 0.5 < before + p[tokens[0, 1]] + 0.1
+    seqs = [None, torch.cat((seqs[1], step.input_ids[1]))]
+    for _ in range(2):
+        lens = step.lens.tolist()
+        mgr._setup_forward_batch(["a", "b"], seq_lens=[1, 1])
+        got = step.run(mgr).logits
+        assert bool(got[0].isnan().all()) and step.placed.tolist() == [0, 1] and step.lens.tolist() == [32, lens[1] + 1]
+        torch.testing.assert_close(got[1].float(), whole(mgr, seqs[1], "b")[-1].float(), atol=ATOL, rtol=ATOL)
+        seqs[1] = torch.cat((seqs[1], step.input_ids[1]))
+
+
+@torch.inference_mode()
+def test_prompts_that_the_pool_cannot_hold_are_refused(dev):
+    mgr, cfg, step, _ = short_of_pages()
+    lens, held = step.lens.tolist(), step.kv.state.held.tolist()
+    ids = torch.zeros(40, dtype=torch.long, device=dev)
+    with pytest.raises(ValueError, match="4 pages"):
+        step.prefill(mgr, [ids, ids[:16]], ["a", "b"])
+    assert step.lens.tolist() == lens and step.kv.state.held.tolist() == held
+    step.prefill(mgr, [ids[:32], ids[:16]], ["a", "b"])
+    assert step.kv.state.held.tolist() == [2, 1]
+
+
+@torch.inference_mode()
+def test_captured_steps_short_of_pages_equal_direct_ones(dev):
+    mgr, cfg, direct, _ = short_of_pages()
+    recorded = short_of_pages()[2]
+    mgr._setup_forward_batch(["a", "b"], seq_lens=[1, 1])
+    graph, out = capture_graph(mgr, recorded)
+    for turn in range(6):
+        graph.replay()
+        want = direct.run(mgr).logits
+        torch.cuda.synchronize()
+        assert torch.equal(out.logits.isnan(), want.isnan())
+        assert torch.equal(torch.nan_to_num(out.logits), torch.nan_to_num(want))
+        assert torch.equal(recorded.lens, direct.lens) and torch.equal(recorded.placed, direct.placed)
+        nxt = torch.where(direct.placed[:, None] > 0, want.argmax(-1, keepdim=True), direct.input_ids)
+        recorded.input_ids.copy_(nxt)
+        direct.input_ids.copy_(nxt)
+    assert direct.lens.tolist() == [16, 21] and direct.placed.tolist() == [0, 1]
+
+
+@torch.inference_mode()
+def test_captured_verification_short_of_pages_equals_the_direct_one(dev):
+    mgr, cfg, direct, _ = short_of_pages()
+    recorded = short_of_pages()[2]
+    g = torch.Generator(dev).manual_seed(3)
+    drafts, u, last = torch.zeros(2, 3, dtype=torch.long, device=dev), torch.zeros(2, 3, device=dev), torch.zeros(2, device=dev)
+    mgr._setup_forward_batch(["a", "b"], seq_lens=[4, 4])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        recorded.verify(mgr, drafts, None, u, last)
+        recorded.rewind()
+    recorded.input_ids.copy_(direct.input_ids)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        res = recorded.verify(mgr, drafts, None, u, last)
+    torch.cuda.current_stream().wait_stream(side)
+    seen = set()
+    for _ in range(8):
+        drafts.random_(0, cfg.vocab_size, generator=g)
+        u.copy_(torch.randint(0, 2, (2, 3), generator=g, device=dev))
+        last.uniform_(generator=g)
+        graph.replay()
+        want = direct.verify(mgr, drafts, None, u, last)
+        torch.cuda.synchronize()
+        for x, y in zip((*res, recorded.lens, recorded.placed, recorded.input_ids),
+                        (*want, direct.lens, direct.placed, direct.input_ids)):
+            assert torch.equal(x, y)
+        seen |= set(direct.placed.tolist())
+    assert 0 in seen and 4 in seen and len(seen) > 2
