@@ -465,8 +465,9 @@ int mlora_rotary_paged_write(const void* q, int64_t q_row_stride, const void* k,
  *   out[row, h] = sum_l softmax_l(scale * q[row, h] . k[l, h / rep]) * v[l, h / rep]
  * over the positions l <= the row's own; fp32 sums, P rounded to the data type
  * for its product with V, one rounding of the result.  `step` is one that
- * mlora_page_tables filled for these heads (its plan is followed unchecked).  Rows behind the last request's
- * are left as they were.  A row that would attend to a page outside the pool,
+ * mlora_page_tables filled for these heads; what its plan says outside the
+ * call's bounds (one never filled, say) is skipped, and rows that no other item
+ * has are left as they were.  So are rows behind the last request's.  A row that would attend to a page outside the pool,
  * or past the table, is NaN.  What lies in positions that a row does not
  * attend to (NaN too) does not reach it.
  * Requirements (else -2): bf16 or fp16; D 64 or 128; 16-byte aligned rows of

@@ -907,6 +907,7 @@ int mlora_paged_attention(const void* q, int64_t q_row_stride, const void* keys,
   a.num_pages = pages->num_pages, a.page_shift = shift;
   a.table = pages->table, a.table_stride = pages->table_stride, a.width = pages->width;
   a.plan = step->plan;
+  a.n = pages->n, a.rows = step->rows;
   a.out = out, a.out_stride = out_row_stride;
   a.workspace = static_cast<char*>(step->workspace);
   a.kv_heads = kv_heads, a.rep = heads / kv_heads;

@@ -106,6 +106,7 @@ struct PagedAttnArgs {
   int64_t table_stride;
   int width;
   const int32_t* plan;
+  int n, rows;       // requests, packed rows
   void* out;
   int64_t out_stride;
   // Of each kind at its offsets: sums [slot][kv_heads][bm][D], and the

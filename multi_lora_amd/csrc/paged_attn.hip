@@ -73,13 +73,22 @@ struct Item {
   int first, c, past;  // its request's first packed row, new tokens, and position of the first
   int rows;            // query rows of the tile, at most bm
 };
+__device__ __forceinline__ bool below(int v, int end) { return static_cast<uint32_t>(v) < static_cast<uint32_t>(end); }
 __device__ __forceinline__ bool load_item(const PagedAttnArgs& a, const PagedKind& kd, int counter, int item, Item* t) {
   if (item >= min(a.plan[counter], kd.item_cap)) return false;
   const int32_t* w = a.plan + kd.items_off + static_cast<int64_t>(item) * kApItemWords;
   t->req = w[0], t->row0 = w[1], t->kv0 = w[2], t->kv1 = w[3], t->slot = w[4];
   t->first = w[5], t->c = w[6], t->past = w[7];
+  // The list is the page tables' own, but a step can be used without one: the
+  // launch that fills it may stand in a graph that has not run yet.  What does
+  // not fit the call's bounds is skipped, and nothing outside them touched.
+  const int room = static_cast<int>(min(static_cast<int64_t>(a.width) << a.page_shift, static_cast<int64_t>(1 << 30)));
+  if (!below(t->req, a.n) || !below(t->c, a.rows + 1) || !below(t->first, a.rows - t->c + 1) || !below(t->past, 1 << 30) ||
+      !below(t->row0, t->c * a.rep) || t->kv0 < 0 || (t->kv0 < t->kv1 && (t->kv0 & 63) != 0) || t->kv1 > room ||
+      t->slot >= kd.slot_cap)
+    return false;
   t->rows = min(kd.bm, t->c * a.rep - t->row0);
-  return t->rows > 0;
+  return true;
 }
 
 // Element offset of query row m of a request inside q or out.
@@ -677,7 +686,7 @@ __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(PagedAttnArgs a) {
   } s;
   const int item = blockIdx.x / a.kv_heads;
   const int head = blockIdx.x - item * a.kv_heads;
-  const int long_items = min(a.plan[kApLong], a.shape.kind[1].item_cap);
+  const int long_items = max(min(a.plan[kApLong], a.shape.kind[1].item_cap), 0);
   if (item < long_items)
     tile_item<T, D>(a, s.tile, item, head);
   else
@@ -699,7 +708,11 @@ __device__ __forceinline__ void join_rows(const PagedAttnArgs& a, int k, int joi
   const int slot0 = w[2], parts = w[3];
   Item it;
   it.first = w[0], it.row0 = w[1], it.rows = w[4];
-  if (block * RB >= it.rows) return;
+  if (!below(it.rows, kd.bm + 1) || block * RB >= it.rows) return;
+  // As in load_item.
+  if (!below(it.first, a.rows) || !below(it.row0, 1 << 30) || (it.row0 + it.rows - 1) / a.rep >= a.rows - it.first ||
+      !below(parts - 1, kd.slot_cap) || !below(slot0, kd.slot_cap - parts + 1))
+    return;
   const int group = threadIdx.x / (RB * C);
   const int i = threadIdx.x - group * (RB * C);
   const int r = min(block * RB + i / C, it.rows - 1);
@@ -748,9 +761,10 @@ constexpr int join_block(int d, int kind) { return kind ? 1024 / d : 256 / d; } 
 template <class T, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedAttnArgs a, int long_per) {
   __shared__ f32x4 os[256];
-  const int short_per = cdiv(a.plan[kApJoinRows], join_block(D, 0));
-  const int long_blocks = a.plan[kApLong + 1] * a.kv_heads * long_per;
-  const int blocks = long_blocks + a.plan[kApShort + 1] * a.kv_heads * short_per;
+  const PagedKind &few = a.shape.kind[0], &many = a.shape.kind[1];
+  const int short_per = cdiv(max(min(a.plan[kApJoinRows], few.bm), 0), join_block(D, 0));
+  const int long_blocks = max(min(a.plan[kApLong + 1], many.join_cap), 0) * a.kv_heads * long_per;
+  const int blocks = long_blocks + max(min(a.plan[kApShort + 1], few.join_cap), 0) * a.kv_heads * short_per;
   for (int u = blockIdx.x; u < blocks; u += gridDim.x) {
     if (u < long_blocks) {
       const int tile = u / long_per;

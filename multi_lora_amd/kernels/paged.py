@@ -312,7 +312,9 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, s
     (``heads / kv_heads`` each).  ``step`` is ``page_tables``' of this step,
     made for these heads; one step serves every layer.  Sums are fp32 and the
     result is rounded once.  Rows behind the last request's are left as they
-    were in ``out`` (undefined without one).
+    were in ``out`` (undefined without one).  A step whose ``page_tables`` was
+    only recorded holds a work list once the graph has run; before, the result
+    is undefined.
     """
     if not step.filled:
         raise ValueError("the step is empty: page_tables fills it")

@@ -534,3 +534,26 @@ def test_two_steps_of_one_state_on_two_streams(dev):
         a = [paged_attention(q1, keys, values, step1, 0.1) for _ in range(8)]
         torch.cuda.synchronize()
         assert all(torch.equal(x, want[0]) for x in a) and all(torch.equal(x, want[1]) for x in b)
+
+
+@pytest.mark.parametrize("new,start,rows", [([1] * 4, [900, 2000, 300, 77], 4), ([300, 1, 7], [900, 2000, 0], 308)])
+def test_a_step_that_was_only_recorded(dev, new, start, rows):
+    """The launch that fills a step's work list stands in a graph that has not run: whatever the list's memory holds, the
+    call keeps to its tensors.  Once the graph has run it answers."""
+    q, keys, values, table, eager = cache_case(dev, new, start, 8, 2, 128, 16, torch.bfloat16, 1)
+    want = paged_attention(q, keys, values, eager, 0.1)
+    step = PagedStep(eager.state, rows, max(new), 8, 2, 128)
+    first, more = i32(start, dev), i32(new, dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        page_tables(eager.state, first, more, step=step)
+    out = torch.full_like(q, 7.0)
+    for junk in (-1, 2 ** 31 - 1, -2 ** 31, 0, 1000, 1 << 24):
+        step._ints.fill_(junk)
+        paged_attention(q, keys, values, step, 0.1, out=out)
+        assert bool((out == 7.0).all())
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(paged_attention(q, keys, values, step, 0.1), want)
