@@ -17,9 +17,11 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <ATen/core/grad_mode.h>
 #include <c10/core/InferenceMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 
 #include <algorithm>
@@ -530,6 +532,16 @@ bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
   return false;
 }
 
+// A trace may be recording what torch runs (the caller then says so).
+bool maybe_traced() { return torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::any_modes_set(); }
+
+// A forward-mode tangent, which a launch past torch would drop.
+bool has_tangent(std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    if (t->_fw_grad(0).defined()) return true;
+  return false;
+}
+
 // Inference tensors are written in inference mode only (no version counter).
 bool may_write(const at::Tensor& t) { return !t.is_inference() || c10::InferenceMode::is_enabled(); }
 
@@ -564,7 +576,7 @@ struct Pool {
 Took page_tables(PyObject* const* args) {
   Step st;
   const at::Tensor *start = tensor_of(args[1]), *add = tensor_of(args[2]);
-  if (!st.read(args[0]) || start == nullptr || add == nullptr || !start->is_cuda()) return Took::kNo;
+  if (!st.read(args[0]) || start == nullptr || add == nullptr || !start->is_cuda() || maybe_traced()) return Took::kNo;
   const at::Device dev = start->device();
   if (!is_current(dev) || dev.index() != st.device || !is_i32(start, dev, st.pages->n) || !is_i32(add, dev, st.pages->n)) return Took::kNo;
   const hipStream_t stream = stream_of(dev);
@@ -585,6 +597,7 @@ PyObject* paged_attention(PyObject* const* args, Took* took) {
   const at::ScalarType dt = k->scalar_type();
   const int64_t rows = st.step->rows, width = static_cast<int64_t>(st.heads) * st.head_dim;
   if (!is_current(dev) || dev.index() != st.device || st.step->plan == nullptr || rows == 0 || wants_grad({q, k, v}) ||
+      maybe_traced() || has_tangent({q, k, v}) ||
       !is_rows_of(q, dev, dt, rows, width) || pool.kv_heads != st.kv_heads || pool.d != st.head_dim ||
       pool.page != st.pages->page || pool.pages < st.pages->num_pages)
     return nullptr;
@@ -625,7 +638,7 @@ PyObject* paged_write(PyObject* const* args, Took* took) {
   const int64_t rows = q->size(0), heads = q->size(1) / pool.d;
   if (!is_rows_of(q, dev, dt, rows, heads * pool.d) || !is_rows_of(k, dev, dt, rows, pool.kv_heads * pool.d) ||
       !is_rows_of(v, dev, dt, rows, pool.kv_heads * pool.d) || !is_i32(slots, dev, rows) ||
-      wants_grad({q, k, v, cs, sn, kp, vp}))
+      wants_grad({q, k, v, cs, sn, kp, vp}) || maybe_traced() || has_tangent({q, k, v, cs, sn, kp, vp}))
     return nullptr;
   if (!may_write(*kp) || !may_write(*vp)) return nullptr;
   int64_t rot[2];
@@ -676,7 +689,7 @@ PyObject* verify_drafts(PyObject* const* args, Took* took) {
     return nullptr;
   const at::Device dev = target->device();
   const int code = dtype_code(target->scalar_type());
-  if (!is_current(dev) || code < 0 || target->dim() != 2 || tokens->dim() != 2 || target->size(0) == 0 || target->size(1) == 0 ||
+  if (!is_current(dev) || code < 0 || maybe_traced() || target->dim() != 2 || tokens->dim() != 2 || target->size(0) == 0 || target->size(1) == 0 ||
       !fits_i32(target->size(0)) || !fits_i32(target->size(1)))
     return nullptr;
   const int64_t rows = target->size(0), vocab = target->size(1), n = tokens->size(0), most = tokens->size(1);

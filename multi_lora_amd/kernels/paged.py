@@ -12,7 +12,8 @@ Pools of one layer: keys ``[num_pages, kv_heads, page, d]`` and values
 ``[num_pages, kv_heads, d, page]`` (transposed inside a page, so that a chunk
 of eight positions is one load of the second product's operand).  Data in
 float16 or bfloat16, ``d`` 64 or 128, pages of a power of two positions from 8
-to 1024.  There is no CPU path and no backward pass.
+to 1024.  There is no CPU path and no derivative in either mode: inputs that ask
+for one are refused, and so are calls under a trace, which would not see them.
 
 No counterpart in the reference, whose decode runs over
 ``transformers.StaticCache`` (multi_lora/graph_decode.py:23-111).
@@ -27,6 +28,7 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _ffi
 
@@ -41,6 +43,17 @@ def _on_gpu(what: str, *tensors: torch.Tensor) -> torch.device:
         if t.device != first:
             raise ValueError(f"{what}: tensors on {t.device} and {first}")
     return first
+
+
+def _untraced(what: str) -> None:
+    """The launch goes past torch: a trace would keep this call's result as a constant."""
+    if torch.jit.is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError(f"{what} is not a torch operation and cannot be traced")
+
+
+def _no_tangent(what: str, *tensors: torch.Tensor) -> None:
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative; call it on tensors without tangents")
 
 
 def _no_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -213,6 +226,7 @@ def page_tables(state: PageState, start_lens: torch.Tensor, new_lens: torch.Tens
         step.filled = True
         return step
     dev = _on_gpu("page_tables", state.table, start_lens, new_lens)
+    _untraced("page_tables")
     n = state.table.shape[0]
     _i32("start_lens", start_lens, n)
     _i32("new_lens", new_lens, n)
@@ -262,7 +276,9 @@ def rotary_paged_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: t
     if done is not None:
         return done if out is None else out
     dev = _on_gpu("rotary_paged_write", q, k, v, cos, sin, keys, values, slots)
+    _untraced("rotary_paged_write")
     _no_grad("rotary_paged_write", q, k, v, cos, sin, keys, values)
+    _no_tangent("rotary_paged_write", q, k, v, cos, sin, keys, values)
     pages, kv_heads, page, d = _pool("rotary_paged_write", keys, values)
     rows = q.shape[0] if q.dim() == 2 else -1
     if rows < 0 or q.shape[1] == 0 or q.shape[1] % d:
@@ -322,7 +338,9 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, s
     if done is not None:
         return done if out is None else out
     dev = _on_gpu("paged_attention", q, keys, values, step.row_indptr)
+    _untraced("paged_attention")
     _no_grad("paged_attention", q, keys, values)
+    _no_tangent("paged_attention", q, keys, values)
     pages, kv_heads, page, d = _pool("paged_attention", keys, values)
     if not step.has_plan:
         raise ValueError("the step has no work list: give page_tables the heads")
@@ -382,6 +400,7 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
         return done
     given = [t for t in (target, draft, tokens, row_indptr, accept, last) if t is not None]
     dev = _on_gpu("verify_drafts", *given)
+    _untraced("verify_drafts")
     if tokens.dim() != 2 or tokens.dtype != torch.int64 or (tokens.numel() > 0 and tokens.stride(1) != 1):
         raise ValueError("tokens must be int64 [n, most] with contiguous rows")
     n, most = tokens.shape

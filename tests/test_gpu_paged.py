@@ -5,6 +5,8 @@ from types import SimpleNamespace
 
 import pytest
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from multi_lora_amd import _ffi
 from multi_lora_amd.kernels import PagedStep, PageState, page_tables, paged_attention, rotary_paged_write, verify_drafts
@@ -557,3 +559,42 @@ def test_a_step_that_was_only_recorded(dev, new, start, rows):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(paged_attention(q, keys, values, step, 0.1), want)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_what_torch_has_to_see_is_refused(dev, monkeypatch, native):
+    """A launch past torch would drop a tangent, and a trace would keep its result as a constant."""
+    q, keys, values, table, step = cache_case(dev, [3, 1], [0, 20], 4, 2, 64, 16, torch.float16, 3)
+    k, cos = torch.randn(4, 128, device=dev).half(), torch.randn(4, 64, device=dev).half()
+    target, tokens = probabilities(torch.Generator(dev).manual_seed(1), (4, 50), torch.float32, dev), torch.zeros(2, 1, dtype=torch.int64, device=dev)
+    u, start, new, indptr = torch.zeros(2, 1, device=dev), i32([0, 20], dev), i32([3, 1], dev), i32([0, 2, 4], dev)
+    if not native:
+        none = lambda *a: None  # noqa: E731
+        monkeypatch.setattr(_ffi, "calls", lambda: SimpleNamespace(page_tables=none, paged_write=none, paged_attention=none,
+                                                                   verify_drafts=none))
+
+    def attend(q, keys=keys, values=values):
+        return paged_attention(q, keys, values, step, 0.125)
+
+    def write(q, k=k, v=k, cos=cos):
+        return rotary_paged_write(q, k, v, cos, cos, keys, values, step.slots)
+
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: attend(dual(q)), lambda: attend(q, keys=dual(keys)), lambda: attend(q, values=dual(values)),
+                     lambda: write(dual(q)), lambda: write(q, k=dual(k)), lambda: write(q, v=dual(k)), lambda: write(q, cos=dual(cos))):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+        got = attend(q)  # without a tangent
+    assert torch.equal(got, attend(q))
+    for f, x in ((lambda x: attend(x), q), (lambda x: write(x), q), (lambda p: verify_drafts(p, None, tokens, indptr, u, u[:, 0])[1], target),
+                 (lambda c: page_tables(step.state, start, c, step=step).slots, new)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, (x,), check_trace=False)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(f)(x)
+        f(x)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(attend)(q[None])
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(attend, (q,), (q,))
