@@ -343,7 +343,12 @@ class Decoder(nn.Module):
                 cache_position: Optional[torch.Tensor] = None, use_cache: bool = True,
                 paged_step: Optional[PagedStep] = None, logit_rows: Optional[torch.Tensor] = None, **_):
         if isinstance(past_key_values, PagedKV):
+            if any(v is not None for v in (attention_mask, position_ids, cache_position)) or not use_cache:
+                raise ValueError("over a PagedKV the step says which positions the rows have and see: no attention_mask, "
+                                 "position_ids, cache_position or use_cache=False")
             return SimpleNamespace(logits=self.forward_paged(input_ids.reshape(-1), past_key_values, paged_step, logit_rows))
+        if paged_step is not None or logit_rows is not None:
+            raise ValueError("paged_step and logit_rows go with a PagedKV")
         b, t = input_ids.shape
         dev = input_ids.device
         kv = past_key_values if use_cache else None
@@ -367,6 +372,10 @@ class Decoder(nn.Module):
         row, or of ``logit_rows``; those of rows behind the last request's mean
         nothing.  No host synchronisation: over resident tensors the step can
         be captured in a graph and replayed with new ids and lengths."""
+        if step is None or step.state is not kv.state or not (step.has_plan and step.filled):
+            raise ValueError("a PagedKV needs the paged_step that its new_step made and its tables filled")
+        if ids.shape != (step.rows,):
+            raise ValueError(f"{step.rows} packed token ids expected, got {tuple(ids.shape)}")
         x = self.embed_tokens(ids)
         rot = Rotary.make(step.positions, self.inv_freq, x.dtype)
         pending = None

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from multi_lora_amd import _ffi
+from multi_lora_amd.decoder import Decoder, DecoderConfig, PagedKV, StaticKV
 from multi_lora_amd.kernels import PagedStep, PageState, page_tables, paged_attention, rotary_paged_write, verify_drafts
 from tests import paged_ref as ref
 
@@ -158,3 +159,34 @@ def test_the_plain_allocator_itself():
             sim.step(again, [0] * 6, 0)
             assert sim.stack == before and sim.held == had
         lens = [h * 8 for h in sim.held]
+
+
+def test_decoder_arguments():
+    """What a paged step does not follow is refused, not ignored."""
+    cfg = DecoderConfig()
+    model, ids = Decoder(cfg), torch.zeros(1, 4, dtype=torch.long)
+    kv, other = PagedKV(cfg, 2, 40, "cpu", torch.float32), PagedKV(cfg, 2, 40, "cpu", torch.float32)
+    step = kv.new_step(4, 4)
+
+    def call(**kw):
+        return model(input_ids=ids, **{"past_key_values": kv, "paged_step": step, **kw})
+
+    with pytest.raises(ValueError, match="its tables filled"):
+        call()
+    step.filled = True
+    for kw in (dict(attention_mask=torch.ones(1, 4)), dict(position_ids=torch.zeros(1, 4, dtype=torch.long)),
+               dict(cache_position=torch.arange(4)), dict(use_cache=False)):
+        with pytest.raises(ValueError, match="no attention_mask"):
+            call(**kw)
+    for kw in (dict(paged_step=None), dict(past_key_values=other), dict(paged_step=PagedStep(kv.state, 4, 4))):
+        with pytest.raises(ValueError, match="needs the paged_step"):
+            call(**kw)
+    with pytest.raises(ValueError, match="4 packed token ids"):
+        model(input_ids=ids[:, :3], past_key_values=kv, paged_step=step)
+    with pytest.raises(RuntimeError, match="no CPU fallback"), torch.no_grad():
+        call()
+    for kw in (dict(), dict(past_key_values=StaticKV(cfg, 1, 8, "cpu", torch.float32))):
+        with pytest.raises(ValueError, match="go with a PagedKV"):
+            model(input_ids=ids, paged_step=step, **kw)
+        with pytest.raises(ValueError, match="go with a PagedKV"):
+            model(input_ids=ids, logit_rows=torch.tensor([1]), **kw)
