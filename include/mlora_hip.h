@@ -440,7 +440,7 @@ int32_t mlora_page_tables_scratch(int32_t n);
  * request's), and, if the step has a plan, the work list for `heads` query
  * heads over `kv_heads` key heads of head_dim.  A new length above the step's
  * max_new counts as max_new, and requests that the step's rows do not hold get
- * fewer or none (row_indptr says so).  start_lens and new_lens may be the
+ * fewer or none (row_indptr says so), and pages for those only.  start_lens and new_lens may be the
  * step's own kv_lens.  Table entries past the pages held are left as they
  * were.  rows at most 2^20, num_pages * page and n *
  * width below 2^31. */

@@ -47,13 +47,13 @@ __device__ __forceinline__ int pages_for(int tokens, const TablesArgs& a) {
   return static_cast<int>(min(p, static_cast<int64_t>(a.width)));
 }
 
-// Tokens request i keeps and gets, as the caller gives them: sums stay inside
-// 31 bits, and max_new is kept, for the work list has room for no more.
+// Tokens request i keeps and asks for, as the caller gives them: sums stay
+// inside 31 bits, and max_new is kept, for the work list has room for no more.
 __device__ __forceinline__ int2 given_lens(const TablesArgs& a, int i) {
   return make_int2(min(max(a.start[i], 0), (1 << 30) - 1), min(max(a.add[i], 0), a.max_new));
 }
-// The same from scratch, once the first kernel has put them there (the
-// caller's may be the step's own kv_lens).
+// Tokens it keeps and gets, from scratch, where the first kernel has put them
+// (the caller's may be the step's own kv_lens).
 __device__ __forceinline__ int2 lens_of(const TablesArgs& a, int i) {
   const int32_t* start0 = a.scratch + kTsArrays + 7 * a.n;
   return make_int2(start0[i], start0[a.n + i]);
@@ -261,16 +261,26 @@ __global__ __launch_bounds__(kScanThreads) void tables_small_kernel(TablesArgs a
     start = l.x;
     need = pages_for(l.x + l.y, a);
     held = min(max(a.held[i], 0), a.width);
-    v[0] = min(l.y, a.rows);
+    v[0] = min(l.y, a.rows + 1);
     v[1] = max(held - need, 0);
     v[2] = max(need - held, 0);
   }
   int c = v[0];
   scan(v, total, tmp);
-  const int rows = min(total[0], a.rows), freed = total[1], taken = total[2];
+  const int rows = min(total[0], a.rows), first = min(v[0], a.rows);
+  c = min(c, a.rows - first);
+  int freed = total[1], taken = total[2];
+  if (total[0] > a.rows) {  // some get fewer tokens than asked for, and pages for those only
+    int w[2] = {0, 0}, t[2];
+    if (i < a.n) {
+      need = pages_for(start + c, a);
+      w[0] = max(held - need, 0);
+      w[1] = max(need - held, 0);
+    }
+    scan(w, t, tmp);
+    v[1] = w[0], v[2] = w[1], freed = t[0], taken = t[1];
+  }
   if (i < a.n) {
-    const int first = min(v[0], a.rows);
-    c = min(c, a.rows - first);
     len = start + c;
     first_s[i] = first;
     freed_s[i] = v[1];
@@ -386,25 +396,36 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
     const int i = i0 + threadIdx.x;
     int v[3] = {0, 0, 0}, total[3];
     int2 l = make_int2(0, 0);
+    int held = 0;
     if (i < a.n) {
       l = given_lens(a, i);
       const int need = pages_for(l.x + l.y, a);
-      const int held = min(max(a.held[i], 0), a.width);
-      v[0] = min(l.y, a.rows);
+      held = min(max(a.held[i], 0), a.width);
+      v[0] = min(l.y, a.rows + 1);
       v[1] = max(held - need, 0);
       v[2] = max(need - held, 0);
       held0[i] = held;
     }
     const int c = v[0];
     scan(v, total, tmp);
+    // Rows saturate at the call's rows: later requests then get none.
+    const int first = min(rows + v[0], a.rows);
+    const int mine = min(c, a.rows - first);
+    if (rows + total[0] > a.rows) {  // as in the small kernel
+      int w[2] = {0, 0}, t[2];
+      if (i < a.n) {
+        const int need = pages_for(l.x + mine, a);
+        w[0] = max(held - need, 0);
+        w[1] = max(need - held, 0);
+      }
+      scan(w, t, tmp);
+      v[1] = w[0], v[2] = w[1], total[1] = t[0], total[2] = t[1];
+    }
     if (i < a.n) {
-      // Rows saturate at the call's rows: later requests then get none.
-      const int first = min(rows + v[0], a.rows);
-      const int mine = min(c, a.rows - first);
       a.row_indptr[i] = first;
       a.kv_lens[i] = l.x + mine;
       parts0[a.n + i] = l.x;
-      parts0[2 * a.n + i] = l.y;
+      parts0[2 * a.n + i] = mine;
       freed0[i] = freed + v[1];
       taken0[i] = taken + v[2];
       if (plan) {
@@ -443,7 +464,7 @@ __global__ __launch_bounds__(kScanThreads) void tables_scan_kernel(TablesArgs a)
       const int need = pages_for(l.x + l.y, a);
       const int held = held0[i];
       a.held[i] = need > held ? held + min(need - held, max(have - taken0[i], 0)) : need;
-      c = min(l.y, a.rows - a.row_indptr[i]);
+      c = l.y;
       len = min(l.x + c, room);
     }
     if (!plan) continue;

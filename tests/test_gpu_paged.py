@@ -598,3 +598,18 @@ def test_what_torch_has_to_see_is_refused(dev, monkeypatch, native):
         torch.func.vmap(attend)(q[None])
     with pytest.raises(RuntimeError):
         torch.func.jvp(attend, (q,), (q,))
+
+
+@pytest.mark.parametrize("n", [5, 1200, 2100])  # one launch, and two
+@pytest.mark.parametrize("rows", [0, 3, 15, 40])
+def test_pages_go_to_the_tokens_that_the_rows_hold(dev, n, rows):
+    """A request that gets fewer rows than it asked for takes pages for those only, and gives back the others."""
+    start, new = [7, 20, 0, 0, 33] + [0] * (n - 5), [40, 12, 30, 60, 17] + [1] * (n - 5)
+    state, sim = PageState.new(n, 64, 20 + n, 16, dev), ref.Pages(n, 4, 20 + n, 16)
+    for starts, asked, room in (([0] * n, start, sum(start)), (start, new, rows), (start, [0] * n, 0), (start, new, rows + 9)):
+        left, got = room, []
+        for c in asked:
+            got.append(min(c, left))
+            left -= got[-1]
+        step = page_tables(state, i32(starts, dev), i32(asked, dev), rows=room, max_new=60, heads=2, kv_heads=1, head_dim=64)
+        check_step(state, sim, step, sim.step(starts, got, room), room)
