@@ -166,7 +166,7 @@ __device__ __forceinline__ void split_lengths(const TablesArgs& a, const Ranges&
   for (int k = 0; k < 2; ++k) {
     const unsigned long long part = (r.work[k] * a.kv_heads + target - 1) / target;
     const unsigned long long least = max(part, static_cast<unsigned long long>(k ? kApMinSplitLong : kApMinSplit));
-    split[k] = static_cast<int>((min(least, 1ull << 29) + 63) / 64 * 64);
+    split[k] = static_cast<int>((min(least, 1ull << 30) + 63) / 64 * 64);  // (no range is longer than 2^30)
     if (r.tiles[k] * a.kv_heads >= kApWhole * target) split[k] = INT32_MAX;
   }
   const unsigned long long filled = min(2 * r.tiles[0] * a.kv_heads, target);
@@ -731,10 +731,15 @@ bool paged_shape(int n, int rows, int max_new, int64_t max_kv, int heads, int kv
     const int64_t tiles = !occurs ? 0
                           : k == 0 ? std::min(n, rows)
                                    : all / kd.bm + std::min<int64_t>(n, all / (s->kind[0].bm + 1));
-    // Parts of a tile: at most its length / split + 1, and the lengths of all
-    // tiles over the split are at most the parts that fill the chip.
+    // A range splits into parts only where it is longer than `split`, and the
+    // lengths of all tiles over the split are at most the parts that fill the
+    // chip, target / kv_heads.  So the parts past each tile's first are at most
+    // that many; and so are all parts of long tiles that split (they round
+    // down), while those of short ones, which round a ratio above 1 up, are
+    // fewer than twice as many.  4096 rows of 64 requests, 8 key heads of 128:
+    // 43 MB; with room for two parts of every tile it would be 145.
     const int64_t extra = !occurs || max_kv <= (k ? kApMinSplitLong : kApMinSplit + kApKeep) ? 0 : s->target / kv_heads + 1;
-    const int64_t slots = extra > 0 ? std::min(tiles, static_cast<int64_t>(kApWhole) * s->target / kv_heads + 1) + extra : 0;
+    const int64_t slots = extra > 0 ? std::min(tiles + extra, static_cast<int64_t>(k ? 1 : 2) * s->target / kv_heads) : 0;
     if (tiles + extra > INT32_MAX / 64) return false;
     kd.item_cap = static_cast<int>(tiles + extra);
     kd.slot_cap = static_cast<int>(slots);

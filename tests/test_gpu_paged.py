@@ -613,3 +613,11 @@ def test_pages_go_to_the_tokens_that_the_rows_hold(dev, n, rows):
             left -= got[-1]
         step = page_tables(state, i32(starts, dev), i32(asked, dev), rows=room, max_new=60, heads=2, kv_heads=1, head_dim=64)
         check_step(state, sim, step, sim.step(starts, got, room), room)
+
+
+def test_as_many_parts_as_a_step_can_have(dev):
+    """Eight tiles of 64 parts each: the workspace has room for 512 parts of one key head's long tiles."""
+    new, start = [16] * 8, [65520] * 8
+    q, keys, values, table, step = cache_case(dev, new, start, 8, 1, 64, 256, torch.bfloat16, 5)
+    assert step._c.workspace_bytes == (512 * 128 + 521 * 16) * 66 * 4
+    check_attention(paged_attention(q, keys, values, step, 0.125), q, keys, values, table, start, new, 0.125, torch.bfloat16)

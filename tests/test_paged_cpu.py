@@ -190,3 +190,56 @@ def test_decoder_arguments():
             model(input_ids=ids, paged_step=step, **kw)
         with pytest.raises(ValueError, match="go with a PagedKV"):
             model(input_ids=ids, logit_rows=torch.tensor([1]), **kw)
+
+
+CUS = 256                      # without a GPU the library counts these
+SPLIT_FROM = (256 + 384, 1024)  # longest range that no step splits, short and long
+
+
+def slot_caps(n, rows, max_new, max_kv, heads, kv_heads):
+    """(rows a tile, parts of split ranges that the workspace holds) of both kinds of a step's work items."""
+    rep, target = heads // kv_heads, 2 * CUS
+    most, every = min(max_new, rows) * rep, rows * rep
+    bm = 32 if 16 < most <= 32 else 16
+    caps = []
+    for k, tile, tiles in ((0, bm, min(n, rows)), (1, 128, every // 128 + min(n, every // (bm + 1)) if most > bm else 0)):
+        extra = target // kv_heads + 1 if tiles and max_kv > SPLIT_FROM[k] else 0
+        caps.append((tile, min(tiles + extra, (1 if k else 2) * target // kv_heads) if extra else 0))
+    return caps
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_a_steps_workspace_holds_the_parts_of_any_lengths(seed):
+    """The workspace has room for every part that the split rule can make of a step's ranges, and for little more."""
+    rng = random.Random(seed)
+    full = 0.0
+    for _ in range(400):
+        kv_heads = rng.choice((1, 2, 4, 8, 32, 600))
+        rep = rng.choice((1, 4, 7, 8, 16)) if kv_heads < 600 else 1
+        d, n, page = rng.choice((64, 128)), rng.choice((1, 3, 20, 300)), 16
+        new = [rng.choice((1, 1, 5, rng.randint(1, 3000))) for _ in range(n)]
+        lens = [c + (0 if rng.random() < 0.1 else rng.choice((rng.randint(0, 500), 2048, 65536 - c % 4, rng.randint(0, 200000)))) for c in new]
+        if rng.random() < 0.3:
+            new, lens = [16] * n, [65536] * n
+        max_kv = -(-max(lens) // page) * page
+        caps = slot_caps(n, sum(new), max(new), max_kv, kv_heads * rep, kv_heads)
+        plan, ws = ctypes.c_size_t(), ctypes.c_size_t()
+        assert _ffi.lib().mlora_paged_step_bytes(n, sum(new), max(new), max_kv, kv_heads * rep, kv_heads, d, ctypes.byref(plan),
+                                                 ctypes.byref(ws)) == 0
+        assert ws.value == sum(slots * kv_heads * tile * (d + 2) * 4 for tile, slots in caps)
+        # The split rule, on exact numbers: the least length of a part, and the parts of each tile.
+        tiles = [[], []]
+        for c, length in zip(new, lens):
+            k = c * rep > caps[0][0]
+            tiles[k] += [length] * (-(-c * rep // caps[k][0]))
+        for k in (0, 1):
+            split = -(-max(-(-sum(tiles[k]) * kv_heads // (2 * CUS)), (256, 1024)[k]) // 64) * 64
+            if len(tiles[k]) * kv_heads >= 4 * 2 * CUS:
+                continue
+            parts = [max(length // split, 1) if k else -(-length // split) for length in tiles[k]]
+            if k == 0 and max(tiles[0], default=0) - 384 <= split:
+                continue
+            used = sum(p for p in parts if p > 1)
+            assert used <= caps[k][1]
+            full = max(full, used / max(caps[k][1], 1))
+    assert full == 1.0
