@@ -812,7 +812,7 @@ int mlora_page_tables(const mlora_pages* pages, const int32_t* start_lens, const
     if (step->plan_bytes < a.shape.plan_bytes)
       return fail(kWorkspace, "plan of %zu bytes, needs %zu", step->plan_bytes, a.shape.plan_bytes);
   }
-  if (pages->n == 0 && step->rows == 0 && step->plan == nullptr) return 0;
+  if (pages->n == 0 && step->rows == 0 && step->plan == nullptr && step->row_indptr == nullptr) return 0;
   if (scratch == nullptr || step->row_indptr == nullptr || (step->rows > 0 && (!step->positions || !step->slots)) ||
       (pages->n > 0 && (!pages->table || !pages->held || !start_lens || !new_lens || !step->kv_lens)) ||
       pages->counts == nullptr || (pages->num_pages > 0 && pages->free == nullptr))

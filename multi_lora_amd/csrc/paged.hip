@@ -759,7 +759,6 @@ bool paged_shape(int n, int rows, int max_new, int64_t max_kv, int heads, int kv
 }
 
 hipError_t launch_page_tables(const TablesArgs& a, hipStream_t stream) {
-  if (a.n == 0 && a.rows == 0) return hipSuccess;
   const int64_t row_blocks = (static_cast<int64_t>(a.rows) + 255) / 256;
   const int64_t blocks = row_blocks + (static_cast<int64_t>(a.n) + 3) / 4;
   if (!grid_fits(blocks)) return hipErrorInvalidConfiguration;

@@ -621,3 +621,20 @@ def test_as_many_parts_as_a_step_can_have(dev):
     q, keys, values, table, step = cache_case(dev, new, start, 8, 1, 64, 256, torch.bfloat16, 5)
     assert step._c.workspace_bytes == (512 * 128 + 521 * 16) * 66 * 4
     check_attention(paged_attention(q, keys, values, step, 0.125), q, keys, values, table, start, new, 0.125, torch.bfloat16)
+
+
+@pytest.mark.parametrize("rows", [0, 5])
+def test_a_step_of_no_requests(dev, rows):
+    state = PageState.new(0, 64, 4, 16, dev)
+    none = i32([], dev)
+    for heads in ({}, dict(heads=2, kv_heads=1, head_dim=64)):
+        step = PagedStep(state, rows, 1, **heads)
+        step._ints.fill_(77)
+        state.counts[1] = 3
+        page_tables(state, none, none, step=step)
+        assert step.row_indptr.tolist() == [0] and step.positions.tolist() == [0] * rows and step.slots.tolist() == [-1] * rows
+        assert state.counts.tolist() == [4, 0]
+    out = torch.full((rows, 128), 7.0, device=dev).half()
+    pool = torch.zeros(4, 1, 16, 64, device=dev).half()
+    paged_attention(torch.zeros_like(out), pool, pool.view(4, 1, 64, 16), step, 0.1, out=out)
+    assert bool((out == 7.0).all())
