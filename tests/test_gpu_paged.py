@@ -638,3 +638,56 @@ def test_a_step_of_no_requests(dev, rows):
     pool = torch.zeros(4, 1, 16, 64, device=dev).half()
     paged_attention(torch.zeros_like(out), pool, pool.view(4, 1, 64, 16), step, 0.1, out=out)
     assert bool((out == 7.0).all())
+
+
+# ---------------------------------------------------------------- work lists of large steps (built by two launches)
+def many_requests(seed, n):
+    """Lengths of ``n`` requests: mostly short, some without tokens, long ranges and prompts among the first and the last."""
+    rng = random.Random(seed)
+    new = [rng.choice((0, 1, 1, 1, 3)) for _ in range(n)]
+    start = [rng.randint(0, 60) for _ in range(n)]
+    for i in (5, 700, n - 9):
+        new[i], start[i] = 1, rng.randint(2500, 6000)
+    for i in (17, n - 30):
+        new[i], start[i] = rng.randint(100, 300), rng.randint(0, 3000)
+    return new, start
+
+
+LARGE = [
+    # new, start, heads, kv_heads, d, page: more than 2048 rows, ranges of both kinds split
+    ([1500, 1, 1, 700, 5, 0, 1], [4000, 9000, 3000, 0, 1200, 50, 0], 8, 2, 64, 16),
+    ([2, 2100, 1, 40], [7000, 1100, 0, 2500], 16, 2, 128, 32),
+    # more than 1024 requests: two and three rounds of the scan
+    (*many_requests(1, 1300), 4, 1, 64, 16), (*many_requests(2, 2300), 2, 1, 128, 8),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", range(len(LARGE)))
+def test_attention_of_large_steps(dev, case, dtype):
+    new, start, heads, kv_heads, d, page = LARGE[case]
+    assert sum(new) > 2048 or len(new) > 1024
+    q, keys, values, table, step = cache_case(dev, new, start, heads, kv_heads, d, page, dtype, case)
+    got = paged_attention(q, keys, values, step, d ** -0.5)
+    check_attention(got, q, keys, values, table, start, new, d ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_both_work_lists_of_one_step_agree(dev, seed):
+    """One launch builds the list of a small step, two that of a step with room for many rows: the same items and parts,
+    so the same results bit for bit."""
+    rng = random.Random(seed)
+    heads, kv_heads, d = rng.choice(((32, 8, 128), (4, 1, 64), (12, 2, 64), (8, 8, 128)))
+    n = (1, 3, 30, 200, 900, 1024, 40, 9)[seed]
+    new = [rng.choice((0, 1, 1, 2)) if n > 100 else rng.choice((0, 1, 4, rng.randint(5, 1200 // n + 5))) for _ in range(n)]
+    new[0] = max(new[0], 1)
+    start = [rng.choice((0, rng.randint(0, 100), rng.randint(0, 100), rng.randint(0, 3000 if n < 100 else 200))) for _ in range(n)]
+    start[-1] = 4000
+    q, keys, values, table, step = cache_case(dev, new, start, heads, kv_heads, d, 16, torch.bfloat16, seed)
+    rows = sum(new)
+    assert rows <= 2048
+    roomy = page_tables(step.state, i32(start, dev), i32(new, dev), rows=2500, max_new=max(new), heads=heads, kv_heads=kv_heads,
+                        head_dim=d)
+    assert torch.equal(roomy.slots[:rows], step.slots) and torch.equal(roomy.row_indptr, step.row_indptr)
+    wide = torch.cat((q, torch.zeros(2500 - rows, heads * d, dtype=q.dtype, device=dev)))
+    assert torch.equal(paged_attention(wide, keys, values, roomy, d ** -0.5)[:rows], paged_attention(q, keys, values, step, d ** -0.5))
