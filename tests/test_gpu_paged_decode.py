@@ -9,6 +9,8 @@ from multi_lora_amd.decoder import Decoder, DecoderConfig, PagedKV
 from multi_lora_amd.graph_decode import capture_graph
 from multi_lora_amd.paged_decode import PagedDecode
 
+from tests import paged_ref as ref
+
 pytestmark = pytest.mark.gpu
 
 PROJ = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj", "mlp.gate_proj", "mlp.up_proj",
@@ -312,3 +314,61 @@ def test_captured_verification_short_of_pages_equals_the_direct_one(dev):
             assert torch.equal(x, y)
         seen |= set(direct.placed.tolist())
     assert 0 in seen and 4 in seen and len(seen) > 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@torch.inference_mode()
+def test_drawn_drafts(dev, dtype):
+    """Drafts drawn from given probabilities, in steps between which requests decode: accepted as the definition says from
+    the model's own probabilities, and what is kept gives the logits of the whole sequences."""
+    mgr, cfg = build(dtype)
+    ps = prompts(cfg, 9)
+    k = 3
+    g = torch.Generator(dev).manual_seed(6)
+    step, twin = PagedDecode.new(mgr, 4, 112), PagedDecode.new(mgr, 4, 112)
+    for s in (step, twin):
+        s.input_ids.copy_(s.prefill(mgr, ps, NAMES))
+    seqs = [torch.cat((p, t)) for p, t in zip(ps, step.input_ids)]
+    kept = []
+    for _ in range(3):
+        q = torch.softmax(torch.randn(4, k, cfg.vocab_size, generator=g, device=dev) * 0.6, -1)
+        drafts = q.view(-1, cfg.vocab_size).multinomial(1, generator=g).view(4, k)
+        u, last = torch.rand(4, k, generator=g, device=dev), torch.rand(4, generator=g, device=dev)
+        mgr._setup_forward_batch(NAMES, seq_lens=[k + 1] * 4)
+        st = twin.kv.tables(twin.lens, torch.full_like(twin.lens, k + 1), twin.kv.new_step(4 * (k + 1), k + 1))
+        logits = mgr.model(input_ids=torch.cat((twin.input_ids, drafts), 1), past_key_values=twin.kv, paged_step=st).logits
+        want = ref.verify(torch.softmax(logits.float(), -1), q, drafts, st.row_indptr.tolist(), u, last)
+        accepted, tokens = step.verify(mgr, drafts, q, u, last)
+        assert accepted.tolist() == want[0] and tokens.tolist() == want[1] and step.placed.tolist() == [k + 1] * 4
+        kept += want[0]
+        seqs = [torch.cat((s, d[:a], t)) for s, d, a, t in zip(seqs, drafts, want[0], step.input_ids)]
+        mgr._setup_forward_batch(NAMES, seq_lens=[1] * 4)
+        got = step.run(mgr).logits
+        rows = torch.stack([whole(mgr, s, n)[-1] for s, n in zip(seqs, NAMES)])
+        torch.testing.assert_close(got.float(), rows.float(), atol=ATOL, rtol=ATOL)
+        step.input_ids.copy_(got.argmax(-1, keepdim=True))
+        seqs = [torch.cat((s, t)) for s, t in zip(seqs, step.input_ids)]
+        # The other decoder keeps the same tokens.
+        twin.lens.copy_(step.lens - 1)
+        twin.input_ids.copy_(torch.stack([s[-2:-1] for s in seqs]))
+        mgr._setup_forward_batch(NAMES, seq_lens=[1] * 4)
+        assert torch.equal(twin.run(mgr).logits, got)
+        twin.input_ids.copy_(step.input_ids)
+    assert min(kept) < k and max(kept) > 0
+
+
+@torch.inference_mode()
+def test_ragged_float16_prompts_and_steps_equal_whole_sequences(dev):
+    mgr, cfg = build(torch.float16)
+    ps = prompts(cfg, 12)
+    step = PagedDecode.new(mgr, 4, 96, page=32)
+    step.input_ids.copy_(step.prefill(mgr, ps, NAMES))
+    seqs = list(ps)
+    for _ in range(3):
+        seqs = [torch.cat((s, t)) for s, t in zip(seqs, step.input_ids)]
+        mgr._setup_forward_batch(NAMES, seq_lens=[1] * 4)
+        got = step.run(mgr).logits
+        want = torch.stack([whole(mgr, s, n)[-1] for s, n in zip(seqs, NAMES)])
+        torch.testing.assert_close(got.float(), want.float(), atol=ATOL, rtol=ATOL)
+        step.input_ids.copy_(got.argmax(-1, keepdim=True))
+    assert step.placed.tolist() == [1] * 4
