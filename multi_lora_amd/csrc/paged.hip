@@ -7,12 +7,12 @@
 // the free stack, so nothing is claimed by atomics and a step gives the same
 // pages every time.  The bytes are kilobytes: launches and the chain of reads
 // bound it, hence one workgroup and one launch for all but the largest steps:
-// 168 requests of one token 5.6 us on average, of a step and its taking back.
-// Beyond, two launches: 7.0 + 2.8 us for 4139 rows of 72 requests.
+// 168 requests of one token 5.6 us, the average of a step and its taking back.
+// Beyond, two launches: 8.1 + 3.9 us on average for 4139 rows of 72 requests.
 //
 // Write: bound by its bytes, read and written once each.  4075 rows of 32 + 2 *
-// 8 heads of 128, 102 MB, take 20.2 us, 5.1 TB/s, the rate of a large copy; 64
-// rows 3.8.
+// 8 heads of 128, 102 MB, take 20.5 us on average, 5.0 TB/s, where a copy of 1
+// GB has 5.15; 64 rows 3.6.
 #include <algorithm>
 
 #include "kernels.h"

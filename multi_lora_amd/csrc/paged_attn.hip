@@ -14,7 +14,9 @@
 //
 // Roundings: the weights, for the second product, to the data type (half a
 // step of each; their sum is taken before), the result once; scores, sums and
-// rescaling are fp32.
+// rescaling are fp32.  (The decoder's q is rounded by the write before.  The
+// matrix units take 16-bit operands only; the static cache's attention, which
+// uses none, rounds neither.)
 //
 // Masked places: their scores become -inf by selection, and where a tile has
 // any, values that are not finite are left out of the product and added in
@@ -118,10 +120,10 @@ struct StreamLds {
 
 // Short items: wave w of NW takes tiles w, w + NW, ... of 32 positions,
 // straight from memory into MFMA operands; the waves meet in LDS at the end.
-// Bound by the bytes of K and V, read once each: 68 decoding requests of 200
-// to 3985 positions, 295 MB, 59.1 us (5.0 TB/s); 64 of 4096 5.5 to 5.8 TB/s.
-// Few short ranges are bound by their chain: work list, page number, keys,
-// values, meeting (4.4 us for one request of a few positions).
+// Bound by the bytes of K and V, read once each: 64 decoding requests of 200
+// to 3985 positions, 295 MB, 60.6 us on average (4.9 TB/s).  Few short ranges
+// are bound by their chain: work list, page number, keys, values, meeting (4.7
+// us for one request of 203 positions).
 template <class T, int D, int NW, int MT>
 __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, StreamLds<D, NW, MT>& s, int item, int head) {
   using raw = typename T::raw_t;
@@ -351,8 +353,9 @@ constexpr int kBlock = 68;
 // step go straight into LDS, a step ahead, in one of two buffers.  Chunk p of
 // a row lies at p ^ (row's low bits), which spreads a fragment's rows over the
 // banks.  Bound by the matrix units and the exponentials beside them: 444
-// GFLOP (chunks of 4096, 777 and 1301 tokens, 32 heads of 128) take 456 to 505
-// us, 880 to 970 TFLOP/s where a large library product has 1142 to 1218.  The
+// GFLOP (chunks of 4096, 777 and 1301 tokens, 32 heads of 128) take 465 to 474
+// us a call, 935 to 955 TFLOP/s where a library product of 8192^3 has 1200 to
+// 1212 on the same card (504 on average under the profiler, 468 at best).  The
 // matrix units are busy in 44 % of the cycles, at 1.9 GHz under this load.
 // Without the exponentials it takes 4 % less, without the loads 17 %, with half
 // of the second product 12 %.

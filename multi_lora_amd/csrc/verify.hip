@@ -6,16 +6,19 @@
 // max(p_j - q_j, 0) at the first rejection j (certain drafts: q is 1 at x_j,
 // 0 elsewhere), from p_k after k acceptances: the lowest x whose cumulated
 // mass exceeds w times the row's mass.  Products, sums and cumulated sums are
-// fp64, so a draw does not depend on how the row is cut.  Mass that is not
-// positive (NaN too) counts as none; a residual without mass falls back to
-// p_j, and a row without mass has no answer (-1).
+// fp64 and always added in the same order: an answer repeats, and differs from
+// that of adding column by column only where w times the mass is within some
+// vocab * 2^-53 of it of a column's border.  Mass that is not positive (NaN
+// too) counts as none; a residual without mass falls back to p_j, and a row
+// without mass has no answer (-1).
 //
 // Two launches, for one row's sums are needed before its draw: a workgroup
 // per 2048 columns of a request's row, which finds the row itself, then a
 // workgroup per request that reads the one chunk its draw falls in.  Rows of
-// up to 4096 columns are one launch, bound by its chain of reads: 4.3 us for
+// up to 4096 columns are one launch, bound by its chain of reads: 5.3 us for
 // one request.  Thirty-two requests of 128,256 fp32 columns (31.8 MB with the
-// drafts' rows) take 7.6 us for the sums, 4.2 TB/s, and 4.4 us for the draw.
+// drafts' rows) take 8.5 us for the sums, 3.7 TB/s, and 4.7 us for the draw
+// (averages).
 #include "kernels.h"
 #include "loads.h"
 #include "paged.h"
@@ -304,6 +307,8 @@ __global__ __launch_bounds__(draw_threads(ONE)) void verify_draw_kernel(VerifyAr
       last_s[wave] = last_mass;
     }
     __syncthreads();
+    // No hit where w is 1 or more, or where the chunk's own sum, added in another
+    // order, says so within a rounding: the last column with mass.
     for (int v = 0; v < kWaves; ++v) token = max(token, static_cast<int64_t>(last_s[v]));
     for (int v = kWaves - 1; v >= 0; --v)
       if (hit_s[v] >= 0) token = hit_s[v];

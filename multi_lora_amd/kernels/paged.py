@@ -138,7 +138,8 @@ class PagedStep:
     row_indptr[i + 1])``, the last of its ``kv_lens[i]`` positions.  Filled by
     ``page_tables``; with ``heads``, it carries the attention's work list and
     the workspace of its split ranges, so steps whose attention may overlap in
-    time (on different streams) need to be different ``PagedStep``s.
+    time (on different streams) need to be different ``PagedStep``s, kept until
+    those streams are done with them.
 
     ``row_indptr [n + 1]``, ``kv_lens [n]``, ``positions [rows]`` and ``slots
     [rows]`` (page * page size + offset; -1: no place) are int32 tensors.
@@ -393,7 +394,8 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
     Returns ``accepted [n]`` (int32) and ``[n, most + 1]`` (int64): the accepted
     drafts, the next token, then -1.  A request without rows gets 0 and -1; a
     row without any mass, -1.  Probabilities are float32, float16 or bfloat16;
-    all sums are fp64.
+    all sums are fp64, so a draw differs from that of exact sums only where
+    ``last[i]`` lies within about ``vocab * 2**-53`` of a column's border.
     """
     done = _ffi.calls().verify_drafts(target, draft, tokens, row_indptr, accept, last)
     if done is not None:
