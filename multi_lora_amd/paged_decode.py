@@ -64,8 +64,9 @@ class PagedDecode:
         return self.lens
 
     def rewind(self) -> None:
-        """Every request back to the end of its prompt; the pages after it go back to the pool."""
-        self.lens.copy_(self.start_lens)
+        """Every request back to the end of its prompt; the pages after it go
+        back to the pool.  One that is not that far (it has left) stays."""
+        torch.minimum(self.lens, self.start_lens, out=self.lens)
         self.kv.tables(self.lens, self.none, self.kv.new_step(0, 0))
 
     def prefill(self, mgr, prompts: Sequence[torch.Tensor], lora_names) -> torch.Tensor:

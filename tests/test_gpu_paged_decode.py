@@ -372,3 +372,19 @@ def test_ragged_float16_prompts_and_steps_equal_whole_sequences(dev):
         torch.testing.assert_close(got.float(), want.float(), atol=ATOL, rtol=ATOL)
         step.input_ids.copy_(got.argmax(-1, keepdim=True))
     assert step.placed.tolist() == [1] * 4
+
+
+@torch.inference_mode()
+def test_rewinding_after_a_request_has_left(dev):
+    """Its prompt is no longer cached: it is not taken back to the prompt's end."""
+    mgr, cfg, step, seqs = short_of_pages()
+    step_and_compare(mgr, step, seqs, ["a", "b"], (0, 1))
+    step.lens[1] = 0
+    seqs[1] = step.input_ids[1].clone()
+    step.input_ids[0] = 3
+    step_and_compare(mgr, step, [torch.cat((seqs[0], step.input_ids[0])), seqs[1]], ["a", "b"], (0, 1))
+    step.rewind()
+    assert step.lens.tolist() == [14, 1] and step.kv.state.held.tolist() == [1, 1]
+    step.input_ids.copy_(torch.tensor([[5], [6]]))
+    seqs = [torch.cat((seqs[0][:14], step.input_ids[0])), torch.cat((seqs[1], step.input_ids[1]))]
+    step_and_compare(mgr, step, seqs, ["a", "b"], (0, 1))
