@@ -82,12 +82,14 @@ class PagedDecode:
         ends = torch.tensor(counts, dtype=torch.int32).cumsum(0) - 1
         self.start = max(counts)
         self.start_lens.copy_(torch.tensor(counts, dtype=torch.int32))
+        self.lens.zero_()  # and so it stays if the prompts do not get through
         self.kv.tables(self.none, self.none, self.kv.new_step(0, 0))
         step = self.kv.tables(self.none, self.start_lens, self.kv.new_step(sum(counts), max(counts)))
         out = mgr.forward_with_lora(input_ids=torch.cat([p.reshape(-1) for p in prompts]).to(device), lora_names=lora_names,
                                     seq_lens=counts, past_key_values=self.kv, paged_step=step,
                                     logit_rows=ends.to(device))
         self.lens.copy_(self.start_lens)
+        self.placed.copy_(self.start_lens)
         return out.logits.argmax(dim=-1, keepdim=True)
 
     def run(self, mgr):

@@ -388,3 +388,17 @@ def test_rewinding_after_a_request_has_left(dev):
     step.input_ids.copy_(torch.tensor([[5], [6]]))
     seqs = [torch.cat((seqs[0][:14], step.input_ids[0])), torch.cat((seqs[1], step.input_ids[1]))]
     step_and_compare(mgr, step, seqs, ["a", "b"], (0, 1))
+
+
+@torch.inference_mode()
+def test_prompts_that_do_not_get_through_leave_an_empty_cache(dev):
+    mgr, cfg, step, _ = short_of_pages()
+    assert step.placed.tolist() == [14, 15]
+    ids = torch.arange(20, dtype=torch.long, device=dev)
+    with pytest.raises(ValueError):
+        step.prefill(mgr, [ids, ids[:3]], ["a"])  # one name for two prompts
+    assert step.lens.tolist() == [0, 0]
+    step.rewind()
+    assert step.lens.tolist() == [0, 0] and step.kv.state.counts.tolist() == [3, 0]
+    step.input_ids.copy_(ids[4:6, None])
+    step_and_compare(mgr, step, [ids[4:5], ids[5:6]], ["a", "b"], (0, 1))
