@@ -402,3 +402,18 @@ def test_prompts_that_do_not_get_through_leave_an_empty_cache(dev):
     assert step.lens.tolist() == [0, 0] and step.kv.state.counts.tolist() == [3, 0]
     step.input_ids.copy_(ids[4:6, None])
     step_and_compare(mgr, step, [ids[4:5], ids[5:6]], ["a", "b"], (0, 1))
+
+
+@torch.inference_mode()
+def test_fused_projections_over_the_paged_cache(dev, monkeypatch):
+    """q, k and v as columns of one fused output."""
+    monkeypatch.setenv("MULTI_LORA_FUSED_QKV", "all")
+    monkeypatch.setenv("MULTI_LORA_FUSED_GATE_UP", "1")
+    mgr, cfg = build()
+    ps = prompts(cfg, 14)
+    step = PagedDecode.new(mgr, 4, 96)
+    step.input_ids.copy_(step.prefill(mgr, ps, NAMES))
+    mgr._setup_forward_batch(NAMES, seq_lens=[1] * 4)
+    got = step.run(mgr).logits
+    want = torch.stack([whole(mgr, torch.cat((p, t)), n)[-1] for p, t, n in zip(ps, step.input_ids, NAMES)])
+    torch.testing.assert_close(got.float(), want.float(), atol=ATOL, rtol=ATOL)
