@@ -471,7 +471,7 @@ int mlora_rotary_paged_write(const void* q, int64_t q_row_stride, const void* k,
  * or past the table, is NaN.  What lies in positions that a row does not
  * attend to (NaN too) does not reach it.
  * Requirements (else -2): bf16 or fp16; D 64 or 128; 16-byte aligned rows of
- * q, out and pages. */
+ * q, out and pages; pages less than 2^30 elements apart. */
 int mlora_paged_attention(const void* q, int64_t q_row_stride, const void* keys, int64_t key_page_stride,
                           const void* values, int64_t value_page_stride, const mlora_pages* pages,
                           const mlora_paged_step* step, void* out, int64_t out_row_stride, int32_t heads,
