@@ -296,6 +296,7 @@ def test_captured_verification_short_of_pages_equals_the_direct_one(dev):
     with torch.cuda.stream(side):
         recorded.verify(mgr, drafts, None, u, last)
         recorded.rewind()
+    torch.cuda.current_stream().wait_stream(side)
     recorded.input_ids.copy_(direct.input_ids)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=side):
