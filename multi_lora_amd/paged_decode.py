@@ -112,6 +112,9 @@ class PagedDecode:
         and its tokens are -1."""
         k = int(drafts.shape[1])
         if k not in self._chunks:
+            if self.lens.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"the step of {k} drafts does not exist yet: its lengths would only be written when the "
+                                   "graph runs; verify as many drafts once before capturing")
             self._chunks[k] = (self.kv.new_step(self.batch * (k + 1), k + 1), torch.full_like(self.one, k + 1))
         step, new = self._chunks[k]
         self.kv.tables(self.lens, new, step)

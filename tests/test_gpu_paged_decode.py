@@ -418,3 +418,23 @@ def test_fused_projections_over_the_paged_cache(dev, monkeypatch):
     got = step.run(mgr).logits
     want = torch.stack([whole(mgr, torch.cat((p, t)), n)[-1] for p, t, n in zip(ps, step.input_ids, NAMES)])
     torch.testing.assert_close(got.float(), want.float(), atol=ATOL, rtol=ATOL)
+
+
+@torch.inference_mode()
+def test_verification_is_not_captured_before_its_first_call(dev):
+    """What its step is made of would be filled by the graph alone, and an eager call before that read memory as it was."""
+    mgr, cfg, step, _ = short_of_pages()
+    other = short_of_pages()[2]
+    drafts, u, last = torch.zeros(2, 2, dtype=torch.long, device=dev), torch.ones(2, 2, device=dev), torch.zeros(2, device=dev)
+    stream = torch.cuda.Stream()
+    mgr._setup_forward_batch(["a", "b"], seq_lens=[3, 3])
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        other.verify(mgr, drafts, None, u, last)  # the adapters' workspace of the stream exists
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="once before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+            step.verify(mgr, drafts, None, u, last)
+    accepted, _ = step.verify(mgr, drafts, None, u, last)
+    assert accepted.tolist() == [0, 0] and step.placed.tolist() == [3, 1] and step.lens.tolist() == [15, 16]
