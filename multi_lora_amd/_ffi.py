@@ -51,6 +51,10 @@ EXPORTS = (
     "mlora_paged_attention",
     "mlora_verify_workspace_bytes",
     "mlora_verify_drafts",
+    "mlora_quantize_rows",
+    "mlora_int8_matmul",
+    "mlora_int8_linear_workspace_bytes",
+    "mlora_int8_linear",
 )
 
 # include/mlora_hip.h: MLORA_STATIC_SCRATCH_BYTES
@@ -237,6 +241,16 @@ _SIGNATURES = {
         [_vp, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _sz,
          _vp],
     ),
+    "mlora_quantize_rows": (ctypes.c_int, [_vp, _i64, _i32, _i32, _vp, _i64, _vp, _i32, _vp]),
+    "mlora_int8_matmul": (
+        ctypes.c_int,
+        [_vp, _i64, _vp, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i64, _i32, _vp],
+    ),
+    "mlora_int8_linear_workspace_bytes": (_sz, [_i32, _i32]),
+    "mlora_int8_linear": (
+        ctypes.c_int,
+        [_vp, _i64, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i64, _i32, _vp, _sz, _vp],
+    ),
     "mlora_build_plan": (ctypes.c_int, [ctypes.POINTER(SegMeta), _i32, _vp, _i32, _vp]),
     "mlora_rmsnorm_apply_grouped": (
         ctypes.c_int,
@@ -280,7 +294,8 @@ _CALLS_FUNCTIONS = ("mlora_last_error", "mlora_shrink_workspace_bytes", "mlora_s
                     "mlora_apply_segments_workspace_bytes", "mlora_apply_segments", "mlora_rmsnorm",
                     "mlora_add_rmsnorm", "mlora_grouped_workspace_bytes", "mlora_apply_grouped",
                     "mlora_rmsnorm_apply_grouped", "mlora_page_tables", "mlora_rotary_paged_write",
-                    "mlora_paged_attention", "mlora_verify_workspace_bytes", "mlora_verify_drafts")
+                    "mlora_paged_attention", "mlora_verify_workspace_bytes", "mlora_verify_drafts",
+                    "mlora_int8_linear_workspace_bytes", "mlora_int8_linear")
 _calls_module = None
 
 

@@ -50,6 +50,8 @@ struct Library {
   decltype(&mlora_paged_attention) paged_attention;
   decltype(&mlora_verify_workspace_bytes) verify_ws;
   decltype(&mlora_verify_drafts) verify;
+  decltype(&mlora_int8_linear_workspace_bytes) int8_ws;
+  decltype(&mlora_int8_linear) int8_linear;
 };
 Library lib{};
 PyObject* launch_error = nullptr;  // exception type of a failed launch
@@ -723,6 +725,48 @@ PyObject* verify_drafts(PyObject* const* args, Took* took) {
   return a.p != nullptr && o.p != nullptr ? PyTuple_Pack(2, a.p, o.p) : nullptr;
 }
 
+// kernels.int8.int8_linear of a new output.
+PyObject* int8_linear(PyObject* const* args, Took* took) {
+  const at::Tensor *x = tensor_of(args[0]), *codes = tensor_of(args[1]), *scales = tensor_of(args[2]);
+  const at::Tensor* bias = args[4] == Py_None ? nullptr : tensor_of(args[4]);
+  if (x == nullptr || codes == nullptr || scales == nullptr || (bias == nullptr && args[4] != Py_None) || args[5] != Py_None ||
+      !PyLong_CheckExact(args[3]))
+    return nullptr;
+  const at::Device dev = x->device();
+  const at::ScalarType dt = x->scalar_type();
+  const long k = PyLong_AsLong(args[3]);
+  if (!is_current(dev) || (dt != at::kBFloat16 && dt != at::kHalf) || !is_rows(*x) || x->size(0) == 0 || x->size(1) != k ||
+      !is_rows_of(x, dev, dt, x->size(0), k) || wants_grad({x}) || maybe_traced() || has_tangent({x}))
+    return nullptr;
+  // Int8Rows has checked what its tensors look like.
+  if (codes->dim() != 2 || codes->device() != dev || codes->scalar_type() != at::kChar || !fits_i32(codes->size(0)) ||
+      scales->device() != dev || scales->scalar_type() != at::kFloat)
+    return nullptr;
+  const int64_t m = x->size(0), n = codes->size(0);
+  if (n == 0) return nullptr;
+  if (bias != nullptr && (bias->device() != dev || bias->scalar_type() != dt || bias->dim() != 1 || bias->size(0) != n ||
+                          !bias->is_contiguous() || wants_grad({bias}) || has_tangent({bias})))
+    return nullptr;
+  at::Tensor out = at::empty({m, n}, x->options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+  const size_t need = lib.int8_ws(static_cast<int32_t>(m), static_cast<int32_t>(k));
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({static_cast<int64_t>(need)}, scales->options().dtype(at::kByte));
+  const hipStream_t stream = stream_of(dev);
+  const void *xp = x->data_ptr(), *bp = bias != nullptr ? bias->data_ptr() : nullptr;
+  const int8_t* cp = static_cast<const int8_t*>(codes->data_ptr());
+  const float* sp = scales->data_ptr<float>();
+  void *op = out.data_ptr(), *wp = need > 0 ? ws.data_ptr() : nullptr;
+  const int64_t xs = row_stride(*x), cs = row_stride(*codes);
+  const int code = dtype_code(dt);
+  const int rc = unlocked([&] {
+    return lib.int8_linear(xp, xs, static_cast<int32_t>(m), cp, cs, sp, static_cast<int32_t>(n), static_cast<int32_t>(k), bp,
+                           op, n, code, wp, need, stream);
+  });
+  *took = outcome(rc, "mlora_int8_linear");
+  if (*took != Took::kYes) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+}
+
 // f(&took) -> a new reference or nullptr, as the module's functions return it:
 // None when the call was not taken.  No C++ exception gets out (an error of
 // torch's, as for a tensor without storage, leaves the call to the caller).
@@ -808,14 +852,19 @@ PyObject* py_verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&](Took* took) { return verify_drafts(args, took); });
 }
 
+PyObject* py_int8_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!arity(n, 6)) return nullptr;
+  return guarded([&](Took* took) { return int8_linear(args, took); });
+}
+
 // set_library(addresses, launch_error, meta_type): the library's functions in
 // the order of the struct Library.
 PyObject* py_set_library(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!arity(n, 3)) return nullptr;
-  constexpr int kFns = 16;
+  constexpr int kFns = 18;
   void* p[kFns];
   if (!PyTuple_CheckExact(args[0]) || PyTuple_GET_SIZE(args[0]) != kFns) {
-    PyErr_SetString(PyExc_TypeError, "a tuple of the library's sixteen addresses is expected");
+    PyErr_SetString(PyExc_TypeError, "a tuple of the library's eighteen addresses is expected");
     return nullptr;
   }
   for (int i = 0; i < kFns; ++i) {
@@ -841,6 +890,8 @@ PyObject* py_set_library(PyObject*, PyObject* const* args, Py_ssize_t n) {
   lib.paged_attention = reinterpret_cast<decltype(lib.paged_attention)>(p[13]);
   lib.verify_ws = reinterpret_cast<decltype(lib.verify_ws)>(p[14]);
   lib.verify = reinterpret_cast<decltype(lib.verify)>(p[15]);
+  lib.int8_ws = reinterpret_cast<decltype(lib.int8_ws)>(p[16]);
+  lib.int8_linear = reinterpret_cast<decltype(lib.int8_linear)>(p[17]);
   Py_INCREF(args[1]);
   Py_INCREF(args[2]);
   Py_XSETREF(launch_error, args[1]);
@@ -866,6 +917,7 @@ PyMethodDef methods[] = {
                  "(q, k, v, cos, sin, keys, values, slots, out or None) -> out, or None"),
     MLORA_METHOD("verify_drafts", py_verify_drafts,
                  "(target, draft or None, tokens, row_indptr, accept, last) -> (accepted, tokens), or None"),
+    MLORA_METHOD("int8_linear", py_int8_linear, "(x, codes, scales, k, bias or None, out or None) -> new tensor, or None"),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Native form of the entry points' ordinary calls.", -1, methods,
                       nullptr,               nullptr,  nullptr,                                            nullptr};

@@ -1,0 +1,50 @@
+// Products in 8-bit integers: argument structs shared by csrc/int8.hip and the
+// C entry points (the layouts callers see are in include/mlora_hip.h).
+#pragma once
+
+#include "common.h"
+
+namespace mlora {
+
+// Codes of a row are padded with zeros to a multiple of this many.
+constexpr int kInt8Pad = 128;
+constexpr int64_t int8_padded(int64_t k) { return (k + kInt8Pad - 1) / kInt8Pad * kInt8Pad; }
+// 127^2 * 2^17 < 2^31: sums of this many products fit 32 bits.
+constexpr int kInt8MaxK = 1 << 17;
+
+struct QuantArgs {
+  const void* x;
+  int64_t x_stride;
+  int rows, k;
+  int8_t* codes;
+  int64_t codes_stride;
+  float* scales;
+};
+hipError_t launch_quantize_rows(const QuantArgs& a, int dtype, bool aligned, hipStream_t stream);
+
+struct Int8Args {
+  // Activations: codes and scales, or (of calls with few of them) the 16-bit
+  // rows themselves.
+  const int8_t* a;
+  int64_t a_stride;
+  const float* a_scales;
+  const void* x;
+  int64_t x_stride;
+  int x_aligned;
+  int m;
+  // Weight.
+  const int8_t* b;
+  int64_t b_stride;
+  const float* b_scales;
+  int n;
+  int k;              // of x; the codes have int8_padded(k)
+  const void* bias;   // [n] of the data type, or nullptr
+  void* out;
+  int64_t out_stride;
+  int vec;            // four outputs of a row can be stored at once
+};
+// Whether a call of 16-bit rows is quantised inside the product's own launch.
+bool int8_fused(int m, int k);
+hipError_t launch_int8_matmul(const Int8Args& a, int dtype, int cus, hipStream_t stream);
+
+}  // namespace mlora

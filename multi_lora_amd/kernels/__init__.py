@@ -1,5 +1,6 @@
 """HIP segment-LoRA kernels (export surface of multi_lora/kernels/__init__.py:3-7)."""
 
+from .int8 import Int8Rows, int8_linear, int8_matmul, quantize_rows
 from .lora_ops import (
     Workspace,
     sgemm_lora_a_fwd,
@@ -27,4 +28,8 @@ __all__ = [
     "rotary_paged_write",
     "paged_attention",
     "verify_drafts",
+    "Int8Rows",
+    "quantize_rows",
+    "int8_matmul",
+    "int8_linear",
 ]

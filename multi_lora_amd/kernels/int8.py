@@ -1,0 +1,227 @@
+"""Products of 16-bit activations with 8-bit weights, on the HIP kernels.
+
+``quantize_rows`` turns every row of a matrix into 8-bit integers and one fp32
+scale; ``int8_matmul`` multiplies two such matrices (a scale for each token,
+and for each output channel), ``int8_linear`` quantises its activations on the
+way.  ``layers.Int8Linear`` is the module over it, ``layers.quantize_base``
+puts it in a model's place of its linear layers, beneath the adapters.
+
+A row's scale is ``max|x| / 127``, its codes ``round(x / scale)``, ties to
+even.  Sums of products are exact, so a result differs from that of exact
+arithmetic on the codes only by its fp32 scaling and one rounding, and repeats
+bit for bit.  Results are float16 or bfloat16.  There is no CPU path and no
+derivative in either mode: inputs that ask for one are refused, and so are
+calls under a trace, which would not see them.
+
+No counterpart in the reference, whose base products are the model's own
+(multi_lora/layers.py:42-88).
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Sequence
+
+import torch
+
+from .. import _ffi
+from .paged import _DTYPES, _guard, _no_grad, _no_tangent, _on_gpu, _untraced, _writes
+
+PAD = 128        # columns of codes come in multiples of it
+MAX_K = 1 << 17  # longer sums of products could leave 32 bits
+
+
+def _padded(k: int) -> int:
+    return -(-k // PAD) * PAD
+
+
+@dataclass(frozen=True)
+class Int8Rows:
+    """Quantised rows ``[rows, k]``: ``codes [rows, k rounded up to 128]`` (zeros
+    behind column ``k``) and ``scales [rows]``.  Row ``r`` stands for
+    ``codes[r, :k] * scales[r]``."""
+
+    codes: torch.Tensor   # int8
+    scales: torch.Tensor  # float32
+    k: int
+
+    def __post_init__(self) -> None:
+        c, s = self.codes, self.scales
+        if not 1 <= self.k <= MAX_K:
+            raise ValueError(f"rows of 1 to {MAX_K} elements, got {self.k}")
+        if c.dtype != torch.int8 or c.dim() != 2 or c.shape[1] != _padded(self.k) or (c.numel() > 0 and c.stride(1) != 1):
+            raise ValueError(f"codes must be int8 [rows, {_padded(self.k)}] with contiguous rows, got {tuple(c.shape)} {c.dtype}")
+        if c.shape[0] > 1 and (c.stride(0) % 16 or c.stride(0) < c.shape[1]) or c.data_ptr() % 16:
+            raise ValueError("codes need rows at multiples of 16 bytes")
+        if s.dtype != torch.float32 or tuple(s.shape) != (c.shape[0],) or not s.is_contiguous():
+            raise ValueError(f"scales must be a contiguous float32 tensor of {c.shape[0]} numbers, got {tuple(s.shape)} {s.dtype}")
+        if s.device != c.device:
+            raise ValueError(f"codes on {c.device}, scales on {s.device}")
+
+    @property
+    def shape(self):
+        """``(rows, k)``."""
+        return torch.Size((self.codes.shape[0], self.k))
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Int8Rows":
+        """Rows quantised elsewhere: ``codes [rows, k]`` int8 and ``scales [rows]``; copied into the padded layout."""
+        if codes.dtype != torch.int8 or codes.dim() != 2:
+            raise ValueError(f"codes must be int8 [rows, k], got {tuple(codes.shape)} {codes.dtype}")
+        rows, k = codes.shape
+        if not 1 <= k <= MAX_K:
+            raise ValueError(f"rows of 1 to {MAX_K} elements, got {k}")
+        padded = torch.zeros((rows, _padded(k)), dtype=torch.int8, device=codes.device)
+        padded[:, :k] = codes
+        return cls(padded, scales.to(torch.float32).contiguous(), k)
+
+    def rows(self, start: int, end: int) -> "Int8Rows":
+        """A view of rows ``[start, end)``."""
+        return Int8Rows(self.codes[start:end], self.scales[start:end], self.k)
+
+    @classmethod
+    def cat(cls, parts: Sequence["Int8Rows"]) -> "Int8Rows":
+        """The rows of several, one after the other."""
+        if len({p.k for p in parts}) != 1:
+            raise ValueError(f"rows of different lengths {[p.k for p in parts]}")
+        return cls(torch.cat([p.codes for p in parts]), torch.cat([p.scales for p in parts]), parts[0].k)
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values the codes stand for, ``[rows, k]``."""
+        return (self.codes[:, :self.k].float() * self.scales[:, None]).to(dtype)
+
+
+def _matrix(what: str, t: torch.Tensor, dtypes) -> None:
+    if t.dim() != 2 or t.dtype not in dtypes or (t.numel() > 0 and t.stride(1) != 1):
+        names = " or ".join(str(d).replace("torch.", "") for d in dtypes)
+        raise ValueError(f"{what} must be 2-D {names} with contiguous rows, got {tuple(t.shape)} {t.dtype}")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{what}: the rows overlap")
+
+
+def _stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two matrices share memory; columns of one buffer side by side do not."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    size, (sa, sb) = a.element_size(), (_stride(a), _stride(b))
+    pa, pb = a.data_ptr(), b.data_ptr()
+    ends = [p + ((t.shape[0] - 1) * s + t.shape[1]) * size for p, t, s in ((pa, a, sa), (pb, b, sb))]
+    if ends[0] <= pb or ends[1] <= pa:
+        return False
+    apart = (pb - pa) // size % sa
+    return sa != sb or apart < a.shape[1] or apart + b.shape[1] > sa
+
+
+def quantize_rows(x: torch.Tensor) -> Int8Rows:
+    """``x [rows, k]`` (float32, float16 or bfloat16) as 8-bit integers with a scale for each row.
+
+    The maximum counts as at least ``2**-100``.  A row with an infinity or a
+    NaN has a NaN scale (and a product with it a NaN result).  Codes of 16-bit
+    rows are those of exact arithmetic; of float32 rows, those of fp32
+    arithmetic, which may round a quotient next to halfway the other way.
+    """
+    dev = _on_gpu("quantize_rows", x)
+    _untraced("quantize_rows")
+    _no_grad("quantize_rows", x)
+    _no_tangent("quantize_rows", x)
+    _matrix("x", x, (torch.float32, *_DTYPES))
+    rows, k = x.shape
+    if not 1 <= k <= MAX_K:
+        raise ValueError(f"rows of 1 to {MAX_K} elements, got {k}")
+    codes = torch.empty((rows, _padded(k)), dtype=torch.int8, device=dev)
+    scales = torch.empty(rows, dtype=torch.float32, device=dev)
+    with _guard(dev):
+        rc = _ffi.lib().mlora_quantize_rows(x.data_ptr(), _stride(x), rows, k, codes.data_ptr(), codes.shape[1],
+                                            scales.data_ptr(), _ffi.dtype_code(x.dtype), _ffi.stream_ptr(dev))
+    _ffi.check(rc, "mlora_quantize_rows")
+    return Int8Rows(codes, scales, k)
+
+
+def _result(what: str, rows: int, weight: Int8Rows, bias: Optional[torch.Tensor], out: Optional[torch.Tensor],
+            dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    """The checked or new output, and the bias checked."""
+    n = weight.shape[0]
+    if bias is not None:
+        _on_gpu(what, weight.codes, bias)
+        _no_grad(what, bias)
+        _no_tangent(what, bias)
+        if tuple(bias.shape) != (n,) or bias.dtype != dtype or not bias.is_contiguous():
+            raise ValueError(f"bias must be a contiguous {dtype} tensor of {n} numbers, got {tuple(bias.shape)} {bias.dtype}")
+    if out is None:
+        return torch.empty((rows, n), dtype=dtype, device=dev)
+    _on_gpu(what, weight.codes, out)
+    _writes(what, out)
+    _no_tangent(what, out)
+    _matrix("out", out, (dtype,))
+    if tuple(out.shape) != (rows, n):
+        raise ValueError(f"out must be [{rows}, {n}], got {tuple(out.shape)}")
+    return out
+
+
+def _address(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def int8_matmul(a: Int8Rows, b: Int8Rows, dtype: torch.dtype, bias: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``a [m, k] @ b [n, k].T + bias`` of quantised rows, ``[m, n]`` in ``dtype`` (float16 or bfloat16; in ``out``
+    if given, which may be a column slice of a wider tensor)."""
+    dev = _on_gpu("int8_matmul", a.codes, b.codes)
+    _untraced("int8_matmul")
+    if a.k != b.k:
+        raise ValueError(f"rows of {a.k} and of {b.k} elements")
+    if dtype not in _DTYPES:
+        raise ValueError(f"int8_matmul: float16 or bfloat16, got {dtype}")
+    m, n = a.shape[0], b.shape[0]
+    given = out is not None
+    out = _result("int8_matmul", m, b, bias, out, dtype, dev)
+    with _guard(dev):
+        rc = _ffi.lib().mlora_int8_matmul(a.codes.data_ptr(), _stride(a.codes), a.scales.data_ptr(), m, b.codes.data_ptr(),
+                                          _stride(b.codes), b.scales.data_ptr(), n, a.k, _address(bias), out.data_ptr(),
+                                          _stride(out), _ffi.dtype_code(dtype), _ffi.stream_ptr(dev))
+    _ffi.check(rc, "mlora_int8_matmul")
+    if given:
+        torch.autograd.graph.increment_version(out)
+    return out
+
+
+def int8_linear(x: torch.Tensor, weight: Int8Rows, bias: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x [rows, k] @ weight.T + bias`` with the rows of ``x`` (float16 or bfloat16) quantised as ``quantize_rows``
+    does; ``[rows, n]`` in x's type (in ``out`` if given, which may be a column slice of a wider tensor, and must not
+    overlap ``x``).  A row with an infinity or a NaN gives NaN."""
+    # The ordinary call, checked and launched natively; what it does not take (None) runs, or raises, below.
+    done = _ffi.calls().int8_linear(x, weight.codes, weight.scales, weight.k, bias, out)
+    if done is not None:
+        return done if out is None else out
+    dev = _on_gpu("int8_linear", x, weight.codes)
+    _untraced("int8_linear")
+    _no_grad("int8_linear", x)
+    _no_tangent("int8_linear", x)
+    _matrix("x", x, _DTYPES)
+    rows, k = x.shape
+    if k != weight.k:
+        raise ValueError(f"x has rows of {k} elements, the weight of {weight.k}")
+    given = out is not None
+    out = _result("int8_linear", rows, weight, bias, out, x.dtype, dev)
+    if given and _overlap(x, out):
+        raise ValueError("int8_linear: out overlaps x")
+    lib = _ffi.lib()
+    need = lib.mlora_int8_linear_workspace_bytes(rows, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _guard(dev):
+        rc = lib.mlora_int8_linear(x.data_ptr(), _stride(x), rows, weight.codes.data_ptr(), _stride(weight.codes),
+                                   weight.scales.data_ptr(), weight.shape[0], k, _address(bias), out.data_ptr(),
+                                   _stride(out), _ffi.dtype_code(x.dtype), _address(ws), need, _ffi.stream_ptr(dev))
+    _ffi.check(rc, "mlora_int8_linear")
+    if given:
+        torch.autograd.graph.increment_version(out)
+    return out
