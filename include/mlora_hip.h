@@ -496,6 +496,40 @@ int mlora_verify_drafts(const void* target, int64_t target_row_stride, int32_t r
                         int32_t n, int32_t most, int32_t vocab, int32_t* accepted, int64_t* out, int32_t dtype,
                         void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- the paged KV cache in 8 bits ----------------------------------------
+ * Pools of e4m3 codes (4 exponent, 3 mantissa bits; NaN 0x7f, no infinity) in
+ * the layout of the 16-bit ones,
+ *   keys   [num_pages, kv_heads, page, D]
+ *   values [num_pages, kv_heads, D, page]
+ * with pages of 16 to 1024 positions, 16-byte aligned, and an exponent byte for
+ * each block of 16 positions of a key head,
+ *   key_scales, value_scales [num_pages, kv_heads, page / 16], contiguous:
+ * a code c of a block with byte b stands for c * 2^(b - 127), exactly a number of
+ * the data type.  Steps and page tables are those of the 16-bit cache. */
+
+/* mlora_rotary_paged_write into such pools: fp32 math, one rounding to a code.
+ * A block's exponent e is the least with max|new rows| <= 448 * 2^e within
+ * [-117, 120] (bf16) or [-15, 8] (fp16; at the upper end codes stop at 240), or
+ * the one it has if that is larger and the block holds earlier rows (its first
+ * new row is not its first position); those rows' codes are then rounded again
+ * if it grows.  Infinities and NaN (fp16: what rounds to infinity, too) become
+ * NaN and do not count.  Rows of one block must be neighbours in ascending
+ * order, as mlora_page_tables lists them. */
+int mlora_rotary_paged_write_fp8(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
+                                 int64_t v_row_stride, const void* cos, const void* sin, int64_t rot_row_stride,
+                                 int32_t rot_dtype, const int32_t* slots, int32_t rows, int32_t heads, int32_t kv_heads,
+                                 int32_t head_dim, void* keys, int64_t key_page_stride, void* values,
+                                 int64_t value_page_stride, uint8_t* key_scales, uint8_t* value_scales, int32_t num_pages,
+                                 int32_t page, void* q_out, int64_t q_out_row_stride, int32_t dtype, void* stream);
+
+/* mlora_paged_attention over such pools: the result for the values that the
+ * codes stand for, computed and rounded as there. */
+int mlora_paged_attention_fp8(const void* q, int64_t q_row_stride, const void* keys, int64_t key_page_stride,
+                              const void* values, int64_t value_page_stride, const uint8_t* key_scales,
+                              const uint8_t* value_scales, const mlora_pages* pages, const mlora_paged_step* step, void* out,
+                              int64_t out_row_stride, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale,
+                              int32_t dtype, void* stream);
+
 /* ---- products in 8-bit integers -----------------------------------------
  * A quantised row of k elements is `scale = max|x| / 127` (fp32; the maximum
  * counts as at least 2^-100) and codes rint(x / scale), ties to even, padded

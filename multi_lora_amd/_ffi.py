@@ -55,6 +55,8 @@ EXPORTS = (
     "mlora_int8_matmul",
     "mlora_int8_linear_workspace_bytes",
     "mlora_int8_linear",
+    "mlora_rotary_paged_write_fp8",
+    "mlora_paged_attention_fp8",
 )
 
 # include/mlora_hip.h: MLORA_STATIC_SCRATCH_BYTES
@@ -241,6 +243,16 @@ _SIGNATURES = {
         [_vp, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _sz,
          _vp],
     ),
+    "mlora_rotary_paged_write_fp8": (
+        ctypes.c_int,
+        [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp, _i64,
+         _vp, _vp, _i32, _i32, _vp, _i64, _i32, _vp],
+    ),
+    "mlora_paged_attention_fp8": (
+        ctypes.c_int,
+        [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, ctypes.POINTER(Pages), ctypes.POINTER(PagedStep), _vp, _i64, _i32,
+         _i32, _i32, _f32, _i32, _vp],
+    ),
     "mlora_quantize_rows": (ctypes.c_int, [_vp, _i64, _i32, _i32, _vp, _i64, _vp, _i32, _vp]),
     "mlora_int8_matmul": (
         ctypes.c_int,
@@ -295,7 +307,8 @@ _CALLS_FUNCTIONS = ("mlora_last_error", "mlora_shrink_workspace_bytes", "mlora_s
                     "mlora_add_rmsnorm", "mlora_grouped_workspace_bytes", "mlora_apply_grouped",
                     "mlora_rmsnorm_apply_grouped", "mlora_page_tables", "mlora_rotary_paged_write",
                     "mlora_paged_attention", "mlora_verify_workspace_bytes", "mlora_verify_drafts",
-                    "mlora_int8_linear_workspace_bytes", "mlora_int8_linear")
+                    "mlora_int8_linear_workspace_bytes", "mlora_int8_linear", "mlora_rotary_paged_write_fp8",
+                    "mlora_paged_attention_fp8")
 _calls_module = None
 
 

@@ -297,6 +297,105 @@ int expand_impl(const void* mid, int64_t mid_row_stride, int32_t num_rows, const
   return 0;
 }
 
+int paged_write_call(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
+                     int64_t v_row_stride, const void* cos, const void* sin, int64_t rot_row_stride,
+                     int32_t rot_dtype, const int32_t* slots, int32_t rows, int32_t heads, int32_t kv_heads,
+                     int32_t head_dim, void* keys, int64_t key_page_stride, void* values,
+                     int64_t value_page_stride, int32_t num_pages, int32_t page, uint8_t* key_scales,
+                     uint8_t* value_scales, bool kv8, void* q_out, int64_t q_out_row_stride, int32_t dtype, void* stream) {
+  g_err[0] = '\0';
+  if (dtype != MLORA_BF16 && dtype != MLORA_F16) return fail(kUnsupported, "paged write needs bf16 or fp16, got dtype %d", dtype);
+  if (rot_dtype != dtype && rot_dtype != MLORA_F32) return fail(kUnsupported, "rotary tables of the data type or fp32, got dtype %d", rot_dtype);
+  if (head_dim != 64 && head_dim != 128) return fail(kUnsupported, "head_dim 64 or 128, got %d", head_dim);
+  mlora_pages p{};
+  p.num_pages = num_pages, p.page = page, p.width = 1;
+  int shift;
+  if (const int rc = check_pages(&p, &shift)) return rc;
+  if (rows < 0 || heads < 1 || kv_heads < 1) return fail(kBadArg, "rows %d, heads %d, kv_heads %d", rows, heads, kv_heads);
+  const int64_t qw = static_cast<int64_t>(heads) * head_dim, kw = static_cast<int64_t>(kv_heads) * head_dim;
+  if (q_row_stride < qw || k_row_stride < kw || v_row_stride < kw || q_out_row_stride < qw || rot_row_stride < 0 ||
+      key_page_stride < kw * page || value_page_stride < kw * page)
+    return fail(kBadArg, "strides do not hold the rows or pages");
+  if (kv8 && page < mlora::kScaleBlock) return fail(kUnsupported, "8-bit pages of 16 positions or more, got %d", page);
+  if (rows == 0) return 0;
+  if (!q || !k || !v || !cos || !sin || !slots || !keys || !values || !q_out || (kv8 && (!key_scales || !value_scales)))
+    return fail(kBadArg, "null pointer");
+  mlora::WriteArgs a{};
+  a.q = q, a.k = k, a.v = v;
+  a.q_stride = q_row_stride, a.k_stride = k_row_stride, a.v_stride = v_row_stride;
+  a.cos = cos, a.sin = sin, a.rot_stride = rot_row_stride, a.rot_f32 = rot_dtype == MLORA_F32;
+  a.slots = slots;
+  a.rows = rows, a.heads = heads, a.kv_heads = kv_heads;
+  a.keys = keys, a.values = values;
+  a.key_stride = key_page_stride, a.value_stride = value_page_stride;
+  a.num_pages = num_pages, a.page_shift = shift;
+  a.q_out = q_out, a.q_out_stride = q_out_row_stride;
+  const bool aligned = al16(q) && al16(k) && al16(v) && al16(keys) && al16(values) && al16(q_out) && al16(cos) && al16(sin) &&
+                       q_row_stride % 8 == 0 && k_row_stride % 8 == 0 && v_row_stride % 8 == 0 && q_out_row_stride % 8 == 0 &&
+                       rot_row_stride % 8 == 0 && key_page_stride % 8 == 0 && value_page_stride % 8 == 0;
+  hipError_t e;
+  if (kv8) {
+    if (!al16(keys) || !al16(values) || key_page_stride % 16 != 0 || value_page_stride % 16 != 0)
+      return fail(kUnsupported, "8-bit pages need 16-byte alignment");
+    e = mlora::launch_rotary_paged_write8({a, key_scales, value_scales}, dtype, head_dim, aligned, static_cast<hipStream_t>(stream));
+  } else {
+    e = mlora::launch_rotary_paged_write(a, dtype, head_dim, aligned, static_cast<hipStream_t>(stream));
+  }
+  if (e != hipSuccess) return hip_fail(e, "paged write launch");
+  return 0;
+}
+
+int paged_attention_call(const void* q, int64_t q_row_stride, const void* keys, int64_t key_page_stride,
+                         const void* values, int64_t value_page_stride, const uint8_t* key_scales,
+                         const uint8_t* value_scales, bool kv8, const mlora_pages* pages,
+                         const mlora_paged_step* step, void* out, int64_t out_row_stride, int32_t heads,
+                         int32_t kv_heads, int32_t head_dim, float scale, int32_t dtype, void* stream) {
+  g_err[0] = '\0';
+  if (dtype != MLORA_BF16 && dtype != MLORA_F16) return fail(kUnsupported, "paged attention needs bf16 or fp16, got dtype %d", dtype);
+  int shift;
+  if (const int rc = check_pages(pages, &shift)) return rc;
+  if (const int rc = check_step(step)) return rc;
+  mlora::PagedAttnArgs a{};
+  const int64_t max_kv = static_cast<int64_t>(pages->width) * pages->page;
+  if (!paged_step_shape(pages->n, step->rows, step->max_new, max_kv, heads, kv_heads, head_dim, &a.shape)) return kUnsupported;
+  const int64_t qw = static_cast<int64_t>(heads) * head_dim, pw = static_cast<int64_t>(kv_heads) * head_dim * pages->page;
+  if (q_row_stride < qw || out_row_stride < qw || key_page_stride < pw || value_page_stride < pw)
+    return fail(kBadArg, "strides do not hold the rows or pages");
+  if (key_page_stride > INT32_MAX / 2 || value_page_stride > INT32_MAX / 2)
+    return fail(kUnsupported, "pages more than 2^30 elements apart");
+  if (kv8 && pages->page < mlora::kScaleBlock) return fail(kUnsupported, "8-bit pages of 16 positions or more, got %d", pages->page);
+  if (pages->n == 0 || step->rows == 0 || pages->num_pages == 0 || pages->width == 0) {
+    if (pages->n > 0 && step->rows > 0) return fail(kBadArg, "attention over a cache without pages");
+    return 0;
+  }
+  if (!q || !keys || !values || !out || !pages->table || !step->row_indptr || !step->kv_lens || !step->plan ||
+      (kv8 && (!key_scales || !value_scales)))
+    return fail(kBadArg, "null pointer");
+  if (!al16(q) || !al16(keys) || !al16(values) || !al16(out) || q_row_stride % 8 != 0 || out_row_stride % 8 != 0 ||
+      key_page_stride % (kv8 ? 16 : 8) != 0 || value_page_stride % (kv8 ? 16 : 8) != 0)
+    return fail(kUnsupported, "paged attention needs 16-byte aligned rows and pages");
+  if (step->plan_bytes < a.shape.plan_bytes || step->workspace_bytes < a.shape.ws_bytes ||
+      (a.shape.ws_bytes > 0 && step->workspace == nullptr))
+    return fail(kWorkspace, "plan of %zu bytes and workspace of %zu, needs %zu and %zu", step->plan_bytes,
+                step->workspace_bytes, a.shape.plan_bytes, a.shape.ws_bytes);
+  a.q = q, a.q_stride = q_row_stride;
+  a.keys = keys, a.values = values;
+  a.key_stride = key_page_stride, a.value_stride = value_page_stride;
+  a.num_pages = pages->num_pages, a.page_shift = shift;
+  a.table = pages->table, a.table_stride = pages->table_stride, a.width = pages->width;
+  a.plan = step->plan;
+  a.n = pages->n, a.rows = step->rows;
+  a.out = out, a.out_stride = out_row_stride;
+  a.workspace = static_cast<char*>(step->workspace);
+  a.kv_heads = kv_heads, a.rep = heads / kv_heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.key_scales = key_scales, a.value_scales = value_scales;
+  const auto launch = kv8 ? mlora::launch_paged_attention8 : mlora::launch_paged_attention;
+  const hipError_t e = launch(a, std::min(step->max_new, step->rows), dtype, head_dim, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "paged attention launch");
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -858,83 +957,37 @@ int mlora_rotary_paged_write(const void* q, int64_t q_row_stride, const void* k,
                              int32_t head_dim, void* keys, int64_t key_page_stride, void* values,
                              int64_t value_page_stride, int32_t num_pages, int32_t page, void* q_out,
                              int64_t q_out_row_stride, int32_t dtype, void* stream) {
-  g_err[0] = '\0';
-  if (dtype != MLORA_BF16 && dtype != MLORA_F16) return fail(kUnsupported, "paged write needs bf16 or fp16, got dtype %d", dtype);
-  if (rot_dtype != dtype && rot_dtype != MLORA_F32) return fail(kUnsupported, "rotary tables of the data type or fp32, got dtype %d", rot_dtype);
-  if (head_dim != 64 && head_dim != 128) return fail(kUnsupported, "head_dim 64 or 128, got %d", head_dim);
-  mlora_pages p{};
-  p.num_pages = num_pages, p.page = page, p.width = 1;
-  int shift;
-  if (const int rc = check_pages(&p, &shift)) return rc;
-  if (rows < 0 || heads < 1 || kv_heads < 1) return fail(kBadArg, "rows %d, heads %d, kv_heads %d", rows, heads, kv_heads);
-  const int64_t qw = static_cast<int64_t>(heads) * head_dim, kw = static_cast<int64_t>(kv_heads) * head_dim;
-  if (q_row_stride < qw || k_row_stride < kw || v_row_stride < kw || q_out_row_stride < qw || rot_row_stride < 0 ||
-      key_page_stride < kw * page || value_page_stride < kw * page)
-    return fail(kBadArg, "strides do not hold the rows or pages");
-  if (rows == 0) return 0;
-  if (!q || !k || !v || !cos || !sin || !slots || !keys || !values || !q_out) return fail(kBadArg, "null pointer");
-  mlora::WriteArgs a{};
-  a.q = q, a.k = k, a.v = v;
-  a.q_stride = q_row_stride, a.k_stride = k_row_stride, a.v_stride = v_row_stride;
-  a.cos = cos, a.sin = sin, a.rot_stride = rot_row_stride, a.rot_f32 = rot_dtype == MLORA_F32;
-  a.slots = slots;
-  a.rows = rows, a.heads = heads, a.kv_heads = kv_heads;
-  a.keys = keys, a.values = values;
-  a.key_stride = key_page_stride, a.value_stride = value_page_stride;
-  a.num_pages = num_pages, a.page_shift = shift;
-  a.q_out = q_out, a.q_out_stride = q_out_row_stride;
-  const bool aligned = al16(q) && al16(k) && al16(v) && al16(keys) && al16(values) && al16(q_out) && al16(cos) && al16(sin) &&
-                       q_row_stride % 8 == 0 && k_row_stride % 8 == 0 && v_row_stride % 8 == 0 && q_out_row_stride % 8 == 0 &&
-                       rot_row_stride % 8 == 0 && key_page_stride % 8 == 0 && value_page_stride % 8 == 0;
-  const hipError_t e = mlora::launch_rotary_paged_write(a, dtype, head_dim, aligned, static_cast<hipStream_t>(stream));
-  if (e != hipSuccess) return hip_fail(e, "paged write launch");
-  return 0;
+  return paged_write_call(q, q_row_stride, k, k_row_stride, v, v_row_stride, cos, sin, rot_row_stride, rot_dtype, slots, rows,
+                          heads, kv_heads, head_dim, keys, key_page_stride, values, value_page_stride, num_pages, page,
+                          nullptr, nullptr, false, q_out, q_out_row_stride, dtype, stream);
+}
+
+int mlora_rotary_paged_write_fp8(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
+                                 int64_t v_row_stride, const void* cos, const void* sin, int64_t rot_row_stride,
+                                 int32_t rot_dtype, const int32_t* slots, int32_t rows, int32_t heads, int32_t kv_heads,
+                                 int32_t head_dim, void* keys, int64_t key_page_stride, void* values,
+                                 int64_t value_page_stride, uint8_t* key_scales, uint8_t* value_scales, int32_t num_pages,
+                                 int32_t page, void* q_out, int64_t q_out_row_stride, int32_t dtype, void* stream) {
+  return paged_write_call(q, q_row_stride, k, k_row_stride, v, v_row_stride, cos, sin, rot_row_stride, rot_dtype, slots, rows,
+                          heads, kv_heads, head_dim, keys, key_page_stride, values, value_page_stride, num_pages, page,
+                          key_scales, value_scales, true, q_out, q_out_row_stride, dtype, stream);
 }
 
 int mlora_paged_attention(const void* q, int64_t q_row_stride, const void* keys, int64_t key_page_stride,
                           const void* values, int64_t value_page_stride, const mlora_pages* pages,
                           const mlora_paged_step* step, void* out, int64_t out_row_stride, int32_t heads,
                           int32_t kv_heads, int32_t head_dim, float scale, int32_t dtype, void* stream) {
-  g_err[0] = '\0';
-  if (dtype != MLORA_BF16 && dtype != MLORA_F16) return fail(kUnsupported, "paged attention needs bf16 or fp16, got dtype %d", dtype);
-  int shift;
-  if (const int rc = check_pages(pages, &shift)) return rc;
-  if (const int rc = check_step(step)) return rc;
-  mlora::PagedAttnArgs a{};
-  const int64_t max_kv = static_cast<int64_t>(pages->width) * pages->page;
-  if (!paged_step_shape(pages->n, step->rows, step->max_new, max_kv, heads, kv_heads, head_dim, &a.shape)) return kUnsupported;
-  const int64_t qw = static_cast<int64_t>(heads) * head_dim, pw = static_cast<int64_t>(kv_heads) * head_dim * pages->page;
-  if (q_row_stride < qw || out_row_stride < qw || key_page_stride < pw || value_page_stride < pw)
-    return fail(kBadArg, "strides do not hold the rows or pages");
-  if (key_page_stride > INT32_MAX / 2 || value_page_stride > INT32_MAX / 2)
-    return fail(kUnsupported, "pages more than 2^30 elements apart");
-  if (pages->n == 0 || step->rows == 0 || pages->num_pages == 0 || pages->width == 0) {
-    if (pages->n > 0 && step->rows > 0) return fail(kBadArg, "attention over a cache without pages");
-    return 0;
-  }
-  if (!q || !keys || !values || !out || !pages->table || !step->row_indptr || !step->kv_lens || !step->plan)
-    return fail(kBadArg, "null pointer");
-  if (!al16(q) || !al16(keys) || !al16(values) || !al16(out) || q_row_stride % 8 != 0 || out_row_stride % 8 != 0 ||
-      key_page_stride % 8 != 0 || value_page_stride % 8 != 0)
-    return fail(kUnsupported, "paged attention needs 16-byte aligned rows and pages");
-  if (step->plan_bytes < a.shape.plan_bytes || step->workspace_bytes < a.shape.ws_bytes ||
-      (a.shape.ws_bytes > 0 && step->workspace == nullptr))
-    return fail(kWorkspace, "plan of %zu bytes and workspace of %zu, needs %zu and %zu", step->plan_bytes,
-                step->workspace_bytes, a.shape.plan_bytes, a.shape.ws_bytes);
-  a.q = q, a.q_stride = q_row_stride;
-  a.keys = keys, a.values = values;
-  a.key_stride = key_page_stride, a.value_stride = value_page_stride;
-  a.num_pages = pages->num_pages, a.page_shift = shift;
-  a.table = pages->table, a.table_stride = pages->table_stride, a.width = pages->width;
-  a.plan = step->plan;
-  a.n = pages->n, a.rows = step->rows;
-  a.out = out, a.out_stride = out_row_stride;
-  a.workspace = static_cast<char*>(step->workspace);
-  a.kv_heads = kv_heads, a.rep = heads / kv_heads;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  const hipError_t e = mlora::launch_paged_attention(a, std::min(step->max_new, step->rows), dtype, head_dim, static_cast<hipStream_t>(stream));
-  if (e != hipSuccess) return hip_fail(e, "paged attention launch");
-  return 0;
+  return paged_attention_call(q, q_row_stride, keys, key_page_stride, values, value_page_stride, nullptr, nullptr, false,
+                              pages, step, out, out_row_stride, heads, kv_heads, head_dim, scale, dtype, stream);
+}
+
+int mlora_paged_attention_fp8(const void* q, int64_t q_row_stride, const void* keys, int64_t key_page_stride,
+                              const void* values, int64_t value_page_stride, const uint8_t* key_scales,
+                              const uint8_t* value_scales, const mlora_pages* pages, const mlora_paged_step* step, void* out,
+                              int64_t out_row_stride, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale,
+                              int32_t dtype, void* stream) {
+  return paged_attention_call(q, q_row_stride, keys, key_page_stride, values, value_page_stride, key_scales, value_scales,
+                              true, pages, step, out, out_row_stride, heads, kv_heads, head_dim, scale, dtype, stream);
 }
 
 size_t mlora_verify_workspace_bytes(int32_t n, int32_t vocab) {

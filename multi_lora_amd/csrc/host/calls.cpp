@@ -52,6 +52,8 @@ struct Library {
   decltype(&mlora_verify_drafts) verify;
   decltype(&mlora_int8_linear_workspace_bytes) int8_ws;
   decltype(&mlora_int8_linear) int8_linear;
+  decltype(&mlora_rotary_paged_write_fp8) paged_write8;
+  decltype(&mlora_paged_attention_fp8) paged_attention8;
 };
 Library lib{};
 PyObject* launch_error = nullptr;  // exception type of a failed launch
@@ -561,9 +563,25 @@ int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t
 // One layer's pools, pages contiguous.
 struct Pool {
   int64_t pages, kv_heads, page, d, key_stride, value_stride;
+  at::ScalarType rows;  // of the rows that are written and attend
+  // 8-bit pools (kernels.paged8.Fp8Pool has checked what they look like): exponents
+  const at::Tensor *key_scales = nullptr, *value_scales = nullptr;
+  bool read8(const at::Tensor* k, const at::Tensor* v, const at::Tensor* ks, const at::Tensor* vs, PyObject* code) {
+    if (k == nullptr || ks == nullptr || vs == nullptr || !PyLong_CheckExact(code) || k->scalar_type() != at::kFloat8_e4m3fn ||
+        ks->device() != k->device() || vs->device() != k->device())
+      return false;
+    key_scales = ks, value_scales = vs;
+    rows = PyLong_AsLong(code) == MLORA_BF16 ? at::kBFloat16 : at::kHalf;
+    return read_layout(k, v);
+  }
   bool read(const at::Tensor* k, const at::Tensor* v) {
-    if (k == nullptr || v == nullptr || k->dim() != 4 || v->dim() != 4 || !k->is_cuda() || v->device() != k->device()) return false;
-    if ((k->scalar_type() != at::kBFloat16 && k->scalar_type() != at::kHalf) || v->scalar_type() != k->scalar_type()) return false;
+    if (k == nullptr || (k->scalar_type() != at::kBFloat16 && k->scalar_type() != at::kHalf)) return false;
+    rows = k->scalar_type();
+    return read_layout(k, v);
+  }
+  bool read_layout(const at::Tensor* k, const at::Tensor* v) {
+    if (v == nullptr || k->dim() != 4 || v->dim() != 4 || !k->is_cuda() || v->device() != k->device()) return false;
+    if (v->scalar_type() != k->scalar_type()) return false;
     pages = k->size(0), kv_heads = k->size(1), page = k->size(2), d = k->size(3);
     if (pages < 1 || !fits_i32(pages) || v->size(0) != pages || v->size(1) != kv_heads || v->size(2) != d || v->size(3) != page) return false;
     if (k->stride(3) != 1 || k->stride(2) != d || k->stride(1) != page * d) return false;
@@ -590,13 +608,12 @@ Took page_tables(PyObject* const* args) {
 }
 
 // kernels.paged.paged_attention: the output, new or given.
-PyObject* paged_attention(PyObject* const* args, Took* took) {
-  const at::Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *v = tensor_of(args[2]);
+PyObject* attend(const at::Tensor* q, const at::Tensor* k, const at::Tensor* v, const Pool& pool, PyObject* pstep,
+                 PyObject* pscale, PyObject* pout, Took* took) {
   Step st;
-  Pool pool;
-  if (q == nullptr || !pool.read(k, v) || !st.read(args[3]) || !PyFloat_CheckExact(args[4])) return nullptr;
+  if (q == nullptr || !st.read(pstep) || !PyFloat_CheckExact(pscale)) return nullptr;
   const at::Device dev = k->device();
-  const at::ScalarType dt = k->scalar_type();
+  const at::ScalarType dt = pool.rows;
   const int64_t rows = st.step->rows, width = static_cast<int64_t>(st.heads) * st.head_dim;
   if (!is_current(dev) || dev.index() != st.device || st.step->plan == nullptr || rows == 0 || wants_grad({q, k, v}) ||
       maybe_traced() || has_tangent({q, k, v}) ||
@@ -604,45 +621,65 @@ PyObject* paged_attention(PyObject* const* args, Took* took) {
       pool.page != st.pages->page || pool.pages < st.pages->num_pages)
     return nullptr;
   at::Tensor out;
-  if (args[5] == Py_None) {
+  if (pout == Py_None) {
     out = at::empty({rows, width}, q->options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
   } else {
-    const at::Tensor* o = tensor_of(args[5]);
+    const at::Tensor* o = tensor_of(pout);
     if (!is_rows_of(o, dev, dt, rows, width) || wants_grad({o}) || !may_write(*o)) return nullptr;
     out = *o;
   }
-  const float scale = static_cast<float>(PyFloat_AS_DOUBLE(args[4]));
+  const float scale = static_cast<float>(PyFloat_AS_DOUBLE(pscale));
   const hipStream_t stream = stream_of(dev);
   const void *qp = q->data_ptr(), *kp = k->data_ptr(), *vp = v->data_ptr();
   void* op = out.data_ptr();
   const int code = dtype_code(dt);
   const int64_t qs = row_stride(*q), os = row_stride(out);
+  const uint8_t *ksp = pool.key_scales != nullptr ? pool.key_scales->data_ptr<uint8_t>() : nullptr;
+  const uint8_t *vsp = pool.value_scales != nullptr ? pool.value_scales->data_ptr<uint8_t>() : nullptr;
   const int rc = unlocked([&] {
+    if (pool.key_scales != nullptr)
+      return lib.paged_attention8(qp, qs, kp, pool.key_stride, vp, pool.value_stride, ksp, vsp, st.pages, st.step, op, os,
+                                  st.heads, st.kv_heads, st.head_dim, scale, code, stream);
     return lib.paged_attention(qp, qs, kp, pool.key_stride, vp, pool.value_stride, st.pages, st.step, op, os, st.heads,
                                st.kv_heads, st.head_dim, scale, code, stream);
   });
-  *took = outcome(rc, "mlora_paged_attention");
+  *took = outcome(rc, ksp != nullptr ? "mlora_paged_attention_fp8" : "mlora_paged_attention");
   if (*took != Took::kYes) return nullptr;
-  if (args[5] != Py_None) out.unsafeGetTensorImpl()->bump_version();  // written in place
+  if (pout != Py_None) out.unsafeGetTensorImpl()->bump_version();  // written in place
   return THPVariable_Wrap(std::move(out));
 }
 
-// kernels.paged.rotary_paged_write: the rotated q, new or given.
-PyObject* paged_write(PyObject* const* args, Took* took) {
-  const at::Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *v = tensor_of(args[2]), *cs = tensor_of(args[3]),
-                   *sn = tensor_of(args[4]), *kp = tensor_of(args[5]), *vp = tensor_of(args[6]), *slots = tensor_of(args[7]);
+PyObject* paged_attention(PyObject* const* args, Took* took) {
+  const at::Tensor *k = tensor_of(args[1]), *v = tensor_of(args[2]);
   Pool pool;
-  if (q == nullptr || k == nullptr || v == nullptr || cs == nullptr || sn == nullptr || !pool.read(kp, vp)) return nullptr;
+  return pool.read(k, v) ? attend(tensor_of(args[0]), k, v, pool, args[3], args[4], args[5], took) : nullptr;
+}
+
+// kernels.paged8.paged_attention_fp8.
+PyObject* paged_attention8(PyObject* const* args, Took* took) {
+  const at::Tensor *k = tensor_of(args[1]), *v = tensor_of(args[2]);
+  Pool pool;
+  return pool.read8(k, v, tensor_of(args[3]), tensor_of(args[4]), args[5])
+             ? attend(tensor_of(args[0]), k, v, pool, args[6], args[7], args[8], took) : nullptr;
+}
+
+// kernels.paged.rotary_paged_write: the rotated q, new or given.
+PyObject* write_rows(PyObject* const* args, const at::Tensor* kp, const at::Tensor* vp, const Pool& pool, const int32_t* slotd,
+                     PyObject* pout, Took* took) {
+  const at::Tensor *q = tensor_of(args[0]), *k = tensor_of(args[1]), *v = tensor_of(args[2]), *cs = tensor_of(args[3]),
+                   *sn = tensor_of(args[4]);
+  if (q == nullptr || k == nullptr || v == nullptr || cs == nullptr || sn == nullptr) return nullptr;
   const at::Device dev = kp->device();
-  const at::ScalarType dt = kp->scalar_type();
+  const at::ScalarType dt = pool.rows;
   if (!is_current(dev) || q->dim() != 2 || q->size(0) == 0 || !fits_i32(q->size(0)) || q->size(1) == 0 || q->size(1) % pool.d != 0)
     return nullptr;
   const int64_t rows = q->size(0), heads = q->size(1) / pool.d;
   if (!is_rows_of(q, dev, dt, rows, heads * pool.d) || !is_rows_of(k, dev, dt, rows, pool.kv_heads * pool.d) ||
-      !is_rows_of(v, dev, dt, rows, pool.kv_heads * pool.d) || !is_i32(slots, dev, rows) ||
+      !is_rows_of(v, dev, dt, rows, pool.kv_heads * pool.d) ||
       wants_grad({q, k, v, cs, sn, kp, vp}) || maybe_traced() || has_tangent({q, k, v, cs, sn, kp, vp}))
     return nullptr;
   if (!may_write(*kp) || !may_write(*vp)) return nullptr;
+  if (pool.key_scales != nullptr && (!may_write(*pool.key_scales) || !may_write(*pool.value_scales))) return nullptr;
   int64_t rot[2];
   const at::Tensor* tabs[2] = {cs, sn};
   for (int i = 0; i < 2; ++i) {
@@ -655,31 +692,62 @@ PyObject* paged_write(PyObject* const* args, Took* took) {
   }
   if (rot[0] != rot[1] || (cs->scalar_type() != dt && cs->scalar_type() != at::kFloat)) return nullptr;
   at::Tensor out;
-  if (args[8] == Py_None) {
+  if (pout == Py_None) {
     out = at::empty({rows, heads * pool.d}, q->options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
   } else {
-    const at::Tensor* o = tensor_of(args[8]);
+    const at::Tensor* o = tensor_of(pout);
     if (!is_rows_of(o, dev, dt, rows, heads * pool.d) || wants_grad({o}) || !may_write(*o)) return nullptr;
     out = *o;
   }
   const hipStream_t stream = stream_of(dev);
   const void *qd = q->data_ptr(), *kd = k->data_ptr(), *vd = v->data_ptr(), *cd = cs->data_ptr(), *sd = sn->data_ptr();
-  const int32_t* slotd = slots->data_ptr<int32_t>();
   void *keyd = kp->data_ptr(), *vald = vp->data_ptr(), *od = out.data_ptr();
   const int64_t qs = row_stride(*q), ks = row_stride(*k), vs = row_stride(*v), os = row_stride(out);
   const int code = dtype_code(dt), rot_code = dtype_code(cs->scalar_type());
+  uint8_t *ksp = pool.key_scales != nullptr ? pool.key_scales->data_ptr<uint8_t>() : nullptr;
+  uint8_t *vsp = pool.value_scales != nullptr ? pool.value_scales->data_ptr<uint8_t>() : nullptr;
   const int rc = unlocked([&] {
+    if (ksp != nullptr)
+      return lib.paged_write8(qd, qs, kd, ks, vd, vs, cd, sd, rot[0], rot_code, slotd, static_cast<int32_t>(rows),
+                              static_cast<int32_t>(heads), static_cast<int32_t>(pool.kv_heads), static_cast<int32_t>(pool.d),
+                              keyd, pool.key_stride, vald, pool.value_stride, ksp, vsp, static_cast<int32_t>(pool.pages),
+                              static_cast<int32_t>(pool.page), od, os, code, stream);
     return lib.paged_write(qd, qs, kd, ks, vd, vs, cd, sd, rot[0], rot_code, slotd, static_cast<int32_t>(rows),
                            static_cast<int32_t>(heads), static_cast<int32_t>(pool.kv_heads), static_cast<int32_t>(pool.d),
                            keyd, pool.key_stride, vald, pool.value_stride, static_cast<int32_t>(pool.pages),
                            static_cast<int32_t>(pool.page), od, os, code, stream);
   });
-  *took = outcome(rc, "mlora_rotary_paged_write");
+  *took = outcome(rc, ksp != nullptr ? "mlora_rotary_paged_write_fp8" : "mlora_rotary_paged_write");
   if (*took != Took::kYes) return nullptr;
   kp->unsafeGetTensorImpl()->bump_version();  // written in place
   vp->unsafeGetTensorImpl()->bump_version();
-  if (args[8] != Py_None) out.unsafeGetTensorImpl()->bump_version();
+  if (ksp != nullptr) {
+    pool.key_scales->unsafeGetTensorImpl()->bump_version();
+    pool.value_scales->unsafeGetTensorImpl()->bump_version();
+  }
+  if (pout != Py_None) out.unsafeGetTensorImpl()->bump_version();
   return THPVariable_Wrap(std::move(out));
+}
+
+PyObject* paged_write(PyObject* const* args, Took* took) {
+  const at::Tensor *q = tensor_of(args[0]), *kp = tensor_of(args[5]), *vp = tensor_of(args[6]), *slots = tensor_of(args[7]);
+  Pool pool;
+  if (q == nullptr || q->dim() != 2 || !pool.read(kp, vp) || !is_i32(slots, kp->device(), q->size(0))) return nullptr;
+  return write_rows(args, kp, vp, pool, slots->data_ptr<int32_t>(), args[8], took);
+}
+
+// kernels.paged8.rotary_paged_write_fp8: the slots are those of a step that page_tables filled.
+PyObject* paged_write8(PyObject* const* args, Took* took) {
+  const at::Tensor *q = tensor_of(args[0]), *kp = tensor_of(args[5]), *vp = tensor_of(args[6]);
+  Pool pool;
+  Step st;
+  if (q == nullptr || q->dim() != 2 || !pool.read8(kp, vp, tensor_of(args[7]), tensor_of(args[8]), args[9]) ||
+      !st.read(args[10]) || args[11] != Py_True)
+    return nullptr;
+  if (st.device != kp->device().index() || st.step->rows != q->size(0) || st.pages->page != pool.page ||
+      pool.pages < st.pages->num_pages)
+    return nullptr;
+  return write_rows(args, kp, vp, pool, st.step->slots, args[12], took);
 }
 
 // kernels.paged.verify_drafts: (accepted, tokens).
@@ -852,6 +920,16 @@ PyObject* py_verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&](Took* took) { return verify_drafts(args, took); });
 }
 
+PyObject* py_paged_attention8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!arity(n, 9)) return nullptr;
+  return guarded([&](Took* took) { return paged_attention8(args, took); });
+}
+
+PyObject* py_paged_write8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (!arity(n, 13)) return nullptr;
+  return guarded([&](Took* took) { return paged_write8(args, took); });
+}
+
 PyObject* py_int8_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!arity(n, 6)) return nullptr;
   return guarded([&](Took* took) { return int8_linear(args, took); });
@@ -861,10 +939,10 @@ PyObject* py_int8_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // the order of the struct Library.
 PyObject* py_set_library(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (!arity(n, 3)) return nullptr;
-  constexpr int kFns = 18;
+  constexpr int kFns = 20;
   void* p[kFns];
   if (!PyTuple_CheckExact(args[0]) || PyTuple_GET_SIZE(args[0]) != kFns) {
-    PyErr_SetString(PyExc_TypeError, "a tuple of the library's eighteen addresses is expected");
+    PyErr_SetString(PyExc_TypeError, "a tuple of the library's twenty addresses is expected");
     return nullptr;
   }
   for (int i = 0; i < kFns; ++i) {
@@ -892,6 +970,8 @@ PyObject* py_set_library(PyObject*, PyObject* const* args, Py_ssize_t n) {
   lib.verify = reinterpret_cast<decltype(lib.verify)>(p[15]);
   lib.int8_ws = reinterpret_cast<decltype(lib.int8_ws)>(p[16]);
   lib.int8_linear = reinterpret_cast<decltype(lib.int8_linear)>(p[17]);
+  lib.paged_write8 = reinterpret_cast<decltype(lib.paged_write8)>(p[18]);
+  lib.paged_attention8 = reinterpret_cast<decltype(lib.paged_attention8)>(p[19]);
   Py_INCREF(args[1]);
   Py_INCREF(args[2]);
   Py_XSETREF(launch_error, args[1]);
@@ -917,6 +997,11 @@ PyMethodDef methods[] = {
                  "(q, k, v, cos, sin, keys, values, slots, out or None) -> out, or None"),
     MLORA_METHOD("verify_drafts", py_verify_drafts,
                  "(target, draft or None, tokens, row_indptr, accept, last) -> (accepted, tokens), or None"),
+    MLORA_METHOD("paged_attention8", py_paged_attention8,
+                 "(q, keys, values, key_scales, value_scales, dtype code, step's native, scale, out or None) -> out, or None"),
+    MLORA_METHOD("paged_write8", py_paged_write8,
+                 "(q, k, v, cos, sin, keys, values, key_scales, value_scales, dtype code, step's native, filled, out or None)"
+                 " -> out, or None"),
     MLORA_METHOD("int8_linear", py_int8_linear, "(x, codes, scales, k, bias or None, out or None) -> new tensor, or None"),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Native form of the entry points' ordinary calls.", -1, methods,

@@ -1,5 +1,5 @@
 // The paged KV cache: argument structs and sizes shared by csrc/paged.hip,
-// csrc/paged_attn.hip, csrc/verify.hip and the C entry points (the layouts
+// csrc/paged8.hip, csrc/paged_attn.h, csrc/verify.hip and the C entry points (the layouts
 // callers see are in include/mlora_hip.h).
 #pragma once
 
@@ -96,11 +96,22 @@ struct WriteArgs {
 };
 hipError_t launch_rotary_paged_write(const WriteArgs& a, int dtype, int head_dim, bool aligned, hipStream_t stream);
 
+// 8-bit pages: the codes of a block of this many positions share an exponent,
+// kept as a byte that is kScaleBias more.
+constexpr int kScaleBlock = 16;
+constexpr int kScaleBias = 127;
+struct Write8Args {
+  WriteArgs w;       // keys and values are e4m3 codes
+  uint8_t *key_scales, *value_scales;  // [num_pages][kv_heads][page / 16]
+};
+hipError_t launch_rotary_paged_write8(const Write8Args& a, int dtype, int head_dim, bool aligned, hipStream_t stream);
+
 struct PagedAttnArgs {
   const void* q;
   int64_t q_stride;
   const void *keys, *values;
   int64_t key_stride, value_stride;
+  const uint8_t *key_scales, *value_scales;  // 8-bit pages: [num_pages][kv_heads][page / 16]
   int num_pages, page_shift;
   const int32_t* table;
   int64_t table_stride;
@@ -117,6 +128,8 @@ struct PagedAttnArgs {
   PagedShape shape;
 };
 hipError_t launch_paged_attention(const PagedAttnArgs& a, int max_new, int dtype, int head_dim, hipStream_t stream);
+// The same over 8-bit pages (of 16 positions or more).
+hipError_t launch_paged_attention8(const PagedAttnArgs& a, int max_new, int dtype, int head_dim, hipStream_t stream);
 
 struct VerifyArgs {
   const void* target;

@@ -9,6 +9,7 @@ from .lora_ops import (
     sgemm_lora_b_multi_fwd,
 )
 from .paged import PagedStep, PageState, page_tables, paged_attention, rotary_paged_write, verify_drafts
+from .paged8 import Fp8Pool, paged_attention_fp8, rotary_paged_write_fp8
 from .rmsnorm import fuse_rmsnorm, fused_add_rmsnorm, rmsnorm_fwd
 from .scatter_bank import scatter_stage
 
@@ -28,6 +29,9 @@ __all__ = [
     "rotary_paged_write",
     "paged_attention",
     "verify_drafts",
+    "Fp8Pool",
+    "rotary_paged_write_fp8",
+    "paged_attention_fp8",
     "Int8Rows",
     "quantize_rows",
     "int8_matmul",
