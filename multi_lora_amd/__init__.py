@@ -14,8 +14,8 @@ from .batch_info import (
     write_kernel_input_metadata,
 )
 from .eviction import EvictionPolicy
-from .layers import (LinearWithLoRA, QKVProjGroup, fuse_gate_up_projections, fuse_qkv_projections, lora_delta,
-                     set_lora_enabled)
+from .layers import (Int8Linear, LinearWithLoRA, QKVProjGroup, fuse_gate_up_projections, fuse_qkv_projections,
+                     lora_delta, quantize_base, set_lora_enabled)
 from .manager import MultiLoRAManager
 from .pool import LoRAMemoryPool
 from .weights import AdapterWeights
@@ -25,6 +25,7 @@ __all__ = [
     "BatchLoRAInfo",
     "EvictionPolicy",
     "HipLoRABackend",
+    "Int8Linear",
     "KernelInputMetaData",
     "LinearWithLoRA",
     "LoRABackend",
@@ -38,6 +39,7 @@ __all__ = [
     "get_lora_backend",
     "group_rows",
     "lora_delta",
+    "quantize_base",
     "segment_lens",
     "set_lora_enabled",
     "write_kernel_input_metadata",

@@ -29,7 +29,9 @@ use_cache) and returns an object with ``.logits``.
 Ragged requests share a ``PagedKV``: ``forward_paged`` (``forward`` given one)
 runs the packed rows of a ``kernels.PagedStep``, whole prompts, chunks of them,
 decoding requests and drafted tokens alike, every row over its own request's
-pages (``kernels/paged.py``; GPU, 16-bit data).
+pages (``kernels/paged.py``; GPU, 16-bit data; the cache in 16 bits, or in 8:
+``kernels/paged8.py``).  ``layers.quantize_base`` puts 8-bit weights in the
+projections' place.
 """
 
 from __future__ import annotations
@@ -45,6 +47,7 @@ import torch.nn.functional as F
 
 from .kernels.decode_attn import decode_attention, silu_mul
 from .kernels.paged import PagedStep, PageState, page_tables, paged_attention, rotary_paged_write
+from .kernels.paged8 import Fp8Pool, paged_attention_fp8, rotary_paged_write_fp8
 
 
 @dataclass
@@ -104,15 +107,22 @@ class PagedKV:
     """Per-layer pools of pages that up to ``seqs`` requests of up to
     ``max_len`` positions share, and the page tables: keys ``[num_pages,
     kv_heads, page, head_dim]``, values ``[num_pages, kv_heads, head_dim,
-    page]``.  By default there are pages for all of them at full length."""
+    page]``.  By default there are pages for all of them at full length.  With
+    ``fp8`` the pools hold 8-bit codes (``pools``: an ``Fp8Pool`` a layer, whose
+    codes ``keys`` and ``values`` are)."""
 
     def __init__(self, config: DecoderConfig, seqs: int, max_len: int, device, dtype, *, page: int = 16,
-                 num_pages: Optional[int] = None) -> None:
+                 num_pages: Optional[int] = None, fp8: bool = False) -> None:
         self.config, self.max_len, self.page = config, max_len, page
         if num_pages is None:
             num_pages = seqs * -(-max_len // page)
         g, d = config.num_key_value_heads, config.head_dim
         self.state = PageState.new(seqs, max_len, num_pages, page, device)
+        self.pools: Optional[List[Fp8Pool]] = None
+        if fp8:
+            self.pools = [Fp8Pool.new(num_pages, g, page, d, dtype, device) for _ in range(config.num_hidden_layers)]
+            self.keys, self.values = [p.keys for p in self.pools], [p.values for p in self.pools]
+            return
         self.keys: List[torch.Tensor] = [torch.zeros((num_pages, g, page, d), device=device, dtype=dtype)
                                          for _ in range(config.num_hidden_layers)]
         self.values: List[torch.Tensor] = [torch.zeros((num_pages, g, d, page), device=device, dtype=dtype)
@@ -250,6 +260,10 @@ class Attention(nn.Module):
 
     def forward_paged(self, x, rot: Rotary, kv: PagedKV, layer: int, step: PagedStep):
         """Packed rows ``x [rows, hidden]`` of a step over the paged cache."""
+        if kv.pools is not None:
+            pool = kv.pools[layer]
+            q = rotary_paged_write_fp8(self.q_proj(x), self.k_proj(x), self.v_proj(x), rot.cos, rot.sin, pool, step)
+            return self.o_proj(paged_attention_fp8(q, pool, step, self.scale))
         q = rotary_paged_write(self.q_proj(x), self.k_proj(x), self.v_proj(x), rot.cos, rot.sin, kv.keys[layer],
                                kv.values[layer], step.slots)
         return self.o_proj(paged_attention(q, kv.keys[layer], kv.values[layer], step, self.scale))

@@ -6,17 +6,24 @@ strided view (a column slice of a fused QKV output) and is never copied.
 ``QKVProjGroup`` fuses the q/k/v base GEMMs of one attention block in decode;
 when the backend offers ``apply_lora_multi`` the three LoRA deltas are also
 applied by one shrink (x read once) and one three-slice expand.
+
+``Int8Linear`` is a linear layer whose weight is held in 8-bit integers
+(``kernels.int8``); ``quantize_base`` puts it in place of a model's ``nn.Linear``
+layers, wrapped ones too.  The adapters above stay as they are: a delta is
+added to the layer's 16-bit result from its 16-bit input.  No counterpart in
+the reference.
 """
 
 from __future__ import annotations
 
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Sequence, Union
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
 from .backend.base import LoRABackend
+from .kernels.int8 import Int8Rows, int8_linear, quantize_rows
 
 # Process-wide switch: when off, wrapped layers return the base output only.
 LORA_ENABLED = True
@@ -72,6 +79,49 @@ class LinearWithLoRA(nn.Module):
         return y_flat.reshape(y_base.shape)
 
 
+class Int8Linear(nn.Module):
+    """``y = x @ weight.T + bias`` for 16-bit ``x``, with the weight in 8-bit
+    integers and a scale for each output channel, and x's rows quantised at
+    every call.  GPU only; no gradients (a model that serves)."""
+
+    def __init__(self, weight: Int8Rows, bias: Optional[torch.Tensor] = None) -> None:
+        super().__init__()
+        self.register_buffer("codes", None)
+        self.register_buffer("scales", None)
+        self.register_buffer("bias", None if bias is None else bias.detach())
+        self.weight = weight
+
+    @classmethod
+    def from_linear(cls, layer: nn.Linear) -> "Int8Linear":
+        """The layer with its weight quantised (on the GPU)."""
+        return cls(quantize_rows(layer.weight.detach()), layer.bias)
+
+    @property
+    def weight(self) -> Int8Rows:
+        return self._weight
+
+    @weight.setter
+    def weight(self, weight: Int8Rows) -> None:
+        self.out_features, self.in_features = weight.shape
+        self.codes, self.scales = weight.codes, weight.scales
+        self._weight = weight
+
+    def _apply(self, fn, recurse: bool = True):
+        scales = self.scales
+        super()._apply(fn, recurse)
+        if self.scales.dtype != scales.dtype:  # a change of the model's type is not one of the scales'
+            self.scales = scales.to(self.scales.device)
+        self._weight = Int8Rows(self.codes, self.scales, self.in_features)
+        return self
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        y = int8_linear(x.reshape(-1, self.in_features), self._weight, self.bias)
+        return y.view(*x.shape[:-1], self.out_features)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
 class QKVProjGroup:
     """One base GEMM and one multi-slice LoRA call for sibling projections
     that read the same input: q/k/v of an attention block
@@ -87,11 +137,17 @@ class QKVProjGroup:
             raise RuntimeError("QKV fusion requires bias=None")
         self.wrappers = list(wrappers)
         widths = [int(w.base_layer.weight.shape[0]) for w in wrappers]
-        self.weight = torch.cat([w.base_layer.weight.detach() for w in wrappers], dim=0)
+        quantised = {isinstance(w.base_layer, Int8Linear) for w in wrappers}
+        if len(quantised) != 1:
+            raise RuntimeError("fusion of 8-bit and 16-bit projections")
+        self.weight: Union[torch.Tensor, Int8Rows] = (
+            Int8Rows.cat([w.base_layer.weight for w in wrappers]) if quantised == {True}
+            else torch.cat([w.base_layer.weight.detach() for w in wrappers], dim=0))
         col = 0
         for w, width in zip(wrappers, widths):
             # Each layer's weight becomes a view of the fused weight: no extra memory.
-            w.base_layer.weight = nn.Parameter(self.weight[col : col + width], requires_grad=False)
+            w.base_layer.weight = (self.weight.rows(col, col + width) if quantised == {True}
+                                   else nn.Parameter(self.weight[col : col + width], requires_grad=False))
             w.qkv_slice = (col, col + width)
             w.qkv_group = self
             col += width
@@ -109,12 +165,17 @@ class QKVProjGroup:
             and len({w.A_buffer.shape[1] for w in self.wrappers}) == 1
         )
 
+    def _base(self, x: torch.Tensor) -> torch.Tensor:
+        if isinstance(self.weight, Int8Rows):
+            return int8_linear(x.reshape(-1, x.shape[-1]), self.weight).view(*x.shape[:-1], self.weight.shape[0])
+        return F.linear(x, self.weight)
+
     def forward(self, wrapper: LinearWithLoRA, x: torch.Tensor) -> torch.Tensor:
         if x.shape[-2] != 1 and not self.all_shapes:
             return wrapper.add_delta(x, wrapper.base_layer(x))
         if self._cached_x is not x:
             self._cached_x = x
-            self._cached_out = F.linear(x, self.weight)
+            self._cached_out = self._base(x)
             self._delta_done = False
             if self._multi_ready():
                 first = self.wrappers[0]
@@ -165,3 +226,25 @@ def fuse_gate_up_projections(wrappers: Dict[str, LinearWithLoRA], all_shapes: bo
     """The same for every MLP whose gate and up projections are both wrapped:
     one base GEMM and one two-slice LoRA call over their shared input."""
     return _fuse_siblings(wrappers, GATE_UP_LEAVES, all_shapes)
+
+
+def quantize_base(model: nn.Module, skip: Sequence[str] = ("lm_head",)) -> int:
+    """Replace the model's ``nn.Linear`` layers (on the GPU), those beneath
+    ``LinearWithLoRA`` too, by ``Int8Linear``; returns how many.  Layers whose
+    last name is in ``skip`` stay, and so does what is not a float16 or
+    bfloat16 layer.  Call it before projections are fused; adapters may be
+    registered and layers wrapped before or after."""
+    count = 0
+    for name, module in list(model.named_modules()):
+        if isinstance(module, LinearWithLoRA) and module.qkv_group is not None:
+            raise RuntimeError(f"{name} is part of a fused group: quantise the base before fusing projections")
+    for name, module in list(model.named_modules()):
+        leaf = [part for part in name.split(".") if part != "base_layer"][-1:]
+        if type(module) is not nn.Linear or not leaf or leaf[0] in skip:
+            continue
+        if module.weight.dtype not in (torch.float16, torch.bfloat16):
+            continue
+        parent, _, child = name.rpartition(".")
+        setattr(model.get_submodule(parent) if parent else model, child, Int8Linear.from_linear(module))
+        count += 1
+    return count

@@ -33,7 +33,7 @@ from .batch_info import (
     group_rows,
     write_kernel_input_metadata,
 )
-from .layers import LinearWithLoRA, fuse_gate_up_projections, fuse_qkv_projections
+from .layers import Int8Linear, LinearWithLoRA, fuse_gate_up_projections, fuse_qkv_projections
 from .pool import LoRAMemoryPool, LoraName
 from .weights import AdapterWeights
 
@@ -99,13 +99,13 @@ class MultiLoRAManager:
         return any(key.endswith(sfx) for sfx in self.lora_target_suffixes)
 
     def convert_to_lora_layers(self) -> None:
-        """Wrap every ``nn.Linear`` whose name some adapter targets."""
+        """Wrap every ``nn.Linear`` (or ``Int8Linear``) whose name some adapter targets."""
         keys = set()
         for w in self._weight_store.values():
             keys.update(w.modules.keys())
         keys.update(self.pool.buffers.A.keys())
         for name, module in list(self.model.named_modules()):
-            if name in keys and isinstance(module, nn.Linear) and self._target(name):
+            if name in keys and isinstance(module, (nn.Linear, Int8Linear)) and self._target(name):
                 parent_name, _, child = name.rpartition(".")
                 parent = self.model.get_submodule(parent_name) if parent_name else self.model
                 wrapper = LinearWithLoRA(module)

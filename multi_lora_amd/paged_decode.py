@@ -39,12 +39,13 @@ from .kernels.paged import PagedStep, verify_drafts
 
 
 class PagedDecode:
-    """Resident state of ``batch`` requests; the pool holds ``num_pages`` pages of ``page`` positions."""
+    """Resident state of ``batch`` requests; the pool holds ``num_pages`` pages of ``page`` positions, in 8 bits with ``fp8``."""
 
-    def __init__(self, mgr, batch: int, max_len: int, *, page: int = 16, num_pages: Optional[int] = None) -> None:
+    def __init__(self, mgr, batch: int, max_len: int, *, page: int = 16, num_pages: Optional[int] = None,
+                 fp8: bool = False) -> None:
         device, dtype = mgr.pool.device, mgr.pool.dtype
         self.batch, self.max_len, self.start = batch, max_len, 0
-        self.kv = PagedKV(mgr.model.config, batch, max_len, device, dtype, page=page, num_pages=num_pages)
+        self.kv = PagedKV(mgr.model.config, batch, max_len, device, dtype, page=page, num_pages=num_pages, fp8=fp8)
         i32 = dict(dtype=torch.int32, device=device)
         self.input_ids = torch.zeros((batch, 1), dtype=torch.long, device=device)
         self.lens = torch.zeros(batch, **i32)         # cached positions of each request
