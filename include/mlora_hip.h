@@ -532,27 +532,33 @@ int mlora_paged_attention_fp8(const void* q, int64_t q_row_stride, const void* k
 
 /* ---- products in 8-bit integers -----------------------------------------
  * A quantised row of k elements is `scale = max|x| / 127` (fp32; the maximum
- * counts as at least 2^-100) and codes rint(x / scale), ties to even, padded
- * with zeros to a multiple of 128; rows of codes are 16-byte aligned.  A row
- * with an infinity or a NaN has a NaN scale.  No counterpart in the
- * reference, whose base products are the model's own. */
+ * counts as at least 2^-100) and codes rint(x / scale), ties to even.  A row
+ * with an infinity or a NaN has a NaN scale.  Codes are kept in the order in
+ * which the matrix units take them, 16-byte aligned: blocks of 16 rows by 64
+ * columns, 1 KB each, in which columns 16 c to 16 c + 15 of row r are at byte
+ * 16 (16 c + r).  The blocks of the same columns lie side by side; `stride` bytes
+ * on (at least 1 KB a block) are those of the next 64 columns.  Columns are
+ * padded with zeros to a multiple of 128; what the last block of rows holds
+ * behind them does not matter.  No counterpart in the reference, whose base
+ * products are the model's own. */
 
-/* Rows x [rows, k] (F16, BF16 or F32) to codes and scales; k at most 2^17. */
-int mlora_quantize_rows(const void* x, int64_t x_row_stride, int32_t rows, int32_t k, int8_t* codes,
-                        int64_t codes_row_stride, float* scales, int32_t dtype, void* stream);
+/* Rows x [rows, k] (F16, BF16 or F32) to codes (of stride 1 KB times the blocks
+ * of rows) and scales; k at most 2^17. */
+int mlora_quantize_rows(const void* x, int64_t x_row_stride, int32_t rows, int32_t k, int8_t* codes, float* scales,
+                        int32_t dtype, void* stream);
 
 /* out[m, n] = a_scales[m] * b_scales[n] * sum_k a[m, k] * b[n, k] + bias[n]
  * for quantised rows a and b; the sum is exact, the rest fp32 with one
  * rounding to `dtype` (bf16 or fp16, bias too; else -2).  bias may be NULL. */
-int mlora_int8_matmul(const int8_t* a_codes, int64_t a_row_stride, const float* a_scales, int32_t m, const int8_t* b_codes,
-                      int64_t b_row_stride, const float* b_scales, int32_t n, int32_t k, const void* bias, void* out,
+int mlora_int8_matmul(const int8_t* a_codes, int64_t a_stride, const float* a_scales, int32_t m, const int8_t* b_codes,
+                      int64_t b_stride, const float* b_scales, int32_t n, int32_t k, const void* bias, void* out,
                       int64_t out_row_stride, int32_t dtype, void* stream);
 
 /* mlora_quantize_rows of x [m, k] (bf16 or fp16) into the workspace, then the
  * product; a few rows are quantised inside the product's launch and need no
- * workspace (0 bytes). */
+ * workspace (0 bytes).  out must not overlap x. */
 size_t mlora_int8_linear_workspace_bytes(int32_t m, int32_t k);
-int mlora_int8_linear(const void* x, int64_t x_row_stride, int32_t m, const int8_t* b_codes, int64_t b_row_stride,
+int mlora_int8_linear(const void* x, int64_t x_row_stride, int32_t m, const int8_t* b_codes, int64_t b_stride,
                       const float* b_scales, int32_t n, int32_t k, const void* bias, void* out, int64_t out_row_stride,
                       int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -253,7 +253,7 @@ _SIGNATURES = {
         [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, ctypes.POINTER(Pages), ctypes.POINTER(PagedStep), _vp, _i64, _i32,
          _i32, _i32, _f32, _i32, _vp],
     ),
-    "mlora_quantize_rows": (ctypes.c_int, [_vp, _i64, _i32, _i32, _vp, _i64, _vp, _i32, _vp]),
+    "mlora_quantize_rows": (ctypes.c_int, [_vp, _i64, _i32, _i32, _vp, _vp, _i32, _vp]),
     "mlora_int8_matmul": (
         ctypes.c_int,
         [_vp, _i64, _vp, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i64, _i32, _vp],

@@ -115,15 +115,16 @@ int check_step(const mlora_paged_step* s) {
 bool rows_aligned(const void* x, int64_t stride, int k) { return al16(x) && stride % 8 == 0 && k % 8 == 0; }
 
 // What the products in 8-bit integers share; the pointers are the caller's to check.
-int int8_args(int32_t m, const int8_t* codes, int64_t row_stride, const float* scales, int32_t n, int32_t k, const void* bias,
+int int8_args(int32_t m, const int8_t* codes, int64_t stride, const float* scales, int32_t n, int32_t k, const void* bias,
               void* out, int64_t out_row_stride, int32_t dtype, mlora::Int8Args* a) {
   if (dtype != MLORA_BF16 && dtype != MLORA_F16) return fail(kUnsupported, "int8 products give bf16 or fp16, got dtype %d", dtype);
   if (m < 0 || n < 0 || k < 1) return fail(kBadArg, "m %d, n %d, k %d", m, n, k);
   if (k > mlora::kInt8MaxK) return fail(kUnsupported, "rows of %d elements, at most %d", k, mlora::kInt8MaxK);
-  if (row_stride < mlora::int8_padded(k) || out_row_stride < n) return fail(kBadArg, "row strides do not hold the rows");
-  if (!al16(codes) || row_stride % 16 != 0) return fail(kUnsupported, "codes need 16-byte aligned rows");
+  if (out_row_stride < n) return fail(kBadArg, "row strides do not hold the rows");
+  if (stride < mlora::int8_bands(n) * mlora::kInt8Block) return fail(kBadArg, "strides do not hold the blocks");
+  if (!al16(codes) || stride % 16 != 0) return fail(kUnsupported, "codes need 16-byte alignment");
   a->m = m, a->n = n, a->k = k;
-  a->b = codes, a->b_stride = row_stride, a->b_scales = scales;
+  a->b = codes, a->b_step = stride, a->b_scales = scales;
   a->bias = bias;
   a->out = out, a->out_stride = out_row_stride;
   a->vec = (reinterpret_cast<uintptr_t>(out) & 7u) == 0 && out_row_stride % 4 == 0;
@@ -1027,37 +1028,37 @@ int mlora_verify_drafts(const void* target, int64_t target_row_stride, int32_t r
   return 0;
 }
 
-int mlora_quantize_rows(const void* x, int64_t x_row_stride, int32_t rows, int32_t k, int8_t* codes,
-                        int64_t codes_row_stride, float* scales, int32_t dtype, void* stream) {
+int mlora_quantize_rows(const void* x, int64_t x_row_stride, int32_t rows, int32_t k, int8_t* codes, float* scales,
+                        int32_t dtype, void* stream) {
   g_err[0] = '\0';
   if (!valid_dtype(dtype)) return fail(kBadArg, "bad dtype %d", dtype);
   if (rows < 0 || k < 1) return fail(kBadArg, "rows %d, k %d", rows, k);
   if (k > mlora::kInt8MaxK) return fail(kUnsupported, "rows of %d elements, at most %d", k, mlora::kInt8MaxK);
-  if (x_row_stride < k || codes_row_stride < mlora::int8_padded(k)) return fail(kBadArg, "row strides do not hold the rows");
+  if (x_row_stride < k) return fail(kBadArg, "row strides do not hold the rows");
   if (rows == 0) return 0;
   if (!x || !codes || !scales) return fail(kBadArg, "null pointer");
-  if (!al16(codes) || codes_row_stride % 16 != 0) return fail(kUnsupported, "codes need 16-byte aligned rows");
+  if (!al16(codes)) return fail(kUnsupported, "codes need 16-byte alignment");
   mlora::QuantArgs a{};
   a.x = x, a.x_stride = x_row_stride;
   a.rows = rows, a.k = k;
-  a.codes = codes, a.codes_stride = codes_row_stride;
+  a.codes = codes;
   a.scales = scales;
   const hipError_t e = mlora::launch_quantize_rows(a, dtype, rows_aligned(x, x_row_stride, k), static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "row quantisation launch");
   return 0;
 }
 
-int mlora_int8_matmul(const int8_t* a_codes, int64_t a_row_stride, const float* a_scales, int32_t m, const int8_t* b_codes,
-                      int64_t b_row_stride, const float* b_scales, int32_t n, int32_t k, const void* bias, void* out,
+int mlora_int8_matmul(const int8_t* a_codes, int64_t a_stride, const float* a_scales, int32_t m, const int8_t* b_codes,
+                      int64_t b_stride, const float* b_scales, int32_t n, int32_t k, const void* bias, void* out,
                       int64_t out_row_stride, int32_t dtype, void* stream) {
   g_err[0] = '\0';
   mlora::Int8Args a{};
-  if (const int rc = int8_args(m, b_codes, b_row_stride, b_scales, n, k, bias, out, out_row_stride, dtype, &a)) return rc;
-  if (a_row_stride < mlora::int8_padded(k)) return fail(kBadArg, "row strides do not hold the rows");
+  if (const int rc = int8_args(m, b_codes, b_stride, b_scales, n, k, bias, out, out_row_stride, dtype, &a)) return rc;
+  if (a_stride < mlora::int8_bands(m) * mlora::kInt8Block) return fail(kBadArg, "strides do not hold the blocks");
   if (m == 0 || n == 0) return 0;
   if (!a_codes || !a_scales || !b_codes || !b_scales || !out) return fail(kBadArg, "null pointer");
-  if (!al16(a_codes) || a_row_stride % 16 != 0) return fail(kUnsupported, "codes need 16-byte aligned rows");
-  a.a = a_codes, a.a_stride = a_row_stride, a.a_scales = a_scales;
+  if (!al16(a_codes) || a_stride % 16 != 0) return fail(kUnsupported, "codes need 16-byte alignment");
+  a.a = a_codes, a.a_step = a_stride, a.a_scales = a_scales;
   const hipError_t e = mlora::launch_int8_matmul(a, dtype, num_cus(), static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "int8 product launch");
   return 0;
@@ -1065,15 +1066,15 @@ int mlora_int8_matmul(const int8_t* a_codes, int64_t a_row_stride, const float* 
 
 size_t mlora_int8_linear_workspace_bytes(int32_t m, int32_t k) {
   if (m < 1 || k < 1 || k > mlora::kInt8MaxK || mlora::int8_fused(m, k)) return 0;
-  return static_cast<size_t>(m) * mlora::int8_padded(k) + static_cast<size_t>(m) * sizeof(float);
+  return static_cast<size_t>(mlora::int8_bytes(m, k)) + static_cast<size_t>(m) * sizeof(float);
 }
 
-int mlora_int8_linear(const void* x, int64_t x_row_stride, int32_t m, const int8_t* b_codes, int64_t b_row_stride,
+int mlora_int8_linear(const void* x, int64_t x_row_stride, int32_t m, const int8_t* b_codes, int64_t b_stride,
                       const float* b_scales, int32_t n, int32_t k, const void* bias, void* out, int64_t out_row_stride,
                       int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
   g_err[0] = '\0';
   mlora::Int8Args a{};
-  if (const int rc = int8_args(m, b_codes, b_row_stride, b_scales, n, k, bias, out, out_row_stride, dtype, &a)) return rc;
+  if (const int rc = int8_args(m, b_codes, b_stride, b_scales, n, k, bias, out, out_row_stride, dtype, &a)) return rc;
   if (x_row_stride < k) return fail(kBadArg, "row strides do not hold the rows");
   if (m == 0 || n == 0) return 0;
   if (!x || !b_codes || !b_scales || !out) return fail(kBadArg, "null pointer");
@@ -1081,21 +1082,20 @@ int mlora_int8_linear(const void* x, int64_t x_row_stride, int32_t m, const int8
   hipError_t e;
   if (mlora::int8_fused(m, k)) {
     a.x = x, a.x_stride = x_row_stride, a.x_aligned = aligned;
-    e = mlora::launch_int8_matmul(a, dtype, num_cus(), static_cast<hipStream_t>(stream));
-    if (e != hipSuccess) return hip_fail(e, "int8 product launch");
-    return 0;
+  } else {
+    const size_t need = mlora_int8_linear_workspace_bytes(m, k);
+    if (workspace == nullptr || workspace_bytes < need)
+      return fail(kWorkspace, "workspace of %zu bytes, needs %zu", workspace_bytes, need);
+    if (!al16(workspace)) return fail(kUnsupported, "the workspace needs 16-byte alignment");
+    mlora::QuantArgs q{};
+    q.x = x, q.x_stride = x_row_stride;
+    q.rows = m, q.k = k;
+    q.codes = static_cast<int8_t*>(workspace);
+    q.scales = reinterpret_cast<float*>(q.codes + mlora::int8_bytes(m, k));
+    e = mlora::launch_quantize_rows(q, dtype, aligned, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "row quantisation launch");
+    a.a = q.codes, a.a_step = mlora::int8_bands(m) * mlora::kInt8Block, a.a_scales = q.scales;
   }
-  const size_t need = mlora_int8_linear_workspace_bytes(m, k);
-  if (workspace == nullptr || workspace_bytes < need) return fail(kWorkspace, "workspace of %zu bytes, needs %zu", workspace_bytes, need);
-  if (!al16(workspace)) return fail(kUnsupported, "the workspace needs 16-byte alignment");
-  mlora::QuantArgs q{};
-  q.x = x, q.x_stride = x_row_stride;
-  q.rows = m, q.k = k;
-  q.codes = static_cast<int8_t*>(workspace), q.codes_stride = mlora::int8_padded(k);
-  q.scales = reinterpret_cast<float*>(q.codes + static_cast<size_t>(m) * q.codes_stride);
-  e = mlora::launch_quantize_rows(q, dtype, aligned, static_cast<hipStream_t>(stream));
-  if (e != hipSuccess) return hip_fail(e, "row quantisation launch");
-  a.a = q.codes, a.a_stride = q.codes_stride, a.a_scales = q.scales;
   e = mlora::launch_int8_matmul(a, dtype, num_cus(), static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "int8 product launch");
   return 0;

@@ -807,10 +807,10 @@ PyObject* int8_linear(PyObject* const* args, Took* took) {
       !is_rows_of(x, dev, dt, x->size(0), k) || wants_grad({x}) || maybe_traced() || has_tangent({x}))
     return nullptr;
   // Int8Rows has checked what its tensors look like.
-  if (codes->dim() != 2 || codes->device() != dev || codes->scalar_type() != at::kChar || !fits_i32(codes->size(0)) ||
-      scales->device() != dev || scales->scalar_type() != at::kFloat)
+  if (codes->dim() != 5 || codes->device() != dev || codes->scalar_type() != at::kChar || scales->dim() != 1 ||
+      !fits_i32(scales->size(0)) || scales->device() != dev || scales->scalar_type() != at::kFloat)
     return nullptr;
-  const int64_t m = x->size(0), n = codes->size(0);
+  const int64_t m = x->size(0), n = scales->size(0);
   if (n == 0) return nullptr;
   if (bias != nullptr && (bias->device() != dev || bias->scalar_type() != dt || bias->dim() != 1 || bias->size(0) != n ||
                           !bias->is_contiguous() || wants_grad({bias}) || has_tangent({bias})))
@@ -824,11 +824,11 @@ PyObject* int8_linear(PyObject* const* args, Took* took) {
   const int8_t* cp = static_cast<const int8_t*>(codes->data_ptr());
   const float* sp = scales->data_ptr<float>();
   void *op = out.data_ptr(), *wp = need > 0 ? ws.data_ptr() : nullptr;
-  const int64_t xs = row_stride(*x), cs = row_stride(*codes);
+  const int64_t xs = row_stride(*x), cs = codes->stride(0);
   const int code = dtype_code(dt);
   const int rc = unlocked([&] {
-    return lib.int8_linear(xp, xs, static_cast<int32_t>(m), cp, cs, sp, static_cast<int32_t>(n), static_cast<int32_t>(k), bp,
-                           op, n, code, wp, need, stream);
+    return lib.int8_linear(xp, xs, static_cast<int32_t>(m), cp, cs, sp, static_cast<int32_t>(n), static_cast<int32_t>(k), bp, op,
+                           n, code, wp, need, stream);
   });
   *took = outcome(rc, "mlora_int8_linear");
   if (*took != Took::kYes) return nullptr;

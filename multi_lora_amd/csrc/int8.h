@@ -6,9 +6,18 @@
 
 namespace mlora {
 
-// Codes of a row are padded with zeros to a multiple of this many.
+// Codes lie in blocks of 16 rows (a band) by 64 columns, 1 KB each: the 16 bytes
+// at 16 (16 c + r) of a block are columns 16 c to 16 c + 15 of row r.  That is how
+// lane 16 c + r of a wave holds an operand of the matrix units.  Blocks of the
+// same columns lie side by side, band after band: what a tile, or all tiles at
+// work at one time, read is one run of memory.
+// Columns are padded with zeros to a multiple of 128, rows to one of 16.
 constexpr int kInt8Pad = 128;
-constexpr int64_t int8_padded(int64_t k) { return (k + kInt8Pad - 1) / kInt8Pad * kInt8Pad; }
+constexpr int kInt8Block = 1024;
+__host__ __device__ constexpr int64_t int8_padded(int64_t k) { return (k + kInt8Pad - 1) / kInt8Pad * kInt8Pad; }
+__host__ __device__ constexpr int64_t int8_bands(int64_t rows) { return (rows + 15) / 16; }
+constexpr int64_t int8_bytes(int64_t rows, int64_t k) { return int8_bands(rows) * 16 * int8_padded(k); }
+
 // 127^2 * 2^17 < 2^31: sums of this many products fit 32 bits.
 constexpr int kInt8MaxK = 1 << 17;
 
@@ -16,8 +25,7 @@ struct QuantArgs {
   const void* x;
   int64_t x_stride;
   int rows, k;
-  int8_t* codes;
-  int64_t codes_stride;
+  int8_t* codes;      // of these rows alone
   float* scales;
 };
 hipError_t launch_quantize_rows(const QuantArgs& a, int dtype, bool aligned, hipStream_t stream);
@@ -26,7 +34,7 @@ struct Int8Args {
   // Activations: codes and scales, or (of calls with few of them) the 16-bit
   // rows themselves.
   const int8_t* a;
-  int64_t a_stride;
+  int64_t a_step;     // bytes from a block to that of the next columns
   const float* a_scales;
   const void* x;
   int64_t x_stride;
@@ -34,7 +42,7 @@ struct Int8Args {
   int m;
   // Weight.
   const int8_t* b;
-  int64_t b_stride;
+  int64_t b_step;
   const float* b_scales;
   int n;
   int k;              // of x; the codes have int8_padded(k)

@@ -7,17 +7,13 @@
 #include <algorithm>
 
 #include "int8.h"
+#include "int8_tile.h"
 #include "kernels.h"
 #include "loads.h"
 
 namespace mlora {
 
 namespace {
-
-typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
-typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
-typedef const __attribute__((address_space(1))) void gvoid_t;
-typedef __attribute__((address_space(3))) void lvoid_t;
 
 constexpr float kLeast = 7.888609052210118e-31f;  // 2^-100: a row's least maximum, so that neither scale leaves fp32
 constexpr uint32_t kInfBits = 0x7f800000u;
@@ -74,6 +70,8 @@ __device__ __forceinline__ void load8(const typename T::raw_t* row, int e, int k
   }
 }
 
+constexpr int kFusedStep = 8 * 64 * 8;  // elements of one chunk a thread of the register form's workgroup
+
 constexpr int kQuantKeep = 4;  // chunks of eight elements a thread keeps; longer rows are read twice
 
 // TPR threads a row, eight elements at a time.  Bound by bytes: 2 in and 1 out
@@ -88,6 +86,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
   const int row = blockIdx.x * RPB + sub;
   const raw* x = static_cast<const raw*>(a.x) + static_cast<int64_t>(min(row, a.rows - 1)) * a.x_stride;
   const int padded = static_cast<int>(int8_padded(a.k));
+  const int64_t step = int8_bands(a.rows) * kInt8Block;
   float keep[kQuantKeep][8];
   uint32_t top = 0;
 #pragma unroll
@@ -115,13 +114,13 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
   if (row >= a.rows) return;
   const RowScale s = row_scale(top);
   if (t == 0) a.scales[row] = s.scale;
-  int8_t* out = a.codes + row * a.codes_stride;
+  int8_t* out = a.codes + static_cast<int64_t>(row >> 4) * kInt8Block + (row & 15) * 16;
   auto put = [&](int e, const float* f) {
     if (e >= padded) return;
     int q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = code_of(f[i], s);
-    *reinterpret_cast<uint2*>(out + e) = make_uint2(pack4(q), pack4(q + 4));
+    *reinterpret_cast<uint2*>(out + (e >> 6) * step + (e >> 4 & 3) * 256 + (e & 8)) = make_uint2(pack4(q), pack4(q + 4));
   };
 #pragma unroll
   for (int c = 0; c < kQuantKeep; ++c) put((c * TPR + t) * 8, keep[c]);
@@ -131,6 +130,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
     put(e, f);
   }
 }
+
 
 // Four columns of a row of the result, n to n + 3.
 template <class T>
@@ -154,54 +154,55 @@ __device__ __forceinline__ void store4(const Int8Args& a, int m, int n, const i3
 }
 
 // Few rows: a workgroup has 16 NT output columns of up to 16 MT rows; its
-// waves take the 128-byte pieces of the weight's rows in turn, straight from
-// memory into operands (lane l: row l & 15, the 16 bytes 16 (l >> 4) on and
-// those 64 further), and add their sums in LDS.
-template <class T, int MT, int NT, int NW, int U, bool FUSE>
+// waves take the blocks of the bands in turn, straight from memory into
+// operands, and add their sums in LDS: no barrier while weights stream.
+// KEEP: the rows themselves (of at most KEEP chunks of eight elements a thread)
+// are read and quantised by every workgroup, while its first blocks are on
+// their way.
+template <class T, int MT, int NT, int NW, int U, int KEEP>
 __global__ __launch_bounds__(NW * 64) void int8_rows_kernel(Int8Args a) {
   using raw = typename T::raw_t;
+  constexpr bool FUSE = KEEP > 0;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 15;
-  const int g = lane >> 4;
   const int n0 = blockIdx.x * 16 * NT;
   const int m0 = blockIdx.y * 16 * MT;
   const int padded = static_cast<int>(int8_padded(a.k));
-  const int pieces = padded / 128;
+  const int pieces = padded / 64;
 
   const int8_t* wp[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) wp[t] = a.b + static_cast<int64_t>(min(n0 + t * 16 + col, a.n - 1)) * a.b_stride + g * 16;
   const int8_t* xp[MT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    wp[t] = a.b + static_cast<int64_t>(min(n0 / 16 + t, (a.n - 1) / 16)) * kInt8Block + lane * 16;
   if constexpr (!FUSE) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) xp[t] = a.a + static_cast<int64_t>(min(m0 + t * 16 + col, a.m - 1)) * a.a_stride + g * 16;
+    for (int t = 0; t < MT; ++t)
+      xp[t] = a.a + static_cast<int64_t>(min(m0 / 16 + t, (a.m - 1) / 16)) * kInt8Block + lane * 16;
   }
-  u32x4 wf[U][NT][2], xf[U][MT][2];
+  u32x4 wf[U][NT], xf[U][MT];
   auto load = [&](int u, int piece) {
-    const int p = min(piece, pieces - 1) * 128;
+    const int64_t p = min(piece, pieces - 1);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) wf[u][t][0] = ld_chunk(wp[t] + p), wf[u][t][1] = ld_chunk(wp[t] + p + 64);
+    for (int t = 0; t < NT; ++t) wf[u][t] = ld_chunk(wp[t] + p * a.b_step);
     if constexpr (!FUSE) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t) xf[u][t][0] = ld_chunk(xp[t] + p), xf[u][t][1] = ld_chunk(xp[t] + p + 64);
+      for (int t = 0; t < MT; ++t) xf[u][t] = ld_chunk(xp[t] + p * a.a_step);
     }
   };
 #pragma unroll
   for (int u = 0; u < U; ++u) load(u, wave + u * NW);
 
-  // The workgroup's rows as codes in LDS, rows 64 bytes further apart than
-  // they are long: the rows of a fragment then lie in different banks.
-  const int pitch = padded + 64;
+  // The workgroup's rows as codes in LDS, in the order of blocks of m rows: the
+  // 16 bytes at 16 (m c + r) are those of row r and columns 16 c on.
   uint32_t* tops = reinterpret_cast<uint32_t*>(lds);
   int8_t* codes = reinterpret_cast<int8_t*>(lds) + 64;
   if constexpr (FUSE) {
-    static_assert(MT == 1, "one tile of rows");
+    static_assert(MT == 1, "one band of rows");
     if (threadIdx.x < 16) tops[threadIdx.x] = 0;
     lds_barrier();
     const int chunks = padded / 8;
-    constexpr int KEEP = 8;  // chunks of a thread: int8_fused
     float keep[KEEP][8];
 #pragma unroll
     for (int c = 0; c < KEEP; ++c) {
@@ -211,10 +212,18 @@ __global__ __launch_bounds__(NW * 64) void int8_rows_kernel(Int8Args a) {
       const raw* x = static_cast<const raw*>(a.x) + r * a.x_stride;
       if (a.x_aligned) load8<T, true>(x, (i - r * chunks) * 8, a.k, keep[c]);
       else load8<T, false>(x, (i - r * chunks) * 8, a.k, keep[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < KEEP; ++c) {
+      const int i = c * NW * 64 + threadIdx.x;
+      const int r = i / chunks;
       uint32_t top = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, abs_bits(keep[c][e]));
-      atomicMax(&tops[r], top);
+      for (int e = 0; e < 8; ++e) top = max(top, r < a.m ? abs_bits(keep[c][e]) : 0u);
+      // A row has at least 16 chunks: groups of 16 lanes have one row each.
+#pragma unroll
+      for (int off = 1; off < 16; off <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, kWave)));
+      if ((lane & 15) == 0 && r < a.m) atomicMax(&tops[r], top);
     }
     lds_barrier();
 #pragma unroll
@@ -222,41 +231,43 @@ __global__ __launch_bounds__(NW * 64) void int8_rows_kernel(Int8Args a) {
       const int i = c * NW * 64 + threadIdx.x;
       const int r = i / chunks;
       if (r >= a.m) continue;
+      const int e = i - r * chunks;
       const RowScale s = row_scale(tops[r]);
       int q[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = code_of(keep[c][e], s);
-      *reinterpret_cast<uint2*>(codes + r * pitch + (i - r * chunks) * 8) = make_uint2(pack4(q), pack4(q + 4));
+      for (int j = 0; j < 8; ++j) q[j] = code_of(keep[c][j], s);
+      *reinterpret_cast<uint2*>(codes + ((e >> 1) * a.m + r) * 16 + (e & 1) * 8) = make_uint2(pack4(q), pack4(q + 4));
     }
     lds_barrier();
   }
-  const int8_t* xl = codes + min(col, a.m - 1) * pitch + g * 16;
+  const int8_t* xl = codes + ((lane >> 4) * a.m + min(lane & 15, a.m - 1)) * 16;
 
   i32x4 acc[NT][MT];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[n][m] = i32x4{0, 0, 0, 0};
-  for (int p0 = wave; p0 < pieces; p0 += U * NW) {
+  auto multiply = [&](int u, int p) {
+    if constexpr (FUSE) xf[u][0] = *reinterpret_cast<const u32x4*>(xl + p * 64 * a.m);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        acc[n][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wf[u][n]), __builtin_bit_cast(i32x4, xf[u][m]),
+                                                          acc[n][m], 0, 0, 0);
+  };
+  int p = wave;
+  for (; p + U * NW < pieces; p += U * NW)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int p = p0 + u * NW;
-      if (p < pieces) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if constexpr (FUSE) xf[u][0][h] = *reinterpret_cast<const u32x4*>(xl + p * 128 + h * 64);
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-              acc[n][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, wf[u][n][h]),
-                                                                __builtin_bit_cast(i32x4, xf[u][m][h]), acc[n][m], 0, 0, 0);
-        }
-      }
-      load(u, p + U * NW);
+      multiply(u, p + u * NW);
+      load(u, p + (u + U) * NW);
     }
-  }
-  // Lane l has rows l & 15 of the tile's m and 4 (l >> 4) on of its n.
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (p + u * NW < pieces) multiply(u, p + u * NW);
+  // Lane l has row l & 15 of a band's m and 4 (l >> 4) to + 3 of its n.
+  const int col = lane & 15;
   const uint32_t mine = FUSE ? tops[min(col, a.m - 1)] : 0;
   lds_barrier();  // the codes have been read
   i32x4* part = reinterpret_cast<i32x4*>(lds);
@@ -271,127 +282,65 @@ __global__ __launch_bounds__(NW * 64) void int8_rows_kernel(Int8Args a) {
 #pragma unroll
     for (int w = 1; w < NW; ++w) sum += part[w * S + i];
     const int t = i >> 6;
-    const int n = n0 + (t / MT) * 16 + g * 4;
+    const int n = n0 + (t / MT) * 16 + (lane >> 4) * 4;
     const int m = m0 + (t % MT) * 16 + col;
     if (m < a.m && n < a.n) store4<T>(a, m, n, sum, FUSE ? row_scale(mine).scale : a.a_scales[m]);
   }
 }
 
-constexpr int kRowsWaves = 8;
-constexpr int kFusedElems = kRowsWaves * 64 * 8 * 8;  // that many elements a workgroup keeps in registers
-
-// Many rows: tiles of TN weight rows by TM rows over K, 128 bytes of each at a
-// time in LDS, loaded straight there one step ahead.  Chunk c (16 bytes) of row
-// r lies at c ^ (r & 7): a fragment's eight neighbouring rows then lie in
-// different banks.
-template <class T, int TN, int TM, int WN, int WM>
-__global__ __launch_bounds__(WN * WM * 64) void int8_tile_kernel(Int8Args a, int tiles_n, int tiles_m) {
-  constexpr int NW = WN * WM;
-  constexpr int FN = TN / WN / 32, FM = TM / WM / 32;  // 32x32 blocks of a wave
-  constexpr int BLOCKS = (TN + TM) / 8;                // 1 KB blocks (8 rows) of a step
-  constexpr int LOADS = BLOCKS / NW;
-  static_assert(BLOCKS % NW == 0, "whole blocks a wave");
-  constexpr int STAGE = (TN + TM) * 128;
-  __shared__ __align__(16) char lds[2 * STAGE];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int steps = static_cast<int>(int8_padded(a.k)) / 128;
-  const int tile_n = blockIdx.x % tiles_n, tile_m = blockIdx.x / tiles_n;
-  const int n0 = tile_n * TN, m0 = tile_m * TM;
-
-  // Block b of a step: rows 8 b to 8 b + 7 of the weight's tile, then of the other.
-  const int8_t* from[LOADS];
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    const int r = (wave * LOADS + i) * 8 + (lane >> 3);
-    const int chunk = (lane & 7) ^ (r & 7);
-    from[i] = (r < TN ? a.b + static_cast<int64_t>(min(n0 + r, a.n - 1)) * a.b_stride
-                      : a.a + static_cast<int64_t>(min(m0 + r - TN, a.m - 1)) * a.a_stride) + chunk * 16;
-  }
-  auto load = [&](int step, int buf) {
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i)
-      __builtin_amdgcn_global_load_lds((gvoid_t*)(from[i] + static_cast<int64_t>(step) * 128),
-                                       (lvoid_t*)(lds + buf * STAGE + (wave * LOADS + i) * 1024), 16, 0, 0);
-  };
-  const int wn = wave % WN, wm = wave / WN;
-  const int row = lane & 31, h = lane >> 5;
-  const char* nb = lds + (wn * (TN / WN) + row) * 128;
-  const char* mb = lds + (TN + wm * (TM / WM) + row) * 128;
-  i32x16 acc[FN][FM];
-#pragma unroll
-  for (int i = 0; i < FN; ++i)
-#pragma unroll
-    for (int j = 0; j < FM; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
-  load(0, 0);
-  int buf = 0;
-  for (int s = 0; s < steps; ++s, buf ^= 1) {
-    wait_vmcnt<0>();
-    lds_barrier();  // the step has landed, and nobody reads the other buffer
-    if (s + 1 < steps) load(s + 1, buf ^ 1);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int c = ((k * 2 + h) ^ (row & 7)) * 16 + buf * STAGE;
-      i32x4 nf[FN], mf[FM];
-#pragma unroll
-      for (int i = 0; i < FN; ++i) nf[i] = *reinterpret_cast<const i32x4*>(nb + c + i * 32 * 128);
-#pragma unroll
-      for (int j = 0; j < FM; ++j) mf[j] = *reinterpret_cast<const i32x4*>(mb + c + j * 32 * 128);
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(nf[i], mf[j], acc[i][j], 0, 0, 0);
-    }
-  }
-  // Lane l has row l & 31 of a block's m; register r its n 8 (r >> 2) + 4 (l >> 5) + (r & 3).
-#pragma unroll
-  for (int j = 0; j < FM; ++j) {
-    const int m = m0 + wm * (TM / WM) + j * 32 + row;
-    if (m >= a.m) continue;
-    const float as = a.a_scales[m];
-#pragma unroll
-    for (int i = 0; i < FN; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = n0 + wn * (TN / WN) + i * 32 + q * 8 + h * 4;
-        if (n < a.n) store4<T>(a, m, n, i32x4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]}, as);
-      }
-  }
-}
-
-template <class T, int MT, int NT, int U, bool FUSE>
+template <class T, int MT, int NT, int NW, int U, int KEEP>
 hipError_t launch_rows(const Int8Args& a, hipStream_t stream) {
-  constexpr int NW = kRowsWaves;
-  const int codes = FUSE ? 64 + a.m * (static_cast<int>(int8_padded(a.k)) + 64) : 0;
+  const int codes = KEEP > 0 ? 64 + a.m * static_cast<int>(int8_padded(a.k)) : 0;
   const int bytes = std::max(codes, NW * NT * MT * 64 * 16);  // at most 64 KB
-  const auto kernel = int8_rows_kernel<T, MT, NT, NW, U, FUSE>;
+  const auto kernel = int8_rows_kernel<T, MT, NT, NW, U, KEEP>;
   const dim3 grid(cdiv(a.n, 16 * NT), cdiv(a.m, 16 * MT));
   if (!grid_fits(2 * static_cast<int64_t>(grid.x))) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL(kernel, grid, dim3(NW * 64), bytes, stream, a);
   return hipGetLastError();
 }
 
-template <class T, int TN, int TM, int WN, int WM>
-hipError_t launch_tile(const Int8Args& a, hipStream_t stream) {
-  const int64_t tn = (static_cast<int64_t>(a.n) + TN - 1) / TN, tm = (static_cast<int64_t>(a.m) + TM - 1) / TM;
-  if (!grid_fits(tn * tm * (WN * WM / 4))) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL((int8_tile_kernel<T, TN, TM, WN, WM>), dim3(static_cast<unsigned>(tn * tm)), dim3(WN * WM * 64), 0, stream, a,
-                     static_cast<int>(tn), static_cast<int>(tm));
-  return hipGetLastError();
-}
+// Rows of a workgroup of the register form, and its columns, in bands: as many
+// products as give the chip kFew workgroups, since every band is read anew by
+// each workgroup that uses it.  Times in us (K 4096; in a graph, weights cold):
+// 64 rows to 4096 columns 5.8 with 2 x 2 bands (256 workgroups), 7.1 with 2 x 4,
+// 7.2 with 2 x 1; 128 rows 7.1 with 2 x 4, 8.0 with 2 x 2; 256 rows 10.3 with
+// 4 x 4, 10.9 with 2 x 4; 16 rows to 28672 22.4 with 1 x 4, 24.3 with 1 x 1.
+constexpr int kFew = 192;
+// The register form's loads grow with the rows, and tiles from LDS take over
+// where there are more workgroups of 4 x 4 bands than this: 512 rows to 4096
+// columns (512 of them) 16.2 against 18.6, and with K 14336 52 against 76; to
+// 6144 (768) 24.9 against 22.1; 128 rows to 28672 (896) 44.3 against 34.3.
+constexpr int kRegisterTiles = 512;
 
 template <class T>
 hipError_t launch(const Int8Args& a, int cus, hipStream_t stream) {
-  if (a.a == nullptr) return launch_rows<T, 1, 1, 4, true>(a, stream);
-  if (a.m <= 16) return launch_rows<T, 1, 1, 4, false>(a, stream);
-  if (a.m <= 32) return launch_rows<T, 2, 2, 4, false>(a, stream);
-  if (a.m <= 64) return launch_rows<T, 4, 2, 4, false>(a, stream);
   auto tiles = [&](int tn, int tm) { return static_cast<int64_t>(cdiv(a.n, tn)) * cdiv(a.m, tm); };
-  if (tiles(256, 256) >= cus) return launch_tile<T, 256, 256, 2, 4>(a, stream);
-  if (tiles(128, 128) >= cus) return launch_tile<T, 128, 128, 2, 2>(a, stream);
-  return launch_tile<T, 64, 64, 2, 2>(a, stream);
+  if (a.a == nullptr) {
+    // One or two chunks a thread; one band of columns, or four where they fill the chip all the same.
+    const bool wide = tiles(64, 16) >= kFew, one = int8_padded(a.k) * a.m <= kFusedStep;
+    if (wide) return one ? launch_rows<T, 1, 4, 8, 2, 1>(a, stream) : launch_rows<T, 1, 4, 8, 2, 2>(a, stream);
+    return one ? launch_rows<T, 1, 1, 8, 2, 1>(a, stream) : launch_rows<T, 1, 1, 8, 4, 2>(a, stream);
+  }
+  if (tiles(64, 64) <= kRegisterTiles) {
+    if (a.m > 32 && tiles(64, 64) >= kFew) return launch_rows<T, 4, 4, 4, 2, 0>(a, stream);
+    if (a.m > 16 && tiles(64, 32) >= kFew) return launch_rows<T, 2, 4, 8, 2, 0>(a, stream);
+    if (a.m <= 16 && tiles(64, 16) >= kFew) return launch_rows<T, 1, 4, 8, 2, 0>(a, stream);
+    if (a.m > 16 && tiles(32, 32) >= kFew) return launch_rows<T, 2, 2, 8, 2, 0>(a, stream);
+    if (tiles(32, 16) >= kFew) return launch_rows<T, 1, 2, 8, 4, 0>(a, stream);
+    return launch_rows<T, 1, 1, 8, 2, 0>(a, stream);
+  }
+  // Tiles: the shape whose rounds over the chip take least, by what a step of a
+  // round takes (in hundredths of a us, over all of the CUs; two workgroups of
+  // 128 x 128 share a CU).  4075 rows to 6144 columns 98 us with 192 x 256 (2
+  // rounds), 104 with 128 x 128 (6), 110 with 256 x 256 (1.5, so 2); 512 to 28672
+  // 63 with 256 x 256 (1), 80 with 128 x 128 (3.5); 2048 to 4096 37 with 128 x 128
+  // (2), 45 with 192 x 256 (1), 54 with 256 x 256 (1).
+  auto rounds = [&](int tn, int tm) { return (tiles(tn, tm) + cus - 1) / cus; };
+  const int64_t small = rounds(128, 128) == 1 ? 80 : 60 * rounds(128, 128);
+  const int64_t middle = 154 * rounds(192, 256), large = 187 * rounds(256, 256);
+  if (small <= middle && small <= large) return launch_tile<T, TileShape<128, 128, 4, 2, 2>>(a, stream);
+  if (middle <= large) return launch_tile<T, TileShape<192, 256, 2, 4, 2>>(a, stream);
+  return launch_tile<T, TileShape<256, 256, 2, 4, 2>>(a, stream);
 }
 
 template <class T, int TPR>
@@ -411,7 +360,10 @@ hipError_t quant_of(const QuantArgs& a, bool aligned, hipStream_t stream) {
 
 }  // namespace
 
-bool int8_fused(int m, int k) { return m <= 8 && m * int8_padded(k) <= kFusedElems; }
+// Quantising inside the product's launch saves the other one's 3.3 us and costs
+// every workgroup the rows: one row of 4096 5.8 to 6.0 us against 8.0, two 7.0
+// against 8.1, but four 8.9 against 8.1, and one of 14336 16.3 against 16.0.
+bool int8_fused(int m, int k) { return m <= 8 && m * int8_padded(k) <= 2 * kFusedStep; }
 
 hipError_t launch_quantize_rows(const QuantArgs& a, int dtype, bool aligned, hipStream_t stream) {
   if (a.rows == 0) return hipSuccess;

@@ -28,18 +28,25 @@ from .. import _ffi
 from .paged import _DTYPES, _guard, _no_grad, _no_tangent, _on_gpu, _untraced, _writes
 
 PAD = 128        # columns of codes come in multiples of it
+BAND = 16        # rows, too
 MAX_K = 1 << 17  # longer sums of products could leave 32 bits
 
 
-def _padded(k: int) -> int:
-    return -(-k // PAD) * PAD
+def _code_shape(rows: int, k: int):
+    return (-(-k // PAD) * (PAD // 64), -(-rows // BAND), 4, BAND, 16)
 
 
 @dataclass(frozen=True)
 class Int8Rows:
-    """Quantised rows ``[rows, k]``: ``codes [rows, k rounded up to 128]`` (zeros
-    behind column ``k``) and ``scales [rows]``.  Row ``r`` stands for
-    ``codes[r, :k] * scales[r]``."""
+    """Quantised rows ``[rows, k]``: 8-bit ``codes`` and ``scales [rows]``.  Row
+    ``r`` stands for ``to_rows()[r] * scales[r]``.
+
+    Codes lie in the order in which the matrix units take them, ``[k / 64,
+    rows / 16, 4, 16, 16]`` (rounded up; ``k`` to a multiple of 128, zeros behind
+    it): ``codes[e // 64, r // 16, e // 16 % 4, r % 16, e % 16]`` is column ``e``
+    of row ``r``, and what the last rows' blocks hold behind them does not
+    matter.  A slice of the second dimension is one, too.
+    """
 
     codes: torch.Tensor   # int8
     scales: torch.Tensor  # float32
@@ -49,19 +56,20 @@ class Int8Rows:
         c, s = self.codes, self.scales
         if not 1 <= self.k <= MAX_K:
             raise ValueError(f"rows of 1 to {MAX_K} elements, got {self.k}")
-        if c.dtype != torch.int8 or c.dim() != 2 or c.shape[1] != _padded(self.k) or (c.numel() > 0 and c.stride(1) != 1):
-            raise ValueError(f"codes must be int8 [rows, {_padded(self.k)}] with contiguous rows, got {tuple(c.shape)} {c.dtype}")
-        if c.shape[0] > 1 and (c.stride(0) % 16 or c.stride(0) < c.shape[1]) or c.data_ptr() % 16:
-            raise ValueError("codes need rows at multiples of 16 bytes")
-        if s.dtype != torch.float32 or tuple(s.shape) != (c.shape[0],) or not s.is_contiguous():
-            raise ValueError(f"scales must be a contiguous float32 tensor of {c.shape[0]} numbers, got {tuple(s.shape)} {s.dtype}")
+        if s.dtype != torch.float32 or s.dim() != 1 or not s.is_contiguous():
+            raise ValueError(f"scales must be a contiguous float32 tensor of a number a row, got {tuple(s.shape)} {s.dtype}")
+        shape = _code_shape(s.shape[0], self.k)
+        if (c.dtype != torch.int8 or tuple(c.shape) != shape or not c[0].is_contiguous() or c.data_ptr() % 16 or c.stride(0) % 16
+                or c.stride(0) < shape[1] * 1024):
+            raise ValueError(f"codes must be int8 of shape {shape} with contiguous blocks at multiples of 16 bytes, got "
+                             f"{tuple(c.shape)} {c.dtype}")
         if s.device != c.device:
             raise ValueError(f"codes on {c.device}, scales on {s.device}")
 
     @property
     def shape(self):
         """``(rows, k)``."""
-        return torch.Size((self.codes.shape[0], self.k))
+        return torch.Size((self.scales.shape[0], self.k))
 
     @property
     def device(self) -> torch.device:
@@ -69,30 +77,44 @@ class Int8Rows:
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Int8Rows":
-        """Rows quantised elsewhere: ``codes [rows, k]`` int8 and ``scales [rows]``; copied into the padded layout."""
+        """Rows quantised elsewhere: ``codes [rows, k]`` int8 and ``scales [rows]``; copied into the layout here."""
         if codes.dtype != torch.int8 or codes.dim() != 2:
             raise ValueError(f"codes must be int8 [rows, k], got {tuple(codes.shape)} {codes.dtype}")
         rows, k = codes.shape
         if not 1 <= k <= MAX_K:
             raise ValueError(f"rows of 1 to {MAX_K} elements, got {k}")
-        padded = torch.zeros((rows, _padded(k)), dtype=torch.int8, device=codes.device)
-        padded[:, :k] = codes
+        blocks, bands = _code_shape(rows, k)[:2]
+        padded = torch.zeros((bands * BAND, blocks * 64), dtype=torch.int8, device=codes.device)
+        padded[:rows, :k] = codes
+        padded = padded.view(bands, BAND, blocks, 4, 16).permute(2, 0, 3, 1, 4).contiguous()
         return cls(padded, scales.to(torch.float32).contiguous(), k)
 
+    def to_rows(self) -> torch.Tensor:
+        """The codes as a matrix, int8 ``[rows, k]``."""
+        blocks, bands = self.codes.shape[:2]
+        return self.codes.permute(1, 3, 0, 2, 4).reshape(bands * BAND, blocks * 64)[:self.shape[0], :self.k]
+
     def rows(self, start: int, end: int) -> "Int8Rows":
-        """A view of rows ``[start, end)``."""
-        return Int8Rows(self.codes[start:end], self.scales[start:end], self.k)
+        """Rows ``[start, end)``: a view, where ``start`` is a multiple of 16, otherwise a copy."""
+        start, end, _ = slice(start, end).indices(self.shape[0])
+        end = max(start, end)
+        if start % BAND == 0:
+            return Int8Rows(self.codes[:, start // BAND:-(-end // BAND)], self.scales[start:end], self.k)
+        return Int8Rows.from_codes(self.to_rows()[start:end], self.scales[start:end])
 
     @classmethod
     def cat(cls, parts: Sequence["Int8Rows"]) -> "Int8Rows":
         """The rows of several, one after the other."""
         if len({p.k for p in parts}) != 1:
             raise ValueError(f"rows of different lengths {[p.k for p in parts]}")
-        return cls(torch.cat([p.codes for p in parts]), torch.cat([p.scales for p in parts]), parts[0].k)
+        scales = torch.cat([p.scales for p in parts])
+        if all(p.shape[0] % BAND == 0 for p in parts[:-1]):
+            return cls(torch.cat([p.codes for p in parts], 1), scales, parts[0].k)
+        return cls.from_codes(torch.cat([p.to_rows() for p in parts]), scales)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values the codes stand for, ``[rows, k]``."""
-        return (self.codes[:, :self.k].float() * self.scales[:, None]).to(dtype)
+        return (self.to_rows().float() * self.scales[:, None]).to(dtype)
 
 
 def _matrix(what: str, t: torch.Tensor, dtypes) -> None:
@@ -136,11 +158,11 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     rows, k = x.shape
     if not 1 <= k <= MAX_K:
         raise ValueError(f"rows of 1 to {MAX_K} elements, got {k}")
-    codes = torch.empty((rows, _padded(k)), dtype=torch.int8, device=dev)
+    codes = torch.empty(_code_shape(rows, k), dtype=torch.int8, device=dev)
     scales = torch.empty(rows, dtype=torch.float32, device=dev)
     with _guard(dev):
-        rc = _ffi.lib().mlora_quantize_rows(x.data_ptr(), _stride(x), rows, k, codes.data_ptr(), codes.shape[1],
-                                            scales.data_ptr(), _ffi.dtype_code(x.dtype), _ffi.stream_ptr(dev))
+        rc = _ffi.lib().mlora_quantize_rows(x.data_ptr(), _stride(x), rows, k, codes.data_ptr(), scales.data_ptr(),
+                                            _ffi.dtype_code(x.dtype), _ffi.stream_ptr(dev))
     _ffi.check(rc, "mlora_quantize_rows")
     return Int8Rows(codes, scales, k)
 
@@ -184,8 +206,8 @@ def int8_matmul(a: Int8Rows, b: Int8Rows, dtype: torch.dtype, bias: Optional[tor
     given = out is not None
     out = _result("int8_matmul", m, b, bias, out, dtype, dev)
     with _guard(dev):
-        rc = _ffi.lib().mlora_int8_matmul(a.codes.data_ptr(), _stride(a.codes), a.scales.data_ptr(), m, b.codes.data_ptr(),
-                                          _stride(b.codes), b.scales.data_ptr(), n, a.k, _address(bias), out.data_ptr(),
+        rc = _ffi.lib().mlora_int8_matmul(a.codes.data_ptr(), a.codes.stride(0), a.scales.data_ptr(), m, b.codes.data_ptr(),
+                                          b.codes.stride(0), b.scales.data_ptr(), n, a.k, _address(bias), out.data_ptr(),
                                           _stride(out), _ffi.dtype_code(dtype), _ffi.stream_ptr(dev))
     _ffi.check(rc, "mlora_int8_matmul")
     if given:
@@ -218,9 +240,9 @@ def int8_linear(x: torch.Tensor, weight: Int8Rows, bias: Optional[torch.Tensor] 
     need = lib.mlora_int8_linear_workspace_bytes(rows, k)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     with _guard(dev):
-        rc = lib.mlora_int8_linear(x.data_ptr(), _stride(x), rows, weight.codes.data_ptr(), _stride(weight.codes),
-                                   weight.scales.data_ptr(), weight.shape[0], k, _address(bias), out.data_ptr(),
-                                   _stride(out), _ffi.dtype_code(x.dtype), _address(ws), need, _ffi.stream_ptr(dev))
+        rc = lib.mlora_int8_linear(x.data_ptr(), _stride(x), rows, weight.codes.data_ptr(), weight.codes.stride(0),
+                                   weight.scales.data_ptr(), weight.shape[0], k, _address(bias), out.data_ptr(), _stride(out),
+                                   _ffi.dtype_code(x.dtype), _address(ws), need, _ffi.stream_ptr(dev))
     _ffi.check(rc, "mlora_int8_linear")
     if given:
         torch.autograd.graph.increment_version(out)

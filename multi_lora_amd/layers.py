@@ -145,7 +145,8 @@ class QKVProjGroup:
             else torch.cat([w.base_layer.weight.detach() for w in wrappers], dim=0))
         col = 0
         for w, width in zip(wrappers, widths):
-            # Each layer's weight becomes a view of the fused weight: no extra memory.
+            # Each layer's weight becomes a view of the fused weight: no extra memory (8-bit rows: where it begins at a
+            # multiple of 16).
             w.base_layer.weight = (self.weight.rows(col, col + width) if quantised == {True}
                                    else nn.Parameter(self.weight[col : col + width], requires_grad=False))
             w.qkv_slice = (col, col + width)

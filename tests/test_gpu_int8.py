@@ -65,8 +65,9 @@ def test_codes_are_those_of_exact_arithmetic(m, k, dtype):
     x = activations(m, k, dtype, m * k)
     rows = quantize_rows(x.to(DEV))
     codes, scales = codes_of(x)
-    assert torch.equal(rows.codes[:, :k].cpu().double(), codes)
-    assert not rows.codes[:, k:].any()
+    assert torch.equal(rows.to_rows().cpu().double(), codes)
+    tail = rows.codes.permute(1, 3, 0, 2, 4).reshape(-1, rows.codes.shape[0] * 64)[:m, k:]
+    assert not tail.any()  # zeros behind column k
     torch.testing.assert_close(rows.scales.cpu().double(), scales, rtol=2.0 ** -24, atol=0)
 
 
@@ -78,7 +79,7 @@ def test_every_quotient_of_a_type_is_rounded_as_exactly():
     for top in tops:
         x = every[every.abs() <= top][None]
         rows = quantize_rows(x.to(DEV))
-        assert torch.equal(rows.codes[:, :x.shape[1]].cpu().double(), codes_of(x)[0]), float(top)
+        assert torch.equal(rows.to_rows().cpu().double(), codes_of(x)[0]), float(top)
 
 
 def test_float32_weights():
@@ -86,7 +87,7 @@ def test_float32_weights():
     rows = quantize_rows(w.to(DEV))
     codes, scales = codes_of(w)
     # fp32 quotients next to halfway may round the other way: by one code, and the number is then next to the border.
-    off = (rows.codes[:, :777].cpu().double() - codes).abs()
+    off = (rows.to_rows().cpu().double() - codes).abs()
     assert off.max() <= 1 and off.mean() < 1e-4
     near = (w.double() / scales[:, None] - codes).abs()[off > 0]
     assert bool((near > 0.5 - 1e-4).all())
@@ -108,7 +109,11 @@ def test_slices_of_wider_tensors(m):
     k, n = 200, 50
     wide = activations(m, 3 * k + 1, torch.float16, m)
     codes, scales = weight(3 * n, k, m)
-    w = Int8Rows.from_codes(codes.to(DEV), scales.to(DEV)).rows(n, 2 * n)
+    whole = Int8Rows.from_codes(codes.to(DEV), scales.to(DEV))
+    w = whole.rows(n, 2 * n)
+    view = whole.rows(48, 48 + n)  # blocks further apart than they are long
+    assert view.codes.data_ptr() != w.codes.data_ptr() and not view.codes.is_contiguous()
+    check(int8_linear(wide.to(DEV)[:, :k], view), *product(*codes_of(wide[:, :k]), codes[48:48 + n], scales[48:48 + n]))
     bias = torch.randn(n, generator=gen(2)).half()
     for at in (0, 1, k):
         x = wide.to(DEV)[:, at:at + k]

@@ -26,7 +26,7 @@ class PlainInt8(nn.Module):
 
     def __init__(self, layer: Int8Linear) -> None:
         super().__init__()
-        self.w = layer.weight.codes[:, :layer.in_features].double() * layer.weight.scales.double()[:, None]
+        self.w = layer.weight.to_rows().double() * layer.weight.scales.double()[:, None]
         self.bias = None
 
     def forward(self, x):
@@ -166,11 +166,11 @@ def test_fused_projections(dev, monkeypatch):
     fused = MultiLoRAManager.from_adapters(model, store, max_loras_per_batch=4, max_lora_rank=16)
     for name, w in fused.lora_wrappers.items():
         x = torch.randn(5, 1, w.base_layer.in_features, device=dev).bfloat16()
-        assert torch.equal(w.base_layer.weight.codes, weights[name].codes)
+        assert torch.equal(w.base_layer.weight.to_rows(), weights[name].to_rows())
         if w.qkv_group is not None:
             a, b = w.qkv_slice
             assert torch.equal(w.qkv_group._base(x)[..., a:b], w.base_layer(x))
-            assert w.base_layer.weight.codes.data_ptr() == w.qkv_group.weight.codes[a:].data_ptr()  # a view
+            assert w.base_layer.weight.codes.data_ptr() == w.qkv_group.weight.codes[:, a // 16:].data_ptr()  # a view
     ids = torch.randint(0, cfg.vocab_size, (1, 33), generator=torch.Generator().manual_seed(1)).to(dev)
     got = fused.forward_with_lora(input_ids=ids, lora_names=["a"], seq_lens=[33], use_cache=False).logits
     monkeypatch.setenv("MULTI_LORA_FUSED_QKV", "0")
