@@ -111,8 +111,11 @@ int check_step(const mlora_paged_step* s) {
   return 0;
 }
 
-// 16-bit rows readable as 16-byte chunks of whole rows.
-bool rows_aligned(const void* x, int64_t stride, int k) { return al16(x) && stride % 8 == 0 && k % 8 == 0; }
+// Rows readable as 16-byte chunks from end to end.
+bool rows_aligned(const void* x, int64_t stride, int k, int dtype) {
+  const int v = vec_elems(dtype);
+  return al16(x) && stride % v == 0 && k % v == 0;
+}
 
 // What the products in 8-bit integers share; the pointers are the caller's to check.
 int int8_args(int32_t m, const int8_t* codes, int64_t stride, const float* scales, int32_t n, int32_t k, const void* bias,
@@ -1043,7 +1046,7 @@ int mlora_quantize_rows(const void* x, int64_t x_row_stride, int32_t rows, int32
   a.rows = rows, a.k = k;
   a.codes = codes;
   a.scales = scales;
-  const hipError_t e = mlora::launch_quantize_rows(a, dtype, rows_aligned(x, x_row_stride, k), static_cast<hipStream_t>(stream));
+  const hipError_t e = mlora::launch_quantize_rows(a, dtype, rows_aligned(x, x_row_stride, k, dtype), static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return hip_fail(e, "row quantisation launch");
   return 0;
 }
@@ -1078,7 +1081,7 @@ int mlora_int8_linear(const void* x, int64_t x_row_stride, int32_t m, const int8
   if (x_row_stride < k) return fail(kBadArg, "row strides do not hold the rows");
   if (m == 0 || n == 0) return 0;
   if (!x || !b_codes || !b_scales || !out) return fail(kBadArg, "null pointer");
-  const bool aligned = rows_aligned(x, x_row_stride, k);
+  const bool aligned = rows_aligned(x, x_row_stride, k, dtype);
   hipError_t e;
   if (mlora::int8_fused(m, k)) {
     a.x = x, a.x_stride = x_row_stride, a.x_aligned = aligned;

@@ -24,36 +24,33 @@ __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x
 
 // A row's maximum as codes and scale need it.
 struct RowScale {
-  float top, half;  // divided by 2^8, so that 127 times the maximum stays finite
-  float inv, scale;
+  float top, inv;  // the maximum divided by 2^8, so that 127 times it stays finite, and 1 over that
+  float scale;
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t bits) {
   RowScale s;
   const float top = fmaxf(__uint_as_float(min(bits, kInfBits)), kLeast);
   s.top = top * 0x1p-8f;
-  s.half = top * 0x1p-9f;
-  s.inv = 127.f / top;
+  s.inv = 1.f / s.top;
   s.scale = bits >= kInfBits ? NAN : top / 127.f;
   return s;
 }
 
-// rint(127 x / top), ties to even.  x * inv is off by some 2^-22 of itself, so
-// the nearest integer is off by one only where the quotient is that close to
-// halfway; the remainder 127 x - r * top says so exactly (a 16-bit x has at most
-// 11 bits, 127 and r have 7, and r is 0 or x at least 2^-8 of top).
-__device__ __forceinline__ int code_of(float x, const RowScale& s) {
-  float r = __builtin_rintf(x * s.inv);
-  const float d = __builtin_fmaf(-r, s.top, x * (127.f * 0x1p-8f));
-  const float ad = fabsf(d);
-  if (ad >= s.half) {
-    const bool odd = (static_cast<int>(r) & 1) != 0;
-    if (ad > s.half || odd) r += copysignf(1.f, d);
-  }
-  return static_cast<int>(r);
+// rint(127 x / top), ties to even, in the low byte.  The quotient is corrected
+// by its remainder, which is exact (127 x has at most 18 bits for a 16-bit x), and
+// with that right to its last bit but one: a tie comes out as one, and no other
+// quotient is within 2^-19 of itself of one.  Adding 1.5 * 2^23 rounds.
+__device__ __forceinline__ uint32_t code_of(float x, const RowScale& s) {
+  const float t = x * (127.f * 0x1p-8f);
+  const float q = t * s.inv;
+  const float exact = __builtin_fmaf(__builtin_fmaf(-q, s.top, t), s.inv, q);
+  return __float_as_uint(exact + 12582912.f);
 }
 
-__device__ __forceinline__ uint32_t pack4(const int* c) {
-  return (c[0] & 0xff) | (c[1] & 0xff) << 8 | (c[2] & 0xff) << 16 | static_cast<uint32_t>(c[3]) << 24;
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t pack4(const uint32_t* c) {
+  const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u);
+  return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 
 // Eight elements of a row from element e on, zeros behind its end.
@@ -70,67 +67,91 @@ __device__ __forceinline__ void load8(const typename T::raw_t* row, int e, int k
   }
 }
 
+// Rows from which on a workgroup has four of them.  Times in us: 300 rows of 4096
+// 3.5 with one each, 3.9 with four; 512 rows 4.8 and 4.2; 64 of 14336 3.8 and 7.4;
+// 2048 of 4096 6.7 with four, 8.7 with eight, 8192 of 1024 6.6 and 6.7; 1088 of
+// 14336 19.3 and 17.6.
+constexpr int kQuantMany = 400;
 constexpr int kFusedStep = 8 * 64 * 8;  // elements of one chunk a thread of the register form's workgroup
 
-constexpr int kQuantKeep = 4;  // chunks of eight elements a thread keeps; longer rows are read twice
-
-// TPR threads a row, eight elements at a time.  Bound by bytes: 2 in and 1 out
-// an element.
-template <class T, int TPR, bool AL>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
-  using raw = typename T::raw_t;
-  constexpr int RPB = 256 / TPR;
-  __shared__ uint32_t tops[RPB][TPR / 64];
-  const int sub = threadIdx.x / TPR;
-  const int t = threadIdx.x - sub * TPR;
-  const int row = blockIdx.x * RPB + sub;
-  const raw* x = static_cast<const raw*>(a.x) + static_cast<int64_t>(min(row, a.rows - 1)) * a.x_stride;
-  const int padded = static_cast<int>(int8_padded(a.k));
-  const int64_t step = int8_bands(a.rows) * kInt8Block;
-  float keep[kQuantKeep][8];
-  uint32_t top = 0;
+// The widest of a chunk's elements, as the bits of a float.
+template <class T>
+__device__ __forceinline__ uint32_t widest(const u32x4& v, uint32_t top) {
+  if constexpr (sizeof(typename T::raw_t) == 2) {
+    // Of 16-bit numbers, too, magnitudes order as integers; two at a time.
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 t = __builtin_bit_cast(u16x2, v[0] & 0x7fff7fffu);
 #pragma unroll
-  for (int c = 0; c < kQuantKeep; ++c) {
-    load8<T, AL>(x, (c * TPR + t) * 8, a.k, keep[c]);
-  }
+    for (int i = 1; i < 4; ++i) t = __builtin_elementwise_max(t, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+    return max(top, abs_bits(T::to_f32(max(t[0], t[1]))));
+  } else {
 #pragma unroll
-  for (int c = 0; c < kQuantKeep; ++c)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(keep[c][i]));
-  for (int e = (kQuantKeep * TPR + t) * 8; e < a.k; e += TPR * 8) {
-    float f[8];
-    load8<T, AL>(x, e, a.k, f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(f[i]));
-  }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, kWave)));
-  if constexpr (TPR > 64) {
-    if ((t & 63) == 0) tops[sub][t >> 6] = top;
-    lds_barrier();
-#pragma unroll
-    for (int w = 0; w < TPR / 64; ++w) top = max(top, tops[sub][w]);
-  }
-  if (row >= a.rows) return;
-  const RowScale s = row_scale(top);
-  if (t == 0) a.scales[row] = s.scale;
-  int8_t* out = a.codes + static_cast<int64_t>(row >> 4) * kInt8Block + (row & 15) * 16;
-  auto put = [&](int e, const float* f) {
-    if (e >= padded) return;
-    int q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = code_of(f[i], s);
-    *reinterpret_cast<uint2*>(out + (e >> 6) * step + (e >> 4 & 3) * 256 + (e & 8)) = make_uint2(pack4(q), pack4(q + 4));
-  };
-#pragma unroll
-  for (int c = 0; c < kQuantKeep; ++c) put((c * TPR + t) * 8, keep[c]);
-  for (int e = (kQuantKeep * TPR + t) * 8; e < padded; e += TPR * 8) {
-    float f[8];
-    load8<T, AL>(x, e, a.k, f);
-    put(e, f);
+    for (int i = 0; i < 4; ++i) top = max(top, v[i] & 0x7fffffffu);
+    return top;
   }
 }
 
+// R rows a workgroup (of one band); lane l has row l % R and chunks of 16
+// columns.  With four rows, four lanes write 64 bytes side by side, and a wave
+// reads 512 of each row.  KEEP chunks stay in registers, what a row has more of
+// is read twice.  Bound by bytes, 2 in and 1 out an element, and nearly as much
+// by its arithmetic.
+template <class T, int R, int NW, int KEEP, bool AL>
+__global__ __launch_bounds__(NW * 64) void quantize_rows_kernel(QuantArgs a) {
+  using raw = typename T::raw_t;
+  constexpr int V = 16 / T::VEC;              // 16-byte loads of a chunk
+  constexpr int STEP = NW * (64 / R) * 16;    // columns of all waves
+  __shared__ uint32_t tops[NW][R];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = blockIdx.x * R + lane % R;
+  const raw* x = static_cast<const raw*>(a.x) + static_cast<int64_t>(min(row, a.rows - 1)) * a.x_stride;
+  const int padded = static_cast<int>(int8_padded(a.k));
+  const int e0 = (wave * (64 / R) + lane / R) * 16;
+  auto load = [&](int e, u32x4 (&v)[V]) {
+#pragma unroll
+    for (int h = 0; h < V; ++h)
+      v[h] = load_row_chunk<T, AL>(x, e + h * T::VEC, min(max(a.k - e - h * T::VEC, 0), static_cast<int>(T::VEC)));
+  };
+  u32x4 keep[KEEP][V];
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < KEEP; ++c) load(e0 + c * STEP, keep[c]);
+#pragma unroll
+  for (int c = 0; c < KEEP; ++c)
+#pragma unroll
+    for (int h = 0; h < V; ++h) top = widest<T>(keep[c][h], top);
+  for (int e = e0 + KEEP * STEP; e < a.k; e += STEP) {
+    u32x4 v[V];
+    load(e, v);
+#pragma unroll
+    for (int h = 0; h < V; ++h) top = widest<T>(v[h], top);
+  }
+#pragma unroll
+  for (int off = R; off < 64; off <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, kWave)));
+  if (lane < R) tops[wave][lane] = top;
+  lds_barrier();
+#pragma unroll
+  for (int w = 0; w < NW; ++w) top = max(top, tops[w][lane % R]);
+  if (row >= a.rows) return;
+  const RowScale s = row_scale(top);
+  if (threadIdx.x < R) a.scales[row] = s.scale;
+  const int64_t step = int8_bands(a.rows) * kInt8Block;
+  int8_t* out = a.codes + static_cast<int64_t>(row >> 4) * kInt8Block + (row & 15) * 16;
+  auto put = [&](int e, const u32x4 (&v)[V]) {
+    if (e >= padded) return;
+    uint32_t q[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) q[i] = code_of(chunk_elem<T>(v[i / T::VEC], i % T::VEC), s);
+    st_chunk(out + (e >> 6) * step + (e >> 4 & 3) * 256, u32x4{pack4(q), pack4(q + 4), pack4(q + 8), pack4(q + 12)});
+  };
+#pragma unroll
+  for (int c = 0; c < KEEP; ++c) put(e0 + c * STEP, keep[c]);
+  for (int e = e0 + KEEP * STEP; e < padded; e += STEP) {
+    u32x4 v[V];
+    load(e, v);
+    put(e, v);
+  }
+}
 
 // Four columns of a row of the result, n to n + 3.
 template <class T>
@@ -233,7 +254,7 @@ __global__ __launch_bounds__(NW * 64) void int8_rows_kernel(Int8Args a) {
       if (r >= a.m) continue;
       const int e = i - r * chunks;
       const RowScale s = row_scale(tops[r]);
-      int q[8];
+      uint32_t q[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) q[j] = code_of(keep[c][j], s);
       *reinterpret_cast<uint2*>(codes + ((e >> 1) * a.m + r) * 16 + (e & 1) * 8) = make_uint2(pack4(q), pack4(q + 4));
@@ -343,19 +364,20 @@ hipError_t launch(const Int8Args& a, int cus, hipStream_t stream) {
   return launch_tile<T, TileShape<256, 256, 2, 4, 2>>(a, stream);
 }
 
-template <class T, int TPR>
+template <class T, int R, int NW, int KEEP>
 hipError_t launch_quant(const QuantArgs& a, bool aligned, hipStream_t stream) {
-  const int64_t blocks = (static_cast<int64_t>(a.rows) + 256 / TPR - 1) / (256 / TPR);
-  if (!grid_fits(blocks)) return hipErrorInvalidConfiguration;
+  const int64_t blocks = (static_cast<int64_t>(a.rows) + R - 1) / R;
+  if (!grid_fits(blocks * (NW / 4))) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (aligned) hipLaunchKernelGGL((quantize_rows_kernel<T, TPR, true>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((quantize_rows_kernel<T, TPR, false>), grid, dim3(256), 0, stream, a);
+  if (aligned) hipLaunchKernelGGL((quantize_rows_kernel<T, R, NW, KEEP, true>), grid, dim3(NW * 64), 0, stream, a);
+  else hipLaunchKernelGGL((quantize_rows_kernel<T, R, NW, KEEP, false>), grid, dim3(NW * 64), 0, stream, a);
   return hipGetLastError();
 }
 
 template <class T>
 hipError_t quant_of(const QuantArgs& a, bool aligned, hipStream_t stream) {
-  return a.k <= 1024 ? launch_quant<T, 64>(a, aligned, stream) : launch_quant<T, 256>(a, aligned, stream);
+  if (a.rows < kQuantMany) return a.k <= 4096 ? launch_quant<T, 1, 4, 1>(a, aligned, stream) : launch_quant<T, 1, 16, 1>(a, aligned, stream);
+  return a.k <= 1024 ? launch_quant<T, 4, 4, 1>(a, aligned, stream) : launch_quant<T, 4, 8, 2>(a, aligned, stream);
 }
 
 }  // namespace
@@ -369,7 +391,7 @@ hipError_t launch_quantize_rows(const QuantArgs& a, int dtype, bool aligned, hip
   if (a.rows == 0) return hipSuccess;
   if (dtype == MLORA_BF16) return quant_of<BF16>(a, aligned, stream);
   if (dtype == MLORA_F16) return quant_of<F16>(a, aligned, stream);
-  return quant_of<F32>(a, false, stream);
+  return launch_quant<F32, 4, 4, 1>(a, aligned, stream);
 }
 
 hipError_t launch_int8_matmul(const Int8Args& a, int dtype, int cus, hipStream_t stream) {
