@@ -78,43 +78,97 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   return v;
 }
 
-// x * cos + (x rolled by D / 2) * sin of 8 columns of the first half and the 8
-// they pair with; the products are rounded before the sum, as torch's are.
-template <class T, int D, bool AL>
-__device__ __forceinline__ void rotate8(const WriteArgs& a, const typename T::raw_t* x, int r, int e, float* y0, float* y1) {
-#pragma clang fp contract(off)
-  const u32x4 lo = load_row_chunk<T, AL>(x, e, 8);
-  const u32x4 hi = load_row_chunk<T, AL>(x, e + D / 2, 8);
-  float c0[8], c1[8], s0[8], s1[8];
-  const char* cs = static_cast<const char*>(a.cos) + r * a.rot_stride * (a.rot_f32 ? 4 : 2);
-  const char* sn = static_cast<const char*>(a.sin) + r * a.rot_stride * (a.rot_f32 ? 4 : 2);
-  rot_chunk<T, AL>(cs, e, a.rot_f32, c0);
-  rot_chunk<T, AL>(cs, e + D / 2, a.rot_f32, c1);
-  rot_chunk<T, AL>(sn, e, a.rot_f32, s0);
-  rot_chunk<T, AL>(sn, e + D / 2, a.rot_f32, s1);
+// N neighbouring numbers of the data type, or of fp32.
+template <class T, int N, bool AL>
+__device__ __forceinline__ void load_n(const typename T::raw_t* p, float* f) {
+  if constexpr (AL) {
+    uint32_t w[N / 2];
+    if constexpr (N == 8) *reinterpret_cast<u32x4*>(w) = ld_chunk(p);
+    else *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x0 = chunk_elem<T>(lo, i), x1 = chunk_elem<T>(hi, i);
-    const float p0 = x0 * c0[i], p1 = x1 * s0[i], p2 = x1 * c1[i], p3 = x0 * s1[i];
+    for (int i = 0; i < N; ++i) f[i] = T::to_f32(static_cast<uint16_t>((i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xffffu));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = T::to_f32(p[i]);
+  }
+}
+template <class T, int N, bool AL>
+__device__ __forceinline__ void table_n(const void* p, int64_t e, bool f32, float* f) {
+  if (f32) {
+    const float* t = static_cast<const float*>(p) + e;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      if constexpr (AL) *reinterpret_cast<f32x4*>(f + i) = *reinterpret_cast<const f32x4*>(t + i);
+      else f[i] = t[i], f[i + 1] = t[i + 1], f[i + 2] = t[i + 2], f[i + 3] = t[i + 3];
+    }
+  } else {
+    load_n<T, N, AL>(static_cast<const typename T::raw_t*>(p) + e, f);
+  }
+}
+
+// x * cos + (x rolled by D / 2) * sin of N columns of the first half and the N
+// they pair with; the products are rounded before the sum, as torch's are.
+template <class T, int D, int N, bool AL>
+__device__ __forceinline__ void rotate(const WriteArgs& a, const typename T::raw_t* x, int r, int e, float* y0, float* y1) {
+#pragma clang fp contract(off)
+  alignas(16) float lo[N], hi[N], c0[N], c1[N], s0[N], s1[N];
+  load_n<T, N, AL>(x + e, lo);
+  load_n<T, N, AL>(x + e + D / 2, hi);
+  const int64_t at = r * a.rot_stride + e;
+  table_n<T, N, AL>(a.cos, at, a.rot_f32, c0);
+  table_n<T, N, AL>(a.cos, at + D / 2, a.rot_f32, c1);
+  table_n<T, N, AL>(a.sin, at, a.rot_f32, s0);
+  table_n<T, N, AL>(a.sin, at + D / 2, a.rot_f32, s1);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float p0 = lo[i] * c0[i], p1 = hi[i] * s0[i], p2 = hi[i] * c1[i], p3 = lo[i] * s1[i];
     y0[i] = p0 + p1;
     y1[i] = p2 + p3;
   }
 }
 
-// Blocks [0, block_blocks): a wave has the cache blocks that begin in a few
-// rows (of which its first lanes look at the slots), for keys or for values of
-// one head; a block is one wave's alone, so its exponent and codes are changed
-// without atomics.  The rest: a thread rotates 8 columns of a head's first half
-// of q and the 8 they pair with.
+template <class T, int D>
+__device__ __forceinline__ void rotate_one(const WriteArgs& a, const typename T::raw_t* x, int r, int e, float* y0, float* y1) {
+#pragma clang fp contract(off)
+  const int64_t at = r * a.rot_stride + e;
+  auto table = [&](const void* p, int64_t i) {
+    return a.rot_f32 ? static_cast<const float*>(p)[i] : T::to_f32(static_cast<const typename T::raw_t*>(p)[i]);
+  };
+  const float lo = T::to_f32(x[e]), hi = T::to_f32(x[e + D / 2]);
+  const float p0 = lo * table(a.cos, at), p1 = hi * table(a.sin, at);
+  const float p2 = hi * table(a.cos, at + D / 2), p3 = lo * table(a.sin, at + D / 2);
+  *y0 = p0 + p1;
+  *y1 = p2 + p3;
+}
+
+// N (2 or 4) codes in the low bytes of a word.
+template <int N>
+__device__ __forceinline__ void put_codes(uint8_t* p, uint32_t w) {
+  if constexpr (N == 4) *reinterpret_cast<uint32_t*>(p) = w;
+  else *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w);
+}
+template <int N>
+__device__ __forceinline__ uint32_t get_codes(const uint8_t* p) {
+  if constexpr (N == 4) return *reinterpret_cast<const uint32_t*>(p);
+  else return *reinterpret_cast<const uint16_t*>(p);
+}
+
+// Workgroups [0, block_groups): one has the cache blocks that begin in `window`
+// rows, for keys or for values of one head; a block is one workgroup's alone, so
+// its exponent and codes are changed without atomics.  Its 256 threads share a
+// block of 16 x D numbers, 8 (D 64: 4) each: with a wave a block, the kernel's
+// registers (136) left the q rows a third of the waves (4075 rows 30.4 us).  The
+// rest: a thread rotates 8 columns of a head's first half of q and the 8 they
+// pair with.
 template <class T, int D, bool AL>
-__global__ __launch_bounds__(256) void paged_write8_kernel(Write8Args args, int block_blocks, int window) {
+__global__ __launch_bounds__(256) void paged_write8_kernel(Write8Args args, int block_groups, int window) {
   using raw = typename T::raw_t;
   const WriteArgs& a = args.w;
   const int page = 1 << a.page_shift;
   const int64_t slots = static_cast<int64_t>(a.num_pages) << a.page_shift;
-  if (static_cast<int>(blockIdx.x) >= block_blocks) {
+  if (static_cast<int>(blockIdx.x) >= block_groups) {
     constexpr int U = D / 16;  // units a head
-    const int64_t id = (static_cast<int64_t>(blockIdx.x) - block_blocks) * 256 + threadIdx.x;
+    const int64_t id = (static_cast<int64_t>(blockIdx.x) - block_groups) * 256 + threadIdx.x;
     const int per_row = a.heads * U;
     const int r = static_cast<int>(id / per_row);
     if (r >= a.rows) return;
@@ -122,22 +176,20 @@ __global__ __launch_bounds__(256) void paged_write8_kernel(Write8Args args, int 
     const int h = u / U;
     const int e = (u - h * U) * 8;
     float y0[8], y1[8];
-    rotate8<T, D, AL>(a, static_cast<const raw*>(a.q) + r * a.q_stride + h * D, r, e, y0, y1);
+    rotate<T, D, 8, AL>(a, static_cast<const raw*>(a.q) + r * a.q_stride + h * D, r, e, y0, y1);
     raw* to = static_cast<raw*>(a.q_out) + r * a.q_out_stride + h * D;
     store_row_chunk<T, AL>(to + e, pack_chunk<T>(y0), 8);
     store_row_chunk<T, AL>(to + e + D / 2, pack_chunk<T>(y1), 8);
     return;
   }
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const bool is_v = (w & 1) != 0;
-  const int64_t wg = w >> 1;
-  const int64_t first = wg / a.kv_heads * window;
-  if (first >= a.rows) return;
-  const int r0 = static_cast<int>(first);
-  const int head = static_cast<int>(wg % a.kv_heads);
-  const int lane = threadIdx.x & 63;
-  // Lane l looks at row r0 - 1 + l.  Bits of lanes: rows that have a slot and
-  // are the first of their block here, rows that follow one in their block.
+  __shared__ uint32_t tops[2][4];
+  const bool is_v = (blockIdx.x & 1) != 0;
+  const int wg = static_cast<int>(blockIdx.x) >> 1;
+  const int r0 = wg / a.kv_heads * window;
+  const int head = wg % a.kv_heads;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // Lane l of every wave looks at row r0 - 1 + l.  Bits of lanes: rows that have
+  // a slot and are the first of their block here, rows that follow one in their block.
   const int look = r0 - 1 + lane;
   const int seen = lane < window + 16 && look >= 0 && look < a.rows ? a.slots[look] : -1;
   const int before = __shfl_up(seen, 1, kWave);
@@ -145,7 +197,8 @@ __global__ __launch_bounds__(256) void paged_write8_kernel(Write8Args args, int 
   const bool follows = lane > 0 && placed && (seen & (kScaleBlock - 1)) != 0 && seen == before + 1;
   const uint64_t inside = __ballot(follows);
   const uint64_t mine = (((1ull << window) - 1) << 1);
-  for (uint64_t todo = __ballot(placed && !follows) & mine; todo != 0; todo &= todo - 1) {
+  int turn = 0;
+  for (uint64_t todo = __ballot(placed && !follows) & mine; todo != 0; todo &= todo - 1, turn ^= 1) {
     const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(todo));
     const int slot = __builtin_amdgcn_readlane(seen, l);
     const int n = 1 + __builtin_ctzll(~(inside >> (l + 1)));  // rows of the block, at most 16
@@ -157,91 +210,93 @@ __global__ __launch_bounds__(256) void paged_write8_kernel(Write8Args args, int 
     uint8_t* scale = (is_v ? args.value_scales : args.key_scales) + at;
     // A block's exponent counts where earlier rows are in it.
     const int was = min(max(static_cast<int>(*scale) - kScaleBias, ScaleRange<T>::lo), ScaleRange<T>::hi);
+    // The block's exponent from the threads' widest numbers.
+    auto exponent = [&](uint32_t top) {
+      top = wave_max(top);
+      if (lane == 0) tops[turn][wave] = top;
+      lds_barrier();
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = max(top, tops[turn][w]);
+      const int e = exponent_of<T>(top);
+      return off > 0 ? max(e, was) : e;
+    };
     if (!is_v) {
-      // Lane: row lane >> 2, D / 8 columns of each half.
-      constexpr int E = D / 8;
-      const int ri = lane >> 2, c = lane & 3;
-      float y[2][E];
+      // Thread: row tid / 16, E columns of each half.
+      constexpr int E = D / 32;
+      const int ri = threadIdx.x >> 4, c = (threadIdx.x & 15) * E;
+      uint8_t* keys = static_cast<uint8_t*>(a.keys) + id * a.key_stride + (static_cast<int64_t>(head) * page + in_page) * D + c;
+      float y[2][4] = {};
       uint32_t top = 0;
       if (ri < n) {
         const raw* x = static_cast<const raw*>(a.k) + (row + ri) * a.k_stride + head * D;
+        if constexpr (E == 4) {
+          rotate<T, D, 4, AL>(a, x, row + ri, c, y[0], y[1]);
+        } else {
 #pragma unroll
-        for (int e = 0; e < E; e += 8) rotate8<T, D, AL>(a, x, row + ri, c * E + e, y[0] + e, y[1] + e);
+          for (int i = 0; i < E; ++i) rotate_one<T, D>(a, x, row + ri, c + i, &y[0][i], &y[1][i]);
+        }
 #pragma unroll
         for (int i = 0; i < E; ++i) top = max(top, max(counted<T>(y[0][i]), counted<T>(y[1][i])));
       }
-      int e = exponent_of<T>(wave_max(top));
-      if (off > 0) e = max(e, was);
+      const int e = exponent(top);
       const float inv = pow2(-e);
-      uint8_t* keys = static_cast<uint8_t*>(a.keys) + id * a.key_stride + (static_cast<int64_t>(head) * page + in_page) * D + c * E;
+      const bool grows = off > 0 && e > was;
       if (ri < n) {
-        uint32_t* to = reinterpret_cast<uint32_t*>(keys + (off + ri) * D);
 #pragma unroll
-        for (int i = 0; i < E / 4; ++i) {
-          to[i] = codes4<T>(y[0] + 4 * i, inv, e);
-          to[D / 8 + i] = codes4<T>(y[1] + 4 * i, inv, e);
-        }
+        for (int z = 0; z < 2; ++z) put_codes<E>(keys + (off + ri) * D + z * (D / 2), codes4<T>(y[z], inv, e));
       }
-      if (off > 0 && e > was && ri < off) {
+      if (grows && ri < off) {
         const float ratio = ldexpf(1.f, was - e);
-        uint32_t* old = reinterpret_cast<uint32_t*>(keys + ri * D);
 #pragma unroll
-        for (int i = 0; i < E / 4; ++i) {
-          old[i] = moved4(old[i], ratio);
-          old[D / 8 + i] = moved4(old[D / 8 + i], ratio);
+        for (int z = 0; z < 2; ++z) {
+          uint8_t* old = keys + ri * D + z * (D / 2);
+          put_codes<E>(old, moved4(get_codes<E>(old), ratio));
         }
       }
-      if (lane == 0 && (off == 0 || e > was)) *scale = static_cast<uint8_t>(e + kScaleBias);
+      if (threadIdx.x == 0 && (off == 0 || grows)) *scale = static_cast<uint8_t>(e + kScaleBias);
     } else {
-      // Lane: columns lane and lane + 64, all 16 positions.
-      float x[D / kWave][kScaleBlock];
+      // Thread: column tid % D, P positions.
+      constexpr int P = 16 * D / 256;
+      const int d = threadIdx.x & (D - 1), j0 = threadIdx.x / D * P;
+      float x[P];
       uint32_t top = 0;
-      const raw* v = static_cast<const raw*>(a.v) + head * D + lane;
+      const raw* v = static_cast<const raw*>(a.v) + head * D + d;
 #pragma unroll
-      for (int j = 0; j < kScaleBlock; ++j) {
-        const bool has = j >= off && j < off + n;
-#pragma unroll
-        for (int d = 0; d < D / kWave; ++d) {
-          x[d][j] = has ? T::to_f32(v[(row + j - off) * a.v_stride + d * kWave]) : 0.f;
-          top = max(top, counted<T>(x[d][j]));
-        }
+      for (int j = 0; j < P; ++j) {
+        const int i = j0 + j - off;
+        x[j] = i >= 0 && i < n ? T::to_f32(v[(row + i) * a.v_stride]) : 0.f;
       }
-      uint8_t* values = static_cast<uint8_t*>(a.values) + id * a.value_stride + (static_cast<int64_t>(head) * D + lane) * page + in_page;
-      u32x4 old[D / kWave];
-      if (n < kScaleBlock)
+      uint32_t* values = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.values) + id * a.value_stride +
+                                                     (static_cast<int64_t>(head) * D + d) * page + in_page + j0);
+      uint32_t old[P / 4];
 #pragma unroll
-        for (int d = 0; d < D / kWave; ++d) old[d] = ld_chunk(values + static_cast<int64_t>(d) * kWave * page);
-      int e = exponent_of<T>(wave_max(top));
-      if (off > 0) e = max(e, was);
+      for (int w = 0; w < P / 4; ++w) old[w] = n < kScaleBlock ? values[w] : 0u;
+#pragma unroll
+      for (int j = 0; j < P; ++j) top = max(top, counted<T>(x[j]));
+      const int e = exponent(top);
       const float inv = pow2(-e);
+      const bool grows = off > 0 && e > was;
       const float ratio = ldexpf(1.f, was - e);
+      // Positions before `off` are earlier rows, those behind the new ones stay as they are.
 #pragma unroll
-      for (int d = 0; d < D / kWave; ++d) {
-        u32x4 y;
+      for (int w = 0; w < P / 4; ++w) {
+        uint32_t early = 0, late = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = codes4<T>(x[d] + 4 * i, inv, e);
-        if (n < kScaleBlock) {
-          // Positions before `off` are earlier rows, those behind the new ones stay as they are.
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t kept = off > 0 && e > was ? moved4(old[d][i], ratio) : old[d][i];
-            uint32_t early = 0, late = 0;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              if (4 * i + b < off) early |= 0xffu << (8 * b);
-              if (4 * i + b >= off + n) late |= 0xffu << (8 * b);
-            }
-            y[i] = (y[i] & ~(early | late)) | (kept & early) | (old[d][i] & late);
-          }
+        for (int b = 0; b < 4; ++b) {
+          if (j0 + 4 * w + b < off) early |= 0xffu << (8 * b);
+          if (j0 + 4 * w + b >= off + n) late |= 0xffu << (8 * b);
         }
-        st_chunk(values + static_cast<int64_t>(d) * kWave * page, y);
+        const uint32_t kept = grows ? moved4(old[w], ratio) : old[w];
+        old[w] = (codes4<T>(x + 4 * w, inv, e) & ~(early | late)) | (kept & early) | (old[w] & late);
       }
-      if (lane == 0 && (off == 0 || e > was)) *scale = static_cast<uint8_t>(e + kScaleBias);
+      if constexpr (P == 8) *reinterpret_cast<uint2*>(values) = make_uint2(old[0], old[1]);
+      else values[0] = old[0];
+      if (threadIdx.x == 0 && (off == 0 || grows)) *scale = static_cast<uint8_t>(e + kScaleBias);
     }
   }
 }
 
-// Rows whose blocks one wave looks after.
+// Rows whose blocks one workgroup looks after.
 constexpr int window_rows(int rows) { return rows < 512 ? 1 : 16; }
 
 template <class T, int D>
@@ -250,8 +305,7 @@ hipError_t launch_write8(const Write8Args& args, bool aligned, hipStream_t strea
   const int window = window_rows(a.rows);
   const int64_t units = static_cast<int64_t>(a.rows) * a.heads * (D / 16);
   const int64_t rot = (units + 255) / 256;
-  const int64_t waves = (static_cast<int64_t>(a.rows) + window - 1) / window * a.kv_heads * 2;
-  const int64_t blocks = (waves + 3) / 4;
+  const int64_t blocks = (static_cast<int64_t>(a.rows) + window - 1) / window * a.kv_heads * 2;
   if (!grid_fits(rot + blocks)) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(rot + blocks));
   if (aligned)
