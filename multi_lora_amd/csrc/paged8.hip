@@ -153,63 +153,220 @@ __device__ __forceinline__ uint32_t get_codes(const uint8_t* p) {
   else return *reinterpret_cast<const uint16_t*>(p);
 }
 
-// Workgroups [0, block_groups): one has the cache blocks that begin in `window`
-// rows, for keys or for values of one head; a block is one workgroup's alone, so
-// its exponent and codes are changed without atomics.  Its 256 threads share a
-// block of 16 x D numbers, 8 (D 64: 4) each: with a wave a block, the kernel's
-// registers (136) left the q rows a third of the waves (4075 rows 30.4 us).  The
-// rest: a thread rotates 8 columns of a head's first half of q and the 8 they
-// pair with.
+// A thread rotates 8 columns of a head's first half of q and the 8 they pair with.
 template <class T, int D, bool AL>
-__global__ __launch_bounds__(256) void paged_write8_kernel(Write8Args args, int block_groups, int window) {
+__device__ __forceinline__ void rotate_q(const WriteArgs& a, int64_t id) {
+  using raw = typename T::raw_t;
+  constexpr int U = D / 16;  // units a head
+  const int per_row = a.heads * U;
+  const int r = static_cast<int>(id / per_row);
+  if (r >= a.rows) return;
+  const int u = static_cast<int>(id - static_cast<int64_t>(r) * per_row);
+  const int h = u / U;
+  const int e = (u - h * U) * 8;
+  float y0[8], y1[8];
+  rotate<T, D, 8, AL>(a, static_cast<const raw*>(a.q) + r * a.q_stride + h * D, r, e, y0, y1);
+  raw* to = static_cast<raw*>(a.q_out) + r * a.q_out_stride + h * D;
+  store_row_chunk<T, AL>(to + e, pack_chunk<T>(y0), 8);
+  store_row_chunk<T, AL>(to + e + D / 2, pack_chunk<T>(y1), 8);
+}
+
+// The blocks that begin in `window` rows from r0 on.  Lane l looks at row r0 - 1
+// + l; bits of lanes: rows that have a slot and are the first of their block
+// here, rows that follow one in their block.
+struct Blocks {
+  int seen;
+  uint64_t first, inside;
+};
+__device__ __forceinline__ Blocks find_blocks(const WriteArgs& a, int r0, int window) {
+  const int lane = threadIdx.x & 63;
+  const int64_t slots = static_cast<int64_t>(a.num_pages) << a.page_shift;
+  const int look = r0 - 1 + lane;
+  Blocks b;
+  b.seen = lane < window + 16 && look >= 0 && look < a.rows ? a.slots[look] : -1;
+  const int before = __shfl_up(b.seen, 1, kWave);
+  const bool placed = b.seen >= 0 && b.seen < slots;
+  const bool follows = lane > 0 && placed && (b.seen & (kScaleBlock - 1)) != 0 && b.seen == before + 1;
+  b.inside = __ballot(follows);
+  b.first = __ballot(placed && !follows) & (((1ull << window) - 1) << 1);
+  return b;
+}
+// One of them: its first slot's place, the exponent's, and the new rows.
+struct Block {
+  int row, n, off;      // first row, rows (at most 16), position of the first
+  int64_t id;           // page
+  int in_page;          // the block's first position there
+  int64_t at;           // index of its exponent
+};
+__device__ __forceinline__ Block take_block(const WriteArgs& a, const Blocks& b, int l, int r0, int head) {
+  Block k;
+  const int slot = __builtin_amdgcn_readlane(b.seen, l);
+  const int page = 1 << a.page_shift;
+  k.n = 1 + __builtin_ctzll(~(b.inside >> (l + 1)));
+  k.row = r0 - 1 + l;
+  k.off = slot & (kScaleBlock - 1);
+  k.id = slot >> a.page_shift;
+  k.in_page = slot & (page - 1) & ~(kScaleBlock - 1);
+  k.at = ((k.id * a.kv_heads + head) << (a.page_shift - 4)) + (k.in_page >> 4);
+  return k;
+}
+// A stored exponent; it counts where earlier rows are in the block.
+template <class T>
+__device__ __forceinline__ int stored(uint8_t byte) {
+  return min(max(static_cast<int>(byte) - kScaleBias, ScaleRange<T>::lo), ScaleRange<T>::hi);
+}
+// Four positions of a column of values: positions from j on, of which those
+// before `off` keep their (moved) codes and those from `end` on stay as they are.
+__device__ __forceinline__ uint32_t merge4(uint32_t codes, uint32_t moved, uint32_t old, int j, int off, int end) {
+  uint32_t early = 0, late = 0;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    if (j + b < off) early |= 0xffu << (8 * b);
+    if (j + b >= end) late |= 0xffu << (8 * b);
+  }
+  return (codes & ~(early | late)) | (moved & early) | (old & late);
+}
+
+// Few rows, each in a block of its own more often than not: a wave has the
+// block that begins in its row (if one does), for keys or values of one head.
+// Which row it begins with does not depend on the slots, so that is read while
+// they are on their way.  Bound by that chain: slot, exponent and old codes,
+// store.
+template <class T, int D, bool AL>
+__global__ __launch_bounds__(256, 4) void paged_write8_few_kernel(Write8Args args, int block_groups) {
+  using raw = typename T::raw_t;
+  const WriteArgs& a = args.w;
+  if (static_cast<int>(blockIdx.x) >= block_groups) {
+    rotate_q<T, D, AL>(a, (static_cast<int64_t>(blockIdx.x) - block_groups) * 256 + threadIdx.x);
+    return;
+  }
+  constexpr int H = D / 2, N = D / kWave;
+  const int page = 1 << a.page_shift;
+  const int w = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const bool is_v = (w & 1) != 0;
+  const int r0 = (w >> 1) / a.kv_heads;
+  const int head = (w >> 1) % a.kv_heads;
+  if (r0 >= a.rows) return;
+  const int lane = threadIdx.x & 63;
+  const int e = lane & (H - 1);           // D 64: the upper lanes do what the lower do
+  const raw* k = static_cast<const raw*>(a.k) + head * D;
+  const raw* v = static_cast<const raw*>(a.v) + head * D + lane;
+  float x[2][kScaleBlock];                // keys: the two columns of a pair; values: columns lane and lane + 64; of each row
+  auto read = [&](int i) {
+    const int64_t r = r0 + i;
+    if (!is_v) {
+      rotate_one<T, D>(a, k + r * a.k_stride, r0 + i, e, &x[0][i], &x[1][i]);
+    } else {
+#pragma unroll
+      for (int z = 0; z < N; ++z) x[z][i] = T::to_f32(v[r * a.v_stride + z * kWave]);
+      if constexpr (N == 1) x[1][i] = 0.f;
+    }
+  };
+  read(0);
+  const Blocks found = find_blocks(a, r0, 1);
+  if (found.first == 0) return;
+  const Block b = take_block(a, found, 1, r0, head);
+  uint8_t* scale = (is_v ? args.value_scales : args.key_scales) + b.at;
+  const uint8_t byte = *scale;
+  uint8_t* keys = static_cast<uint8_t*>(a.keys) + b.id * a.key_stride + (static_cast<int64_t>(head) * page + b.in_page) * D + e;
+  uint8_t* values = static_cast<uint8_t*>(a.values) + b.id * a.value_stride + (static_cast<int64_t>(head) * D + lane) * page + b.in_page;
+  u32x4 old[N];
+  if (is_v && b.n < kScaleBlock)
+#pragma unroll
+    for (int z = 0; z < N; ++z) old[z] = ld_chunk(values + static_cast<int64_t>(z) * kWave * page);
+#pragma unroll
+  for (int i = 1; i < kScaleBlock; ++i) {
+    if (i < b.n) read(i);
+    else x[0][i] = x[1][i] = 0.f;
+  }
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kScaleBlock; ++i) top = max(top, max(counted<T>(x[0][i]), counted<T>(x[1][i])));
+  const int was = stored<T>(byte);
+  int ex = exponent_of<T>(wave_max(top));
+  if (b.off > 0) ex = max(ex, was);
+  const float inv = pow2(-ex);
+  const bool grows = b.off > 0 && ex > was;
+  const float ratio = ldexpf(1.f, was - ex);
+  if (!is_v) {
+#pragma unroll
+    for (int i = 0; i < kScaleBlock; ++i) {
+      if (i >= b.n) continue;
+      const float y[4] = {x[0][i], x[1][i], 0.f, 0.f};
+      const uint32_t c = codes4<T>(y, inv, ex);
+      if (lane < H) {
+        keys[(b.off + i) * D] = static_cast<uint8_t>(c);
+        keys[(b.off + i) * D + H] = static_cast<uint8_t>(c >> 8);
+      }
+    }
+    if (grows && lane < H) {
+      for (int i = 0; i < b.off; ++i) {
+        const uint32_t c = moved4(keys[i * D] | static_cast<uint32_t>(keys[i * D + H]) << 8, ratio);
+        keys[i * D] = static_cast<uint8_t>(c);
+        keys[i * D + H] = static_cast<uint8_t>(c >> 8);
+      }
+    }
+  } else {
+    // Rows to positions: row i is position off + i.
+    float p[N][kScaleBlock];
+#pragma unroll
+    for (int z = 0; z < N; ++z)
+#pragma unroll
+      for (int j = 0; j < kScaleBlock; ++j) p[z][j] = x[z][0];
+    if (b.n > 1) {
+#pragma unroll
+      for (int j = 0; j < kScaleBlock; ++j)
+#pragma unroll
+        for (int i = 1; i < kScaleBlock; ++i)
+          if (j - b.off == i)
+#pragma unroll
+            for (int z = 0; z < N; ++z) p[z][j] = x[z][i];
+    }
+#pragma unroll
+    for (int z = 0; z < N; ++z) {
+      u32x4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t c = codes4<T>(p[z] + 4 * i, inv, ex);
+        y[i] = b.n < kScaleBlock ? merge4(c, grows ? moved4(old[z][i], ratio) : old[z][i], old[z][i], 4 * i, b.off, b.off + b.n) : c;
+      }
+      st_chunk(values + static_cast<int64_t>(z) * kWave * page, y);
+    }
+  }
+  if (lane == 0 && (b.off == 0 || grows)) *scale = static_cast<uint8_t>(ex + kScaleBias);
+}
+
+// Many rows.  Some workgroups have the cache blocks that begin in kWindow rows, for keys or for values of one head; a block is one workgroup's
+// alone, so its exponent and codes are changed without atomics.  Its 256 threads
+// share a block of 16 x D numbers, 8 (D 64: 4) each: with a wave a block, the
+// kernel's registers (136) left the q rows, which the other workgroups rotate, a
+// third of the waves (4075 rows 30 us).  Bound by bytes: those rows (94 MB) 23.9
+// us, 3.9 TB/s; both kinds of workgroup in turn 24.3 (4096 tokens of one prompt
+// 24.5, and 29.9).
+constexpr int kWindow = 16;
+template <class T, int D, bool AL>
+__global__ __launch_bounds__(256) void paged_write8_kernel(Write8Args args, int block_groups) {
   using raw = typename T::raw_t;
   const WriteArgs& a = args.w;
   const int page = 1 << a.page_shift;
-  const int64_t slots = static_cast<int64_t>(a.num_pages) << a.page_shift;
   if (static_cast<int>(blockIdx.x) >= block_groups) {
-    constexpr int U = D / 16;  // units a head
-    const int64_t id = (static_cast<int64_t>(blockIdx.x) - block_groups) * 256 + threadIdx.x;
-    const int per_row = a.heads * U;
-    const int r = static_cast<int>(id / per_row);
-    if (r >= a.rows) return;
-    const int u = static_cast<int>(id - static_cast<int64_t>(r) * per_row);
-    const int h = u / U;
-    const int e = (u - h * U) * 8;
-    float y0[8], y1[8];
-    rotate<T, D, 8, AL>(a, static_cast<const raw*>(a.q) + r * a.q_stride + h * D, r, e, y0, y1);
-    raw* to = static_cast<raw*>(a.q_out) + r * a.q_out_stride + h * D;
-    store_row_chunk<T, AL>(to + e, pack_chunk<T>(y0), 8);
-    store_row_chunk<T, AL>(to + e + D / 2, pack_chunk<T>(y1), 8);
+    rotate_q<T, D, AL>(a, (static_cast<int64_t>(blockIdx.x) - block_groups) * 256 + threadIdx.x);
     return;
   }
   __shared__ uint32_t tops[2][4];
   const bool is_v = (blockIdx.x & 1) != 0;
   const int wg = static_cast<int>(blockIdx.x) >> 1;
-  const int r0 = wg / a.kv_heads * window;
+  const int r0 = wg / a.kv_heads * kWindow;
   const int head = wg % a.kv_heads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // Lane l of every wave looks at row r0 - 1 + l.  Bits of lanes: rows that have
-  // a slot and are the first of their block here, rows that follow one in their block.
-  const int look = r0 - 1 + lane;
-  const int seen = lane < window + 16 && look >= 0 && look < a.rows ? a.slots[look] : -1;
-  const int before = __shfl_up(seen, 1, kWave);
-  const bool placed = seen >= 0 && seen < slots;
-  const bool follows = lane > 0 && placed && (seen & (kScaleBlock - 1)) != 0 && seen == before + 1;
-  const uint64_t inside = __ballot(follows);
-  const uint64_t mine = (((1ull << window) - 1) << 1);
+  const Blocks found = find_blocks(a, r0, kWindow);  // of every wave
   int turn = 0;
-  for (uint64_t todo = __ballot(placed && !follows) & mine; todo != 0; todo &= todo - 1, turn ^= 1) {
-    const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(todo));
-    const int slot = __builtin_amdgcn_readlane(seen, l);
-    const int n = 1 + __builtin_ctzll(~(inside >> (l + 1)));  // rows of the block, at most 16
-    const int row = r0 - 1 + l;
-    const int off = slot & (kScaleBlock - 1);
-    const int64_t id = slot >> a.page_shift;
-    const int in_page = slot & (page - 1) & ~(kScaleBlock - 1);
-    const int64_t at = ((id * a.kv_heads + head) << (a.page_shift - 4)) + (in_page >> 4);
-    uint8_t* scale = (is_v ? args.value_scales : args.key_scales) + at;
-    // A block's exponent counts where earlier rows are in it.
-    const int was = min(max(static_cast<int>(*scale) - kScaleBias, ScaleRange<T>::lo), ScaleRange<T>::hi);
+  for (uint64_t todo = found.first; todo != 0; todo &= todo - 1, turn ^= 1) {
+    const Block k = take_block(a, found, __builtin_amdgcn_readfirstlane(__builtin_ctzll(todo)), r0, head);
+    const int n = k.n, row = k.row, off = k.off, in_page = k.in_page;
+    const int64_t id = k.id;
+    uint8_t* scale = (is_v ? args.value_scales : args.key_scales) + k.at;
+    const int was = stored<T>(*scale);
     // The block's exponent from the threads' widest numbers.
     auto exponent = [&](uint32_t top) {
       top = wave_max(top);
@@ -277,18 +434,9 @@ __global__ __launch_bounds__(256) void paged_write8_kernel(Write8Args args, int 
       const float inv = pow2(-e);
       const bool grows = off > 0 && e > was;
       const float ratio = ldexpf(1.f, was - e);
-      // Positions before `off` are earlier rows, those behind the new ones stay as they are.
 #pragma unroll
-      for (int w = 0; w < P / 4; ++w) {
-        uint32_t early = 0, late = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          if (j0 + 4 * w + b < off) early |= 0xffu << (8 * b);
-          if (j0 + 4 * w + b >= off + n) late |= 0xffu << (8 * b);
-        }
-        const uint32_t kept = grows ? moved4(old[w], ratio) : old[w];
-        old[w] = (codes4<T>(x + 4 * w, inv, e) & ~(early | late)) | (kept & early) | (old[w] & late);
-      }
+      for (int w = 0; w < P / 4; ++w)
+        old[w] = merge4(codes4<T>(x + 4 * w, inv, e), grows ? moved4(old[w], ratio) : old[w], old[w], j0 + 4 * w, off, off + n);
       if constexpr (P == 8) *reinterpret_cast<uint2*>(values) = make_uint2(old[0], old[1]);
       else values[0] = old[0];
       if (threadIdx.x == 0 && (off == 0 || grows)) *scale = static_cast<uint8_t>(e + kScaleBias);
@@ -296,32 +444,35 @@ __global__ __launch_bounds__(256) void paged_write8_kernel(Write8Args args, int 
   }
 }
 
-// Rows whose blocks one workgroup looks after.
-constexpr int window_rows(int rows) { return rows < 512 ? 1 : 16; }
+// Calls of fewer rows take a wave a row: 256 decoding requests 7.7 us, 12.7 with
+// a workgroup a block; 64 of them 5.1 on the device.
+constexpr int kFewRows = 512;
 
-template <class T, int D>
-hipError_t launch_write8(const Write8Args& args, bool aligned, hipStream_t stream) {
+template <class T, int D, bool AL>
+hipError_t launch_write8(const Write8Args& args, hipStream_t stream) {
   const WriteArgs& a = args.w;
-  const int window = window_rows(a.rows);
-  const int64_t units = static_cast<int64_t>(a.rows) * a.heads * (D / 16);
-  const int64_t rot = (units + 255) / 256;
-  const int64_t blocks = (static_cast<int64_t>(a.rows) + window - 1) / window * a.kv_heads * 2;
+  const bool few = a.rows < kFewRows;
+  const int64_t rot = (static_cast<int64_t>(a.rows) * a.heads * (D / 16) + 255) / 256;
+  const int64_t blocks = few ? (static_cast<int64_t>(a.rows) * a.kv_heads * 2 + 3) / 4
+                             : (static_cast<int64_t>(a.rows) + kWindow - 1) / kWindow * a.kv_heads * 2;
   if (!grid_fits(rot + blocks)) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(rot + blocks));
-  if (aligned)
-    hipLaunchKernelGGL((paged_write8_kernel<T, D, true>), grid, dim3(256), 0, stream, args, static_cast<int>(blocks), window);
-  else
-    hipLaunchKernelGGL((paged_write8_kernel<T, D, false>), grid, dim3(256), 0, stream, args, static_cast<int>(blocks), window);
+  if (few) hipLaunchKernelGGL((paged_write8_few_kernel<T, D, AL>), grid, dim3(256), 0, stream, args, static_cast<int>(blocks));
+  else hipLaunchKernelGGL((paged_write8_kernel<T, D, AL>), grid, dim3(256), 0, stream, args, static_cast<int>(blocks));
   return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_write8_of(const Write8Args& a, int head_dim, bool aligned, hipStream_t stream) {
+  if (head_dim == 64) return aligned ? launch_write8<T, 64, true>(a, stream) : launch_write8<T, 64, false>(a, stream);
+  return aligned ? launch_write8<T, 128, true>(a, stream) : launch_write8<T, 128, false>(a, stream);
 }
 
 }  // namespace
 
 hipError_t launch_rotary_paged_write8(const Write8Args& a, int dtype, int head_dim, bool aligned, hipStream_t stream) {
   if (a.w.rows == 0) return hipSuccess;
-  if (dtype == MLORA_BF16)
-    return head_dim == 64 ? launch_write8<BF16, 64>(a, aligned, stream) : launch_write8<BF16, 128>(a, aligned, stream);
-  return head_dim == 64 ? launch_write8<F16, 64>(a, aligned, stream) : launch_write8<F16, 128>(a, aligned, stream);
+  return dtype == MLORA_BF16 ? launch_write8_of<BF16>(a, head_dim, aligned, stream) : launch_write8_of<F16>(a, head_dim, aligned, stream);
 }
 
 }  // namespace mlora
