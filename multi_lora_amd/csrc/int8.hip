@@ -67,10 +67,8 @@ __device__ __forceinline__ void load8(const typename T::raw_t* row, int e, int k
   }
 }
 
-// Rows from which on a workgroup has four of them.  Times in us: 300 rows of 4096
-// 3.5 with one each, 3.9 with four; 512 rows 4.8 and 4.2; 64 of 14336 3.8 and 7.4;
-// 2048 of 4096 6.7 with four, 8.7 with eight, 8192 of 1024 6.6 and 6.7; 1088 of
-// 14336 19.3 and 17.6.
+// Rows from which on a workgroup has more than one of them, where a row fits the
+// registers of its share of the waves.
 constexpr int kQuantMany = 400;
 constexpr int kFusedStep = 8 * 64 * 8;  // elements of one chunk a thread of the register form's workgroup
 
@@ -92,10 +90,10 @@ __device__ __forceinline__ uint32_t widest(const u32x4& v, uint32_t top) {
 }
 
 // R rows a workgroup (of one band); lane l has row l % R and chunks of 16
-// columns.  With four rows, four lanes write 64 bytes side by side, and a wave
-// reads 512 of each row.  KEEP chunks stay in registers, what a row has more of
+// columns.  With two rows, two lanes write 32 bytes side by side, and a wave
+// reads 1 KB of each row.  KEEP chunks stay in registers, what a row has more of
 // is read twice.  Bound by bytes, 2 in and 1 out an element, and nearly as much
-// by its arithmetic.
+// by its arithmetic: 4075 rows of 4096 13.8 us, 3.6 TB/s.
 template <class T, int R, int NW, int KEEP, bool AL>
 __global__ __launch_bounds__(NW * 64) void quantize_rows_kernel(QuantArgs a) {
   using raw = typename T::raw_t;
@@ -103,7 +101,15 @@ __global__ __launch_bounds__(NW * 64) void quantize_rows_kernel(QuantArgs a) {
   constexpr int STEP = NW * (64 / R) * 16;    // columns of all waves
   __shared__ uint32_t tops[NW][R];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = blockIdx.x * R + lane % R;
+  // Workgroups go to the eight XCDs in turn; those of a band take places of one
+  // XCD, whose L2 puts together the lines that they share.
+  constexpr int PER = 16 / R;
+  int id = blockIdx.x;
+  if (id < static_cast<int>(gridDim.x) / (8 * PER) * (8 * PER)) {
+    const int at = id >> 3;
+    id = (at / PER * 8 + (id & 7)) * PER + at % PER;
+  }
+  const int row = id * R + lane % R;
   const raw* x = static_cast<const raw*>(a.x) + static_cast<int64_t>(min(row, a.rows - 1)) * a.x_stride;
   const int padded = static_cast<int>(int8_padded(a.k));
   const int e0 = (wave * (64 / R) + lane / R) * 16;
@@ -376,8 +382,14 @@ hipError_t launch_quant(const QuantArgs& a, bool aligned, hipStream_t stream) {
 
 template <class T>
 hipError_t quant_of(const QuantArgs& a, bool aligned, hipStream_t stream) {
-  if (a.rows < kQuantMany) return a.k <= 4096 ? launch_quant<T, 1, 4, 1>(a, aligned, stream) : launch_quant<T, 1, 16, 1>(a, aligned, stream);
-  return a.k <= 1024 ? launch_quant<T, 4, 4, 1>(a, aligned, stream) : launch_quant<T, 4, 8, 2>(a, aligned, stream);
+  // Times in us: 1088 rows of 14336 15.8 with one row a workgroup, 17.3 with two,
+  // 18.5 with four; 2048 of 8192 17.2, 14.3 and 14.3; 4075 of 4096 17.1, 13.8 and
+  // 14.0; 450 of 4096 3.5, 3.3 and 4.1; 64 of 14336 3.9, 4.5 and 8.0; 600 of 1024
+  // 2.8, 3.1 and 2.8.
+  if (a.rows < kQuantMany || a.k > 8192)
+    return a.k <= 4096 ? launch_quant<T, 1, 4, 1>(a, aligned, stream) : launch_quant<T, 1, 16, 1>(a, aligned, stream);
+  if (a.k <= 1024) return launch_quant<T, 4, 4, 1>(a, aligned, stream);
+  return a.k <= 4096 ? launch_quant<T, 2, 8, 1>(a, aligned, stream) : launch_quant<T, 2, 8, 2>(a, aligned, stream);
 }
 
 }  // namespace

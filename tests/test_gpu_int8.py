@@ -197,3 +197,15 @@ def test_two_streams_at_once():
                 got[i].append(int8_linear(xs[i], w))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
+@pytest.mark.parametrize("m,k", [(399, 130), (400, 4096), (517, 4097), (1090, 300), (701, 9000), (1025, 1024)])
+def test_codes_of_many_rows(m, k):
+    x = activations(m, k, torch.bfloat16, m * k)
+    rows = quantize_rows(x.to(DEV))
+    codes, scales = codes_of(x)
+    assert torch.equal(rows.to_rows().cpu().double(), codes)
+    torch.testing.assert_close(rows.scales.cpu().double(), scales, rtol=2.0 ** -24, atol=0)
+    # Numbers with few bits: fp32 quotients are then those of the 16-bit type.
+    again = quantize_rows(x.float().to(DEV))
+    assert torch.equal(again.codes[:, :m // 16], rows.codes[:, :m // 16]) and torch.equal(again.scales, rows.scales)
