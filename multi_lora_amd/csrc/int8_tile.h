@@ -37,20 +37,18 @@ struct TileShared {
 };
 
 // Tile of workgroup `id` of `tiles_n * tiles_m`.  Workgroups go to the eight
-// XCDs in turn; each XCD gets a run of neighbouring tiles, in even bands of up
-// to 4 rows of tiles, so that its L2 holds what the tiles share.  (1088 rows
-// to 6144 columns, 9 rows of tiles: 32.3 us with 3, 3 and 3, 33.4 with 4, 4 and 1.)
+// XCDs in turn; each XCD gets a run of neighbouring tiles, in bands of 4 rows
+// of tiles, so that its L2 holds what the tiles share.
 __device__ __forceinline__ void pick_tile8(int id, int tiles_n, int tiles_m, int* tn, int* tm) {
   const int total = tiles_n * tiles_m;
   const int per = total >> 3, more = total & 7;
   const int xcd = id & 7, at = id >> 3;
   const int t = xcd * per + min(xcd, more) + at;
-  const int bands = (tiles_m + 3) >> 2, high = (tiles_m + bands - 1) / bands;
-  const int band = t / (high * tiles_n);
-  const int rows = min(high, tiles_m - band * high);
-  const int in = t - band * high * tiles_n;
+  const int band = t / (4 * tiles_n);
+  const int rows = min(4, tiles_m - band * 4);
+  const int in = t - band * 4 * tiles_n;
   *tn = in / rows;
-  *tm = band * high + in - *tn * rows;
+  *tm = band * 4 + in - *tn * rows;
 }
 
 // A tile over K, 128 bytes of each row a step: blocks are loaded straight into
