@@ -543,7 +543,7 @@ int mlora_paged_attention_fp8(const void* q, int64_t q_row_stride, const void* k
  * products are the model's own. */
 
 /* Rows x [rows, k] (F16, BF16 or F32) to codes (of stride 1 KB times the blocks
- * of rows) and scales; k at most 2^17. */
+ * of rows) and scales; k below 2^17. */
 int mlora_quantize_rows(const void* x, int64_t x_row_stride, int32_t rows, int32_t k, int8_t* codes, float* scales,
                         int32_t dtype, void* stream);
 

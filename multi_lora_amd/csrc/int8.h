@@ -18,8 +18,9 @@ __host__ __device__ constexpr int64_t int8_padded(int64_t k) { return (k + kInt8
 __host__ __device__ constexpr int64_t int8_bands(int64_t rows) { return (rows + 15) / 16; }
 constexpr int64_t int8_bytes(int64_t rows, int64_t k) { return int8_bands(rows) * 16 * int8_padded(k); }
 
-// 127^2 * 2^17 < 2^31: sums of this many products fit 32 bits.
-constexpr int kInt8MaxK = 1 << 17;
+// 128^2 * (2^17 - 1) < 2^31: sums of this many products fit 32 bits (codes
+// quantised elsewhere may be -128).
+constexpr int kInt8MaxK = (1 << 17) - 1;
 
 struct QuantArgs {
   const void* x;

@@ -29,7 +29,7 @@ from .paged import _DTYPES, _guard, _no_grad, _no_tangent, _on_gpu, _untraced, _
 
 PAD = 128        # columns of codes come in multiples of it
 BAND = 16        # rows, too
-MAX_K = 1 << 17  # longer sums of products could leave 32 bits
+MAX_K = (1 << 17) - 1  # longer sums of products could leave 32 bits
 
 
 def _code_shape(rows: int, k: int):

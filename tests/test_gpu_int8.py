@@ -209,3 +209,12 @@ def test_codes_of_many_rows(m, k):
     # Numbers with few bits: fp32 quotients are then those of the 16-bit type.
     again = quantize_rows(x.float().to(DEV))
     assert torch.equal(again.codes[:, :m // 16], rows.codes[:, :m // 16]) and torch.equal(again.scales, rows.scales)
+
+
+@pytest.mark.parametrize("m", [1, 20, 600])
+def test_the_longest_sums(m):
+    """Codes of -128 throughout: the sum is the largest that 32 bits hold but 16383."""
+    k, n = (1 << 17) - 1, 4100 if m == 600 else 5
+    a = Int8Rows.from_codes(torch.full((m, k), -128, dtype=torch.int8, device=DEV), torch.full((m,), 2.0 ** -31, device=DEV))
+    b = Int8Rows.from_codes(torch.full((n, k), -128, dtype=torch.int8, device=DEV), torch.ones(n, device=DEV))
+    assert torch.equal(int8_matmul(a, b, torch.float16), torch.ones(m, n, dtype=torch.float16, device=DEV))

@@ -5,6 +5,7 @@ import torch
 
 from multi_lora_amd import _ffi
 from multi_lora_amd.kernels import Int8Rows, int8_linear, int8_matmul, quantize_rows
+from multi_lora_amd.kernels.int8 import MAX_K
 
 
 def rows(n=4, k=7):
@@ -86,3 +87,14 @@ def test_c_entry_points_check_before_anything_is_read():
     assert lin(m=0) == 0
     assert lib.mlora_int8_linear_workspace_bytes(100, 64) == 112 * 128 + 100 * 4
     assert lib.mlora_int8_linear_workspace_bytes(2, 4096) == 0 == lib.mlora_int8_linear_workspace_bytes(0, 64)
+
+
+def test_sums_fit_32_bits():
+    """The longest rows, every code -128 in both: one element more would wrap."""
+    assert 128 * 128 * MAX_K < 2 ** 31 <= 128 * 128 * (MAX_K + 1)
+    with pytest.raises(ValueError):
+        Int8Rows.from_codes(torch.full((2, 1 << 17), -128, dtype=torch.int8), torch.ones(2))
+    lib = _ffi.lib()
+    p = 0x10000
+    stride = (1 << 17) * 16
+    assert lib.mlora_int8_matmul(p, stride, p, 1, p, stride, p, 1, 1 << 17, None, p, 1, _ffi.MLORA_BF16, None) == -2
