@@ -98,7 +98,10 @@ class Int8Linear(nn.Module):
 
     @property
     def weight(self) -> Int8Rows:
-        return self._weight
+        w = self._weight
+        if w.codes is not self.codes or w.scales is not self.scales:  # buffers replaced (a state dict assigned)
+            w = self._weight = Int8Rows(self.codes, self.scales, self.in_features)
+        return w
 
     @weight.setter
     def weight(self, weight: Int8Rows) -> None:
@@ -111,11 +114,10 @@ class Int8Linear(nn.Module):
         super()._apply(fn, recurse)
         if self.scales.dtype != scales.dtype:  # a change of the model's type is not one of the scales'
             self.scales = scales.to(self.scales.device)
-        self._weight = Int8Rows(self.codes, self.scales, self.in_features)
         return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        y = int8_linear(x.reshape(-1, self.in_features), self._weight, self.bias)
+        y = int8_linear(x.reshape(-1, self.in_features), self.weight, self.bias)
         return y.view(*x.shape[:-1], self.out_features)
 
     def extra_repr(self) -> str:

@@ -1,11 +1,14 @@
 """8-bit products: layouts, refusals and the C entry points' checks (no GPU call is made)."""
 
+import copy
+
 import pytest
 import torch
 
 from multi_lora_amd import _ffi
 from multi_lora_amd.kernels import Int8Rows, int8_linear, int8_matmul, quantize_rows
 from multi_lora_amd.kernels.int8 import MAX_K
+from multi_lora_amd.layers import Int8Linear
 
 
 def rows(n=4, k=7):
@@ -98,3 +101,16 @@ def test_sums_fit_32_bits():
     p = 0x10000
     stride = (1 << 17) * 16
     assert lib.mlora_int8_matmul(p, stride, p, 1, p, stride, p, 1, 1 << 17, None, p, 1, _ffi.MLORA_BF16, None) == -2
+
+
+def test_the_module_follows_its_buffers():
+    """A state dict that is assigned, not copied, and a move: the weight is what the buffers hold."""
+    layer, other = (Int8Linear(Int8Rows.from_codes(torch.full((20, 7), c, dtype=torch.int8), torch.full((20,), float(c)))) for c in (1, 2))
+    layer.load_state_dict(other.state_dict(), assign=True)
+    assert torch.equal(layer.weight.dequantize(), torch.full((20, 7), 4.0))
+    assert layer.weight.codes is layer.codes
+    layer = layer.bfloat16()
+    assert layer.weight.scales.dtype == torch.float32 and torch.equal(layer.weight.dequantize(), torch.full((20, 7), 4.0))
+    copied = copy.deepcopy(layer)
+    copied.codes.zero_()
+    assert not copied.weight.dequantize().any() and layer.weight.dequantize().all()
