@@ -237,6 +237,8 @@ def quantize_base(model: nn.Module, skip: Sequence[str] = ("lm_head",)) -> int:
     last name is in ``skip`` stay, and so does what is not a float16 or
     bfloat16 layer.  Call it before projections are fused; adapters may be
     registered and layers wrapped before or after."""
+    if type(model) is nn.Linear:
+        raise ValueError("a layer cannot replace itself: Int8Linear.from_linear")
     count = 0
     for name, module in list(model.named_modules()):
         if isinstance(module, LinearWithLoRA) and module.qkv_group is not None:

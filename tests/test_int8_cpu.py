@@ -8,7 +8,7 @@ import torch
 from multi_lora_amd import _ffi
 from multi_lora_amd.kernels import Int8Rows, int8_linear, int8_matmul, quantize_rows
 from multi_lora_amd.kernels.int8 import MAX_K
-from multi_lora_amd.layers import Int8Linear
+from multi_lora_amd.layers import Int8Linear, quantize_base
 
 
 def rows(n=4, k=7):
@@ -114,3 +114,8 @@ def test_the_module_follows_its_buffers():
     copied = copy.deepcopy(layer)
     copied.codes.zero_()
     assert not copied.weight.dequantize().any() and layer.weight.dequantize().all()
+
+
+def test_a_layer_alone_is_not_a_model():
+    with pytest.raises(ValueError, match="from_linear"):
+        quantize_base(torch.nn.Linear(4, 4).bfloat16())
