@@ -185,7 +185,9 @@ __device__ __forceinline__ void store4(const Int8Args& a, int m, int n, const i3
 // operands, and add their sums in LDS: no barrier while weights stream.
 // KEEP: the rows themselves (of at most KEEP chunks of eight elements a thread)
 // are read and quantised by every workgroup, while its first blocks are on
-// their way.
+// their way.  Bound by the weight's bytes: 64 rows to 28672 columns, K 4096
+// (117 MB), 27.6 us, 4.3 TB/s; one row to 4096 columns 5.9, of which the bytes
+// need 3.3 and a launch's chain the rest.
 template <class T, int MT, int NT, int NW, int U, int KEEP>
 __global__ __launch_bounds__(NW * 64) void int8_rows_kernel(Int8Args a) {
   using raw = typename T::raw_t;

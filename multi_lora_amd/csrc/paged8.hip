@@ -336,8 +336,8 @@ __global__ __launch_bounds__(256, 4) void paged_write8_few_kernel(Write8Args arg
   if (lane == 0 && (b.off == 0 || grows)) *scale = static_cast<uint8_t>(ex + kScaleBias);
 }
 
-// Many rows.  Some workgroups have the cache blocks that begin in kWindow rows, for keys or for values of one head; a block is one workgroup's
-// alone, so its exponent and codes are changed without atomics.  Its 256 threads
+// Many rows.  Some workgroups have the cache blocks that begin in kWindow rows,
+// for keys or for values of one head; a block is one workgroup's alone, so its exponent and codes are changed without atomics.  Its 256 threads
 // share a block of 16 x D numbers, 8 (D 64: 4) each: with a wave a block, the
 // kernel's registers (136) left the q rows, which the other workgroups rotate, a
 // third of the waves (4075 rows 30 us).  Bound by bytes: those rows (94 MB) 23.9
