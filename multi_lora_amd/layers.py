@@ -79,6 +79,14 @@ class LinearWithLoRA(nn.Module):
         return y_flat.reshape(y_base.shape)
 
 
+def _packed(x: torch.Tensor) -> torch.Tensor:
+    """``x [..., k]`` as rows that lie apart, each contiguous: what the kernels take (copied only if it is not)."""
+    rows = x.reshape(-1, x.shape[-1])
+    if rows.stride(1) != 1 or rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]:
+        rows = rows.clone(memory_format=torch.contiguous_format)
+    return rows
+
+
 class Int8Linear(nn.Module):
     """``y = x @ weight.T + bias`` for 16-bit ``x``, with the weight in 8-bit
     integers and a scale for each output channel, and x's rows quantised at
@@ -117,7 +125,7 @@ class Int8Linear(nn.Module):
         return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        y = int8_linear(x.reshape(-1, self.in_features), self.weight, self.bias)
+        y = int8_linear(_packed(x), self.weight, self.bias)
         return y.view(*x.shape[:-1], self.out_features)
 
     def extra_repr(self) -> str:
@@ -170,7 +178,7 @@ class QKVProjGroup:
 
     def _base(self, x: torch.Tensor) -> torch.Tensor:
         if isinstance(self.weight, Int8Rows):
-            return int8_linear(x.reshape(-1, x.shape[-1]), self.weight).view(*x.shape[:-1], self.weight.shape[0])
+            return int8_linear(_packed(x), self.weight).view(*x.shape[:-1], self.weight.shape[0])
         return F.linear(x, self.weight)
 
     def forward(self, wrapper: LinearWithLoRA, x: torch.Tensor) -> torch.Tensor:

@@ -215,3 +215,17 @@ def test_what_is_replaced(dev):
     assert isinstance(model["a"], Int8Linear) and isinstance(model["c"].base_layer, Int8Linear)
     assert type(model["lm_head"]) is nn.Linear and type(model["b"]) is nn.Linear  # float32 stays
     assert quantize_base(model, skip=()) == 1
+
+
+def test_inputs_of_any_layout(dev):
+    """What nn.Linear takes: expanded rows, transposed ones, an empty batch."""
+    g = torch.Generator("cpu").manual_seed(5)
+    layer = Int8Linear.from_linear(nn.Linear(40, 17, device=dev, dtype=torch.bfloat16))
+    x = torch.randn(6, 40, generator=g).bfloat16().to(dev)
+    with torch.no_grad():
+        y = layer(x)
+        assert torch.equal(layer(x[:1].expand(5, 40)), y[:1].expand(5, 17))
+        assert torch.equal(layer(x[0].expand(2, 3, 40)), y[0].expand(2, 3, 17))
+        assert torch.equal(layer(x.t().contiguous().t()), y)
+        assert torch.equal(layer(x[0]), y[0])
+        assert layer(x[:0]).shape == (0, 17) and layer(x.view(2, 3, 40)[:, :0]).shape == (2, 0, 17)
