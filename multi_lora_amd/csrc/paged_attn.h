@@ -418,7 +418,12 @@ __device__ __forceinline__ void stream8_item(const PagedAttnArgs& a, StreamLds<D
   const uint8_t* keys = static_cast<const uint8_t*>(a.keys) + static_cast<int64_t>(head) * page * D;
   const uint8_t* values = static_cast<const uint8_t*>(a.values) + static_cast<int64_t>(head) * page * D;
 
-  u32x4 qf[MT][2 * KJ];
+  // q as operands; of two tiles in LDS, where it costs no registers: five tokens
+  // for each of 32 requests 17.8 us against 20.4 with 15 of them spilled, for
+  // each of 64 of 200 to 3985 positions 50.2 against 71.5.
+  constexpr bool QL = MT > 1 && D == 128;
+  __shared__ u32x4 q_lds[QL ? MT * 2 * KJ * kWave : 1];
+  u32x4 qf[QL ? 1 : MT][2 * KJ];
   int lim[MT];  // this lane's row sees positions [0, lim)
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
@@ -426,8 +431,12 @@ __device__ __forceinline__ void stream8_item(const PagedAttnArgs& a, StreamLds<D
     lim[t] = past + m / a.rep + 1;
     const raw* q = static_cast<const raw*>(a.q) + row_offset(a, it, head, m, a.q_stride, D);
 #pragma unroll
-    for (int k = 0; k < 2 * KJ; ++k) qf[t][k] = ld_chunk(q + (k >> 1) * 64 + g * 16 + (k & 1) * 8);
+    for (int k = 0; k < 2 * KJ; ++k) {
+      if constexpr (!QL) qf[t][k] = ld_chunk(q + (k >> 1) * 64 + g * 16 + (k & 1) * 8);
+      else if ((t * 2 * KJ + k) % NW == wave) q_lds[(t * 2 * KJ + k) * kWave + lane] = ld_chunk(q + (k >> 1) * 64 + g * 16 + (k & 1) * 8);
+    }
   }
+  if constexpr (QL) lds_barrier();
   const int open = past + row0 / a.rep + 1;  // every row of the tile sees [0, open)
 
   f32x4 acc[MT][DT];
@@ -494,15 +503,23 @@ __device__ __forceinline__ void stream8_item(const PagedAttnArgs& a, StreamLds<D
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int z = 0; z < 4; ++z) sc[t][z] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const u32x4* ql = q_lds + lane + (QL ? opaque_zero() : 0);
 #pragma unroll
-    for (int z = 0; z < 4; ++z)
+    for (int k = 0; k < 2 * KJ; ++k) {
+      u32x4 qk[MT];
 #pragma unroll
-      for (int k = 0; k < 2 * KJ; ++k) {
+      for (int t = 0; t < MT; ++t) {
+        if constexpr (QL) qk[t] = ql[(t * 2 * KJ + k) * kWave];
+        else qk[t] = qf[t][k];
+      }
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
         const u32x4 w = kf[z][k >> 1];
         const u32x4 key = (k & 1) ? widen8<T>(w[2], w[3], kscale) : widen8<T>(w[0], w[1], kscale);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) sc[t][z] = T::mma(sc[t][z], key, qf[t][k]);
+        for (int t = 0; t < MT; ++t) sc[t][z] = T::mma(sc[t][z], key, qk[t]);
       }
+    }
     if (more) load_keys(base + NW * kPos8, kid);
     kid = page_of(base + 2 * NW * kPos8 + kblock * 16);
     const bool masked = base + kPos8 > min(open, kv1);  // wave-uniform
@@ -544,9 +561,9 @@ __device__ __forceinline__ void stream8_item(const PagedAttnArgs& a, StreamLds<D
       for (int i = 0; i < 8; ++i) pf[t][i >> 2][i & 3] = T::pack2(p[2 * i], p[2 * i + 1]);
     }
     // Nothing of the hidden positions' handling between the products where none
-    // is hidden: 64 requests of 200 to 3985 positions 39.1 us against 40.8.  (For
-    // two tiles the second copy costs registers, 83 spills: five tokens for each
-    // of 32 requests 29.9 us against 20.4.)
+    // is hidden: 64 requests of 200 to 3985 positions 39.1 us against 40.8 with
+    // the handling done always, 39.4 with branches around it.  Two tiles have no
+    // registers for a second copy (121 spills) and take the branches.
     if (MT == 1 && !masked) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
@@ -563,16 +580,19 @@ __device__ __forceinline__ void stream8_item(const PagedAttnArgs& a, StreamLds<D
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const u32x4 all[2] = {widen8<T>(vf[d][0], vf[d][1], vscale), widen8<T>(vf[d][2], vf[d][3], vscale)};
-        u32x4 v[2];
+        u32x4 v[2] = {all[0], all[1]};
         bool odd = false;  // a value is not finite
+        if (masked) {
+          asm volatile("");  // (as above)
 #pragma unroll
-        for (int z = 0; z < 2; ++z)
+          for (int z = 0; z < 2; ++z)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t nf = MT == 1 || masked ? nonfinite_mask<T>(all[z][i]) : 0;
-            v[z][i] = all[z][i] & ~nf;
-            odd |= nf != 0;
-          }
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t nf = nonfinite_mask<T>(all[z][i]);
+              v[z][i] = all[z][i] & ~nf;
+              odd |= nf != 0;
+            }
+        }
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
 #pragma unroll
@@ -580,7 +600,7 @@ __device__ __forceinline__ void stream8_item(const PagedAttnArgs& a, StreamLds<D
 #pragma unroll
           for (int z = 0; z < 2; ++z) acc[t][d] = T::mma(acc[t][d], v[z], pf[t][z]);
         }
-        if (__ballot(odd) == 0) continue;
+        if (!masked || __ballot(odd) == 0) continue;
         // The values left out: one position's at a time, for the rows that see it.
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
