@@ -335,15 +335,9 @@ __device__ __forceinline__ void stream_item(const PagedAttnArgs& a, StreamLds<D,
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         p[i] = sc[t][i >> 2][i & 3] * a.scale_log2;
+        if (masked && i >= seen) p[i] = -INFINITY;
+        top = fmaxf(top, p[i]);
       }
-      if (masked) {
-        asm volatile("");  // (stays a branch)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (i >= seen) p[i] = -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, p[i]);
       bad[t] |= missing && seen > 0;
       top = fmaxf(top, __shfl_xor(top, 16, kWave));
       top = fmaxf(top, __shfl_xor(top, 32, kWave));
