@@ -23,7 +23,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .backend.base import LoRABackend
-from .kernels.int8 import Int8Rows, int8_linear, quantize_rows
+from .kernels.int8 import BAND, Int8Rows, int8_linear, quantize_rows
 
 # Process-wide switch: when off, wrapped layers return the base output only.
 LORA_ENABLED = True
@@ -132,6 +132,15 @@ class Int8Linear(nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
 
 
+def _in_bands(parts: Sequence[Int8Rows]) -> Int8Rows:
+    """Their rows one after the other, each part in whole bands of its own, so that a part's blocks hold no other's rows:
+    rows behind a part's last, up to a multiple of 16, have a scale of 0 (and products that nobody looks at)."""
+    if len({p.k for p in parts}) != 1:
+        raise ValueError(f"rows of different lengths {[p.k for p in parts]}")
+    scales = torch.cat([F.pad(p.scales, (0, -p.shape[0] % BAND)) for p in parts])
+    return Int8Rows(torch.cat([p.codes for p in parts], 1), scales, parts[0].k)
+
+
 class QKVProjGroup:
     """One base GEMM and one multi-slice LoRA call for sibling projections
     that read the same input: q/k/v of an attention block
@@ -150,18 +159,19 @@ class QKVProjGroup:
         quantised = {isinstance(w.base_layer, Int8Linear) for w in wrappers}
         if len(quantised) != 1:
             raise RuntimeError("fusion of 8-bit and 16-bit projections")
+        # Where each projection's columns begin: one after the other, 8-bit ones in bands of rows of their own.
+        step = BAND if quantised == {True} else 1
         self.weight: Union[torch.Tensor, Int8Rows] = (
-            Int8Rows.cat([w.base_layer.weight for w in wrappers]) if quantised == {True}
+            _in_bands([w.base_layer.weight for w in wrappers]) if quantised == {True}
             else torch.cat([w.base_layer.weight.detach() for w in wrappers], dim=0))
         col = 0
         for w, width in zip(wrappers, widths):
-            # Each layer's weight becomes a view of the fused weight: no extra memory (8-bit rows: where it begins at a
-            # multiple of 16).
+            # Each layer's weight becomes a view of the fused weight: no extra memory.
             w.base_layer.weight = (self.weight.rows(col, col + width) if quantised == {True}
                                    else nn.Parameter(self.weight[col : col + width], requires_grad=False))
             w.qkv_slice = (col, col + width)
             w.qkv_group = self
-            col += width
+            col += -(-width // step) * step
         self._cached_x: Optional[torch.Tensor] = None
         self._cached_out: Optional[torch.Tensor] = None
         self._delta_done = False

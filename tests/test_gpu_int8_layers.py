@@ -1,0 +1,31 @@
+"""8-bit projections as a model has them (GPU)."""
+
+import pytest
+import torch
+
+from multi_lora_amd.layers import fuse_gate_up_projections, fuse_qkv_projections
+
+from tests.int8_ref import check, codes_of, product
+from tests.test_int8_layers_cpu import states, wrappers
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("rows", [1, 5, 70, 700])
+@pytest.mark.parametrize("widths", [(20, 24, 8), (37, 37), (160, 1, 33)])
+@torch.inference_mode()
+def test_groups_of_odd_widths(dev, widths, rows):
+    """A fused group's columns are its layers' results, bit for bit, also after a state dict has been loaded."""
+    k = 200
+    ws = {n: w.to(dev) for n, w in wrappers(widths, k, 0).items()}
+    (fuse_qkv_projections if len(widths) == 3 else fuse_gate_up_projections)(ws, all_shapes=True)
+    x = torch.randn(rows, 1, k, generator=torch.Generator().manual_seed(rows)).bfloat16().to(dev)
+    for seed in (0, 50):
+        for n, state in states(wrappers(widths, k, seed)).items():
+            ws[n].load_state_dict(state)
+        x = x + 1
+        for n, w in ws.items():
+            got = w(x)
+            assert got.shape == (rows, 1, w.base_layer.out_features) and torch.equal(got, w.base_layer(x))
+            want = w.base_layer.weight
+            check(got[:, 0], *product(*codes_of(x[:, 0]), want.to_rows().cpu(), want.scales.cpu()))
