@@ -195,7 +195,7 @@ class QKVProjGroup:
         if x.shape[-2] != 1 and not self.all_shapes:
             return wrapper.add_delta(x, wrapper.base_layer(x))
         if self._cached_x is not x:
-            self._cached_x = x
+            self._cached_x = None  # if this call raises, the next one computes
             self._cached_out = self._base(x)
             self._delta_done = False
             if self._multi_ready():
@@ -210,6 +210,7 @@ class QKVProjGroup:
                     [w.qkv_slice[0] for w in self.wrappers],
                 )
                 self._delta_done = True
+            self._cached_x = x
         start, end = wrapper.qkv_slice
         y = self._cached_out[..., start:end]
         if self._delta_done:
