@@ -155,27 +155,43 @@ class QKVProjGroup:
         if any(w.base_layer.bias is not None for w in wrappers):
             raise RuntimeError("QKV fusion requires bias=None")
         self.wrappers = list(wrappers)
-        widths = [int(w.base_layer.weight.shape[0]) for w in wrappers]
         quantised = {isinstance(w.base_layer, Int8Linear) for w in wrappers}
         if len(quantised) != 1:
             raise RuntimeError("fusion of 8-bit and 16-bit projections")
-        # Where each projection's columns begin: one after the other, 8-bit ones in bands of rows of their own.
-        step = BAND if quantised == {True} else 1
-        self.weight: Union[torch.Tensor, Int8Rows] = (
-            _in_bands([w.base_layer.weight for w in wrappers]) if quantised == {True}
-            else torch.cat([w.base_layer.weight.detach() for w in wrappers], dim=0))
-        col = 0
-        for w, width in zip(wrappers, widths):
-            # Each layer's weight becomes a view of the fused weight: no extra memory.
-            w.base_layer.weight = (self.weight.rows(col, col + width) if quantised == {True}
-                                   else nn.Parameter(self.weight[col : col + width], requires_grad=False))
-            w.qkv_slice = (col, col + width)
+        self._parts: List[tuple] = []  # 8-bit: codes and scales of each layer, views of the fused weight's
+        self._join()
+        for w in wrappers:
             w.qkv_group = self
-            col += -(-width // step) * step
         self._cached_x: Optional[torch.Tensor] = None
         self._cached_out: Optional[torch.Tensor] = None
         self._delta_done = False
         self.all_shapes = all_shapes
+
+    def _join(self) -> None:
+        """The fused weight; each layer's becomes a view of it: no extra memory."""
+        layers = [w.base_layer for w in self.wrappers]
+        eight = isinstance(layers[0], Int8Linear)
+        # Where a projection's columns begin: one after the other, 8-bit ones in bands of rows of their own.
+        step = BAND if eight else 1
+        self.weight: Union[torch.Tensor, Int8Rows] = (
+            _in_bands([m.weight for m in layers]) if eight else torch.cat([m.weight.detach() for m in layers], dim=0))
+        col = 0
+        for w, m in zip(self.wrappers, layers):
+            width = int(m.weight.shape[0])
+            m.weight = (self.weight.rows(col, col + width) if eight
+                        else nn.Parameter(self.weight[col : col + width], requires_grad=False))
+            w.qkv_slice = (col, col + width)
+            col += -(-width // step) * step
+        if eight:
+            self._parts = [(m.codes, m.scales) for m in layers]
+
+    def _follow(self) -> None:
+        """8-bit: the fused weight again, where a layer's buffers were replaced (a state dict assigned, a move)."""
+        for w, (codes, scales) in zip(self.wrappers, self._parts):
+            held = w.base_layer._buffers
+            if held["codes"] is not codes or held["scales"] is not scales:
+                with torch.inference_mode(False):
+                    return self._join()
 
     def _multi_ready(self) -> bool:
         first = self.wrappers[0]
@@ -188,6 +204,7 @@ class QKVProjGroup:
 
     def _base(self, x: torch.Tensor) -> torch.Tensor:
         if isinstance(self.weight, Int8Rows):
+            self._follow()
             return int8_linear(_packed(x), self.weight).view(*x.shape[:-1], self.weight.shape[0])
         return F.linear(x, self.weight)
 

@@ -29,3 +29,19 @@ def test_groups_of_odd_widths(dev, widths, rows):
             assert got.shape == (rows, 1, w.base_layer.out_features) and torch.equal(got, w.base_layer(x))
             want = w.base_layer.weight
             check(got[:, 0], *product(*codes_of(x[:, 0]), want.to_rows().cpu(), want.scales.cpu()))
+
+
+@torch.inference_mode()
+def test_groups_whose_layers_are_moved_or_replaced(dev):
+    k, widths = 96, (48, 20, 16)
+    ws = wrappers(widths, k, 0)
+    fuse_qkv_projections(ws)  # on the CPU
+    for w in ws.values():
+        w.to(dev)
+    x = torch.randn(6, 1, k, generator=torch.Generator().manual_seed(1)).bfloat16().to(dev)
+    for seed in (None, 50):
+        if seed is not None:
+            ws["layer.v_proj"].load_state_dict(wrappers(widths, k, seed)["layer.v_proj"].to(dev).state_dict(), assign=True)
+        x = x * 2
+        for w in ws.values():
+            assert torch.equal(w(x), w.base_layer(x))

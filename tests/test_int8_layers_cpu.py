@@ -64,3 +64,26 @@ def test_a_fused_group_holds_what_its_layers_load(widths):
     check(again, widths, k, 50)
     assert sum(w.base_layer.codes.untyped_storage().data_ptr() == w.qkv_group.weight.codes.untyped_storage().data_ptr()
                for w in again.values()) == len(widths)  # no second copy of a weight
+
+
+@pytest.mark.parametrize("widths", [(32, 16, 48), (20, 24, 8)])
+def test_a_fused_group_follows_buffers_that_are_replaced(widths):
+    """A state dict that is assigned, not copied, and layers that are given other weights: one of them, then all."""
+    k = 70
+    ws = fused(widths, k, 0)
+    x = torch.zeros(1, 1, k)
+    one = wrappers(widths, k, 50)["layer.k_proj"]
+    ws["layer.k_proj"].load_state_dict(one.state_dict(), assign=True)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        ws["layer.q_proj"](x)  # (the fused product's weight is looked at before the refusal)
+    group = ws["layer.q_proj"].qkv_group
+    for i, (w, n) in enumerate(zip(ws.values(), widths)):
+        want = rows(n, k, i + (50 if i == 1 else 0))
+        start, end = w.qkv_slice
+        assert torch.equal(group.weight.to_rows()[start:end], want.to_rows()), f"projection {i}"
+        assert torch.equal(group.weight.scales[start:end], want.scales) and torch.equal(w.base_layer.weight.to_rows(), want.to_rows())
+    for i, (w, n) in enumerate(zip(ws.values(), widths)):
+        w.base_layer.weight = rows(n, k, 90 + i)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        ws["layer.q_proj"](x)
+    check(ws, widths, k, 90)
