@@ -131,6 +131,7 @@ int int8_args(int32_t m, const int8_t* codes, int64_t stride, const float* scale
   a->bias = bias;
   a->out = out, a->out_stride = out_row_stride;
   a->vec = (reinterpret_cast<uintptr_t>(out) & 7u) == 0 && out_row_stride % 4 == 0;
+  a->wide = al16(out) && out_row_stride % 8 == 0;
   return 0;
 }
 

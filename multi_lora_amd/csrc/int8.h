@@ -51,6 +51,7 @@ struct Int8Args {
   void* out;
   int64_t out_stride;
   int vec;            // four outputs of a row can be stored at once
+  int wide;           // eight can
 };
 // Whether a call of 16-bit rows is quantised inside the product's own launch.
 bool int8_fused(int m, int k);

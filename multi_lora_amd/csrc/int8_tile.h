@@ -180,8 +180,14 @@ __global__ __launch_bounds__(Sh::NW * 64) void int8_tile_kernel(Int8Args a, int 
     if (m0 + m >= a.m || n >= a.n) continue;
     const u32x4 v = *reinterpret_cast<const u32x4*>(s.stage + m * Sh::PITCH + c * 16);
     raw* out = static_cast<raw*>(a.out) + static_cast<int64_t>(m0 + m) * a.out_stride + n;
-    if (a.vec) store_row_chunk<T, true>(out, v, a.n - n);
-    else store_row_chunk<T, false>(out, v, a.n - n);
+    if (a.wide) {
+      store_row_chunk<T, true>(out, v, a.n - n);
+    } else if (a.vec && n + 8 <= a.n) {  // rows that begin at multiples of 8 bytes only
+      *reinterpret_cast<uint2*>(out) = make_uint2(v[0], v[1]);
+      *reinterpret_cast<uint2*>(out + 4) = make_uint2(v[2], v[3]);
+    } else {
+      store_row_chunk<T, false>(out, v, a.n - n);
+    }
   }
 }
 
