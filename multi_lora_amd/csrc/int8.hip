@@ -167,7 +167,7 @@ __device__ __forceinline__ void store4(const Int8Args& a, int m, int n, const i3
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = min(n + i, a.n - 1);
-    y[i] = static_cast<float>(sum[i]) * a.b_scales[c] * as;
+    y[i] = scaled(sum[i], as, a.b_scales[c]);
     if (a.bias != nullptr) y[i] += T::to_f32(static_cast<const raw*>(a.bias)[c]);
   }
   raw* out = static_cast<raw*>(a.out) + m * a.out_stride + n;

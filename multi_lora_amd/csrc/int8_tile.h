@@ -13,6 +13,13 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(1))) void gvoid_t;
 typedef __attribute__((address_space(3))) void lvoid_t;
 
+// sum * a * b, the smaller scale first: the first product then leaves fp32 only
+// where the result does (scales go from 2^-107 to 2^121).  NaN stays.
+__device__ __forceinline__ float scaled(int32_t sum, float a, float b) {
+  const bool less = a < b;
+  return static_cast<float>(sum) * (less ? a : b) * (less ? b : a);
+}
+
 // A tile's shape: TN weight rows by TM rows, waves WN by WM, S steps in LDS.  A
 // step is two blocks (2 KB) of each band.
 template <int TN_, int TM_, int WN_, int WM_, int S_>
@@ -166,7 +173,7 @@ __global__ __launch_bounds__(Sh::NW * 64) void int8_tile_kernel(Int8Args a, int 
       float y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        y[e] = static_cast<float>(acc[i][j][e]) * bs[e] * as;
+        y[e] = scaled(acc[i][j][e], as, bs[e]);
         if (a.bias != nullptr) y[e] += bias[e];
       }
       *reinterpret_cast<uint2*>(s.stage + m * Sh::PITCH + n * 2) = make_uint2(T::pack2(y[0], y[1]), T::pack2(y[2], y[3]));

@@ -28,3 +28,24 @@ def test_columns_of_wider_tensors(dev, m, n, dtype):
             int8_linear(x, w, out=buf[:, col:col + n])
             assert torch.equal(buf[:, col:col + n], first)
             assert bool((buf[:, :col] == 7).all()) and bool((buf[:, col + n:] == 7).all())
+
+
+@pytest.mark.parametrize("m,n", [(1, 40), (5, 33), (40, 50), (520, 4100)])
+def test_scales_far_apart(dev, m, n):
+    """Rows and channels whose scales lie at either end of the type's range, with products in the middle of it: no partial
+    product leaves fp32.  Channels of zeros and rows of zeros stay 0."""
+    k = 200
+    x = activations(m, k, torch.bfloat16, 3)
+    codes, scales = weight(n, k, 4)
+    scales = scales / 0.01  # up to 1
+    for ex, ew in ((-95, 118), (118, -95), (-60, 110), (0, 118), (118, 0)):
+        xs = (x.double() * 2.0 ** ex).to(torch.bfloat16)
+        ws = scales * 2.0 ** ew
+        zero = codes.clone()
+        zero[0] = 0
+        w = Int8Rows.from_codes(zero.to(dev), ws.to(dev))
+        want, slack = product(*codes_of(xs), zero, ws)
+        end = want.abs() < 2.0 ** 127  # (0 and 118: some results leave the type)
+        got = int8_linear(xs.to(dev), w).cpu()
+        check(torch.where(end, got, 0), torch.where(end, want, 0.0), torch.where(end, slack, 0.0))
+        assert not bool(torch.isnan(got).any()) and bool(end[:, 0].all())
