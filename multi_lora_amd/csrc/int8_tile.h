@@ -13,11 +13,13 @@ typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(1))) void gvoid_t;
 typedef __attribute__((address_space(3))) void lvoid_t;
 
-// sum * a * b, the smaller scale first: the first product then leaves fp32 only
-// where the result does (scales go from 2^-107 to 2^121).  NaN stays.
-__device__ __forceinline__ float scaled(int32_t sum, float a, float b) {
-  const bool less = a < b;
-  return static_cast<float>(sum) * (less ? a : b) * (less ? b : a);
+// A sum (below 2^31) times a row's scale and a channel's, the channel's first
+// unless that could leave fp32 where the result does not.  (Scales go from 2^-107
+// to 2^121.)
+constexpr float kFarScale = 0x1p96f;
+__device__ __forceinline__ float scaled(int32_t sum, float row, float channel) {
+  const bool far = channel > kFarScale;
+  return static_cast<float>(sum) * (far ? row : channel) * (far ? channel : row);
 }
 
 // A tile's shape: TN weight rows by TM rows, waves WN by WM, S steps in LDS.  A
@@ -162,20 +164,28 @@ __global__ __launch_bounds__(Sh::NW * 64) void int8_tile_kernel(Int8Args a, int 
   lds_barrier();
   // Lane l has row l & 15 of a band's m and 4 (l >> 4) to + 3 of its n.  The
   // result goes through LDS, so that a row is stored whole.
+  float as[FM];
 #pragma unroll
-  for (int j = 0; j < FM; ++j) {
-    const int m = (wm * FM + j) * 16 + (lane & 15);
-    const float as = a.a_scales[min(m0 + m, a.m - 1)];
+  for (int j = 0; j < FM; ++j) as[j] = a.a_scales[min(m0 + (wm * FM + j) * 16 + (lane & 15), a.m - 1)];
 #pragma unroll
-    for (int i = 0; i < FN; ++i) {
-      const int n = (wn * FN + i) * 16 + (lane >> 4) * 4;
-      const f32x4 bs = *reinterpret_cast<const f32x4*>(&s.scale[n]), bias = *reinterpret_cast<const f32x4*>(&s.bias[n]);
+  for (int i = 0; i < FN; ++i) {
+    const int n = (wn * FN + i) * 16 + (lane >> 4) * 4;
+    const f32x4 bs = *reinterpret_cast<const f32x4*>(&s.scale[n]), bias = *reinterpret_cast<const f32x4*>(&s.bias[n]);
+    const bool far = __any(fmaxf(fmaxf(bs[0], bs[1]), fmaxf(bs[2], bs[3])) > kFarScale);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const int m = (wm * FM + j) * 16 + (lane & 15);
       float y[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = scaled(acc[i][j][e], as, bs[e]);
-        if (a.bias != nullptr) y[e] += bias[e];
+      for (int e = 0; e < 4; ++e) y[e] = static_cast<float>(acc[i][j][e]) * bs[e] * as[j];
+      if (far) {
+        asm volatile("");  // (stays a branch)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = scaled(acc[i][j][e], as[j], bs[e]);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (a.bias != nullptr) y[e] += bias[e];
       *reinterpret_cast<uint2*>(s.stage + m * Sh::PITCH + n * 2) = make_uint2(T::pack2(y[0], y[1]), T::pack2(y[2], y[3]));
     }
   }
