@@ -30,6 +30,7 @@ from .paged import _DTYPES, _guard, _no_grad, _no_tangent, _on_gpu, _untraced, _
 PAD = 128        # columns of codes come in multiples of it
 BAND = 16        # rows, too
 MAX_K = (1 << 17) - 1  # longer sums of products could leave 32 bits
+MAX_ROWS = (1 << 31) - 1  # the launches count rows in 32 bits
 
 
 def _code_shape(rows: int, k: int):
@@ -58,6 +59,8 @@ class Int8Rows:
             raise ValueError(f"rows of 1 to {MAX_K} elements, got {self.k}")
         if s.dtype != torch.float32 or s.dim() != 1 or not s.is_contiguous():
             raise ValueError(f"scales must be a contiguous float32 tensor of a number a row, got {tuple(s.shape)} {s.dtype}")
+        if s.shape[0] > MAX_ROWS:
+            raise ValueError(f"at most {MAX_ROWS} rows, got {s.shape[0]}")
         shape = _code_shape(s.shape[0], self.k)
         if (c.dtype != torch.int8 or tuple(c.shape) != shape or not c[0].is_contiguous() or c.data_ptr() % 16 or c.stride(0) % 16
                 or c.stride(0) < shape[1] * 1024):
@@ -121,6 +124,8 @@ def _matrix(what: str, t: torch.Tensor, dtypes) -> None:
     if t.dim() != 2 or t.dtype not in dtypes or (t.numel() > 0 and t.stride(1) != 1):
         names = " or ".join(str(d).replace("torch.", "") for d in dtypes)
         raise ValueError(f"{what} must be 2-D {names} with contiguous rows, got {tuple(t.shape)} {t.dtype}")
+    if t.shape[0] > MAX_ROWS:
+        raise ValueError(f"{what}: at most {MAX_ROWS} rows, got {t.shape[0]}")
     if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
         raise ValueError(f"{what}: the rows overlap")
 
