@@ -269,23 +269,25 @@ def fuse_gate_up_projections(wrappers: Dict[str, LinearWithLoRA], all_shapes: bo
 
 def quantize_base(model: nn.Module, skip: Sequence[str] = ("lm_head",)) -> int:
     """Replace the model's ``nn.Linear`` layers (on the GPU), those beneath
-    ``LinearWithLoRA`` too, by ``Int8Linear``; returns how many.  Layers whose
-    last name is in ``skip`` stay, and so does what is not a float16 or
-    bfloat16 layer.  Call it before projections are fused; adapters may be
-    registered and layers wrapped before or after."""
+    ``LinearWithLoRA`` too, by ``Int8Linear``; returns how many (one that
+    stands in several places is one, there too).  Layers whose last name is in
+    ``skip`` stay, and so does what is not a float16 or bfloat16 layer.  Call
+    it before projections are fused; adapters may be registered and layers
+    wrapped before or after."""
     if type(model) is nn.Linear:
         raise ValueError("a layer cannot replace itself: Int8Linear.from_linear")
-    count = 0
-    for name, module in list(model.named_modules()):
+    for name, module in model.named_modules():
         if isinstance(module, LinearWithLoRA) and module.qkv_group is not None:
             raise RuntimeError(f"{name} is part of a fused group: quantise the base before fusing projections")
-    for name, module in list(model.named_modules()):
+    replaced: Dict[nn.Module, Int8Linear] = {}
+    for name, module in list(model.named_modules(remove_duplicate=False)):  # a layer in several places: each of them
         leaf = [part for part in name.split(".") if part != "base_layer"][-1:]
         if type(module) is not nn.Linear or not leaf or leaf[0] in skip:
             continue
         if module.weight.dtype not in (torch.float16, torch.bfloat16):
             continue
         parent, _, child = name.rpartition(".")
-        setattr(model.get_submodule(parent) if parent else model, child, Int8Linear.from_linear(module))
-        count += 1
-    return count
+        if module not in replaced:
+            replaced[module] = Int8Linear.from_linear(module)
+        setattr(model.get_submodule(parent) if parent else model, child, replaced[module])
+    return len(replaced)
