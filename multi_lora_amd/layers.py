@@ -267,25 +267,36 @@ def fuse_gate_up_projections(wrappers: Dict[str, LinearWithLoRA], all_shapes: bo
     return _fuse_siblings(wrappers, GATE_UP_LEAVES, all_shapes)
 
 
+# What a module calls besides its forward.
+_HOOKS = ("_forward_pre_hooks", "_forward_hooks", "_backward_pre_hooks", "_backward_hooks", "_state_dict_pre_hooks",
+          "_state_dict_hooks", "_load_state_dict_pre_hooks", "_load_state_dict_post_hooks")
+
+
 def quantize_base(model: nn.Module, skip: Sequence[str] = ("lm_head",)) -> int:
     """Replace the model's ``nn.Linear`` layers (on the GPU), those beneath
     ``LinearWithLoRA`` too, by ``Int8Linear``; returns how many (one that
     stands in several places is one, there too).  Layers whose last name is in
-    ``skip`` stay, and so does what is not a float16 or bfloat16 layer.  Call
-    it before projections are fused; adapters may be registered and layers
-    wrapped before or after."""
+    ``skip`` stay, and so does what is not a float16 or bfloat16 layer, or is of
+    a class derived from ``nn.Linear``; a layer with hooks is refused before any
+    is replaced.  Call it before projections are fused; adapters may be
+    registered and layers wrapped before or after."""
     if type(model) is nn.Linear:
         raise ValueError("a layer cannot replace itself: Int8Linear.from_linear")
     for name, module in model.named_modules():
         if isinstance(module, LinearWithLoRA) and module.qkv_group is not None:
             raise RuntimeError(f"{name} is part of a fused group: quantise the base before fusing projections")
-    replaced: Dict[nn.Module, Int8Linear] = {}
-    for name, module in list(model.named_modules(remove_duplicate=False)):  # a layer in several places: each of them
+    places = []
+    for name, module in model.named_modules(remove_duplicate=False):  # a layer in several places: each of them
         leaf = [part for part in name.split(".") if part != "base_layer"][-1:]
         if type(module) is not nn.Linear or not leaf or leaf[0] in skip:
             continue
         if module.weight.dtype not in (torch.float16, torch.bfloat16):
             continue
+        if any(getattr(module, hooks) for hooks in _HOOKS) or "forward" in module.__dict__:
+            raise RuntimeError(f"{name} has hooks, which would be lost with the layer: remove them, or skip it")
+        places.append((name, module))
+    replaced: Dict[nn.Module, Int8Linear] = {}
+    for name, module in places:
         parent, _, child = name.rpartition(".")
         if module not in replaced:
             replaced[module] = Int8Linear.from_linear(module)
