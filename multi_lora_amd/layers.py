@@ -102,7 +102,7 @@ class Int8Linear(nn.Module):
     @classmethod
     def from_linear(cls, layer: nn.Linear) -> "Int8Linear":
         """The layer with its weight quantised (on the GPU)."""
-        return cls(quantize_rows(layer.weight.detach()), layer.bias)
+        return cls(quantize_rows(layer.weight.detach()), layer.bias).train(layer.training)
 
     @property
     def weight(self) -> Int8Rows:

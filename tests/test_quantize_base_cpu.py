@@ -85,3 +85,10 @@ def test_subclasses_stay():
 
     model = nn.ModuleDict(dict(a=Scaled(8, 6, dtype=torch.bfloat16), b=linear()))
     assert quantize_base(model) == 1 and type(model["a"]) is Scaled
+
+
+@pytest.mark.parametrize("training", [True, False])
+def test_mode_is_kept(training):
+    model = nn.ModuleDict(dict(a=linear())).train(training)
+    quantize_base(model)
+    assert model["a"].training == training
