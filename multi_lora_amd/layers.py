@@ -288,7 +288,7 @@ def quantize_base(model: nn.Module, skip: Sequence[str] = ("lm_head",)) -> int:
     places = []
     for name, module in model.named_modules(remove_duplicate=False):  # a layer in several places: each of them
         leaf = [part for part in name.split(".") if part != "base_layer"][-1:]
-        if type(module) is not nn.Linear or not leaf or leaf[0] in skip:
+        if type(module) is not nn.Linear or (leaf and leaf[0] in skip):
             continue
         if module.weight.dtype not in (torch.float16, torch.bfloat16):
             continue

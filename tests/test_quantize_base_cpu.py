@@ -92,3 +92,9 @@ def test_mode_is_kept(training):
     model = nn.ModuleDict(dict(a=linear())).train(training)
     quantize_base(model)
     assert model["a"].training == training
+
+
+def test_a_wrapper_alone():
+    """A model that is one wrapped layer."""
+    wrapper = LinearWithLoRA(linear())
+    assert quantize_base(wrapper) == 1 and isinstance(wrapper.base_layer, Int8Linear)
