@@ -87,10 +87,19 @@ def _packed(x: torch.Tensor) -> torch.Tensor:
     return rows
 
 
+def _int8_product(x: torch.Tensor, weight: Int8Rows, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x [..., k] @ weight.T + bias``; under autocast x and bias are cast as those of ``F.linear`` are."""
+    if torch.is_autocast_enabled("cuda") and x.dtype != torch.float64:
+        dtype = torch.get_autocast_dtype("cuda")
+        x, bias = x.to(dtype), None if bias is None else bias.to(dtype)
+    return int8_linear(_packed(x), weight, bias).view(*x.shape[:-1], weight.shape[0])
+
+
 class Int8Linear(nn.Module):
-    """``y = x @ weight.T + bias`` for 16-bit ``x``, with the weight in 8-bit
-    integers and a scale for each output channel, and x's rows quantised at
-    every call.  GPU only; no gradients (a model that serves)."""
+    """``y = x @ weight.T + bias`` for 16-bit ``x`` (under autocast also for
+    float32), with the weight in 8-bit integers and a scale for each output
+    channel, and x's rows quantised at every call.  GPU only; no gradients (a
+    model that serves)."""
 
     def __init__(self, weight: Int8Rows, bias: Optional[torch.Tensor] = None) -> None:
         super().__init__()
@@ -125,8 +134,7 @@ class Int8Linear(nn.Module):
         return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        y = int8_linear(_packed(x), self.weight, self.bias)
-        return y.view(*x.shape[:-1], self.out_features)
+        return _int8_product(x, self.weight, self.bias)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
@@ -205,7 +213,7 @@ class QKVProjGroup:
     def _base(self, x: torch.Tensor) -> torch.Tensor:
         if isinstance(self.weight, Int8Rows):
             self._follow()
-            return int8_linear(_packed(x), self.weight).view(*x.shape[:-1], self.weight.shape[0])
+            return _int8_product(x, self.weight)
         return F.linear(x, self.weight)
 
     def forward(self, wrapper: LinearWithLoRA, x: torch.Tensor) -> torch.Tensor:

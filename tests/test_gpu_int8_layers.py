@@ -2,8 +2,11 @@
 
 import pytest
 import torch
+import torch.nn as nn
+import torch.nn.functional as F
 
-from multi_lora_amd.layers import fuse_gate_up_projections, fuse_qkv_projections
+from multi_lora_amd.kernels import int8_linear
+from multi_lora_amd.layers import Int8Linear, fuse_gate_up_projections, fuse_qkv_projections
 
 from tests.int8_ref import check, codes_of, product
 from tests.test_int8_layers_cpu import states, wrappers
@@ -45,3 +48,28 @@ def test_groups_whose_layers_are_moved_or_replaced(dev):
         x = x * 2
         for w in ws.values():
             assert torch.equal(w(x), w.base_layer(x))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("given", [torch.float32, torch.bfloat16, torch.float16])
+@torch.no_grad()
+def test_under_autocast(dev, given, dtype):
+    """Inputs and biases are cast to the region's type, as those of nn.Linear are; outside of one float32 is refused."""
+    torch.manual_seed(3)
+    layer = Int8Linear.from_linear(nn.Linear(72, 40, device=dev, dtype=torch.bfloat16))
+    x = torch.randn(3, 5, 72, device=dev).to(given)
+    want = int8_linear(x.to(dtype).view(15, 72), layer.weight, layer.bias.to(dtype)).view(3, 5, 40)
+    with torch.autocast("cuda", dtype=dtype):
+        got = layer(x)
+        assert F.linear(x, torch.zeros(1, 72, device=dev)).dtype == got.dtype == dtype and torch.equal(got, want)
+        with torch.autocast("cuda", enabled=False):
+            if given == torch.bfloat16:
+                assert layer(x).dtype == given
+            else:
+                with pytest.raises(ValueError):
+                    layer(x)
+    ws = {n: w.to(dev) for n, w in wrappers((48, 20, 16), 72, 0).items()}
+    fuse_qkv_projections(ws, all_shapes=True)
+    with torch.autocast("cuda", dtype=dtype):
+        for w in ws.values():
+            assert torch.equal(w(x), int8_linear(x.to(dtype).view(15, 72), w.base_layer.weight).view(3, 5, -1))
