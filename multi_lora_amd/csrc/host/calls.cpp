@@ -804,7 +804,7 @@ PyObject* int8_linear(PyObject* const* args, Took* took) {
   const at::ScalarType dt = x->scalar_type();
   const long k = PyLong_AsLong(args[3]);
   if (!is_current(dev) || (dt != at::kBFloat16 && dt != at::kHalf) || !is_rows(*x) || x->size(0) == 0 || x->size(1) != k ||
-      !is_rows_of(x, dev, dt, x->size(0), k) || wants_grad({x}) || maybe_traced() || has_tangent({x}))
+      !is_rows_of(x, dev, dt, x->size(0), k) || wants_grad({x, scales}) || maybe_traced() || has_tangent({x, scales}))
     return nullptr;
   // Int8Rows has checked what its tensors look like.
   if (codes->dim() != 5 || codes->device() != dev || codes->scalar_type() != at::kChar || scales->dim() != 1 ||

@@ -203,6 +203,8 @@ def int8_matmul(a: Int8Rows, b: Int8Rows, dtype: torch.dtype, bias: Optional[tor
     if given, which may be a column slice of a wider tensor)."""
     dev = _on_gpu("int8_matmul", a.codes, b.codes)
     _untraced("int8_matmul")
+    _no_grad("int8_matmul", a.scales, b.scales)
+    _no_tangent("int8_matmul", a.scales, b.scales)
     if a.k != b.k:
         raise ValueError(f"rows of {a.k} and of {b.k} elements")
     if dtype not in _DTYPES:
@@ -231,8 +233,8 @@ def int8_linear(x: torch.Tensor, weight: Int8Rows, bias: Optional[torch.Tensor] 
         return done if out is None else out
     dev = _on_gpu("int8_linear", x, weight.codes)
     _untraced("int8_linear")
-    _no_grad("int8_linear", x)
-    _no_tangent("int8_linear", x)
+    _no_grad("int8_linear", x, weight.scales)
+    _no_tangent("int8_linear", x, weight.scales)
     _matrix("x", x, _DTYPES)
     rows, k = x.shape
     if k != weight.k:
