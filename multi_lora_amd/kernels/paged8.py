@@ -189,8 +189,8 @@ def paged_attention_fp8(q: torch.Tensor, pool: Fp8Pool, step: PagedStep, scale: 
     what = "paged_attention_fp8"
     dev = _on_gpu(what, q, pool.keys, step.row_indptr)
     _untraced(what)
-    _no_grad(what, q)
-    _no_tangent(what, q)
+    _no_grad(what, q, pool.keys, pool.values)
+    _no_tangent(what, q, pool.keys, pool.values)
     _checked(what, pool, step)
     if not step.has_plan:
         raise ValueError("the step has no work list: give page_tables the heads")
