@@ -53,18 +53,12 @@ __device__ __forceinline__ uint32_t pack4(const uint32_t* c) {
   return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 
-// Eight elements of a row from element e on, zeros behind its end.
+// Eight elements of a row of a 16-bit type from element e on, zeros behind its end.
 template <class T, bool AL>
 __device__ __forceinline__ void load8(const typename T::raw_t* row, int e, int k, float* f) {
-  const int valid = min(max(k - e, 0), 8);
-  if constexpr (sizeof(typename T::raw_t) == 2) {
-    const u32x4 v = load_row_chunk<T, AL>(row, e, valid);
+  const u32x4 v = load_row_chunk<T, AL>(row, e, min(max(k - e, 0), 8));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = chunk_elem<T>(v, i);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < valid ? T::to_f32(row[e + i]) : 0.f;
-  }
+  for (int i = 0; i < 8; ++i) f[i] = chunk_elem<T>(v, i);
 }
 
 // Rows from which on a workgroup has more than one of them, where a row fits the

@@ -30,13 +30,13 @@ struct TileShape {
   static constexpr int NW = WN * WM;
   static constexpr int FN = TN / WN / 16, FM = TM / WM / 16;  // bands of a wave
   static constexpr int BLOCKS = (TN + TM) / 8;                // of a step
-  static constexpr int LOADS = (BLOCKS + NW - 1) / NW;        // of a wave (the last one is loaded again where they do not come out even)
+  static constexpr int LOADS = BLOCKS / NW;                   // of a wave
   static constexpr int EARLY = (LOADS + 1) / 2;               // of them in the second half of a step, the others in the next one's first
   static constexpr int STAGE = BLOCKS * kInt8Block;
   static constexpr int PITCH = TN * 2 + 16;                   // of a row of the result: 16 bytes more, so that rows begin in different banks
   static constexpr int OUT = TM * PITCH;
   static constexpr int BYTES = S * STAGE > OUT ? S * STAGE : OUT;
-  static_assert(FN * WN * 16 == TN && FM * WM * 16 == TM, "whole bands a wave");
+  static_assert(FN * WN * 16 == TN && FM * WM * 16 == TM && LOADS * NW == BLOCKS, "whole bands and loads a wave");
 };
 
 template <class Sh>
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(Sh::NW * 64) void int8_tile_kernel(Int8Args a, int 
 
   // Block b of a step: half b & 1 of band b >> 1 of the weight's tile, then of the other.
   const int8_t* from[LOADS];
-  auto block = [&](int i) { return Sh::BLOCKS % NW == 0 ? wave * LOADS + i : min(i * NW + wave, Sh::BLOCKS - 1); };
+  auto block = [&](int i) { return wave * LOADS + i; };
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
     const int b = block(i), band = b >> 1;

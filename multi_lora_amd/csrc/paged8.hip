@@ -17,7 +17,6 @@
 #include "kernels.h"
 #include "loads.h"
 #include "paged.h"
-#include "rotary.h"
 
 namespace mlora {
 
@@ -64,7 +63,7 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float inv, int e) {
   return __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
 }
 
-// Four codes rounded again for an exponent that is `down` more.
+// Four codes rounded again for a larger exponent, `ratio` = 2^(old - new).
 __device__ __forceinline__ uint32_t moved4(uint32_t w, float ratio) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
