@@ -160,12 +160,7 @@ class QKVProjGroup:
     """
 
     def __init__(self, wrappers: List[LinearWithLoRA], all_shapes: bool = False) -> None:
-        if any(w.base_layer.bias is not None for w in wrappers):
-            raise RuntimeError("QKV fusion requires bias=None")
         self.wrappers = list(wrappers)
-        quantised = {isinstance(w.base_layer, Int8Linear) for w in wrappers}
-        if len(quantised) != 1:
-            raise RuntimeError("fusion of 8-bit and 16-bit projections")
         self._parts: List[tuple] = []  # 8-bit: codes and scales of each layer, views of the fused weight's
         self._join()
         for w in wrappers:
@@ -178,7 +173,11 @@ class QKVProjGroup:
     def _join(self) -> None:
         """The fused weight; each layer's becomes a view of it: no extra memory."""
         layers = [w.base_layer for w in self.wrappers]
+        if any(m.bias is not None for m in layers):
+            raise RuntimeError("QKV fusion requires bias=None")
         eight = isinstance(layers[0], Int8Linear)
+        if any(isinstance(m, Int8Linear) != eight for m in layers):
+            raise RuntimeError("fusion of 8-bit and 16-bit projections")
         # Where a projection's columns begin: one after the other, 8-bit ones in bands of rows of their own.
         step = BAND if eight else 1
         self.weight: Union[torch.Tensor, Int8Rows] = (
@@ -194,10 +193,10 @@ class QKVProjGroup:
             self._parts = [(m.codes, m.scales) for m in layers]
 
     def _follow(self) -> None:
-        """8-bit: the fused weight again, where a layer's buffers were replaced (a state dict assigned, a move)."""
+        """8-bit: the fused weight again, where a layer or its buffers were replaced (a state dict assigned, a move)."""
         for w, (codes, scales) in zip(self.wrappers, self._parts):
             held = w.base_layer._buffers
-            if held["codes"] is not codes or held["scales"] is not scales:
+            if held.get("codes") is not codes or held.get("scales") is not scales:
                 with torch.inference_mode(False):
                     return self._join()
 
@@ -213,6 +212,7 @@ class QKVProjGroup:
     def _base(self, x: torch.Tensor) -> torch.Tensor:
         if isinstance(self.weight, Int8Rows):
             self._follow()
+        if isinstance(self.weight, Int8Rows):
             return _int8_product(x, self.weight)
         return F.linear(x, self.weight)
 

@@ -87,3 +87,27 @@ def test_a_fused_group_follows_buffers_that_are_replaced(widths):
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         ws["layer.q_proj"](x)
     check(ws, widths, k, 90)
+
+
+def test_a_layer_of_a_group_that_is_replaced():
+    """By another 8-bit layer: the group has its weight.  By a 16-bit one: the group cannot be computed as one."""
+    widths, k = (32, 16, 48), 70
+    ws = fused(widths, k, 0)
+    x = torch.zeros(1, 1, k)
+    ws["layer.k_proj"].base_layer = Int8Linear(rows(16, k, 77))
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        ws["layer.q_proj"](x)
+    assert torch.equal(ws["layer.q_proj"].qkv_group.weight.to_rows()[32:48], rows(16, k, 77).to_rows())
+    ws["layer.v_proj"].base_layer = nn.Linear(k, 48, bias=False)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="8-bit and 16-bit"):
+            ws["layer.q_proj"](x)
+    ws["layer.v_proj"].base_layer = Int8Linear(rows(48, k, 3), torch.zeros(48))
+    with pytest.raises(RuntimeError, match="bias"):
+        ws["layer.q_proj"](x)
+    torch.manual_seed(0)
+    for w, n in zip(ws.values(), widths):  # all of them: a 16-bit group
+        w.base_layer = nn.Linear(k, n, bias=False)
+    x = torch.randn(2, 1, k)
+    for w in ws.values():
+        assert torch.allclose(w(x), w.base_layer(x), atol=1e-6)
