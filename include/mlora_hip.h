@@ -497,7 +497,7 @@ int mlora_verify_drafts(const void* target, int64_t target_row_stride, int32_t r
                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- the paged KV cache in 8 bits ----------------------------------------
- * Pools of e4m3 codes (4 exponent, 3 mantissa bits; NaN 0x7f, no infinity) in
+ * Pools of e4m3 codes (4 exponent, 3 mantissa bits; NaN 0x7f or 0xff, no infinity) in
  * the layout of the 16-bit ones,
  *   keys   [num_pages, kv_heads, page, D]
  *   values [num_pages, kv_heads, D, page]
@@ -513,7 +513,7 @@ int mlora_verify_drafts(const void* target, int64_t target_row_stride, int32_t r
  * the one it has if that is larger and the block holds earlier rows (its first
  * new row is not its first position); those rows' codes are then rounded again
  * if it grows.  Infinities and NaN (fp16: what rounds to infinity, too) become
- * NaN and do not count.  Rows of one block must be neighbours in ascending
+ * NaN (0xff) and do not count.  Rows of one block must be neighbours in ascending
  * order, as mlora_page_tables lists them. */
 int mlora_rotary_paged_write_fp8(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
                                  int64_t v_row_stride, const void* cos, const void* sin, int64_t rot_row_stride,

@@ -87,7 +87,10 @@ __device__ __forceinline__ uint32_t widest(const u32x4& v, uint32_t top) {
 // columns.  With two rows, two lanes write 32 bytes side by side, and a wave
 // reads 1 KB of each row.  KEEP chunks stay in registers, what a row has more of
 // is read twice.  Bound by bytes, 2 in and 1 out an element, and nearly as much
-// by its arithmetic: 4075 rows of 4096 13.8 us, 3.6 TB/s.
+// by its arithmetic: 4075 rows of 4096 13.8 us, 3.6 TB/s, and 11.1 within a call,
+// whose workspace the last-level cache holds; 1088 of 14336, one a workgroup of
+// 16 waves, 15.8.  Rows that are not aligned are read an element at a time, each
+// load behind a branch of its own and waited for: 333 of 1111 4.8 us.
 template <class T, int R, int NW, int KEEP, bool AL>
 __global__ __launch_bounds__(NW * 64) void quantize_rows_kernel(QuantArgs a) {
   using raw = typename T::raw_t;
@@ -179,9 +182,15 @@ __device__ __forceinline__ void store4(const Int8Args& a, int m, int n, const i3
 // operands, and add their sums in LDS: no barrier while weights stream.
 // KEEP: the rows themselves (of at most KEEP chunks of eight elements a thread)
 // are read and quantised by every workgroup, while its first blocks are on
-// their way.  Bound by the weight's bytes: 64 rows to 28672 columns, K 4096
-// (117 MB), 27.6 us, 4.3 TB/s; one row to 4096 columns 5.9, of which the bytes
-// need 3.3 and a launch's chain the rest.
+// their way.  Near the weight's bytes where columns fill the chip: 64 rows to
+// 28672 of them, K 4096 (117 MB), 27.6 to 28.6 us, 4.1 to 4.3 TB/s.  What keeps
+// it from a copy's 5.1: the compiler puts a trip's reloads behind its last
+// product, which has waited for all loads before, so that nothing is on its way
+// then.  One row to 4096 columns 5.7, of which the bytes need 3.3; the rest is a
+// launch's chain and the columns' scales, which are loaded after the products.
+// Few columns leave CUs idle and long rows make long trips, since K is not
+// split over workgroups: 32 rows to 1024 columns 3.2 us (bytes 0.8), of K 14336
+// to 4096 columns 15.8 (11.5), 64 rows 19.3.
 template <class T, int MT, int NT, int NW, int U, int KEEP>
 __global__ __launch_bounds__(NW * 64) void int8_rows_kernel(Int8Args a) {
   using raw = typename T::raw_t;

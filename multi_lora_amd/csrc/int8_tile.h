@@ -66,10 +66,11 @@ __device__ __forceinline__ void pick_tile8(int id, int tiles_n, int tiles_m, int
 // The fragments of the next 64 bytes are read, and loads sent, while this
 // one's products run.  Bound by the matrix units at the clock that this load
 // allows (1.9 GHz; they are busy in 48 to 55 % of the cycles) and by the loads'
-// issue between them: 4075 rows to 6144 columns, K 4096, 94 to 98 us, 2090 to
-// 2190 TOP/s, where a library product without scales takes 118; 8192^3 2300 to
-// 2400 TOP/s (2109).  Three or four places in LDS, steps of 64 bytes and groups
-// of waves that share K were no faster.
+// issue between them: 4075 rows to 6144 columns, K 4096, 95.2 us, 2150 TOP/s
+// (replayed from a graph; 113 under a profiler), where a library product without
+// scales takes 102 to 103; 8192^3 450 us, 2440 TOP/s (443 to 446).  Three or four
+// places in LDS, steps of 64 bytes and groups of waves that share K were no
+// faster.
 template <class T, class Sh>
 __global__ __launch_bounds__(Sh::NW * 64) void int8_tile_kernel(Int8Args a, int tiles_n, int tiles_m) {
   using raw = typename T::raw_t;

@@ -30,6 +30,10 @@ constexpr int kApLongRows = 128;
 // A range is split only into parts of at least this many positions.  A part of
 // a long tile writes and reads again 128 rows of sums: 512 tokens after 2000
 // beside 32 decoding requests 99 us, with 512 or 2048 here 117 and 115.
+// The same rule serves 8-bit pages, of which a wave takes 64 positions at once
+// (us with 128, 256 and 512 here): one of 4000 12.2, 11.6 and 12.4; one of 700 9.3,
+// 9.5 and 9.0; eight of 1500 13.5, 14.1 and 13.7; five drafts of each of 32 26.1, 26.1
+// and 23.0 (32 heads); 64 of 200 to 3985 and three of up to 32,000 the same.
 constexpr int kApMinSplit = 256;
 constexpr int kApMinSplitLong = 1024;
 // Short ranges are split only if the longest is longer than a part by kApKeep,

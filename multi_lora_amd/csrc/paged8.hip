@@ -336,12 +336,14 @@ __global__ __launch_bounds__(256, 4) void paged_write8_few_kernel(Write8Args arg
 }
 
 // Many rows.  Some workgroups have the cache blocks that begin in kWindow rows,
-// for keys or for values of one head; a block is one workgroup's alone, so its exponent and codes are changed without atomics.  Its 256 threads
-// share a block of 16 x D numbers, 8 (D 64: 4) each: with a wave a block, the
-// kernel's registers (136) left the q rows, which the other workgroups rotate, a
-// third of the waves (4075 rows 30 us).  Bound by bytes: those rows (94 MB) 23.9
-// us, 3.9 TB/s; both kinds of workgroup in turn 24.3 (4096 tokens of one prompt
-// 24.5, and 29.9).
+// for keys or for values of one head; a block is one workgroup's alone, so its
+// exponent and codes are changed without atomics.  Its 256 threads share a block
+// of 16 x D numbers, 8 (D 64: 4) each: with a wave a block, the kernel's registers
+// (136) left the q rows, which the other workgroups rotate, a third of the waves
+// (4075 rows 30 us).  Those rows (94 MB) take 24.3 us, 3.9 TB/s; both kinds of
+// workgroup in turn 24.3 (4096 tokens of one prompt 24.5, and 29.9).  Bytes need
+// 18.4; a thread's eight values are loaded one after the other, each of two bytes
+// behind a branch of its own and waited for, after the block's exponent.
 constexpr int kWindow = 16;
 template <class T, int D, bool AL>
 __global__ __launch_bounds__(256) void paged_write8_kernel(Write8Args args, int block_groups) {
@@ -443,8 +445,16 @@ __global__ __launch_bounds__(256) void paged_write8_kernel(Write8Args args, int 
   }
 }
 
-// Calls of fewer rows take a wave a row: 256 decoding requests 7.7 us, 12.7 with
-// a workgroup a block; 64 of them 5.1 on the device.
+// Calls of fewer rows take a wave a row, of more a workgroup a block.  That is
+// best where rows and requests go together, as in steps of decoding requests
+// or of prompts: 64 requests of one token 4.8 us (24 with a workgroup a block),
+// 511 12.5 (38); five drafts of 32 6.5 (8.9), of 64 8.5 (10.4), of 256 18.6 with a
+// wave a row and 16.3 with a workgroup a block; 1024 and 2048 tokens of a prompt
+// 36.7 and 65.5, 8.4 and 13.6.  It is not best for short prompts alone, of which a
+// wave reads 16 rows (64 tokens 12.3 us, 4.3 with a workgroup a block; 300 17.6,
+// 4.8; eight of 40 19, 6.8), nor for many requests of one token, whose blocks a
+// workgroup takes one after the other (600 39.0 us, 13.8 with a wave a row; 2048
+// 81, 39.6): the call has rows and slots, not how many rows a request has.
 constexpr int kFewRows = 512;
 
 template <class T, int D, bool AL>

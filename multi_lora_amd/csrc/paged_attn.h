@@ -28,7 +28,9 @@
 // exponent, for keys and for values.  A code times its power of two is a number
 // of the data type, so the operands are those of a 16-bit cache that holds the
 // values which the codes stand for, and nothing else changes: the conversion
-// instruction takes two codes and the scale.
+// instruction takes two codes and the scale.  (Against 64 bits, relative to the
+// results' norm: 0.0019 to 0.0022 in bf16, where rounding the result alone gives
+// 0.0016; the difference is the weights' rounding.)
 #pragma once
 
 #include <algorithm>
@@ -629,10 +631,11 @@ constexpr int kBlock = 68;
 // step go straight into LDS, a step ahead, in one of two buffers.  Chunk p of
 // a row lies at p ^ (row's low bits), which spreads a fragment's rows over the
 // banks.  Bound by the matrix units and the exponentials beside them: 444
-// GFLOP (chunks of 4096, 777 and 1301 tokens, 32 heads of 128) take 465 to 474
-// us a call, 935 to 955 TFLOP/s where a library product of 8192^3 has 1200 to
-// 1212 on the same card (504 on average under the profiler, 468 at best).  The
-// matrix units are busy in 44 % of the cycles, at 1.9 GHz under this load.
+// GFLOP (chunks of 4096, 777 and 1301 tokens, 32 heads of 128) take 463 to 474
+// us a call, 935 to 960 TFLOP/s, where a library product of 8192^3 has 1606 to
+// 1634 in a long run and 1223 in its first calls (504 on average under the
+// profiler, 468 at best).  The matrix units are busy in 44 % of the cycles, at
+// 1.9 GHz under this load.
 // Without the exponentials it takes 4 % less, without the loads 17 %, with half
 // of the second product 12 %.
 template <int D>
@@ -1021,7 +1024,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_short_kernel(PagedAttnArgs a
 // tokens beside 128 decoding requests, 114 instead of 99 with four times as
 // many of them).  Both kinds in turn from the start: four prompts of 1024
 // beside 128 requests 138 us against 157, but 344 against 288 for 2048 tokens
-// after 4096 beside 64 requests, whose last long items then start late.
+// after 4096 beside 64 requests, whose last long items then start late.  (Over
+// 8-bit pages with D 128 five of its 256 registers are spilled.)
 template <class T, int D, bool KV8>
 __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(PagedAttnArgs a) {
   __shared__ union {

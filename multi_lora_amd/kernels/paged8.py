@@ -126,7 +126,8 @@ def rotary_paged_write_fp8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, co
     rows.  Infinities and NaN, and in float16 what rounds to infinity, are
     written as NaN and do not count.  Rows without a slot are rotated and not
     written.  Rows that replace others of their block (rejected drafts, a step
-    that is run again) leave its exponent as high as those made it.  One write at a time may change a step's requests.
+    that is run again) leave its exponent as high as those made it.  One write
+    at a time may change a step's requests.
     """
     done = _ffi.calls().paged_write8(q, k, v, cos, sin, pool.keys, pool.values, pool.key_scales, pool.value_scales, pool._code,
                                      step._native, step.filled, out)
