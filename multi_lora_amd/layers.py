@@ -165,8 +165,11 @@ class QKVProjGroup:
         self._join()
         for w in wrappers:
             w.qkv_group = self
+        # One call's input (and its version), its result, and the projections that have not taken theirs.
         self._cached_x: Optional[torch.Tensor] = None
+        self._cached_version: Optional[int] = None
         self._cached_out: Optional[torch.Tensor] = None
+        self._waiting: set = set()
         self._delta_done = False
         self.all_shapes = all_shapes
 
@@ -219,7 +222,8 @@ class QKVProjGroup:
     def forward(self, wrapper: LinearWithLoRA, x: torch.Tensor) -> torch.Tensor:
         if x.shape[-2] != 1 and not self.all_shapes:
             return wrapper.add_delta(x, wrapper.base_layer(x))
-        if self._cached_x is not x:
+        version = None if x.is_inference() else x._version
+        if self._cached_x is not x or self._cached_version != version or wrapper not in self._waiting:
             self._cached_x = None  # if this call raises, the next one computes
             self._cached_out = self._base(x)
             self._delta_done = False
@@ -235,9 +239,11 @@ class QKVProjGroup:
                     [w.qkv_slice[0] for w in self.wrappers],
                 )
                 self._delta_done = True
-            self._cached_x = x
+            self._cached_x, self._cached_version = x, version
+            self._waiting = set(self.wrappers)
         start, end = wrapper.qkv_slice
         y = self._cached_out[..., start:end]
+        self._waiting.discard(wrapper)
         if self._delta_done:
             return y
         return wrapper.add_delta(x, y)
