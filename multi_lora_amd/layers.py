@@ -89,7 +89,7 @@ def _packed(x: torch.Tensor) -> torch.Tensor:
 
 def _int8_product(x: torch.Tensor, weight: Int8Rows, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x [..., k] @ weight.T + bias``; under autocast x and bias are cast as those of ``F.linear`` are."""
-    if torch.is_autocast_enabled("cuda") and x.dtype != torch.float64:
+    if torch.is_autocast_enabled("cuda") and x.is_floating_point() and x.dtype != torch.float64:
         dtype = torch.get_autocast_dtype("cuda")
         x, bias = x.to(dtype), None if bias is None else bias.to(dtype)
     return int8_linear(_packed(x), weight, bias).view(*x.shape[:-1], weight.shape[0])

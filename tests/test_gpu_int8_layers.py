@@ -73,3 +73,12 @@ def test_under_autocast(dev, given, dtype):
     with torch.autocast("cuda", dtype=dtype):
         for w in ws.values():
             assert torch.equal(w(x), int8_linear(x.to(dtype).view(15, 72), w.base_layer.weight).view(3, 5, -1))
+
+
+@pytest.mark.parametrize("given", [torch.int64, torch.float64])
+@torch.no_grad()
+def test_autocast_casts_no_others(dev, given):
+    """As with nn.Linear: numbers of 64 bits and whole numbers are not cast, and so not taken."""
+    layer = Int8Linear.from_linear(nn.Linear(72, 40, device=dev, dtype=torch.bfloat16))
+    with torch.autocast("cuda", dtype=torch.bfloat16), pytest.raises(ValueError):
+        layer(torch.ones(2, 72, device=dev, dtype=given))
